@@ -268,6 +268,125 @@ LAIC_API int laic_selftest_peer_timeout(int32_t device, int64_t spin_cycles, int
 LAIC_API int laic_tensor_matvec_noalloc(laic_tensor* t, const float* x_dev, float* y_dev, int32_t batch,
                                         void* stream);
 
+/* ---- serving: a KV cache in pages, attention over it, drafted tokens -------
+ * No counterpart in the reference, which holds one sequence's cache in host
+ * vectors. Every pointer named _dev is device memory of `device`; work runs in
+ * order on `stream` (cudaStream_t), nothing is allocated, and the calls may be
+ * captured into a CUDA graph. The calling thread's current device is left as it
+ * was. Rows of any stride are taken; 16-byte aligned rows are faster. */
+
+/* One layer's KV cache in pages of page_size positions:
+ * k_dev, v_dev [num_pages][kv_heads][page_size][head_dim], binary16. A sequence's
+ * position t lies in page page_table[t / page_size] at offset t % page_size. */
+typedef struct laic_kv_pages {
+    int32_t device;
+    int32_t kv_heads, head_dim;  /* head_dim 32, 64 or 128 */
+    int32_t page_size;           /* 16, 32, 64, 128 or 256 */
+    int32_t num_pages;
+    void* k_dev;
+    void* v_dev;
+    int32_t* err_dev;            /* sticky error word (zero it once): an index on the device that a kernel
+                                    refused leaves its LAIC_KV_BAD_* bits here (laic_kv_check) */
+} laic_kv_pages;
+
+#define LAIC_KV_BAD_SEQ 1   /* seq_dev outside the page table */
+#define LAIC_KV_BAD_POS 2   /* a position or length beyond the page table, the rotation table or a given bound */
+#define LAIC_KV_BAD_PAGE 4  /* a page id outside [0, num_pages) */
+#define LAIC_KV_BAD_GROUP 8 /* group_rows_dev not ascending within the rows, or a group above max_group_rows */
+
+typedef struct laic_kv_append_args {
+    int32_t rows;             /* tokens */
+    int32_t heads;            /* query heads (0: no queries) */
+    int32_t in_type, q_type;  /* LAIC_GGML_F32 or LAIC_GGML_F16: of q, k, v and of q_out */
+    int32_t rope_dim;         /* even, <= head_dim; 0: no rotation */
+    int32_t rope_positions;   /* rows of rope_dev */
+    int32_t nseq, pages_per_seq;
+    int64_t ldq, ldk, ldv, ldqo; /* elements between rows (heads of a row are contiguous) */
+    const void *q_dev, *k_dev, *v_dev;
+    void* q_out_dev;          /* may be q_dev (same type and ld); no other output may overlap an input */
+    const int32_t* pos_dev;   /* [rows] the token's position; negative: padding, nothing of the row is written */
+    const int32_t* seq_dev;   /* [rows] row of the page table (NULL: row t is sequence t) */
+    const int32_t* page_table_dev; /* [nseq][pages_per_seq] */
+    const float* rope_dev;    /* [rope_positions][rope_dim / 2][2]: cos, sin */
+} laic_kv_append_args;
+
+/* For every row t: rotate q[t] and k[t] by the angles of its position (adjacent
+ * pairs, as the reference, src/inference_v2.cpp:25), write q to q_out_dev and
+ * k, v (rounded to binary16) to the position's place in the pages. Two rows must
+ * not name the same place. A row whose indices are out of range is left out and
+ * recorded in err_dev. */
+LAIC_API int laic_kv_append(const laic_kv_pages* pages, const laic_kv_append_args* args, void* stream);
+
+typedef struct laic_kv_attention_args {
+    int32_t rows, heads;      /* query rows (tokens); query heads, a multiple of kv_heads, at most 8 per kv head */
+    int32_t type;             /* of q and out: LAIC_GGML_F32 (products to 22 bits of q and of the weights) or
+                                 LAIC_GGML_F16 (weights rounded to binary16) */
+    int32_t nseq, pages_per_seq;
+    int32_t max_len;          /* bound on len_dev */
+    int32_t groups;           /* groups of rows that share their first positions (0: none) */
+    int32_t max_group_rows, max_shared; /* bounds on the groups' rows and shared lengths */
+    int32_t max_private;      /* bound on a row's positions beyond its group's shared ones (-1: max_len) */
+    float scale;              /* of the scores; 0: 1 / sqrt(head_dim) */
+    int64_t ldq, ldo;
+    const void* q_dev;
+    void* out_dev;
+    const int32_t* len_dev;   /* [rows] positions the row sees, its own included; 0: the output is zeros;
+                                 negative: padding, the output is left as it is */
+    const int32_t* seq_dev;   /* [rows] row of the page table (NULL: row r is sequence r) */
+    const int32_t* page_table_dev;
+    const int32_t* group_rows_dev; /* [groups + 1] ascending: group g is rows [g], ..., [g + 1] - 1 */
+    const int32_t* group_len_dev;  /* [groups] */
+    void* workspace_dev;      /* laic_kv_attention_workspace bytes, 16-byte aligned, of this call alone while it runs */
+    uint64_t workspace_bytes;
+} laic_kv_attention_args;
+
+/* out[r] = softmax(scale * q[r] . K) V over the row's first len_dev[r] positions,
+ * query head h with kv head h / (heads / kv_heads). The rows of group g hold the
+ * same keys and values in positions [0, group_len_dev[g]): the kernels read them
+ * once, through the page table row of the group's first row. Rows that share a
+ * whole sequence with causal lengths (a prompt's tokens, drafted tokens) are a
+ * group whose length is the longest. Masked positions never reach a row's output,
+ * whatever they hold. */
+LAIC_API int laic_kv_attention(const laic_kv_pages* pages, const laic_kv_attention_args* args, void* stream);
+/* Bytes of workspace the call needs (0 possible); reads no pointer of `args`. */
+LAIC_API int laic_kv_attention_workspace(const laic_kv_pages* pages, const laic_kv_attention_args* args,
+                                         uint64_t* bytes);
+/* Synchronise `stream`, read and clear err_dev: LAIC_E_INVALID with the indices' description if any was refused. */
+LAIC_API int laic_kv_check(const laic_kv_pages* pages, void* stream);
+
+/* probs[r] = softmax(logits[r] / temperature[r]); temperature <= 0: one for the
+ * first maximum (sample()'s greedy choice, reference src/inference_v2.cpp:32), zeros elsewhere. A NaN
+ * logit counts as -inf; equal +inf logits share the row; a row of -inf gives zeros. probs_dev
+ * may be logits_dev with the same ld. */
+LAIC_API int laic_logits_probs(int32_t device, int32_t rows, int32_t vocab, const float* logits_dev, int64_t ld_logits,
+                               const float* temperature_dev, float* probs_dev, int64_t ld_probs, void* stream);
+
+#define LAIC_NO_TOKEN 0xFFFFFFFFu
+#define LAIC_MAX_DRAFT 64
+
+typedef struct laic_verify_args {
+    int32_t nseq, max_draft, vocab;  /* max_draft in [0, LAIC_MAX_DRAFT] */
+    int64_t ld_target, ld_draft;     /* elements between probability rows */
+    const float* target_dev;         /* [nseq][max_draft + 1] rows: the target's probabilities after each drafted prefix */
+    const float* draft_dev;          /* [nseq][max_draft] rows the tokens were drawn from; NULL: drafted with certainty */
+    const uint32_t* draft_ids_dev;   /* [nseq][max_draft] */
+    const int32_t* n_draft_dev;      /* [nseq] drafted tokens (above max_draft: max_draft); negative: padding */
+    const float* accept_u_dev;       /* [nseq][max_draft] numbers in [0, 1) */
+    const float* sample_u_dev;       /* [nseq] */
+    uint32_t* out_ids_dev;           /* [nseq][max_draft + 1]: accepted tokens, the sampled one, then LAIC_NO_TOKEN */
+    int32_t* out_n_dev;              /* [nseq] tokens given (accepted + 1) */
+} laic_verify_args;
+
+/* Speculative decoding's check of drafted tokens. With p_j, q_j the target's and
+ * the draft's probabilities at drafted token x_j: accept while
+ * accept_u_j * q_j(x_j) < p_j(x_j) (compared exactly). At the first refusal j the
+ * next token is drawn from max(p_j - q_j, 0) (from p_j where that is zero
+ * everywhere), after n accepted tokens from p_n: the lowest v whose running sum
+ * exceeds sample_u * total, in 64 bits. The tokens follow the target's
+ * distribution. An id outside the vocabulary is refused; negative and NaN
+ * probabilities count as zero. Padding sequences' outputs are left as they are. */
+LAIC_API int laic_verify_drafts(int32_t device, const laic_verify_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

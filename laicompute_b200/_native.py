@@ -24,6 +24,8 @@ EXPORTS = (
     "laic_tensor_matvec", "laic_tensor_dequant", "laic_tensor_bytes", "laic_tensor_matvec_noalloc",
     "laic_dev_prefill_batch", "laic_tensor_check", "laic_selftest_peer_timeout",
     "laic_dev_step_trace", "laic_blocks_convert",
+    "laic_kv_append", "laic_kv_attention", "laic_kv_attention_workspace", "laic_kv_check", "laic_logits_probs",
+    "laic_verify_drafts",
 )
 
 
@@ -54,6 +56,36 @@ class DevStats(ctypes.Structure):
 class KernelRecord(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 16), ("launches", ctypes.c_int32), ("total_us", ctypes.c_double),
                 ("bytes", ctypes.c_double)]
+
+
+class KvPagesDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("device", "kv_heads", "head_dim", "page_size", "num_pages")] + [
+        (n, ctypes.c_void_p) for n in ("k_dev", "v_dev", "err_dev")]
+
+
+class KvAppendArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("rows", "heads", "in_type", "q_type", "rope_dim", "rope_positions", "nseq",
+                                               "pages_per_seq")]
+                + [(n, ctypes.c_int64) for n in ("ldq", "ldk", "ldv", "ldqo")]
+                + [(n, ctypes.c_void_p) for n in ("q_dev", "k_dev", "v_dev", "q_out_dev", "pos_dev", "seq_dev",
+                                                  "page_table_dev", "rope_dev")])
+
+
+class KvAttentionArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("rows", "heads", "type", "nseq", "pages_per_seq", "max_len", "groups",
+                                               "max_group_rows", "max_shared", "max_private")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int64) for n in ("ldq", "ldo")]
+                + [(n, ctypes.c_void_p) for n in ("q_dev", "out_dev", "len_dev", "seq_dev", "page_table_dev",
+                                                  "group_rows_dev", "group_len_dev", "workspace_dev")]
+                + [("workspace_bytes", ctypes.c_uint64)])
+
+
+class VerifyArgs(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("nseq", "max_draft", "vocab")]
+                + [(n, ctypes.c_int64) for n in ("ld_target", "ld_draft")]
+                + [(n, ctypes.c_void_p) for n in ("target_dev", "draft_dev", "draft_ids_dev", "n_draft_dev",
+                                                  "accept_u_dev", "sample_u_dev", "out_ids_dev", "out_n_dev")])
 
 
 class LaicError(RuntimeError):
@@ -107,7 +139,16 @@ def lib() -> ctypes.CDLL:
                                       ctypes.POINTER(I32)]
     L.laic_selftest_peer_timeout.argtypes = [I32, ctypes.c_int64, ctypes.POINTER(I32)]
     L.laic_blocks_convert.argtypes = [I32, P, U64, ctypes.c_uint32, ctypes.POINTER(I32), P, U64, ctypes.POINTER(U64)]
-    for name in ("laic_dev_create", "laic_dev_upload", "laic_dev_prefill", "laic_dev_step", "laic_dev_reset_slot",
+    KP = ctypes.POINTER(KvPagesDesc)
+    I64 = ctypes.c_int64
+    L.laic_kv_append.argtypes = [KP, ctypes.POINTER(KvAppendArgs), P]
+    L.laic_kv_attention.argtypes = [KP, ctypes.POINTER(KvAttentionArgs), P]
+    L.laic_kv_attention_workspace.argtypes = [KP, ctypes.POINTER(KvAttentionArgs), ctypes.POINTER(U64)]
+    L.laic_kv_check.argtypes = [KP, P]
+    L.laic_logits_probs.argtypes = [I32, I32, I32, P, I64, P, P, I64, P]
+    L.laic_verify_drafts.argtypes = [I32, ctypes.POINTER(VerifyArgs), P]
+    for name in ("laic_kv_append", "laic_kv_attention", "laic_kv_attention_workspace", "laic_kv_check",
+                 "laic_logits_probs", "laic_verify_drafts", "laic_dev_create", "laic_dev_upload", "laic_dev_prefill", "laic_dev_step", "laic_dev_reset_slot",
                  "laic_dev_slot_pos", "laic_dev_fill_kv", "laic_dev_sync", "laic_dev_stats_get",
                  "laic_dev_decode", "laic_dev_profile", "laic_nccl_unique_id", "laic_tensor_create", "laic_tensor_matvec",
                  "laic_tensor_dequant", "laic_tensor_matvec_noalloc", "laic_dev_prefill_batch", "laic_tensor_check",

@@ -47,6 +47,7 @@
 #include "nccl_dl.h"
 #include "prefill.cuh"
 #include "sampler.cuh"
+#include "serving.cuh"
 #include "stream_step.cuh"
 
 namespace {
@@ -63,6 +64,12 @@ int fail(int code, const std::string& msg) {
         cudaError_t e_ = (x);                                                                      \
         if (e_ != cudaSuccess) return fail(LAIC_E_CUDA, std::string(#x) + ": " + cudaGetErrorString(e_)); \
     } while (0)
+
+}  // namespace
+
+int laic::api_fail(int code, const std::string& msg) { return fail(code, msg); }
+
+namespace {
 
 using laic::T_F16;
 using laic::T_F32;

@@ -1,0 +1,543 @@
+// Attention over a KV cache in pages, with shared prefixes read once.
+//
+// out[r] = sum_t p_t v_t, p = softmax_t(scale q[r] . k_t) over the positions t < n_r of row r's
+// sequence. The work is cut into items, each a set of score columns (query row, query head of one
+// KV head) over a range of positions:
+//   private item: one row's G = heads / kv_heads columns over a split of [shared, n_r);
+//   shared item: up to 8 NT columns of a group's rows over a split of [0, shared), so the keys and
+//   values of a shared position are read once for all of them.
+// An item keeps, per column, the running maximum m of the scores (log2 domain), l = sum 2^(s - m)
+// and the unnormalised output; where a row has several items the merge kernel joins them by
+// out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
+//
+// Products run transposed on mma.m16n8k16: S^T = K Q^T (16 positions x 8 columns) and
+// O^T = V^T P^T, so the few columns of a decode step fill the narrow side of the tile; P^T goes
+// from accumulators to B fragments by movmatrix. FP32 queries and weights are split into binary16
+// hi + lo (two products, 22 bits); a query row is first scaled by a power of two to [1, 2), so no
+// magnitude leaves binary16's range, and the weights carry a factor 2^10 that keeps small ones
+// out of its subnormals (both sides of the final division have it).
+#pragma once
+#include "common.cuh"
+#include "mma_matvec.cuh"  // smem_u32, mma16816, cp.async
+#include "attention.cuh"   // attn_swz, ldsm_x4
+#include "paged.cuh"
+
+namespace laic {
+
+struct KvAttnParams {
+    const void* q;
+    void* out;
+    long long ldq, ldo;
+    const __half *kp, *vp;
+    int num_pages, page_shift, kv_heads, heads, G;
+    const int *len, *seq, *table;
+    int nseq, pages_per_seq, rows, max_len;
+    int groups, max_group_rows, max_shared, max_private;
+    const int *group_rows, *group_len;
+    float scale_log2;             // scale * log2(e)
+    int lp, nsp;                  // private splits: positions each, count
+    int ls, nss, ctiles;          // shared splits, column tiles per group
+    int shared_items;
+    float* part_o;                // [rows][heads][nss + nsp][head_dim]
+    float2* part_ml;              // [rows][heads][nss + nsp] (m, l)
+    int direct;                   // one item per row: it writes the output
+    int* err;
+};
+
+constexpr int kPaWarps = 4;
+constexpr int kPaChunk = 64;      // positions per ring stage: 16 per warp
+constexpr int kPaMaxSplit = 2048; // positions per item at most (its page ids are held in shared memory)
+constexpr float kPaBias = 10.f;   // log2 of the factor the weights carry
+
+__host__ __device__ constexpr int pa_stages(int D) { return D == 128 ? 3 : 4; }
+__host__ __device__ constexpr size_t pa_ring_bytes(int D) { return (size_t)pa_stages(D) * 2 * kPaChunk * D * 2; }
+__host__ __device__ constexpr size_t pa_smem(int D, int NT, bool hl) {
+    const size_t ring = pa_ring_bytes(D), red = (size_t)kPaWarps * NT * 8 * (D + 4) * 4;
+    return (ring > red ? ring : red) + (size_t)(D / 16) * NT * (hl ? 2 : 1) * 32 * 8;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+// 16 bytes, or 16 zeros where !live (the source is not read then).
+__device__ __forceinline__ void cp_async16_z(uint32_t dst, const void* src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// What the index arrays say about one row.
+struct RowView {
+    int n;       // positions seen (0: none); -1: padding
+    int shared;  // of those, the group's
+    int seq;
+};
+__host__ __device__ inline int kv_clamp_len(const KvAttnParams& p, int n, int bound) {
+    const int most = p.pages_per_seq << p.page_shift, cap = bound < most ? bound : most;
+    if (n > cap) {
+        kv_flag(p.err, kKvBadPos);
+        n = cap;
+    }
+    return n;
+}
+__host__ __device__ inline int row_seq(const KvAttnParams& p, int r) {
+    const int s = p.seq ? p.seq[r] : r;
+    if (s >= 0 && s < p.nseq) return s;
+    kv_flag(p.err, kKvBadSeq);
+    return -1;
+}
+// Rows [r0, r1) of group g, false (and recorded) where they are not within the call's rows and bounds.
+__host__ __device__ inline bool group_rows(const KvAttnParams& p, int g, int& r0, int& r1) {
+    r0 = p.group_rows[g];
+    r1 = p.group_rows[g + 1];
+    if (r0 < 0 || r1 < r0 || r1 > p.rows || r1 - r0 > p.max_group_rows) {
+        kv_flag(p.err, kKvBadGroup);
+        return false;
+    }
+    return true;
+}
+// Shared positions of group g: none where its rows are refused or its first row names no sequence.
+__host__ __device__ inline int group_shared(const KvAttnParams& p, int g, int r0) {
+    if (row_seq(p, r0) < 0) return 0;
+    const int n = kv_clamp_len(p, p.group_len[g], p.max_shared);
+    return n > 0 ? n : 0;
+}
+// The view of row r; the `n` threads tid of one sync domain search the groups together and leave
+// the row's shared length in *found (reset to 0 before, synchronised after, by the caller).
+__device__ __forceinline__ void find_group(const KvAttnParams& p, int r, int tid, int n, int* found) {
+    for (int g = tid; g < p.groups; g += n) {
+        int r0, r1;
+        if (group_rows(p, g, r0, r1) && r >= r0 && r < r1) *found = group_shared(p, g, r0);
+    }
+}
+__host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int shared) {
+    RowView v;
+    v.n = p.len[r];
+    v.seq = -1;
+    v.shared = 0;
+    if (v.n < 0) {
+        v.n = -1;
+        return v;
+    }
+    v.n = kv_clamp_len(p, v.n, p.max_len);
+    v.seq = row_seq(p, r);
+    if (v.seq < 0) v.n = 0;
+    v.shared = v.n < shared ? v.n : shared;
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float q_at(const KvAttnParams& p, int r, int h, int d) {
+    return kv_in<T>(static_cast<const T*>(p.q)[(size_t)r * p.ldq + d + (size_t)h]);
+}
+
+// One item: columns [col0, col0 + 8 NT) of rows r0.. (column = row offset * G + head), positions
+// [t0, t1) of sequence `seq`. Column c sees positions below lim[c] (shared memory; 0: no column).
+// slot: the partial's index among its row's; minlim: the smallest lim of a live column.
+template <int D, int NT, typename T>
+__device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0, int ncol, int kvh, int seq, int t0,
+                                        int t1, int slot, const int* lim, int minlim, int* page_ids, float* cmul,
+                                        uint8_t* smem) {
+    constexpr bool HL = sizeof(T) == 4;
+    constexpr int HN = HL ? 2 : 1;
+    constexpr int KS = D / 16, CPR = D / 8, NC = NT * 8, NW = kPaWarps, NTH = kPaWarps * 32;
+    constexpr int NST = pa_stages(D);
+    constexpr size_t kRed = (size_t)NW * NC * (D + 4) * 4;
+    constexpr size_t kQoff = pa_ring_bytes(D) > kRed ? pa_ring_bytes(D) : kRed;
+    uint32_t* qf = reinterpret_cast<uint32_t*>(smem + kQoff);  // [KS][NT][HN][32 lanes][2]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int gq = lane >> 2, c = lane & 3;
+
+    // ---- the range's page ids, each checked once
+    const int first_page = t0 >> p.page_shift;
+    const int npages = t1 > t0 ? ((t1 - 1) >> p.page_shift) - first_page + 1 : 0;
+    for (int i = tid; i < npages; i += NTH) {
+        int id = p.table[(size_t)seq * p.pages_per_seq + first_page + i];
+        if (id < 0 || id >= p.num_pages) {
+            kv_flag(p.err, kKvBadPage);
+            id = 0;
+        }
+        page_ids[i] = id;
+    }
+    __syncthreads();
+
+    const int nch = (t1 - t0 + kPaChunk - 1) / kPaChunk;
+    const uint32_t ring = smem_u32(smem);
+    const size_t head_run = (size_t)D << p.page_shift;  // elements of a (page, head) pair
+    auto load = [&](int ch) {
+        if (ch < nch) {
+            const uint32_t ks = ring + (uint32_t)(ch % NST) * (2 * kPaChunk * D * 2);
+            const uint32_t vs = ks + kPaChunk * D * 2;
+#pragma unroll
+            for (int i = tid; i < kPaChunk * CPR; i += NTH) {
+                const int r = i / CPR, cc = i % CPR, t = t0 + ch * kPaChunk + r;
+                const bool live = t < t1;
+                const int tt = live ? t : t0;
+                const size_t off = ((size_t)page_ids[(tt >> p.page_shift) - first_page] * p.kv_heads + kvh) * head_run +
+                                   (size_t)(tt & ((1 << p.page_shift) - 1)) * D + cc * 8;
+                cp_async16_z(ks + 2 * attn_swz<D>(r, cc), p.kp + off, live);
+                cp_async16_z(vs + 2 * attn_swz<D>(r, cc), p.vp + off, live);  // rows past the end: zeros
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < NST - 1; ++s) load(s);
+
+    // ---- query fragments: a warp per column
+    for (int col = warp; col < NC; col += NW) {
+        const int cc = col0 + col;
+        const bool live = cc < ncol;
+        const int rr = r0 + (live ? cc / p.G : 0), hh = (kvh * p.G + (live ? cc % p.G : 0)) * D;
+        constexpr int PL = (D / 2 + 31) / 32;  // pairs per lane
+        float a[PL], b[PL], mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < PL; ++i) {
+            const int pi = lane + 32 * i;
+            const bool in = live && pi < D / 2;
+            a[i] = in ? q_at<T>(p, rr, hh, 2 * pi) : 0.f;
+            b[i] = in ? q_at<T>(p, rr, hh, 2 * pi + 1) : 0.f;
+            mx = fmaxf(mx, fmaxf(fabsf(a[i]), fabsf(b[i])));
+        }
+        float fac = 1.f, inv = 1.f;
+        if (HL) {
+            mx = warp_max(mx);
+            const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
+            fac = __uint_as_float((uint32_t)(127 - e) << 23);
+            inv = __uint_as_float((uint32_t)(127 + e) << 23);
+        }
+        if (lane == 0) cmul[col] = p.scale_log2 * inv;
+#pragma unroll
+        for (int i = 0; i < PL; ++i) {
+            const int pi = lane + 32 * i;
+            if (pi < D / 2) {
+                const int ks = pi >> 3, j = (pi >> 2) & 1, cl = pi & 3;
+                uint32_t* dst = qf + (((size_t)(ks * NT + (col >> 3)) * HN) * 32 + (col & 7) * 4 + cl) * 2 + j;
+                const float va = a[i] * fac, vb = b[i] * fac;
+                const __half ha = __float2half_rn(va), hb = __float2half_rn(vb);
+                dst[0] = pack_h2(ha, hb);
+                if (HL) dst[64] = pack_h2(__float2half_rn(va - __half2float(ha)), __float2half_rn(vb - __half2float(hb)));
+            }
+        }
+    }
+
+    float m_[NT][2], l_[NT][2], o[KS][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        m_[nt][0] = m_[nt][1] = -INFINITY;
+        l_[nt][0] = l_[nt][1] = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+    }
+    const int li = lane >> 3, lr = lane & 7;  // ldmatrix: this lane addresses row lr of matrix li
+    const int wp = warp * 16;                 // this warp's first position of a chunk
+
+    for (int ch = 0; ch < nch; ++ch) {
+        cp_async_wait<NST - 2>();
+        __syncthreads();  // chunk ch is in shared memory, and chunk ch - 1 consumed
+        load(ch + NST - 1);
+        const int c0 = t0 + ch * kPaChunk;
+        if (c0 + wp < t1) {
+            const uint32_t ks_a = ring + (uint32_t)(ch % NST) * (2 * kPaChunk * D * 2), vs_a = ks_a + kPaChunk * D * 2;
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                uint32_t a[4];
+                ldsm_x4(ks_a + 2 * attn_swz<D>(wp + (li & 1) * 8 + lr, ks * 2 + (li >> 1)), a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int hl = 0; hl < HN; ++hl) {
+                        const uint2 b = *reinterpret_cast<const uint2*>(qf + (((ks * NT + nt) * HN + hl) * 32 + lane) * 2);
+                        mma16816_acc(s[nt], a[0], a[1], a[2], a[3], b.x, b.y);
+                    }
+            }
+            const int pos = c0 + wp + gq;
+            uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float mx[2] = {-INFINITY, -INFINITY}, corr[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int col = nt * 8 + 2 * c + (e & 1);
+                    s[nt][e] *= cmul[col];
+                    if (pos + (e >> 1) * 8 >= min(t1, lim[col])) s[nt][e] = -INFINITY;
+                    mx[e & 1] = fmaxf(mx[e & 1], s[nt][e]);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16));
+                    const float mnew = fmaxf(m_[nt][h], mx[h]);
+                    const float mu = mnew == -INFINITY ? 0.f : mnew;  // nothing seen yet: every weight is 2^-inf
+                    corr[h] = ex2(m_[nt][h] - mu);
+                    m_[nt][h] = mnew;
+                    mx[h] = mu - kPaBias;
+                }
+                float pv[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    pv[e] = ex2(s[nt][e] - mx[e & 1]);
+                    sum[e & 1] += pv[e];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) l_[nt][h] = fmaf(l_[nt][h], corr[h], sum[h]);  // this lane's positions
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const __half h0 = __float2half_rn(pv[2 * j]), h1 = __float2half_rn(pv[2 * j + 1]);
+                    ph[nt][j] = movm_t(pack_h2(h0, h1));
+                    if (HL)
+                        pl[nt][j] = movm_t(pack_h2(__float2half_rn(pv[2 * j] - __half2float(h0)),
+                                                   __float2half_rn(pv[2 * j + 1] - __half2float(h1))));
+                }
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt) {
+                    o[mt][nt][0] *= corr[0]; o[mt][nt][1] *= corr[1];
+                    o[mt][nt][2] *= corr[0]; o[mt][nt][3] *= corr[1];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] = pv[e];
+            }
+            // a position that some columns see and others do not: where its value is not finite,
+            // 0 * inf would reach the others, so those products are summed one by one
+            bool odd = false;
+            if (min(c0 + wp + 16, t1) > minlim) {
+#pragma unroll
+                for (int i = lane; i < 16 * CPR; i += 32) {
+                    const uint4 w = lds128(vs_a + 2 * attn_swz<D>(wp + i / CPR, i % CPR));
+                    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        odd |= (x[k] & 0x7c00u) == 0x7c00u || (x[k] & 0x7c000000u) == 0x7c000000u;
+                }
+                odd = __any_sync(0xffffffffu, odd);
+            }
+            if (!odd) {
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt) {
+                    uint32_t a[4];
+                    ldsm_x4_t(vs_a + 2 * attn_swz<D>(wp + (li >> 1) * 8 + lr, mt * 2 + (li & 1)), a);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816_acc(o[mt][nt], a[0], a[1], a[2], a[3], ph[nt][0], ph[nt][1]);
+                        if (HL) mma16816_acc(o[mt][nt], a[0], a[1], a[2], a[3], pl[nt][0], pl[nt][1]);
+                    }
+                }
+            } else {
+                const __half* V = reinterpret_cast<const __half*>(smem + (size_t)(ch % NST) * (2 * kPaChunk * D * 2) +
+                                                                  kPaChunk * D * 2);
+#pragma unroll 1
+                for (int i = 0; i < 16; ++i) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {  // the weight of (position i, column 2c + h): lane (i % 8, c)
+                            const float w0 = __shfl_sync(0xffffffffu, s[nt][h], (i & 7) * 4 + c);
+                            const float w1 = __shfl_sync(0xffffffffu, s[nt][2 + h], (i & 7) * 4 + c);
+                            const float w = i < 8 ? w0 : w1;
+                            if (w != 0.f) {
+#pragma unroll
+                                for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+                                    for (int k = 0; k < 2; ++k) {
+                                        const int d = mt * 16 + gq + 8 * k;
+                                        const float x = __half2float(V[attn_swz<D>(wp + i, d >> 3) + (d & 7)]);
+                                        o[mt][nt][2 * k + h] = fmaf(w, x, o[mt][nt][2 * k + h]);
+                                    }
+                            }
+                        }
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v = l_[nt][h];
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 16);
+            l_[nt][h] = v;
+        }
+
+    // ---- join the warps (the ring holds their outputs now)
+    __shared__ float cm[kPaWarps][NC], cl[kPaWarps][NC];
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(smem);  // [warp][column][D + 4]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        if (gq == 0) {
+            cm[warp][nt * 8 + 2 * c] = m_[nt][0]; cm[warp][nt * 8 + 2 * c + 1] = m_[nt][1];
+            cl[warp][nt * 8 + 2 * c] = l_[nt][0]; cl[warp][nt * 8 + 2 * c + 1] = l_[nt][1];
+        }
+#pragma unroll
+        for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                red[((size_t)warp * NC + nt * 8 + 2 * c + (e & 1)) * (D + 4) + mt * 16 + gq + (e >> 1) * 8] = o[mt][nt][e];
+    }
+    __syncthreads();
+    const int ns = p.nss + p.nsp;
+    for (int i = tid; i < NC * (D / 4); i += NTH) {
+        const int col = i / (D / 4), d = (i % (D / 4)) * 4, cc = col0 + col;
+        if (cc >= ncol) continue;
+        float M = -INFINITY, L = 0.f, w[NW];
+#pragma unroll
+        for (int k = 0; k < NW; ++k) M = fmaxf(M, cm[k][col]);
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+            w[k] = cm[k][col] == -INFINITY ? 0.f : ex2(cm[k][col] - M);
+            L = fmaf(cl[k][col], w[k], L);
+            if (w[k] != 0.f) {
+                const float4 v = *reinterpret_cast<const float4*>(red + ((size_t)k * NC + col) * (D + 4) + d);
+                A.x = fmaf(v.x, w[k], A.x); A.y = fmaf(v.y, w[k], A.y);
+                A.z = fmaf(v.z, w[k], A.z); A.w = fmaf(v.w, w[k], A.w);
+            }
+        }
+        const int r = r0 + cc / p.G, h = kvh * p.G + cc % p.G;
+        if (p.direct) {
+            const float iv = M == -INFINITY ? 0.f : 1.f / L;
+            T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)h * D + d;
+            dst[0] = kv_out<T>(A.x * iv); dst[1] = kv_out<T>(A.y * iv);
+            dst[2] = kv_out<T>(A.z * iv); dst[3] = kv_out<T>(A.w * iv);
+        } else {
+            const size_t at = ((size_t)r * p.heads + h) * ns + slot;
+            *reinterpret_cast<float4*>(p.part_o + at * D + d) = A;
+            if (d == 0) p.part_ml[at] = make_float2(M, L);
+        }
+    }
+}
+
+// Grid: the shared items ([group][column tile][kv head][split]), then the private ones ([row][kv head][split]).
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const KvAttnParams p) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int lim[NT * 8], page_ids[kPaMaxSplit / 16 + 2];
+    __shared__ float cmul[NT * 8];
+    __shared__ int found;
+    const int tid = threadIdx.x;
+    int i = blockIdx.x;
+    if (i < p.shared_items) {
+        const int split = i % p.nss;
+        i /= p.nss;
+        const int kvh = i % p.kv_heads;
+        i /= p.kv_heads;
+        const int ct = i % p.ctiles, g = i / p.ctiles;
+        int r0, r1;
+        if (!group_rows(p, g, r0, r1)) return;
+        const int col0 = ct * NT * 8, ncol = (r1 - r0) * p.G;
+        if (col0 >= ncol) return;
+        const int shared = group_shared(p, g, r0);
+        const int t0 = split * p.ls;
+        if (t0 >= shared) return;
+        int mx = 0, mn = 0x7fffffff;  // every thread: the tile's few rows
+        for (int col = col0; col < min(ncol, col0 + NT * 8); ++col) {
+            if (col != col0 && col % p.G) continue;
+            const int n = max(0, row_view(p, r0 + col / p.G, shared).shared);
+            mx = max(mx, n);
+            mn = min(mn, n);
+        }
+        if (tid < NT * 8) {
+            const int col = col0 + tid;
+            lim[tid] = col < ncol ? max(0, row_view(p, r0 + col / p.G, shared).shared) : 0;
+        }
+        const int t1 = min(mx, t0 + p.ls);
+        if (t0 >= t1) return;  // no row of the tile sees this far
+        pa_item<D, NT, T>(p, r0, col0, ncol, kvh, row_seq(p, r0), t0, t1, split, lim, mn, page_ids, cmul, smem);
+    } else {
+        i -= p.shared_items;
+        const int split = i % p.nsp;
+        i /= p.nsp;
+        const int kvh = i % p.kv_heads, r = i / p.kv_heads;
+        if (tid == 0) found = 0;
+        __syncthreads();
+        find_group(p, r, tid, kPaWarps * 32, &found);
+        __syncthreads();
+        const RowView v = row_view(p, r, found);
+        if (v.n < 0) return;
+        if (v.n - v.shared > p.max_private && tid == 0) kv_flag(p.err, kKvBadPos);
+        const int t0 = v.shared + split * p.lp, t1 = min(min(v.n, v.shared + p.max_private), t0 + p.lp);
+        if (t0 >= t1) {
+            if (p.direct) {  // a row that sees nothing
+                T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)kvh * p.G * D;
+                for (int e = tid; e < p.G * D; e += kPaWarps * 32) dst[e] = kv_out<T>(0.f);
+            }
+            return;
+        }
+        if (tid < 8) lim[tid] = tid < p.G ? t1 : 0;
+        pa_item<D, 1, T>(p, r, 0, p.G, kvh, v.seq, t0, t1, p.nss + split, lim, t1, page_ids, cmul, smem);
+    }
+    pdl_launch_dependents();
+}
+
+constexpr int kPmWarps = 4;
+// Join the items of each (row, head): one warp per pair, grid ceil(rows * heads / kPmWarps).
+template <int D, typename T>
+__global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttnParams p) {
+    constexpr int E = D / 32;
+    __shared__ int found[kPmWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int pair = blockIdx.x * kPmWarps + warp;
+    const bool in = pair < p.rows * p.heads;
+    const int r = in ? pair / p.heads : 0, h = in ? pair % p.heads : 0;
+    if (lane == 0) found[warp] = 0;
+    __syncwarp();
+    find_group(p, r, lane, 32, &found[warp]);
+    __syncwarp();
+    const RowView v = row_view(p, r, found[warp]);
+    pdl_wait();
+    if (!in || v.n < 0) return;
+    const int ns = p.nss + p.nsp;
+    const int priv = min(v.n - v.shared, p.max_private);
+    const int live_s = v.shared > 0 ? (v.shared + p.ls - 1) / p.ls : 0;
+    const int live = live_s + (priv > 0 ? (priv + p.lp - 1) / p.lp : 0);
+    const size_t base = (size_t)pair * ns;
+    auto slot = [&](int i) { return i < live_s ? i : p.nss + (i - live_s); };
+    float M = -INFINITY;
+    for (int i = lane; i < live; i += 32) M = fmaxf(M, p.part_ml[base + slot(i)].x);
+    M = warp_max(M);
+    float L = 0.f, acc[E] = {};
+    for (int i0 = 0; i0 < live; i0 += 32) {
+        float w = 0.f;
+        if (i0 + lane < live) {
+            const float2 ml = p.part_ml[base + slot(i0 + lane)];
+            w = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+            L = fmaf(ml.y, w, L);
+        }
+        const int n = min(32, live - i0);
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            const float* src = p.part_o + (base + slot(i0 + i)) * D + lane * E;
+            float x[E];
+            if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
+            else if constexpr (E == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
+            else x[0] = *src;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (wi != 0.f) acc[e] = fmaf(x[e], wi, acc[e]);
+        }
+    }
+    L = warp_sum(L);
+    const float iv = M == -INFINITY ? 0.f : 1.f / L;
+    T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)h * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[e] = kv_out<T>(acc[e] * iv);
+}
+
+}  // namespace laic

@@ -1,0 +1,408 @@
+// The serving operators' entry points: a KV cache in pages (append, attention),
+// probabilities of logits rows and the verification of drafted tokens.
+#include "serving.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <new>
+
+#include "launch.cuh"
+#include "paged.cuh"
+#include "paged_attn.cuh"
+#include "verify.cuh"
+
+namespace laic {
+namespace {
+
+// The pages' device for the call; the thread's current one afterwards.
+struct DeviceGuard {
+    int prev = -1;
+    cudaError_t err = cudaSuccess;
+    explicit DeviceGuard(int device) {
+        int cur = -1;
+        err = cudaGetDevice(&cur);
+        if (err == cudaSuccess && cur != device) {
+            err = cudaSetDevice(device);
+            if (err == cudaSuccess) prev = cur;
+        }
+    }
+    ~DeviceGuard() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+};
+
+int cuda_fail(cudaError_t e, const char* what) {
+    return api_fail(LAIC_E_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool type_ok(int t) { return t == LAIC_GGML_F32 || t == LAIC_GGML_F16; }
+int type_size(int t) { return t == LAIC_GGML_F32 ? 4 : 2; }
+int log2i(int v) {
+    int s = 0;
+    while ((1 << s) < v) ++s;
+    return s;
+}
+
+int check_pages(const laic_kv_pages& g) {
+    if (g.head_dim != 32 && g.head_dim != 64 && g.head_dim != 128)
+        return api_fail(LAIC_E_UNSUPPORTED, "head_dim must be 32, 64 or 128");
+    if (g.kv_heads < 1 || g.num_pages < 1) return api_fail(LAIC_E_INVALID, "kv_heads and num_pages must be >= 1");
+    if (g.page_size < 16 || g.page_size > 256 || (g.page_size & (g.page_size - 1)))
+        return api_fail(LAIC_E_UNSUPPORTED, "page_size must be 16, 32, 64, 128 or 256");
+    return LAIC_OK;
+}
+int check_page_ptrs(const laic_kv_pages& g) {
+    if (!g.k_dev || !g.v_dev || !g.err_dev) return api_fail(LAIC_E_INVALID, "null page or error pointer");
+    if (!aligned16(g.k_dev) || !aligned16(g.v_dev)) return api_fail(LAIC_E_INVALID, "pages must be 16-byte aligned");
+    return LAIC_OK;
+}
+int check_table(int rows, int nseq, int pages_per_seq, int page_size, const int32_t* seq) {
+    if (nseq < 1 || pages_per_seq < 1) return api_fail(LAIC_E_INVALID, "nseq and pages_per_seq must be >= 1");
+    if ((long long)pages_per_seq * page_size > INT_MAX) return api_fail(LAIC_E_INVALID, "page table row too long");
+    if (!seq && nseq < rows) return api_fail(LAIC_E_INVALID, "without seq_dev every row needs its page table row");
+    return LAIC_OK;
+}
+
+// Runs `f` (the launches of a checked call) on `device`.
+template <typename F>
+int on_device(int device, F&& f) {
+    DeviceGuard dg(device);
+    if (dg.err != cudaSuccess) return cuda_fail(dg.err, "device");
+    return f();
+}
+
+template <typename TI, typename TQ>
+void append_launch(bool vec, dim3 grid, int block, cudaStream_t st, const KvAppendParams& p) {
+    if (vec) kv_append_kernel<TI, TQ, true><<<grid, block, 0, st>>>(p);
+    else kv_append_kernel<TI, TQ, false><<<grid, block, 0, st>>>(p);
+}
+
+int device_sms(int dev) {
+    static std::atomic<int> sms[64];
+    if (dev < 0 || dev >= 64) return 148;
+    int n = sms[dev].load();
+    if (!n) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            return 148;
+        }
+        sms[dev].store(n);
+    }
+    return n;
+}
+
+// ---- attention: how a call is cut into items
+struct AttnPlan {
+    int nt = 1;            // column tiles of 8 of a shared item
+    int lp = 64, nsp = 1;  // private splits
+    int ls = 64, nss = 0, ctiles = 0;
+    int shared_items = 0, private_items = 0;
+    bool direct = false;
+    size_t ml_off = 0, bytes = 0;
+};
+
+int round_up(long long v, int m) { return (int)((v + m - 1) / m * m); }
+
+int check_attention(const laic_kv_pages& g, const laic_kv_attention_args& a) {
+    if (int rc = check_pages(g)) return rc;
+    if (a.rows < 0) return api_fail(LAIC_E_INVALID, "rows must be >= 0");
+    if (a.heads < 1 || a.heads % g.kv_heads) return api_fail(LAIC_E_INVALID, "heads must be a multiple of kv_heads");
+    if (a.heads / g.kv_heads > 8) return api_fail(LAIC_E_UNSUPPORTED, "at most 8 query heads per kv head");
+    if (!type_ok(a.type)) return api_fail(LAIC_E_UNSUPPORTED, "query and output type must be F32 or F16");
+    if (a.max_len < 0 || a.groups < 0 || a.max_private < -1) return api_fail(LAIC_E_INVALID, "negative bound");
+    if (a.groups && (a.max_group_rows < 1 || a.max_shared < 0 || a.max_group_rows > a.rows))
+        return api_fail(LAIC_E_INVALID, "groups need max_group_rows in [1, rows] and max_shared >= 0");
+    const long long cap = (long long)a.pages_per_seq * g.page_size;
+    if (a.max_len > cap || (a.groups && a.max_shared > cap))
+        return api_fail(LAIC_E_INVALID, "max_len and max_shared must not exceed pages_per_seq * page_size");
+    return LAIC_OK;
+}
+
+int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, AttnPlan& pl) {
+    const int G = a.heads / g.kv_heads;
+    const int max_private = a.max_private < 0 ? a.max_len : std::min(a.max_private, a.max_len);
+    // splits: about `want` items, each a whole number of chunks, at most kPaMaxSplit positions (its page
+    // ids) and, where there is work enough, 512 (a partial costs 2 % of such an item's bytes)
+    const long long want = 4LL * device_sms(g.device);
+    auto split = [&](long long pairs, int len) {
+        const long long l = ((long long)len * pairs + want - 1) / want;
+        return std::max(kPaChunk, std::min(round_up(l, kPaChunk), 512));
+    };
+    pl.lp = split((long long)a.rows * g.kv_heads, max_private);
+    pl.nsp = std::max(1, (max_private + pl.lp - 1) / pl.lp);
+    if (a.groups) {
+        const int cols = a.max_group_rows * G;
+        pl.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+        pl.ctiles = (cols + 8 * pl.nt - 1) / (8 * pl.nt);
+        pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared);
+        pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
+        if (!max_private) pl.nsp = 1;
+    }
+    const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss;
+    const long long pi = (long long)a.rows * g.kv_heads * pl.nsp;
+    if (si + pi > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
+    pl.shared_items = (int)si;
+    pl.private_items = (int)pi;
+    pl.direct = pl.nss == 0 && pl.nsp == 1;
+    if (!pl.direct) {
+        const size_t parts = (size_t)a.rows * a.heads * (pl.nss + pl.nsp);
+        pl.ml_off = parts * g.head_dim * 4;
+        pl.bytes = pl.ml_off + parts * 8;
+    }
+    return LAIC_OK;
+}
+
+using PaFn = void (*)(KvAttnParams);
+template <int D, typename T>
+PaFn pa_fn_nt(int nt) {
+    return nt == 1 ? paged_attn_kernel<D, 1, T> : nt == 2 ? paged_attn_kernel<D, 2, T> : paged_attn_kernel<D, 4, T>;
+}
+template <typename T>
+PaFn pa_fn(int D, int nt) {
+    return D == 32 ? pa_fn_nt<32, T>(nt) : D == 64 ? pa_fn_nt<64, T>(nt) : pa_fn_nt<128, T>(nt);
+}
+PaFn pa_pick(int D, int nt, int type) { return type == LAIC_GGML_F32 ? pa_fn<float>(D, nt) : pa_fn<__half>(D, nt); }
+template <typename T>
+PaFn pm_fn(int D) {
+    return D == 32 ? paged_merge_kernel<32, T> : D == 64 ? paged_merge_kernel<64, T> : paged_merge_kernel<128, T>;
+}
+
+}  // namespace
+
+cudaError_t serving_set_attributes() {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64 && done[dev].load()) return cudaSuccess;
+    for (int D : {32, 64, 128})
+        for (int nt : {1, 2, 4})
+            for (int type : {LAIC_GGML_F32, LAIC_GGML_F16}) {
+                e = cudaFuncSetAttribute(pa_pick(D, nt, type), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)pa_smem(D, nt, type == LAIC_GGML_F32));
+                if (e != cudaSuccess) return e;
+            }
+    if (dev >= 0 && dev < 64) done[dev].store(true);
+    return cudaSuccess;
+}
+
+std::string kv_error_text(int bits) {
+    std::string s = "paged KV cache:";
+    if (bits & LAIC_KV_BAD_SEQ) s += " sequence index outside the page table;";
+    if (bits & LAIC_KV_BAD_POS) s += " position or length beyond its bound;";
+    if (bits & LAIC_KV_BAD_PAGE) s += " page id out of range;";
+    if (bits & LAIC_KV_BAD_GROUP) s += " group rows out of order or above their bound;";
+    s.pop_back();
+    return s;
+}
+
+int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t st) {
+    if (int rc = check_pages(g)) return rc;
+    if (a.rows < 0 || a.heads < 0) return api_fail(LAIC_E_INVALID, "rows and heads must be >= 0");
+    if (!type_ok(a.in_type) || !type_ok(a.q_type)) return api_fail(LAIC_E_UNSUPPORTED, "q, k and v must be F32 or F16");
+    if (a.rope_dim < 0 || a.rope_dim > g.head_dim || (a.rope_dim & 1)) return api_fail(LAIC_E_INVALID, "invalid RoPE dimension");
+    if (int rc = check_table(a.rows, a.nseq, a.pages_per_seq, g.page_size, a.seq_dev)) return rc;
+    if (a.rows == 0) return LAIC_OK;
+    if (int rc = check_page_ptrs(g)) return rc;
+    if (!a.k_dev || !a.v_dev || !a.pos_dev || !a.page_table_dev || (a.heads && (!a.q_dev || !a.q_out_dev)))
+        return api_fail(LAIC_E_INVALID, "null pointer");
+    if (a.rope_dim && (!a.rope_dev || a.rope_positions < 1)) return api_fail(LAIC_E_INVALID, "rotation without a table");
+    if ((reinterpret_cast<uintptr_t>(a.rope_dev) & 7) && a.rope_dim) return api_fail(LAIC_E_INVALID, "rotation table must be 8-byte aligned");
+    const long long kvw = (long long)g.kv_heads * g.head_dim, qw = (long long)a.heads * g.head_dim;
+    if (a.rows > 1 && (a.ldk < kvw || a.ldv < kvw || (a.heads && (a.ldq < qw || a.ldqo < qw))))
+        return api_fail(LAIC_E_INVALID, "row strides must not be below the rows' widths");
+    if (a.q_out_dev == a.q_dev && a.heads && (a.in_type != a.q_type || (a.rows > 1 && a.ldq != a.ldqo)))
+        return api_fail(LAIC_E_INVALID, "rotation in place needs one type and stride");
+    if (qw + 2 * kvw > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "rows too wide");
+    KvAppendParams p{};
+    p.q = a.q_dev; p.k = a.k_dev; p.v = a.v_dev; p.q_out = a.q_out_dev;
+    p.ldq = a.ldq; p.ldk = a.ldk; p.ldv = a.ldv; p.ldqo = a.ldqo;
+    p.kp = static_cast<__half*>(g.k_dev); p.vp = static_cast<__half*>(g.v_dev);
+    p.heads = a.heads; p.kv_heads = g.kv_heads; p.head_dim = g.head_dim;
+    p.page_shift = log2i(g.page_size); p.num_pages = g.num_pages;
+    p.pos = a.pos_dev; p.seq = a.seq_dev; p.table = a.page_table_dev;
+    p.nseq = a.nseq; p.pages_per_seq = a.pages_per_seq;
+    p.rope = reinterpret_cast<const float2*>(a.rope_dev);
+    p.rope_pairs = a.rope_dim / 2; p.rope_positions = a.rope_dim ? a.rope_positions : INT_MAX;
+    p.err = g.err_dev;
+    const int bi = type_size(a.in_type), bq = type_size(a.q_type);
+    const bool vec = aligned16(a.k_dev) && aligned16(a.v_dev) && a.ldk * bi % 16 == 0 && a.ldv * bi % 16 == 0 &&
+                     (!a.heads || (aligned16(a.q_dev) && aligned16(a.q_out_dev) && a.ldq * bi % 16 == 0 && a.ldqo * bq % 16 == 0));
+    const int units = (a.heads + 2 * g.kv_heads) * (g.head_dim / 8);
+    const int block = std::min(256, (units + 31) / 32 * 32);
+    const dim3 grid(a.rows, std::min(65535, (units + block - 1) / block));
+    return on_device(g.device, [&]() -> int {
+        if (a.in_type == LAIC_GGML_F32) {
+            if (a.q_type == LAIC_GGML_F32) append_launch<float, float>(vec, grid, block, st, p);
+            else append_launch<float, __half>(vec, grid, block, st, p);
+        } else {
+            if (a.q_type == LAIC_GGML_F32) append_launch<__half, float>(vec, grid, block, st, p);
+            else append_launch<__half, __half>(vec, grid, block, st, p);
+        }
+        const cudaError_t e = cudaGetLastError();
+        return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "kv_append");
+    });
+}
+
+int kv_attention_bytes(const laic_kv_pages& g, const laic_kv_attention_args& a, uint64_t* bytes) {
+    AttnPlan pl;
+    if (int rc = check_attention(g, a)) return rc;
+    if (a.rows > 0)
+        if (int rc = plan_attention(g, a, pl)) return rc;
+    *bytes = pl.bytes;
+    return LAIC_OK;
+}
+
+int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaStream_t st) {
+    if (int rc = check_attention(g, a)) return rc;
+    if (int rc = check_table(a.rows, a.nseq, a.pages_per_seq, g.page_size, a.seq_dev)) return rc;
+    if (a.rows == 0) return LAIC_OK;
+    if (int rc = check_page_ptrs(g)) return rc;
+    if (!a.q_dev || !a.out_dev || !a.len_dev || !a.page_table_dev || (a.groups && (!a.group_rows_dev || !a.group_len_dev)))
+        return api_fail(LAIC_E_INVALID, "null pointer");
+    const long long qw = (long long)a.heads * g.head_dim;
+    if (a.rows > 1 && (a.ldq < qw || a.ldo < qw)) return api_fail(LAIC_E_INVALID, "row strides must not be below the rows' widths");
+    AttnPlan pl;
+    if (int rc = plan_attention(g, a, pl)) return rc;
+    if (pl.bytes && (!a.workspace_dev || a.workspace_bytes < pl.bytes))
+        return api_fail(LAIC_E_INVALID, "laic_kv_attention needs " + std::to_string(pl.bytes) + " bytes of workspace");
+    if (pl.bytes && !aligned16(a.workspace_dev)) return api_fail(LAIC_E_INVALID, "the workspace must be 16-byte aligned");
+    KvAttnParams p{};
+    p.q = a.q_dev; p.out = a.out_dev; p.ldq = a.ldq; p.ldo = a.ldo;
+    p.kp = static_cast<const __half*>(g.k_dev); p.vp = static_cast<const __half*>(g.v_dev);
+    p.num_pages = g.num_pages; p.page_shift = log2i(g.page_size);
+    p.kv_heads = g.kv_heads; p.heads = a.heads; p.G = a.heads / g.kv_heads;
+    p.len = a.len_dev; p.seq = a.seq_dev; p.table = a.page_table_dev;
+    p.nseq = a.nseq; p.pages_per_seq = a.pages_per_seq; p.rows = a.rows; p.max_len = a.max_len;
+    p.groups = a.groups; p.max_group_rows = a.max_group_rows; p.max_shared = a.max_shared;
+    p.max_private = a.max_private < 0 ? a.max_len : std::min(a.max_private, a.max_len);
+    p.group_rows = a.group_rows_dev; p.group_len = a.group_len_dev;
+    const float scale = a.scale != 0.f ? a.scale : 1.f / sqrtf((float)g.head_dim);
+    p.scale_log2 = scale * 1.44269504f;
+    p.lp = pl.lp; p.nsp = pl.nsp; p.ls = pl.ls; p.nss = pl.nss; p.ctiles = pl.ctiles; p.shared_items = pl.shared_items;
+    p.direct = pl.direct;
+    if (!pl.direct) {
+        p.part_o = static_cast<float*>(a.workspace_dev);
+        p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace_dev) + pl.ml_off);
+    }
+    p.err = g.err_dev;
+    const bool f32 = a.type == LAIC_GGML_F32;
+    return on_device(g.device, [&]() -> int {
+        cudaError_t e = serving_set_attributes();
+        if (e == cudaSuccess)
+            e = launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(pl.shared_items + pl.private_items), dim3(kPaWarps * 32),
+                         pa_smem(g.head_dim, pl.nt, f32), st, false, p);
+        if (e == cudaSuccess && !pl.direct)
+            e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
+                         dim3((unsigned)(((long long)a.rows * a.heads + kPmWarps - 1) / kPmWarps)), dim3(kPmWarps * 32), 0,
+                         st, true, p);
+        return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "kv_attention");
+    });
+}
+
+int logits_probs(int device, int rows, int vocab, const float* x, long long ldx, const float* temp, float* y, long long ldy,
+                 cudaStream_t st) {
+    if (rows < 0 || vocab < 1) return api_fail(LAIC_E_INVALID, "rows must be >= 0 and vocab >= 1");
+    if (rows == 0) return LAIC_OK;
+    if (!x || !temp || !y) return api_fail(LAIC_E_INVALID, "null pointer");
+    if (rows > 1 && (ldx < vocab || ldy < vocab)) return api_fail(LAIC_E_INVALID, "row strides must not be below the vocabulary");
+    if (x == y && rows > 1 && ldx != ldy) return api_fail(LAIC_E_INVALID, "in place needs one stride");
+    ProbsParams p{x, y, temp, ldx, ldy, vocab};
+    return on_device(device, [&]() -> int {
+        probs_kernel<<<rows, kProbsThreads, 0, st>>>(p);
+        const cudaError_t e = cudaGetLastError();
+        return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "logits_probs");
+    });
+}
+
+int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st) {
+    if (a.nseq < 0 || a.vocab < 1) return api_fail(LAIC_E_INVALID, "nseq must be >= 0 and vocab >= 1");
+    if (a.max_draft < 0) return api_fail(LAIC_E_INVALID, "max_draft must be >= 0");
+    if (a.max_draft > LAIC_MAX_DRAFT) return api_fail(LAIC_E_UNSUPPORTED, "at most 64 drafted tokens per sequence");
+    if (a.nseq > INT_MAX / kVerifyCluster) return api_fail(LAIC_E_UNSUPPORTED, "too many sequences");
+    if (a.nseq == 0) return LAIC_OK;
+    if (!a.target_dev || !a.n_draft_dev || !a.sample_u_dev || !a.out_ids_dev || !a.out_n_dev ||
+        (a.max_draft && (!a.draft_ids_dev || !a.accept_u_dev)))
+        return api_fail(LAIC_E_INVALID, "null pointer");
+    if (a.ld_target < a.vocab || (a.draft_dev && a.ld_draft < a.vocab))
+        return api_fail(LAIC_E_INVALID, "row strides must not be below the vocabulary");
+    VerifyParams p{a.target_dev, a.draft_dev, a.ld_target, a.ld_draft, a.draft_ids_dev, a.n_draft_dev, a.accept_u_dev,
+                   a.sample_u_dev, a.out_ids_dev, a.out_n_dev, a.nseq, a.max_draft, a.vocab};
+    return on_device(device, [&]() -> int {
+        const cudaError_t e = launch_cluster_k(verify_kernel, dim3(a.nseq * kVerifyCluster), dim3(kVerifyThreads), 0, st, false,
+                                               kVerifyCluster, p);
+        return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "verify_drafts");
+    });
+}
+
+}  // namespace laic
+
+using laic::api_fail;
+
+// No exception crosses the C boundary (the checks' messages allocate).
+template <typename F>
+static int guarded(F&& f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc&) {
+        return LAIC_E_INVALID;
+    }
+}
+
+extern "C" {
+
+int laic_kv_append(const laic_kv_pages* pages, const laic_kv_append_args* args, void* stream) {
+    return guarded([&] {
+        if (!pages || !args) return api_fail(LAIC_E_INVALID, "null argument");
+        return laic::kv_append(*pages, *args, (cudaStream_t)stream);
+    });
+}
+
+int laic_kv_attention(const laic_kv_pages* pages, const laic_kv_attention_args* args, void* stream) {
+    return guarded([&] {
+        if (!pages || !args) return api_fail(LAIC_E_INVALID, "null argument");
+        return laic::kv_attention(*pages, *args, (cudaStream_t)stream);
+    });
+}
+
+int laic_kv_attention_workspace(const laic_kv_pages* pages, const laic_kv_attention_args* args, uint64_t* bytes) {
+    return guarded([&] {
+        if (!pages || !args || !bytes) return api_fail(LAIC_E_INVALID, "null argument");
+        return laic::kv_attention_bytes(*pages, *args, bytes);
+    });
+}
+
+int laic_kv_check(const laic_kv_pages* pages, void* stream) {
+    return guarded([&] {
+        if (!pages || !pages->err_dev) return api_fail(LAIC_E_INVALID, "null argument");
+        return laic::on_device(pages->device, [&]() -> int {
+            const cudaStream_t st = (cudaStream_t)stream;
+            int bits = 0;
+            cudaError_t e = cudaMemcpyAsync(&bits, pages->err_dev, 4, cudaMemcpyDeviceToHost, st);
+            if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+            if (e == cudaSuccess && bits) e = cudaMemsetAsync(pages->err_dev, 0, 4, st);
+            if (e == cudaSuccess && bits) e = cudaStreamSynchronize(st);
+            if (e != cudaSuccess) return laic::cuda_fail(e, "laic_kv_check");
+            return bits ? api_fail(LAIC_E_INVALID, laic::kv_error_text(bits)) : LAIC_OK;
+        });
+    });
+}
+
+int laic_logits_probs(int32_t device, int32_t rows, int32_t vocab, const float* logits_dev, int64_t ld_logits,
+                      const float* temperature_dev, float* probs_dev, int64_t ld_probs, void* stream) {
+    return guarded([&] {
+        return laic::logits_probs(device, rows, vocab, logits_dev, ld_logits, temperature_dev, probs_dev, ld_probs,
+                                  (cudaStream_t)stream);
+    });
+}
+
+int laic_verify_drafts(int32_t device, const laic_verify_args* args, void* stream) {
+    return guarded([&] {
+        if (!args) return api_fail(LAIC_E_INVALID, "null argument");
+        return laic::verify_drafts(device, *args, (cudaStream_t)stream);
+    });
+}
+
+}  // extern "C"
