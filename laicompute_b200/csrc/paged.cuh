@@ -46,6 +46,8 @@ struct KvAppendParams {
     int nseq, pages_per_seq;
     const float2* rope;
     int rope_pairs, rope_positions;
+    bool vec_rope;  // rows of the rotation table are 16-byte aligned
+    int units;      // eight-element units of a row: (heads + 2 kv_heads) * head_dim / 8
     int* err;
 };
 
@@ -56,85 +58,104 @@ template <typename T> __device__ __forceinline__ T kv_out(float x);
 template <> __device__ __forceinline__ float kv_out<float>(float x) { return x; }
 template <> __device__ __forceinline__ __half kv_out<__half>(float x) { return __float2half_rn(x); }
 
-// Eight consecutive elements; VEC: the address is 16-byte aligned.
+// Eight consecutive elements as loaded; VEC: the address is 16-byte aligned.
+template <typename T>
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ float at(int i) const { return kv_in<T>(reinterpret_cast<const T*>(w)[i]); }
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+__device__ __forceinline__ void load8(const T* p, Raw8<T>& r) {
     if constexpr (VEC) {
-        constexpr int W = 16 / sizeof(T);
 #pragma unroll
-        for (int j = 0; j < 8 / W; ++j) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p + j * W);
-            const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-            for (int i = 0; i < W; ++i) x[j * W + i] = kv_in<T>(e[i]);
-        }
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) r.w[j] = reinterpret_cast<const uint4*>(p)[j];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = kv_in<T>(p[i]);
+        for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(r.w)[i] = p[i];
     }
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(r.w)[i] = kv_out<T>(x[i]);
     if constexpr (VEC) {
-        constexpr int W = 16 / sizeof(T);
 #pragma unroll
-        for (int j = 0; j < 8 / W; ++j) {
-            uint4 w;
-            T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-            for (int i = 0; i < W; ++i) e[i] = kv_out<T>(x[j * W + i]);
-            *reinterpret_cast<uint4*>(p + j * W) = w;
-        }
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(p)[j] = r.w[j];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = kv_out<T>(x[i]);
+        for (int i = 0; i < 8; ++i) p[i] = reinterpret_cast<const T*>(r.w)[i];
     }
 }
 
-// Grid (rows, slices of the row's eight-element units). A thread owns whole
-// rotation pairs, so q_out may be q itself. The rotation is the reference's
-// unfused multiply and add (src/inference_v2.cpp:25) in FP32; k and v are
-// rounded to binary16 once, which is the cache's precision.
+constexpr int kAppendUnits = 4;  // units per thread
+
+// Grid (rows, slices of a row). A thread owns whole rotation pairs, so q_out may be q itself; it
+// loads all its units before the chain position -> sequence -> page is resolved. The rotation is
+// the reference's unfused multiply and add (src/inference_v2.cpp:25) in FP32; k and v are rounded
+// to binary16 once, which is the cache's precision.
 template <typename TI, typename TQ, bool VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p) {
     const int t = blockIdx.x;
     const int pos = p.pos[t];
-    if (pos < 0) return;
     const int seq = p.seq ? p.seq[t] : t;
+    if (pos < 0) return;
+    const int sh = __ffs(p.head_dim) - 4;  // units per head: 2^sh
+    const int u0 = blockIdx.y * blockDim.x * kAppendUnits + threadIdx.x;
+    Raw8<TI> raw[kAppendUnits];
+#pragma unroll
+    for (int j = 0; j < kAppendUnits; ++j) {
+        const int u = u0 + j * blockDim.x;
+        if (u < p.units) {
+            const int head = u >> sh, hk = head - p.heads, hv = hk - p.kv_heads;
+            const TI* src = hk < 0   ? static_cast<const TI*>(p.q) + (size_t)t * p.ldq + (size_t)u * 8
+                            : hv < 0 ? static_cast<const TI*>(p.k) + (size_t)t * p.ldk + (size_t)(u - (p.heads << sh)) * 8
+                                     : static_cast<const TI*>(p.v) + (size_t)t * p.ldv +
+                                           (size_t)(u - ((p.heads + p.kv_heads) << sh)) * 8;
+            load8<TI, VEC>(src, raw[j]);
+        }
+    }
     int bad;
     const int page = kv_place(seq, pos, p.table, p.nseq, p.pages_per_seq, p.page_shift, p.num_pages, p.rope_positions, bad);
     if (page < 0) {
         if (threadIdx.x == 0 && blockIdx.y == 0) kv_flag(p.err, bad);
         return;
     }
-    const int per_head = p.head_dim >> 3;
-    const int units = (p.heads + 2 * p.kv_heads) * per_head;
     const float2* cs = p.rope + (size_t)pos * p.rope_pairs;
     const int off = pos & ((1 << p.page_shift) - 1);
-    for (int u = blockIdx.y * blockDim.x + threadIdx.x; u < units; u += blockDim.x * gridDim.y) {
-        const int head = u / per_head, d = (u - head * per_head) * 8;
-        const bool isq = head < p.heads, isk = !isq && head < p.heads + p.kv_heads;
-        const int h = isq ? head : isk ? head - p.heads : head - p.heads - p.kv_heads;
-        const TI* src = static_cast<const TI*>(isq ? p.q : isk ? p.k : p.v) + (size_t)t * (isq ? p.ldq : isk ? p.ldk : p.ldv) +
-                        (size_t)h * p.head_dim + d;
-        float x[8];
-        load8<TI, VEC>(src, x);
-        if (isq || isk) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int pr = (d >> 1) + i;
-                if (pr < p.rope_pairs) {
-                    const float2 c = __ldg(cs + pr);
-                    const float a = x[2 * i], b = x[2 * i + 1];
-                    x[2 * i] = __fsub_rn(__fmul_rn(a, c.x), __fmul_rn(b, c.y));
-                    x[2 * i + 1] = __fadd_rn(__fmul_rn(a, c.y), __fmul_rn(b, c.x));
-                }
+    for (int j = 0; j < kAppendUnits; ++j) {
+        const int u = u0 + j * blockDim.x;
+        if (u >= p.units) break;
+        const int head = u >> sh, hk = head - p.heads, hv = hk - p.kv_heads;
+        const int d = (u & ((1 << sh) - 1)) * 8;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = raw[j].at(i);
+        if (hv < 0) {
+            const int pr = d >> 1;
+            float2 c[4];
+            if (p.vec_rope && pr + 4 <= p.rope_pairs) {
+                *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cs + pr));
+                *reinterpret_cast<float4*>(c + 2) = __ldg(reinterpret_cast<const float4*>(cs + pr + 2));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (pr + i < p.rope_pairs) c[i] = __ldg(cs + pr + i);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (pr + i < p.rope_pairs) {
+                    const float a = x[2 * i], b = x[2 * i + 1];
+                    x[2 * i] = __fsub_rn(__fmul_rn(a, c[i].x), __fmul_rn(b, c[i].y));
+                    x[2 * i + 1] = __fadd_rn(__fmul_rn(a, c[i].y), __fmul_rn(b, c[i].x));
+                }
         }
-        if (isq) {
-            store8<TQ, VEC>(static_cast<TQ*>(p.q_out) + (size_t)t * p.ldqo + (size_t)h * p.head_dim + d, x);
+        if (hk < 0) {
+            store8<TQ, VEC>(static_cast<TQ*>(p.q_out) + (size_t)t * p.ldqo + (size_t)u * 8, x);
         } else {
-            __half* dst = (isk ? p.kp : p.vp) +
+            const int h = hv < 0 ? hk : hv;
+            __half* dst = (hv < 0 ? p.kp : p.vp) +
                           (((((size_t)page * p.kv_heads + h) << p.page_shift) + off) * p.head_dim + d);
             store8<__half, true>(dst, x);  // pages are 16-byte aligned and head_dim a multiple of 8
         }

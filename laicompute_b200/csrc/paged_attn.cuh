@@ -15,7 +15,11 @@
 // from accumulators to B fragments by movmatrix. FP32 queries and weights are split into binary16
 // hi + lo (two products, 22 bits); a query row is first scaled by a power of two to [1, 2), so no
 // magnitude leaves binary16's range, and the weights carry a factor 2^10 that keeps small ones
-// out of its subnormals (both sides of the final division have it).
+// out of its subnormals (both sides of the final division have it). The hi and lo products have
+// accumulators of their own: the tensor cores truncate as they accumulate, and lo parts added to a
+// large sum would only lengthen that chain. With at most four columns (a decode step of the usual
+// groups) hi and lo sit side by side in one tile's eight columns (PK), so the split costs no
+// product at all.
 #pragma once
 #include "common.cuh"
 #include "mma_matvec.cuh"  // smem_u32, mma16816, cp.async
@@ -47,7 +51,7 @@ struct KvAttnParams {
 constexpr int kPaWarps = 4;
 constexpr int kPaChunk = 64;      // positions per ring stage: 16 per warp
 constexpr int kPaMaxSplit = 2048; // positions per item at most (its page ids are held in shared memory)
-constexpr float kPaBias = 10.f;   // log2 of the factor the weights carry
+constexpr float kPaGain = 1024.f; // the factor the weights carry
 
 __host__ __device__ constexpr int pa_stages(int D) { return D == 128 ? 3 : 4; }
 __host__ __device__ constexpr size_t pa_ring_bytes(int D) { return (size_t)pa_stages(D) * 2 * kPaChunk * D * 2; }
@@ -143,13 +147,14 @@ __device__ __forceinline__ float q_at(const KvAttnParams& p, int r, int h, int d
 // One item: columns [col0, col0 + 8 NT) of rows r0.. (column = row offset * G + head), positions
 // [t0, t1) of sequence `seq`. Column c sees positions below lim[c] (shared memory; 0: no column).
 // slot: the partial's index among its row's; minlim: the smallest lim of a live column.
-template <int D, int NT, typename T>
+template <int D, int NT, typename T, bool PK>
 __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0, int ncol, int kvh, int seq, int t0,
                                         int t1, int slot, const int* lim, int minlim, int* page_ids, float* cmul,
                                         uint8_t* smem) {
-    constexpr bool HL = sizeof(T) == 4;
+    constexpr bool HL = sizeof(T) == 4 && !PK;  // a second set of products for the lo parts
     constexpr int HN = HL ? 2 : 1;
-    constexpr int KS = D / 16, CPR = D / 8, NC = NT * 8, NW = kPaWarps, NTH = kPaWarps * 32;
+    static_assert(!PK || (NT == 1 && sizeof(T) == 4), "hi and lo side by side: one tile of FP32 columns");
+    constexpr int KS = D / 16, CPR = D / 8, NC = PK ? 4 : NT * 8, NW = kPaWarps, NTH = kPaWarps * 32;
     constexpr int NST = pa_stages(D);
     constexpr size_t kRed = (size_t)NW * NC * (D + 4) * 4;
     constexpr size_t kQoff = pa_ring_bytes(D) > kRed ? pa_ring_bytes(D) : kRed;
@@ -209,7 +214,7 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             mx = fmaxf(mx, fmaxf(fabsf(a[i]), fabsf(b[i])));
         }
         float fac = 1.f, inv = 1.f;
-        if (HL) {
+        if (HL || PK) {
             mx = warp_max(mx);
             const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
             fac = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -225,7 +230,8 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                 const float va = a[i] * fac, vb = b[i] * fac;
                 const __half ha = __float2half_rn(va), hb = __float2half_rn(vb);
                 dst[0] = pack_h2(ha, hb);
-                if (HL) dst[64] = pack_h2(__float2half_rn(va - __half2float(ha)), __float2half_rn(vb - __half2float(hb)));
+                if (HL || PK)  // the next plane, or the column four on
+                    dst[HL ? 64 : 32] = pack_h2(__float2half_rn(va - __half2float(ha)), __float2half_rn(vb - __half2float(hb)));
             }
         }
     }
@@ -248,32 +254,46 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
         const int c0 = t0 + ch * kPaChunk;
         if (c0 + wp < t1) {
             const uint32_t ks_a = ring + (uint32_t)(ch % NST) * (2 * kPaChunk * D * 2), vs_a = ks_a + kPaChunk * D * 2;
-            float s[NT][4];
+            float s[NT][4], sl[NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            for (int nt = 0; nt < NT; ++nt) {
+                s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+                sl[nt][0] = sl[nt][1] = sl[nt][2] = sl[nt][3] = 0.f;
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 uint32_t a[4];
                 ldsm_x4(ks_a + 2 * attn_swz<D>(wp + (li & 1) * 8 + lr, ks * 2 + (li >> 1)), a);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int hl = 0; hl < HN; ++hl) {
-                        const uint2 b = *reinterpret_cast<const uint2*>(qf + (((ks * NT + nt) * HN + hl) * 32 + lane) * 2);
-                        mma16816_acc(s[nt], a[0], a[1], a[2], a[3], b.x, b.y);
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint32_t* qa = qf + (((ks * NT + nt) * HN) * 32 + lane) * 2;
+                    const uint2 b = *reinterpret_cast<const uint2*>(qa);
+                    mma16816_acc(s[nt], a[0], a[1], a[2], a[3], b.x, b.y);
+                    if (HL) {
+                        const uint2 bl = *reinterpret_cast<const uint2*>(qa + 64);
+                        mma16816_acc(sl[nt], a[0], a[1], a[2], a[3], bl.x, bl.y);
                     }
+                }
             }
             const int pos = c0 + wp + gq;
+            const bool full = c0 + wp + 16 <= min(t1, minlim);  // every live column sees all 16 positions
             uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float mx[2] = {-INFINITY, -INFINITY}, corr[2], sum[2] = {0.f, 0.f};
+                float mx[2] = {-INFINITY, -INFINITY}, corr[2], sum[2] = {0.f, 0.f}, cm2[2];
+                int lm[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int col = PK ? (2 * c + h) & 3 : nt * 8 + 2 * c + h;
+                    cm2[h] = cmul[col];
+                    lm[h] = min(t1, lim[col]);
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int col = nt * 8 + 2 * c + (e & 1);
-                    s[nt][e] *= cmul[col];
-                    if (pos + (e >> 1) * 8 >= min(t1, lim[col])) s[nt][e] = -INFINITY;
-                    mx[e & 1] = fmaxf(mx[e & 1], s[nt][e]);
+                    if (HL) s[nt][e] += sl[nt][e];
+                    if (PK) s[nt][e] += __shfl_xor_sync(0xffffffffu, s[nt][e], 2);
+                    const float x = s[nt][e] * cm2[e & 1];
+                    if (full || pos + (e >> 1) * 8 < lm[e & 1]) mx[e & 1] = fmaxf(mx[e & 1], x);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -281,26 +301,31 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
                     mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16));
                     const float mnew = fmaxf(m_[nt][h], mx[h]);
-                    const float mu = mnew == -INFINITY ? 0.f : mnew;  // nothing seen yet: every weight is 2^-inf
+                    const float mu = mnew == -INFINITY ? 0.f : mnew;  // nothing seen yet: every weight is 0
                     corr[h] = ex2(m_[nt][h] - mu);
                     m_[nt][h] = mnew;
-                    mx[h] = mu - kPaBias;
+                    mx[h] = mu;
                 }
                 float pv[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    pv[e] = ex2(s[nt][e] - mx[e & 1]);
+                    pv[e] = ex2(fmaf(s[nt][e], cm2[e & 1], -mx[e & 1]));
+                    if (!full && pos + (e >> 1) * 8 >= lm[e & 1]) pv[e] = 0.f;
                     sum[e & 1] += pv[e];
+                    pv[e] *= kPaGain;
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) l_[nt][h] = fmaf(l_[nt][h], corr[h], sum[h]);  // this lane's positions
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const __half h0 = __float2half_rn(pv[2 * j]), h1 = __float2half_rn(pv[2 * j + 1]);
+                    __half h0 = __float2half_rn(pv[2 * j]), h1 = __float2half_rn(pv[2 * j + 1]);
+                    if (HL || PK) {
+                        const __half l0 = __float2half_rn(pv[2 * j] - __half2float(h0));
+                        const __half l1 = __float2half_rn(pv[2 * j + 1] - __half2float(h1));
+                        if (HL) pl[nt][j] = movm_t(pack_h2(l0, l1));
+                        if (PK && c >= 2) { h0 = l0; h1 = l1; }
+                    }
                     ph[nt][j] = movm_t(pack_h2(h0, h1));
-                    if (HL)
-                        pl[nt][j] = movm_t(pack_h2(__float2half_rn(pv[2 * j] - __half2float(h0)),
-                                                   __float2half_rn(pv[2 * j + 1] - __half2float(h1))));
                 }
 #pragma unroll
                 for (int mt = 0; mt < KS; ++mt) {
@@ -308,12 +333,12 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                     o[mt][nt][2] *= corr[0]; o[mt][nt][3] *= corr[1];
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = pv[e];
+                for (int e = 0; e < 4; ++e) s[nt][e] = PK && c >= 2 ? 0.f : pv[e];
             }
             // a position that some columns see and others do not: where its value is not finite,
             // 0 * inf would reach the others, so those products are summed one by one
             bool odd = false;
-            if (min(c0 + wp + 16, t1) > minlim) {
+            if (!full && min(c0 + wp + 16, t1) > minlim) {
 #pragma unroll
                 for (int i = lane; i < 16 * CPR; i += 32) {
                     const uint4 w = lds128(vs_a + 2 * attn_swz<D>(wp + i / CPR, i % CPR));
@@ -371,7 +396,7 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             v += __shfl_xor_sync(0xffffffffu, v, 4);
             v += __shfl_xor_sync(0xffffffffu, v, 8);
             v += __shfl_xor_sync(0xffffffffu, v, 16);
-            l_[nt][h] = v;
+            l_[nt][h] = v * kPaGain;
         }
 
     // ---- join the warps (the ring holds their outputs now)
@@ -380,15 +405,20 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
     float* red = reinterpret_cast<float*>(smem);  // [warp][column][D + 4]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        if (gq == 0) {
+        const bool mine = !PK || c < 2;  // (PK: the lo columns' outputs are added to the hi columns')
+        if (gq == 0 && mine) {
             cm[warp][nt * 8 + 2 * c] = m_[nt][0]; cm[warp][nt * 8 + 2 * c + 1] = m_[nt][1];
             cl[warp][nt * 8 + 2 * c] = l_[nt][0]; cl[warp][nt * 8 + 2 * c + 1] = l_[nt][1];
         }
 #pragma unroll
         for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                red[((size_t)warp * NC + nt * 8 + 2 * c + (e & 1)) * (D + 4) + mt * 16 + gq + (e >> 1) * 8] = o[mt][nt][e];
+            for (int e = 0; e < 4; ++e) {
+                float v = o[mt][nt][e];
+                if (PK) v += __shfl_xor_sync(0xffffffffu, v, 2);
+                if (mine)
+                    red[((size_t)warp * NC + nt * 8 + 2 * c + (e & 1)) * (D + 4) + mt * 16 + gq + (e >> 1) * 8] = v;
+            }
     }
     __syncthreads();
     const int ns = p.nss + p.nsp;
@@ -458,7 +488,7 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const KvAttnP
         }
         const int t1 = min(mx, t0 + p.ls);
         if (t0 >= t1) return;  // no row of the tile sees this far
-        pa_item<D, NT, T>(p, r0, col0, ncol, kvh, row_seq(p, r0), t0, t1, split, lim, mn, page_ids, cmul, smem);
+        pa_item<D, NT, T, false>(p, r0, col0, ncol, kvh, row_seq(p, r0), t0, t1, split, lim, mn, page_ids, cmul, smem);
     } else {
         i -= p.shared_items;
         const int split = i % p.nsp;
@@ -480,7 +510,14 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const KvAttnP
             return;
         }
         if (tid < 8) lim[tid] = tid < p.G ? t1 : 0;
-        pa_item<D, 1, T>(p, r, 0, p.G, kvh, v.seq, t0, t1, p.nss + split, lim, t1, page_ids, cmul, smem);
+        if constexpr (sizeof(T) == 4) {
+            if (p.G <= 4) {
+                pa_item<D, 1, T, true>(p, r, 0, p.G, kvh, v.seq, t0, t1, p.nss + split, lim, t1, page_ids, cmul, smem);
+                pdl_launch_dependents();
+                return;
+            }
+        }
+        pa_item<D, 1, T, false>(p, r, 0, p.G, kvh, v.seq, t0, t1, p.nss + split, lim, t1, page_ids, cmul, smem);
     }
     pdl_launch_dependents();
 }

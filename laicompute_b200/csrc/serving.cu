@@ -123,12 +123,14 @@ int check_attention(const laic_kv_pages& g, const laic_kv_attention_args& a) {
 int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, AttnPlan& pl) {
     const int G = a.heads / g.kv_heads;
     const int max_private = a.max_private < 0 ? a.max_len : std::min(a.max_private, a.max_len);
-    // splits: about `want` items, each a whole number of chunks, at most kPaMaxSplit positions (its page
-    // ids) and, where there is work enough, 512 (a partial costs 2 % of such an item's bytes)
+    // splits: about `want` items, each a whole number of chunks; not below 128 positions (a join costs
+    // more than another chunk) and a range of 256 stays whole; at most 512 (a partial costs 2 % of such
+    // an item's bytes, and ragged rows balance)
     const long long want = 4LL * device_sms(g.device);
     auto split = [&](long long pairs, int len) {
+        if (len <= 256) return round_up(std::max(len, 1), kPaChunk);
         const long long l = ((long long)len * pairs + want - 1) / want;
-        return std::max(kPaChunk, std::min(round_up(l, kPaChunk), 512));
+        return std::max(128, std::min(round_up(l, kPaChunk), 512));
     };
     pl.lp = split((long long)a.rows * g.kv_heads, max_private);
     pl.nsp = std::max(1, (max_private + pl.lp - 1) / pl.lp);
@@ -230,9 +232,12 @@ int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t
     const int bi = type_size(a.in_type), bq = type_size(a.q_type);
     const bool vec = aligned16(a.k_dev) && aligned16(a.v_dev) && a.ldk * bi % 16 == 0 && a.ldv * bi % 16 == 0 &&
                      (!a.heads || (aligned16(a.q_dev) && aligned16(a.q_out_dev) && a.ldq * bi % 16 == 0 && a.ldqo * bq % 16 == 0));
+    p.vec_rope = a.rope_dim % 4 == 0 && aligned16(a.rope_dev);
     const int units = (a.heads + 2 * g.kv_heads) * (g.head_dim / 8);
-    const int block = std::min(256, (units + 31) / 32 * 32);
-    const dim3 grid(a.rows, std::min(65535, (units + block - 1) / block));
+    p.units = units;
+    const int block = std::min(256, (units + 31) / 32 * 32), cta = block * kAppendUnits;
+    const dim3 grid(a.rows, (units + cta - 1) / cta);
+    if (grid.y > 65535) return api_fail(LAIC_E_UNSUPPORTED, "rows too wide");
     return on_device(g.device, [&]() -> int {
         if (a.in_type == LAIC_GGML_F32) {
             if (a.q_type == LAIC_GGML_F32) append_launch<float, float>(vec, grid, block, st, p);
@@ -305,14 +310,22 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
 int logits_probs(int device, int rows, int vocab, const float* x, long long ldx, const float* temp, float* y, long long ldy,
                  cudaStream_t st) {
     if (rows < 0 || vocab < 1) return api_fail(LAIC_E_INVALID, "rows must be >= 0 and vocab >= 1");
+    if (rows > INT_MAX / 8) return api_fail(LAIC_E_UNSUPPORTED, "too many rows");
     if (rows == 0) return LAIC_OK;
     if (!x || !temp || !y) return api_fail(LAIC_E_INVALID, "null pointer");
     if (rows > 1 && (ldx < vocab || ldy < vocab)) return api_fail(LAIC_E_INVALID, "row strides must not be below the vocabulary");
     if (x == y && rows > 1 && ldx != ldy) return api_fail(LAIC_E_INVALID, "in place needs one stride");
     ProbsParams p{x, y, temp, ldx, ldy, vocab};
     return on_device(device, [&]() -> int {
-        probs_kernel<<<rows, kProbsThreads, 0, st>>>(p);
-        const cudaError_t e = cudaGetLastError();
+        const bool vec = aligned16(x) && aligned16(y) && (rows == 1 || (ldx % 4 == 0 && ldy % 4 == 0));
+        // the smallest cluster whose registers hold the row; for few rows the largest, to spread them over the SMs
+        int c = 1;
+        while (c < 8 && c * kProbsSlice < vocab) c *= 2;
+        if (vocab >= 8 * kProbsThreads && 8LL * rows <= device_sms(device)) c = 8;
+        const bool reg = (long long)c * kProbsSlice >= vocab;
+        if (!reg) c = 1;
+        auto fn = reg ? (vec ? probs_kernel<true, true> : probs_kernel<true, false>) : probs_kernel<false, false>;
+        const cudaError_t e = launch_cluster_k(fn, dim3((unsigned)rows * c), dim3(kProbsThreads), 0, st, false, c, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "logits_probs");
     });
 }
@@ -331,7 +344,9 @@ int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st) {
     VerifyParams p{a.target_dev, a.draft_dev, a.ld_target, a.ld_draft, a.draft_ids_dev, a.n_draft_dev, a.accept_u_dev,
                    a.sample_u_dev, a.out_ids_dev, a.out_n_dev, a.nseq, a.max_draft, a.vocab};
     return on_device(device, [&]() -> int {
-        const cudaError_t e = launch_cluster_k(verify_kernel, dim3(a.nseq * kVerifyCluster), dim3(kVerifyThreads), 0, st, false,
+        const bool vec = aligned16(a.target_dev) && a.ld_target % 4 == 0 &&
+                         (!a.draft_dev || (aligned16(a.draft_dev) && a.ld_draft % 4 == 0));
+        const cudaError_t e = launch_cluster_k(vec ? verify_kernel<true> : verify_kernel<false>, dim3(a.nseq * kVerifyCluster), dim3(kVerifyThreads), 0, st, false,
                                                kVerifyCluster, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "verify_drafts");
     });

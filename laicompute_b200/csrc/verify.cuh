@@ -31,45 +31,138 @@ __device__ __forceinline__ float prob_exp(float x, float m, float k, float kl) {
     return fmaf(p, l * 0.69314718f, p);
 }
 
-// One row per CTA, three passes over it (the second and third from L2).
-constexpr int kProbsThreads = 1024;
+constexpr int kProbsThreads = 512;
+constexpr int kProbsPer = 32;  // elements a thread holds
+constexpr int kProbsSlice = kProbsThreads * kProbsPer;
+
+// The row's slices exchange through this (distributed shared memory).
+struct ProbsPart {
+    float m, s;
+    int at;
+};
+
+// A cluster per row, each CTA a slice held in registers (REG; vocab <= cluster * kProbsSlice), so
+// the row is read once: the slice's maximum and its sum of 2^((x - slice maximum) k) meet in one
+// exchange, then every element is formed against the row's maximum. Else (larger vocabularies) a
+// CTA per row reads it three times. VEC: 16-byte aligned rows.
+template <bool REG, bool VEC>
 __global__ void __launch_bounds__(kProbsThreads) probs_kernel(const ProbsParams p) {
-    __shared__ float red[32];
-    __shared__ int redi[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float* x = p.x + (size_t)blockIdx.x * p.ldx;
-    float* y = p.y + (size_t)blockIdx.x * p.ldy;
-    const float t = p.temp[blockIdx.x];
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = REG ? (int)cluster.num_blocks() : 1, rank = REG ? (int)cluster.block_rank() : 0;
+    const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int NW = kProbsThreads / 32;
+    __shared__ float red[NW];
+    __shared__ int redi[NW];
+    __shared__ ProbsPart part;
+    const float* x = p.x + (size_t)row * p.ldx;
+    float* y = p.y + (size_t)row * p.ldy;
+    const float t = p.temp[row];
+    const bool greedy = !(t > 0.f);
+    const int per = REG ? ((p.vocab + C - 1) / C + 3) & ~3 : p.vocab;
+    const int v0 = min(p.vocab, rank * per), v1 = min(p.vocab, v0 + per);
+    // element e of this thread (its order within the slice follows the index only across e / 4)
+    auto index = [&](int e) { return VEC ? v0 + ((e >> 2) * kProbsThreads + tid) * 4 + (e & 3) : v0 + e * kProbsThreads + tid; };
+    float r[REG ? kProbsPer : 1];
+    auto get = [&](float v) { return v == v ? v : -INFINITY; };  // a NaN cannot be chosen
     float m = -INFINITY;
     int at = 0x7fffffff;
-    for (int i = threadIdx.x; i < p.vocab; i += kProbsThreads) {
-        const float v = x[i];
-        if (v > m) { m = v; at = i; }  // NaN never
-    }
+    if constexpr (REG) {
+        if constexpr (VEC) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float om = __shfl_xor_sync(0xffffffffu, m, o);
-        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-        if (om > m || (om == m && oa < at)) { m = om; at = oa; }
+            for (int e = 0; e < kProbsPer; e += 4) {
+                const int i = index(e);
+                float4 w = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (i + 3 < v1) {
+                    w = *reinterpret_cast<const float4*>(x + i);
+                } else {
+                    if (i < v1) w.x = x[i];
+                    if (i + 1 < v1) w.y = x[i + 1];
+                    if (i + 2 < v1) w.z = x[i + 2];
+                }
+                r[e] = get(w.x); r[e + 1] = get(w.y); r[e + 2] = get(w.z); r[e + 3] = get(w.w);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < kProbsPer; ++e) r[e] = index(e) < v1 ? get(x[index(e)]) : -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < kProbsPer; ++e) m = fmaxf(m, r[e]);
+    } else {
+        for (int i = tid; i < p.vocab; i += kProbsThreads) m = fmaxf(m, get(x[i]));
     }
-    if (lane == 0) { red[warp] = m; redi[warp] = at; }
+    m = warp_max(m);
+    if (lane == 0) red[warp] = m;
     __syncthreads();
-    m = -INFINITY; at = 0x7fffffff;
-    for (int w = 0; w < kProbsThreads / 32; ++w)
-        if (red[w] > m || (red[w] == m && redi[w] < at)) { m = red[w]; at = redi[w]; }
-    __syncthreads();
-    if (!(t > 0.f) || m == -INFINITY) {  // greedy: the first maximum; a row of -inf: zeros
-        for (int i = threadIdx.x; i < p.vocab; i += kProbsThreads) y[i] = i == at && m != -INFINITY ? 1.f : 0.f;
-        return;
-    }
-    const double kd = 1.4426950408889634 / (double)t;
+    m = warp_max(lane < NW ? red[lane] : -INFINITY);
+    const double kd = 1.4426950408889634 / (double)(greedy ? 1.f : t);
     const float k = (float)kd, kl = (float)(kd - (double)k);
-    auto term = [&](float v) { return m == INFINITY ? (v == INFINITY ? 1.f : 0.f) : v == v && v != -INFINITY ? prob_exp(v, m, k, kl) : 0.f; };
     float s = 0.f;
-    for (int i = threadIdx.x; i < p.vocab; i += kProbsThreads) s += term(x[i]);
-    s = block_sum(s, red);
-    const float iv = 1.f / s;
-    for (int i = threadIdx.x; i < p.vocab; i += kProbsThreads) y[i] = term(x[i]) * iv;
+    if (greedy) {  // the slice's first maximum
+        if constexpr (REG) {
+#pragma unroll
+            for (int e = kProbsPer - 1; e >= 0; --e)
+                if (r[e] == m && m != -INFINITY) at = min(at, index(e));
+        } else {
+            for (int i = tid; i < p.vocab; i += kProbsThreads)
+                if (at == 0x7fffffff && m != -INFINITY && x[i] == m) at = i;
+        }
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) redi[warp] = at;
+        __syncthreads();
+        at = __reduce_min_sync(0xffffffffu, lane < NW ? redi[lane] : 0x7fffffff);
+    } else if (m != -INFINITY) {
+        auto rough = [&](float v) { return m == INFINITY ? (v == INFINITY ? 1.f : 0.f) : ex2(__fmul_rn(__fsub_rn(v, m), k)); };
+        if constexpr (REG) {
+#pragma unroll
+            for (int e = 0; e < kProbsPer; ++e) s += rough(r[e]);
+        } else {
+            for (int i = tid; i < p.vocab; i += kProbsThreads) s += rough(get(x[i]));
+        }
+        s = warp_sum(s);
+        __syncthreads();
+        if (lane == 0) red[warp] = s;
+        __syncthreads();
+        s = warp_sum(lane < NW ? red[lane] : 0.f);
+    }
+    float M = m, S = s;
+    if (REG && C > 1) {
+        if (tid == 0) part = ProbsPart{m, s, at};
+        cluster.sync();
+        ProbsPart o{-INFINITY, 0.f, 0x7fffffff};
+        if (lane < C) o = *cluster.map_shared_rank(&part, lane);  // every warp for itself
+        M = warp_max(o.m);
+        S = warp_sum(o.m == -INFINITY ? 0.f : o.m == M ? o.s : o.s * ex2(__fmul_rn(__fsub_rn(o.m, M), k)));
+        at = __reduce_min_sync(0xffffffffu, o.m == M ? o.at : 0x7fffffff);
+        cluster.sync();  // no CTA leaves while another may still read its part
+    }
+    const float iv = 1.f / S;
+    auto term = [&](float v, int i) {
+        if (M == -INFINITY) return 0.f;  // nothing can be chosen
+        if (greedy) return i == at ? 1.f : 0.f;
+        if (M == INFINITY) return v == INFINITY ? iv : 0.f;
+        return prob_exp(v, M, k, kl) * iv;
+    };
+    if constexpr (REG) {
+#pragma unroll
+        for (int e = 0; e < kProbsPer; e += VEC ? 4 : 1) {
+            const int i = index(e);
+            if constexpr (VEC) {
+                const float4 w = make_float4(term(r[e], i), term(r[e + 1], i + 1), term(r[e + 2], i + 2), term(r[e + 3], i + 3));
+                if (i + 3 < v1) {
+                    *reinterpret_cast<float4*>(y + i) = w;
+                } else {
+                    if (i < v1) y[i] = w.x;
+                    if (i + 1 < v1) y[i + 1] = w.y;
+                    if (i + 2 < v1) y[i + 2] = w.z;
+                }
+            } else {
+                if (i < v1) y[i] = term(r[e], i);
+            }
+        }
+    } else {
+        for (int i = tid; i < p.vocab; i += kProbsThreads) y[i] = term(get(x[i]), i);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -92,9 +185,11 @@ constexpr int kVerifyCluster = 8;
 __device__ __forceinline__ float prob_in(float x) { return fmaxf(x, 0.f); }  // negative and NaN: 0
 
 // One cluster per sequence. Every CTA finds the first refused token (the numbers are gathered, a
-// lane per drafted token), then sums its slice of the row the next token is drawn from; the slices'
-// sums meet in distributed shared memory, and the CTA whose slice holds sample_u * total reads it
-// once more in order. Sums are in 64 bits: 128k binary32 terms in 32 would move the drawn token.
+// lane per drafted token), then sums its slice of the row the next token is drawn from, a run of
+// consecutive elements per warp; the slices' sums meet in distributed shared memory, and the warp
+// whose run holds sample_u * total walks it once more. Sums are in 64 bits: 128k binary32 terms in
+// 32 would move the drawn token. VEC: 16-byte aligned rows.
+template <bool VEC>
 __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyParams p) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -102,8 +197,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int NW = kVerifyThreads / 32;
     __shared__ int s_acc;
-    __shared__ double s_sum[2], s_red[NW];
-    __shared__ int s_hit, s_last;
+    __shared__ double s_sum[2], s_run[NW];
     int n = p.n_draft[s];
     if (n < 0) return;  // the whole cluster alike
     n = min(n, p.max_draft);
@@ -116,12 +210,13 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
             bool refuse = false;
             if (j < n) {
                 const unsigned x = ids[j];
+                const float u = p.accept_u[(size_t)s * p.max_draft + j];
                 refuse = true;
                 if (x < (unsigned)p.vocab) {
                     const float pt = prob_in(p.target[((size_t)s * (p.max_draft + 1) + j) * p.ldt + x]);
                     const float qd = p.draft ? prob_in(p.draft[((size_t)s * p.max_draft + j) * p.ldd + x]) : 1.f;
                     // the product of two binary32 numbers is exact in binary64
-                    refuse = !((double)p.accept_u[(size_t)s * p.max_draft + j] * (double)qd < (double)pt);
+                    refuse = !((double)u * (double)qd < (double)pt);
                 }
             }
             no[b] = __ballot_sync(0xffffffffu, refuse);
@@ -134,41 +229,56 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
     const float* Q = acc < n && p.draft ? p.draft + ((size_t)s * p.max_draft + acc) * p.ldd : nullptr;
     const unsigned hole = acc < n && !p.draft ? ids[acc] : LAIC_NO_TOKEN;  // drafted with certainty: p without it
     int mode = acc < n ? 1 : 0;  // 1: what the draft leaves of p; 0: p itself
-    auto value = [&](int v) -> double {
-        const float a = prob_in(P[v]);
-        if (mode == 0) return (double)a;
-        if (Q) return fmax((double)a - (double)prob_in(Q[v]), 0.0);
-        return (unsigned)v == hole ? 0.0 : (double)a;
+    auto value = [&](float a, float b, int v) -> double {  // a = P[v], b = Q[v]
+        if (mode == 0) return (double)prob_in(a);
+        if (Q) return fmax((double)prob_in(a) - (double)prob_in(b), 0.0);
+        return (unsigned)v == hole ? 0.0 : (double)prob_in(a);
     };
-    const int per = ((p.vocab + kVerifyCluster - 1) / kVerifyCluster + 3) & ~3;
-    const int v0 = min(p.vocab, rank * per), v1 = min(p.vocab, v0 + per);
+    // warp w of CTA r: run r * NW + w, a multiple of four elements long
+    const int run_len = ((p.vocab + kVerifyCluster * NW - 1) / (kVerifyCluster * NW) + 3) & ~3;
+    const long long first = (long long)(rank * NW + warp) * run_len;
+    const int v0 = (int)min((long long)p.vocab, first), v1 = min(p.vocab, v0 + run_len);
+    auto four = [&](const float* src, int i, float (&x)[4]) {  // elements i.. of the run, zeros past its end
+        if (VEC && i + 3 < v1) {
+            *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src + i);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = i + e < v1 ? src[i + e] : 0.f;
+        }
+    };
     double total = 0.0, before = 0.0;
     int owner = -1;
     for (int pass = 0; pass < 2; ++pass) {
         double a = 0.0;
-        for (int v = v0 + tid; v < v1; v += kVerifyThreads) a += value(v);
+#pragma unroll 4
+        for (int i = v0 + lane * 4; i < v1; i += 128) {
+            float x[4], q[4] = {};
+            four(P, i, x);
+            if (mode && Q) four(Q, i, q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a += value(x[e], q[e], i + e);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-        if (lane == 0) s_red[warp] = a;
+        if (lane == 0) s_run[warp] = a;
         __syncthreads();
-        if (tid == 0) {
-            double t = 0.0;
-            for (int w = 0; w < NW; ++w) t += s_red[w];
-            s_sum[pass] = t;
+        if (warp == 0) {
+            double t = lane < NW ? s_run[lane] : 0.0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            if (lane == 0) s_sum[pass] = t;
         }
         cluster.sync();
         double part[kVerifyCluster];
         total = 0.0;
 #pragma unroll
-        for (int j = 0; j < kVerifyCluster; ++j) {
-            part[j] = *cluster.map_shared_rank(&s_sum[pass], j);
-            total += part[j];
-        }
+        for (int j = 0; j < kVerifyCluster; ++j) part[j] = *cluster.map_shared_rank(&s_sum[pass], j);
+#pragma unroll
+        for (int j = 0; j < kVerifyCluster; ++j) total += part[j];
         if (total > 0.0 || mode == 0) {
             const double t = (double)p.sample_u[s] * total;
-            double run = 0.0;
+            double run = 0.0, last_before = 0.0;
             int last = -1;
-            double last_before = 0.0;
 #pragma unroll
             for (int j = 0; j < kVerifyCluster; ++j) {
                 if (owner < 0 && part[j] > 0.0) {
@@ -191,47 +301,61 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
         if (tid == 0) p.out_n[s] = acc + 1;
     }
     if (rank != owner) return;
-    // the lowest v of this slice whose running sum exceeds t: each thread a run of consecutive
-    // elements, the runs' sums scanned, then the run that crosses t walked
+    // the lowest v of this slice whose running sum exceeds t: every warp finds the run that crosses
+    // t (or, where rounding put t at the slice's end, the last with a positive sum), its warp walks it
     const double t = (double)p.sample_u[s] * total - before;
-    const int run_len = (v1 - v0 + kVerifyThreads - 1) / kVerifyThreads;
-    const int a0 = min(v1, v0 + tid * run_len), a1 = min(v1, a0 + run_len);
-    double mine = 0.0;
-    for (int v = a0; v < a1; ++v) mine += value(v);
-    double incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const double u = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += u;
+    double base = 0.0, at_base = 0.0;
+    int who = -1;
+    for (int w = 0; w < NW; ++w) {
+        const double a = s_run[w];
+        if (a > 0.0) {
+            who = w;
+            at_base = base;
+            if (base + a > t) break;
+        }
+        base += a;
     }
-    if (lane == 31) s_red[warp] = incl;
-    if (tid == 0) { s_hit = kVerifyThreads; s_last = -1; }
-    __syncthreads();
-    double base = 0.0;
-    for (int w = 0; w < warp; ++w) base += s_red[w];
-    const double end = base + incl;
-    if (mine > 0.0) {
-        atomicMax(&s_last, tid);
-        if (end > t) atomicMin(&s_hit, tid);
-    }
-    __syncthreads();
-    const int who = s_hit < kVerifyThreads ? s_hit : s_last;  // rounding put t at the slice's end: its last element
     if (who < 0) {
         if (tid == 0) out[acc] = 0;  // no positive probability anywhere
         return;
     }
-    if (tid != who) return;
-    double run = end - mine;
-    int pick = a0;
-    for (int v = a0; v < a1; ++v) {
-        const double x = value(v);
-        if (x > 0.0) {
-            pick = v;
-            run += x;
-            if (run > t) break;
+    if (warp != who) return;
+    double run = at_base;
+    int pick = v0;  // the last positive element so far
+    for (int i0 = v0; i0 < v1; i0 += 128) {
+        const int i = i0 + lane * 4;
+        float x[4] = {}, q[4] = {};
+        four(P, i, x);
+        if (mode && Q) four(Q, i, q);
+        double c[4], mine = 0.0;
+        int lastpos = -1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double w = i + e < v1 ? value(x[e], q[e], i + e) : 0.0;
+            if (w > 0.0) lastpos = i + e;
+            mine += w;
+            c[e] = mine;
         }
+        double incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
+        }
+        const double start = run + (incl - mine);
+        int hit = 0x7fffffff;
+#pragma unroll
+        for (int e = 3; e >= 0; --e)
+            if (i + e < v1 && start + c[e] > t && (e == 0 ? c[0] > 0.0 : c[e] > c[e - 1])) hit = i + e;
+        hit = __reduce_min_sync(0xffffffffu, hit);
+        if (hit != 0x7fffffff) {
+            if (lane == 0) out[acc] = (unsigned)hit;
+            return;
+        }
+        pick = max(pick, __reduce_max_sync(0xffffffffu, lastpos));
+        run += __shfl_sync(0xffffffffu, incl, 31);
     }
-    out[acc] = (unsigned)pick;
+    if (lane == 0) out[acc] = (unsigned)pick;
 }
 
 }  // namespace laic
