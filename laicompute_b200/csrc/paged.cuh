@@ -115,34 +115,34 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p) 
             load8<TI, VEC>(src, raw[j]);
         }
     }
+    // the units of a thread lie blockDim.x apart, a whole number of heads: one set of angles
+    const int d = (u0 & ((1 << sh) - 1)) * 8, pr = d >> 1;
+    const float2* cs = p.rope + (size_t)min(pos, p.rope_positions - 1) * p.rope_pairs;
+    float2 c[4];
+    if (p.vec_rope && pr + 4 <= p.rope_pairs) {
+        *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cs + pr));
+        *reinterpret_cast<float4*>(c + 2) = __ldg(reinterpret_cast<const float4*>(cs + pr + 2));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (pr + i < p.rope_pairs) c[i] = __ldg(cs + pr + i);
+    }
     int bad;
     const int page = kv_place(seq, pos, p.table, p.nseq, p.pages_per_seq, p.page_shift, p.num_pages, p.rope_positions, bad);
     if (page < 0) {
         if (threadIdx.x == 0 && blockIdx.y == 0) kv_flag(p.err, bad);
         return;
     }
-    const float2* cs = p.rope + (size_t)pos * p.rope_pairs;
     const int off = pos & ((1 << p.page_shift) - 1);
 #pragma unroll
     for (int j = 0; j < kAppendUnits; ++j) {
         const int u = u0 + j * blockDim.x;
         if (u >= p.units) break;
         const int head = u >> sh, hk = head - p.heads, hv = hk - p.kv_heads;
-        const int d = (u & ((1 << sh) - 1)) * 8;
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = raw[j].at(i);
         if (hv < 0) {
-            const int pr = d >> 1;
-            float2 c[4];
-            if (p.vec_rope && pr + 4 <= p.rope_pairs) {
-                *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cs + pr));
-                *reinterpret_cast<float4*>(c + 2) = __ldg(reinterpret_cast<const float4*>(cs + pr + 2));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (pr + i < p.rope_pairs) c[i] = __ldg(cs + pr + i);
-            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (pr + i < p.rope_pairs) {

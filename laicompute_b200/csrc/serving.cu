@@ -186,6 +186,10 @@ cudaError_t serving_set_attributes() {
                                          (int)pa_smem(D, nt, type == LAIC_GGML_F32));
                 if (e != cudaSuccess) return e;
             }
+    for (auto fn : {probs_kernel<true, true>, probs_kernel<true, false>}) {
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (kProbsSlice + 8) * 4);
+        if (e != cudaSuccess) return e;
+    }
     if (dev >= 0 && dev < 64) done[dev].store(true);
     return cudaSuccess;
 }
@@ -318,14 +322,17 @@ int logits_probs(int device, int rows, int vocab, const float* x, long long ldx,
     ProbsParams p{x, y, temp, ldx, ldy, vocab};
     return on_device(device, [&]() -> int {
         const bool vec = aligned16(x) && aligned16(y) && (rows == 1 || (ldx % 4 == 0 && ldy % 4 == 0));
-        // the smallest cluster whose registers hold the row; for few rows the largest, to spread them over the SMs
+        // the smallest cluster whose shared memory holds the row; for few rows the largest, to spread them over the SMs
         int c = 1;
         while (c < 8 && c * kProbsSlice < vocab) c *= 2;
         if (vocab >= 8 * kProbsThreads && 8LL * rows <= device_sms(device)) c = 8;
-        const bool reg = (long long)c * kProbsSlice >= vocab;
-        if (!reg) c = 1;
-        auto fn = reg ? (vec ? probs_kernel<true, true> : probs_kernel<true, false>) : probs_kernel<false, false>;
-        const cudaError_t e = launch_cluster_k(fn, dim3((unsigned)rows * c), dim3(kProbsThreads), 0, st, false, c, p);
+        const bool sm = (long long)c * kProbsSlice >= vocab;
+        if (!sm) c = 1;
+        const size_t smem = sm ? ((size_t)(vocab + c - 1) / c + 8) * 4 : 0;
+        cudaError_t e = serving_set_attributes();
+        if (e == cudaSuccess)
+            e = launch_cluster_k(sm ? (vec ? probs_kernel<true, true> : probs_kernel<true, false>) : probs_kernel<false, false>,
+                                 dim3((unsigned)rows * c), dim3(kProbsThreads), smem, st, false, c, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "logits_probs");
     });
 }
@@ -334,7 +341,7 @@ int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st) {
     if (a.nseq < 0 || a.vocab < 1) return api_fail(LAIC_E_INVALID, "nseq must be >= 0 and vocab >= 1");
     if (a.max_draft < 0) return api_fail(LAIC_E_INVALID, "max_draft must be >= 0");
     if (a.max_draft > LAIC_MAX_DRAFT) return api_fail(LAIC_E_UNSUPPORTED, "at most 64 drafted tokens per sequence");
-    if (a.nseq > INT_MAX / kVerifyCluster) return api_fail(LAIC_E_UNSUPPORTED, "too many sequences");
+    if (a.nseq > INT_MAX / kVerifyMaxCluster) return api_fail(LAIC_E_UNSUPPORTED, "too many sequences");
     if (a.nseq == 0) return LAIC_OK;
     if (!a.target_dev || !a.n_draft_dev || !a.sample_u_dev || !a.out_ids_dev || !a.out_n_dev ||
         (a.max_draft && (!a.draft_ids_dev || !a.accept_u_dev)))
@@ -346,8 +353,10 @@ int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st) {
     return on_device(device, [&]() -> int {
         const bool vec = aligned16(a.target_dev) && a.ld_target % 4 == 0 &&
                          (!a.draft_dev || (aligned16(a.draft_dev) && a.ld_draft % 4 == 0));
-        const cudaError_t e = launch_cluster_k(vec ? verify_kernel<true> : verify_kernel<false>, dim3(a.nseq * kVerifyCluster), dim3(kVerifyThreads), 0, st, false,
-                                               kVerifyCluster, p);
+        // the largest cluster that still runs in one wave (two CTAs per SM)
+        int c = kVerifyMaxCluster;
+        while (c > 1 && (long long)a.nseq * c > 2LL * device_sms(device)) c /= 2;
+        const cudaError_t e = launch_cluster_k(vec ? verify_kernel<true> : verify_kernel<false>, dim3((unsigned)a.nseq * c), dim3(kVerifyThreads), 0, st, false, c, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "verify_drafts");
     });
 }

@@ -32,8 +32,7 @@ __device__ __forceinline__ float prob_exp(float x, float m, float k, float kl) {
 }
 
 constexpr int kProbsThreads = 512;
-constexpr int kProbsPer = 32;  // elements a thread holds
-constexpr int kProbsSlice = kProbsThreads * kProbsPer;
+constexpr int kProbsSlice = 16384;  // elements of a row's slice in shared memory
 
 // The row's slices exchange through this (distributed shared memory).
 struct ProbsPart {
@@ -41,84 +40,76 @@ struct ProbsPart {
     int at;
 };
 
-// A cluster per row, each CTA a slice held in registers (REG; vocab <= cluster * kProbsSlice), so
+// A cluster per row, each CTA a slice held in shared memory (SM; vocab <= cluster * kProbsSlice), so
 // the row is read once: the slice's maximum and its sum of 2^((x - slice maximum) k) meet in one
 // exchange, then every element is formed against the row's maximum. Else (larger vocabularies) a
 // CTA per row reads it three times. VEC: 16-byte aligned rows.
-template <bool REG, bool VEC>
-__global__ void __launch_bounds__(kProbsThreads) probs_kernel(const ProbsParams p) {
+template <bool SM, bool VEC>
+__global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsParams p) {
     namespace cg = cooperative_groups;
+    extern __shared__ __align__(16) float slice[];
     cg::cluster_group cluster = cg::this_cluster();
-    const int C = REG ? (int)cluster.num_blocks() : 1, rank = REG ? (int)cluster.block_rank() : 0;
+    const int C = SM ? (int)cluster.num_blocks() : 1, rank = SM ? (int)cluster.block_rank() : 0;
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    constexpr int NW = kProbsThreads / 32;
+    constexpr int NW = kProbsThreads / 32, NT = kProbsThreads;
     __shared__ float red[NW];
     __shared__ int redi[NW];
     __shared__ ProbsPart part;
-    const float* x = p.x + (size_t)row * p.ldx;
-    float* y = p.y + (size_t)row * p.ldy;
+    const int per = SM ? ((p.vocab + C - 1) / C + 3) & ~3 : p.vocab;
+    const int v0 = min(p.vocab, rank * per), n = min(p.vocab, v0 + per) - v0;
+    const float* x = p.x + (size_t)row * p.ldx + v0;
+    float* y = p.y + (size_t)row * p.ldy + v0;
+    const float* src = SM ? slice : x;
+    if constexpr (SM) {
+        if constexpr (VEC) {
+            for (int i = tid * 4; i + 3 < n; i += NT * 4) cp_async16(slice + i, x + i);
+            cp_async_commit();
+            if (tid < (n & 3)) slice[(n & ~3) + tid] = x[(n & ~3) + tid];
+        } else {
+#pragma unroll 4
+            for (int i = tid; i < n; i += NT) slice[i] = x[i];
+        }
+    }
     const float t = p.temp[row];
     const bool greedy = !(t > 0.f);
-    const int per = REG ? ((p.vocab + C - 1) / C + 3) & ~3 : p.vocab;
-    const int v0 = min(p.vocab, rank * per), v1 = min(p.vocab, v0 + per);
-    // element e of this thread (its order within the slice follows the index only across e / 4)
-    auto index = [&](int e) { return VEC ? v0 + ((e >> 2) * kProbsThreads + tid) * 4 + (e & 3) : v0 + e * kProbsThreads + tid; };
-    float r[REG ? kProbsPer : 1];
+    const double kd = 1.4426950408889634 / (double)(greedy ? 1.f : t);
+    const float k = (float)kd, kl = (float)(kd - (double)k);
+    if constexpr (SM) {
+        if constexpr (VEC) cp_async_wait_all();
+        __syncthreads();
+    }
     auto get = [&](float v) { return v == v ? v : -INFINITY; };  // a NaN cannot be chosen
-    float m = -INFINITY;
-    int at = 0x7fffffff;
-    if constexpr (REG) {
-        if constexpr (VEC) {
-#pragma unroll
-            for (int e = 0; e < kProbsPer; e += 4) {
-                const int i = index(e);
-                float4 w = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (i + 3 < v1) {
-                    w = *reinterpret_cast<const float4*>(x + i);
-                } else {
-                    if (i < v1) w.x = x[i];
-                    if (i + 1 < v1) w.y = x[i + 1];
-                    if (i + 2 < v1) w.z = x[i + 2];
-                }
-                r[e] = get(w.x); r[e + 1] = get(w.y); r[e + 2] = get(w.z); r[e + 3] = get(w.w);
+    // f(element, its index) over this thread's elements, in ascending order
+    auto each = [&](auto&& f) {
+        if constexpr (SM) {
+#pragma unroll 2
+            for (int i = tid * 4; i < n; i += NT * 4) {
+                const float4 w = *reinterpret_cast<const float4*>(slice + i);  // (the slice is padded to four)
+                f(w.x, i);
+                if (i + 1 < n) f(w.y, i + 1);
+                if (i + 2 < n) f(w.z, i + 2);
+                if (i + 3 < n) f(w.w, i + 3);
             }
         } else {
-#pragma unroll
-            for (int e = 0; e < kProbsPer; ++e) r[e] = index(e) < v1 ? get(x[index(e)]) : -INFINITY;
+            for (int i = tid; i < n; i += NT) f(src[i], i);
         }
-#pragma unroll
-        for (int e = 0; e < kProbsPer; ++e) m = fmaxf(m, r[e]);
-    } else {
-        for (int i = tid; i < p.vocab; i += kProbsThreads) m = fmaxf(m, get(x[i]));
-    }
+    };
+    float m = -INFINITY, s = 0.f;
+    int at = 0x7fffffff;
+    each([&](float v, int) { m = fmaxf(m, v); });  // (fmaxf passes a NaN over)
     m = warp_max(m);
     if (lane == 0) red[warp] = m;
     __syncthreads();
     m = warp_max(lane < NW ? red[lane] : -INFINITY);
-    const double kd = 1.4426950408889634 / (double)(greedy ? 1.f : t);
-    const float k = (float)kd, kl = (float)(kd - (double)k);
-    float s = 0.f;
     if (greedy) {  // the slice's first maximum
-        if constexpr (REG) {
-#pragma unroll
-            for (int e = kProbsPer - 1; e >= 0; --e)
-                if (r[e] == m && m != -INFINITY) at = min(at, index(e));
-        } else {
-            for (int i = tid; i < p.vocab; i += kProbsThreads)
-                if (at == 0x7fffffff && m != -INFINITY && x[i] == m) at = i;
-        }
+        each([&](float v, int i) { if (v == m) at = min(at, i + v0); });
         at = __reduce_min_sync(0xffffffffu, at);
         if (lane == 0) redi[warp] = at;
         __syncthreads();
         at = __reduce_min_sync(0xffffffffu, lane < NW ? redi[lane] : 0x7fffffff);
     } else if (m != -INFINITY) {
-        auto rough = [&](float v) { return m == INFINITY ? (v == INFINITY ? 1.f : 0.f) : ex2(__fmul_rn(__fsub_rn(v, m), k)); };
-        if constexpr (REG) {
-#pragma unroll
-            for (int e = 0; e < kProbsPer; ++e) s += rough(r[e]);
-        } else {
-            for (int i = tid; i < p.vocab; i += kProbsThreads) s += rough(get(x[i]));
-        }
+        if (m == INFINITY) each([&](float v, int) { s += v == INFINITY ? 1.f : 0.f; });
+        else each([&](float v, int) { s += ex2(__fmul_rn(__fsub_rn(get(v), m), k)); });
         s = warp_sum(s);
         __syncthreads();
         if (lane == 0) red[warp] = s;
@@ -126,7 +117,7 @@ __global__ void __launch_bounds__(kProbsThreads) probs_kernel(const ProbsParams 
         s = warp_sum(lane < NW ? red[lane] : 0.f);
     }
     float M = m, S = s;
-    if (REG && C > 1) {
+    if (SM && C > 1) {
         if (tid == 0) part = ProbsPart{m, s, at};
         cluster.sync();
         ProbsPart o{-INFINITY, 0.f, 0x7fffffff};
@@ -139,29 +130,25 @@ __global__ void __launch_bounds__(kProbsThreads) probs_kernel(const ProbsParams 
     const float iv = 1.f / S;
     auto term = [&](float v, int i) {
         if (M == -INFINITY) return 0.f;  // nothing can be chosen
-        if (greedy) return i == at ? 1.f : 0.f;
+        if (greedy) return i + v0 == at ? 1.f : 0.f;
         if (M == INFINITY) return v == INFINITY ? iv : 0.f;
-        return prob_exp(v, M, k, kl) * iv;
+        return prob_exp(v, M, k, kl) * iv;  // (0 for a NaN: its exponent is not above any bound)
     };
-    if constexpr (REG) {
-#pragma unroll
-        for (int e = 0; e < kProbsPer; e += VEC ? 4 : 1) {
-            const int i = index(e);
-            if constexpr (VEC) {
-                const float4 w = make_float4(term(r[e], i), term(r[e + 1], i + 1), term(r[e + 2], i + 2), term(r[e + 3], i + 3));
-                if (i + 3 < v1) {
-                    *reinterpret_cast<float4*>(y + i) = w;
-                } else {
-                    if (i < v1) y[i] = w.x;
-                    if (i + 1 < v1) y[i + 1] = w.y;
-                    if (i + 2 < v1) y[i + 2] = w.z;
-                }
+    if constexpr (SM && VEC) {
+#pragma unroll 2
+        for (int i = tid * 4; i < n; i += NT * 4) {
+            const float4 w = *reinterpret_cast<const float4*>(slice + i);
+            const float4 o = make_float4(term(w.x, i), term(w.y, i + 1), term(w.z, i + 2), term(w.w, i + 3));
+            if (i + 3 < n) {
+                *reinterpret_cast<float4*>(y + i) = o;
             } else {
-                if (i < v1) y[i] = term(r[e], i);
+                y[i] = o.x;
+                if (i + 1 < n) y[i + 1] = o.y;
+                if (i + 2 < n) y[i + 2] = o.z;
             }
         }
     } else {
-        for (int i = tid; i < p.vocab; i += kProbsThreads) y[i] = term(get(x[i]), i);
+        for (int i = tid; i < n; i += NT) y[i] = term(src[i], i);
     }
 }
 
@@ -180,7 +167,7 @@ struct VerifyParams {
 };
 
 constexpr int kVerifyThreads = 512;
-constexpr int kVerifyCluster = 8;
+constexpr int kVerifyMaxCluster = 8;
 
 __device__ __forceinline__ float prob_in(float x) { return fmaxf(x, 0.f); }  // negative and NaN: 0
 
@@ -190,10 +177,10 @@ __device__ __forceinline__ float prob_in(float x) { return fmaxf(x, 0.f); }  // 
 // whose run holds sample_u * total walks it once more. Sums are in 64 bits: 128k binary32 terms in
 // 32 would move the drawn token. VEC: 16-byte aligned rows.
 template <bool VEC>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyParams p) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyParams p) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank(), s = blockIdx.x / kVerifyCluster;
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), s = blockIdx.x / C;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int NW = kVerifyThreads / 32;
     __shared__ int s_acc;
@@ -235,7 +222,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
         return (unsigned)v == hole ? 0.0 : (double)prob_in(a);
     };
     // warp w of CTA r: run r * NW + w, a multiple of four elements long
-    const int run_len = ((p.vocab + kVerifyCluster * NW - 1) / (kVerifyCluster * NW) + 3) & ~3;
+    const int run_len = ((p.vocab + C * NW - 1) / (C * NW) + 3) & ~3;
     const long long first = (long long)(rank * NW + warp) * run_len;
     const int v0 = (int)min((long long)p.vocab, first), v1 = min(p.vocab, v0 + run_len);
     auto four = [&](const float* src, int i, float (&x)[4]) {  // elements i.. of the run, zeros past its end
@@ -250,7 +237,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
     int owner = -1;
     for (int pass = 0; pass < 2; ++pass) {
         double a = 0.0;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = v0 + lane * 4; i < v1; i += 128) {
             float x[4], q[4] = {};
             four(P, i, x);
@@ -269,18 +256,18 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyPara
             if (lane == 0) s_sum[pass] = t;
         }
         cluster.sync();
-        double part[kVerifyCluster];
+        double part[kVerifyMaxCluster];
         total = 0.0;
 #pragma unroll
-        for (int j = 0; j < kVerifyCluster; ++j) part[j] = *cluster.map_shared_rank(&s_sum[pass], j);
+        for (int j = 0; j < kVerifyMaxCluster; ++j) part[j] = j < C ? *cluster.map_shared_rank(&s_sum[pass], j) : 0.0;
 #pragma unroll
-        for (int j = 0; j < kVerifyCluster; ++j) total += part[j];
+        for (int j = 0; j < kVerifyMaxCluster; ++j) total += part[j];
         if (total > 0.0 || mode == 0) {
             const double t = (double)p.sample_u[s] * total;
             double run = 0.0, last_before = 0.0;
             int last = -1;
 #pragma unroll
-            for (int j = 0; j < kVerifyCluster; ++j) {
+            for (int j = 0; j < kVerifyMaxCluster; ++j) {
                 if (owner < 0 && part[j] > 0.0) {
                     last = j;
                     last_before = run;
