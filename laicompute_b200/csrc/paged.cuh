@@ -11,7 +11,7 @@
 
 namespace laic {
 
-enum : int { kKvBadSeq = 1, kKvBadPos = 2, kKvBadPage = 4, kKvBadGroup = 8 };
+enum : int { kKvBadSeq = 1, kKvBadPos = 2, kKvBadPage = 4, kKvBadGroup = 8, kKvWait = 16 };
 
 __host__ __device__ inline void kv_flag(int* err, int bits) {
 #ifdef __CUDA_ARCH__

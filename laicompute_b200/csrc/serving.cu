@@ -10,6 +10,7 @@
 #include "launch.cuh"
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "paged_bulk.cuh"
 #include "verify.cuh"
 
 namespace laic {
@@ -98,10 +99,14 @@ struct AttnPlan {
     int nt = 1;            // column tiles of 8 of a shared item
     int lp = 64, nsp = 1;  // private splits
     int ls = 64, nss = 0, ctiles = 0;
-    int shared_items = 0, private_items = 0;
+    int lb = 64, nbs = 0, pairs = 0;  // bulk splits of the shared part
+    int shared_items = 0, private_items = 0, bulk_items = 0;
     bool direct = false;
     size_t ml_off = 0, bytes = 0;
 };
+
+// A group goes to the bulk kernel from this many columns (query rows x heads per kv head) and shared positions on.
+constexpr int kBulkMinCols = 48, kBulkMinShared = 256;
 
 int round_up(long long v, int m) { return (int)((v + m - 1) / m * m); }
 
@@ -141,6 +146,18 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
         pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared);
         pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
         if (!max_private) pl.nsp = 1;
+        const long long pool_rows = (long long)g.num_pages * g.kv_heads * g.page_size;
+        if (g.head_dim >= 64 && cols >= kBulkMinCols && a.max_shared >= kBulkMinShared && pool_rows <= INT_MAX) {
+            // about one item per SM (a bulk CTA fills one), in whole tiles
+            pl.pairs = (cols + kBulkCols - 1) / kBulkCols;
+            const int tile = bulk_keys(a.type == LAIC_GGML_F32);
+            const long long sets = (long long)a.groups * pl.pairs * g.kv_heads;
+            const int splits = (int)std::max<long long>(1, device_sms(g.device) / sets);
+            pl.lb = std::min(kBulkMaxSplit, std::max(2 * tile, round_up((a.max_shared + splits - 1) / splits, tile)));
+            pl.nbs = (a.max_shared + pl.lb - 1) / pl.lb;
+            if (sets * pl.nbs > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
+            pl.bulk_items = (int)(sets * pl.nbs);
+        }
     }
     const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss;
     const long long pi = (long long)a.rows * g.kv_heads * pl.nsp;
@@ -149,7 +166,7 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
     pl.private_items = (int)pi;
     pl.direct = pl.nss == 0 && pl.nsp == 1;
     if (!pl.direct) {
-        const size_t parts = (size_t)a.rows * a.heads * (pl.nss + pl.nsp);
+        const size_t parts = (size_t)a.rows * a.heads * (pl.nbs + pl.nss + pl.nsp);
         pl.ml_off = parts * g.head_dim * 4;
         pl.bytes = pl.ml_off + parts * 8;
     }
@@ -171,6 +188,37 @@ PaFn pm_fn(int D) {
     return D == 32 ? paged_merge_kernel<32, T> : D == 64 ? paged_merge_kernel<64, T> : paged_merge_kernel<128, T>;
 }
 
+using BulkFn = void (*)(KvAttnParams, CUtensorMap, CUtensorMap);
+BulkFn bulk_pick(int D, bool f32) {
+    if (D == 64) return f32 ? paged_bulk_kernel<64, float> : paged_bulk_kernel<64, __half>;
+    return f32 ? paged_bulk_kernel<128, float> : paged_bulk_kernel<128, __half>;
+}
+
+using EncodeFn = decltype(&cuTensorMapEncodeTiled);
+EncodeFn tensor_map_encode() {
+    static std::atomic<EncodeFn> fn{nullptr};
+    EncodeFn f = fn.load();
+    if (!f) {
+        void* at = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &at, cudaEnableDefault, &found) == cudaSuccess &&
+            found == cudaDriverEntryPointSuccess)
+            fn.store(f = reinterpret_cast<EncodeFn>(at));
+    }
+    return f;
+}
+// One pool as rows of head_dim binary16 values; a box is 64 columns (x 0 or 64: whole 128-byte lines) of
+// up to a page's positions, so it never leaves a (page, head) run.
+bool encode_pages(const laic_kv_pages& g, void* pool, int tile, CUtensorMap* map) {
+    const EncodeFn f = tensor_map_encode();
+    if (!f) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_pages * g.kv_heads * g.page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)g.head_dim * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)std::min(g.page_size, tile)}, step[2] = {1, 1};
+    return f(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 cudaError_t serving_set_attributes() {
@@ -186,6 +234,11 @@ cudaError_t serving_set_attributes() {
                                          (int)pa_smem(D, nt, type == LAIC_GGML_F32));
                 if (e != cudaSuccess) return e;
             }
+    for (int D : {64, 128})
+        for (bool f32 : {false, true}) {
+            e = cudaFuncSetAttribute(bulk_pick(D, f32), cudaFuncAttributeMaxDynamicSharedMemorySize, bulk_smem(D, f32));
+            if (e != cudaSuccess) return e;
+        }
     for (auto fn : {probs_kernel<true, true>, probs_kernel<true, false>}) {
         e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (kProbsSlice + 8) * 4);
         if (e != cudaSuccess) return e;
@@ -200,6 +253,7 @@ std::string kv_error_text(int bits) {
     if (bits & LAIC_KV_BAD_POS) s += " position or length beyond its bound;";
     if (bits & LAIC_KV_BAD_PAGE) s += " page id out of range;";
     if (bits & LAIC_KV_BAD_GROUP) s += " group rows out of order or above their bound;";
+    if (bits & kKvWait) s += " a device wait timed out;";
     s.pop_back();
     return s;
 }
@@ -292,6 +346,8 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     p.scale_log2 = scale * 1.44269504f;
     p.lp = pl.lp; p.nsp = pl.nsp; p.ls = pl.ls; p.nss = pl.nss; p.ctiles = pl.ctiles; p.shared_items = pl.shared_items;
     p.direct = pl.direct;
+    p.lb = pl.lb; p.nbs = pl.nbs; p.pairs = pl.pairs; p.bulk_tile = bulk_keys(a.type == LAIC_GGML_F32);
+    p.q_vec = aligned16(a.q_dev) && (a.rows == 1 || a.ldq * type_size(a.type) % 16 == 0);
     if (!pl.direct) {
         p.part_o = static_cast<float*>(a.workspace_dev);
         p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace_dev) + pl.ml_off);
@@ -300,9 +356,16 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     const bool f32 = a.type == LAIC_GGML_F32;
     return on_device(g.device, [&]() -> int {
         cudaError_t e = serving_set_attributes();
+        if (e == cudaSuccess && pl.bulk_items) {
+            CUtensorMap mk, mv;
+            if (!encode_pages(g, g.k_dev, p.bulk_tile, &mk) || !encode_pages(g, g.v_dev, p.bulk_tile, &mv))
+                return api_fail(LAIC_E_CUDA, "kv_attention: tensor map");
+            e = launch_k(bulk_pick(g.head_dim, f32), dim3(pl.bulk_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32), st,
+                         false, p, mk, mv);
+        }
         if (e == cudaSuccess)
             e = launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(pl.shared_items + pl.private_items), dim3(kPaWarps * 32),
-                         pa_smem(g.head_dim, pl.nt, f32), st, false, p);
+                         pa_smem(g.head_dim, pl.nt, f32), st, pl.bulk_items > 0, p);
         if (e == cudaSuccess && !pl.direct)
             e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
                          dim3((unsigned)(((long long)a.rows * a.heads + kPmWarps - 1) / kPmWarps)), dim3(kPmWarps * 32), 0,

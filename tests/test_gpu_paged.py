@@ -239,6 +239,66 @@ def test_attention_shared_prefix(heads, hkv, d, nrows, shared, page, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("heads,hkv,d,nrows,shared,page", [
+    (8, 2, 128, 12, 256, 16), (8, 2, 128, 12, 300, 64), (8, 2, 64, 40, 700, 16), (8, 1, 128, 33, 1111, 256),
+    (9, 3, 64, 90, 520, 32), (2, 2, 64, 130, 640, 128), (8, 1, 64, 70, 2500, 64), (4, 1, 128, 65, 2048, 32)])
+def test_attention_wide_groups(heads, hkv, d, nrows, shared, page, dtype):
+    """Groups of many columns behind long prefixes (whole tiles of theirs go to the tensor-memory kernel), one
+    or two column pairs, partly filled ones, and rows that see less, nothing, or are padding."""
+    rng = random.Random(shared)
+    lens = [shared + rng.randint(0, 70) for _ in range(nrows)] + [shared // 2 + 20] * (nrows // 2 + 3) + [17]
+    groups = ([0, nrows, nrows + nrows // 2 + 3], [shared, shared // 2])
+    cache = Cache(lens, hkv, d, page, seed=shared, shared=[(list(range(nrows)), shared),
+                                                           (list(range(nrows, len(lens) - 1)), shared // 2)])
+    q = _q(len(lens), heads, d, dtype, seed=nrows)
+    rows = list(range(0, len(lens), 5)) + [nrows - 1, nrows, len(lens) - 2, len(lens) - 1]  # checked in 64 bits
+    out = attend(cache, q, lens, groups=groups)
+    cache.pages().check()
+    ref, tol = reference(cache, q[rows], [lens[r] for r in rows], rows)
+    close(out[rows], ref, tol)
+    plain = attend(cache, q, lens)
+    assert (out.double() - plain.double()).abs().max() <= 2 * tol.max()
+    short = list(lens)
+    short[1], short[2], short[nrows - 1], short[nrows] = shared - 3, 0, -1, 5
+    out = attend(cache, q, short, groups=groups)
+    cache.pages().check()
+    rows = [r for r in rows + [1, nrows] if short[r] > 0]
+    ref, tol = reference(cache, q[rows], [short[r] for r in rows], rows)
+    close(out[rows], ref, tol)
+    assert not out[2].any() and torch.all(out[nrows - 1] == 7.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("heads,hkv,d,start,nrows,page", [(8, 2, 128, 400, 150, 64), (9, 3, 64, 900, 100, 16),
+                                                          (8, 1, 64, 0, 400, 128), (8, 2, 128, 2000, 16, 32)])
+def test_attention_prompt_rows(heads, hkv, d, start, nrows, page, dtype):
+    """A prompt's rows behind cached ones: whole tiles seen by all rows of a column pair, causal edges beyond."""
+    total = start + nrows
+    cache = Cache([total], hkv, d, page, seed=nrows)
+    lens = [start + j + 1 for j in range(nrows)]
+    q = _q(nrows, heads, d, dtype, seed=start + 2)
+    buf = torch.zeros(nrows, heads * d + 3, dtype=q.dtype, device="cuda")  # rows that are not 16-byte aligned
+    buf[:, 1:heads * d + 1] = q
+    rows = sorted({0, 1, nrows // 3, nrows // 2, nrows - 2, nrows - 1})
+    ref, tol = reference(cache, q[rows], [lens[r] for r in rows], [0] * len(rows))
+    for x in (q, buf[:, 1:heads * d + 1]):
+        out = attend(cache, x, lens, seqs=[0] * nrows, groups=([0, nrows], [total]))
+        cache.pages().check()
+        close(out[rows], ref, tol)
+
+
+@pytest.mark.parametrize("scale", [-0.05, 1e-30, 3.0])
+def test_attention_wide_group_scales(scale):
+    """Negative, vanishing and large scales (maxima that outgrow their reference again and again)."""
+    cache = Cache([1000] * 20, 1, 64, 64, seed=4, shared=[(list(range(20)), 1000)])
+    q = _q(20, 4, 64, F32, seed=3)
+    out = attend(cache, q, [1000] * 20, groups=([0, 20], [1000]), scale=scale)
+    rows = [0, 7, 19]
+    ref, tol = reference(cache, q[rows], [1000] * 3, rows, scale=scale)
+    close(out[rows], ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
 def test_attention_rows_shorter_than_their_prefix(dtype):
     """Rows that see less than the shared positions, nothing, or are padding."""
     lens = [300, 10, 0, 150, -1, 129, 1]
