@@ -42,10 +42,9 @@ struct KvAttnParams {
     int lp, nsp;                  // private splits: positions each, count
     int ls, nss, ctiles;          // shared splits, column tiles per group
     int shared_items;
-    int lb, nbs, pairs, bulk_tile; // bulk splits (paged_bulk.cuh; nbs 0: none), column pairs per group, keys per tile
     bool q_vec;                   // rows of q are 16-byte aligned
-    float* part_o;                // [rows][heads][nbs + nss + nsp][head_dim]
-    float2* part_ml;              // [rows][heads][nbs + nss + nsp] (m, l)
+    float* part_o;                // [rows][heads][nss + nsp][head_dim]
+    float2* part_ml;              // [rows][heads][nss + nsp] (m, l)
     int direct;                   // one item per row: it writes the output
     int* err;
 };
@@ -111,51 +110,35 @@ __host__ __device__ inline bool group_rows(const KvAttnParams& p, int g, int& r0
     }
     return true;
 }
-// Shared positions of group g: none where its rows are refused or its first row names no sequence.
-__host__ __device__ inline int group_shared(const KvAttnParams& p, int g, int r0) {
-    if (row_seq(p, r0) < 0) return 0;
+// Shared positions of group g.
+__host__ __device__ inline int group_shared(const KvAttnParams& p, int g) {
     const int n = kv_clamp_len(p, p.group_len[g], p.max_shared);
     return n > 0 ? n : 0;
 }
-// The group of row r: `n` threads tid of one sync domain search together and leave it in *found
-// (shared reset to 0 before, synchronised after, by the caller).
-struct GroupView {
-    int shared, r0, r1;
-};
-__device__ __forceinline__ void find_group(const KvAttnParams& p, int r, int tid, int n, GroupView* found) {
+// The shared length of row r's group: `n` threads tid of one sync domain search together and leave it
+// in *found (reset to 0 before, synchronised after, by the caller).
+__device__ __forceinline__ void find_group(const KvAttnParams& p, int r, int tid, int n, int* found) {
     for (int g = tid; g < p.groups; g += n) {
         int r0, r1;
-        if (group_rows(p, g, r0, r1) && r >= r0 && r < r1) *found = GroupView{group_shared(p, g, r0), r0, r1};
+        if (group_rows(p, g, r0, r1) && r >= r0 && r < r1) *found = group_shared(p, g);
     }
 }
 __host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int shared) {
     RowView v;
-    v.n = p.len[r];
+    const int n = p.len[r], s = p.seq ? p.seq[r] : r;  // (both loads at once)
+    v.n = -1;
     v.seq = -1;
     v.shared = 0;
-    if (v.n < 0) {
-        v.n = -1;
-        return v;
+    if (n < 0) return v;
+    v.n = kv_clamp_len(p, n, p.max_len);
+    if (s >= 0 && s < p.nseq) {
+        v.seq = s;
+    } else {
+        kv_flag(p.err, kKvBadSeq);
+        v.n = 0;
     }
-    v.n = kv_clamp_len(p, v.n, p.max_len);
-    v.seq = row_seq(p, r);
-    if (v.seq < 0) v.n = 0;
     v.shared = v.n < shared ? v.n : shared;
     return v;
-}
-
-constexpr int kBulkCols = 256;  // columns of a bulk item (paged_bulk.cuh): a pair of tiles
-
-// Shared positions that the bulk items of a column pair take: every row of the pair's columns sees
-// them (rows that see nothing do not count), in whole tiles. The lanes of a warp search together.
-__device__ __forceinline__ int pair_bulk(const KvAttnParams& p, int r0, int r1, int pair, int shared, int lane) {
-    const int ncol = (r1 - r0) * p.G, ca = pair * kBulkCols, cb = min(ncol, ca + kBulkCols);
-    int mn = shared;
-    for (int r = r0 + ca / p.G + lane; r <= r0 + (cb - 1) / p.G; r += 32) {
-        const RowView v = row_view(p, r, shared);
-        if (v.n > 0) mn = min(mn, v.shared);
-    }
-    return __reduce_min_sync(0xffffffffu, mn) / p.bulk_tile * p.bulk_tile;
 }
 
 template <typename T>
@@ -440,7 +423,7 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             }
     }
     __syncthreads();
-    const int ns = p.nbs + p.nss + p.nsp;
+    const int ns = p.nss + p.nsp;
     for (int i = tid; i < NC * (D / 4); i += NTH) {
         const int col = i / (D / 4), d = (i % (D / 4)) * 4, cc = col0 + col;
         if (cc >= ncol) continue;
@@ -474,18 +457,18 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
 
 // One row's own positions: item i of [row][kv head][split].
 template <int D, typename T>
-__device__ __forceinline__ void private_item(const KvAttnParams& p, int i, int* lim, int* page_ids, float* cmul, GroupView* found,
+__device__ __forceinline__ void private_item(const KvAttnParams& p, int i, int* lim, int* page_ids, float* cmul, int* found,
                                              uint8_t* smem) {
     const int tid = threadIdx.x, split = i % p.nsp;
     i /= p.nsp;
     const int kvh = i % p.kv_heads, r = i / p.kv_heads;
     int shared = 0;
     if (p.groups) {
-        if (tid == 0) found->shared = 0;
+        if (tid == 0) *found = 0;
         __syncthreads();
         find_group(p, r, tid, kPaWarps * 32, found);
         __syncthreads();
-        shared = found->shared;
+        shared = *found;
     }
     const RowView v = row_view(p, r, shared);
     if (v.n < 0) return;
@@ -499,7 +482,7 @@ __device__ __forceinline__ void private_item(const KvAttnParams& p, int i, int* 
         return;
     }
     if (tid < 8) lim[tid] = tid < p.G ? t1 : 0;
-    const int slot = p.nbs + p.nss + split;
+    const int slot = p.nss + split;
     if constexpr (sizeof(T) == 4) {
         if (p.G <= 4) {
             pa_item<D, 1, T, true>(p, r, 0, p.G, kvh, v.seq, t0, t1, slot, lim, t1, page_ids, cmul, smem);
@@ -509,7 +492,7 @@ __device__ __forceinline__ void private_item(const KvAttnParams& p, int i, int* 
     pa_item<D, 1, T, false>(p, r, 0, p.G, kvh, v.seq, t0, t1, slot, lim, t1, page_ids, cmul, smem);
 }
 
-// One tile of a group's columns over a split of the shared positions the bulk items leave:
+// One tile of a group's columns over a split of the shared positions:
 // item i of [group][column tile][kv head][split].
 template <int D, int NT, typename T>
 __device__ __forceinline__ void shared_item(const KvAttnParams& p, int i, int* lim, int* page_ids, float* cmul, int* range,
@@ -523,9 +506,8 @@ __device__ __forceinline__ void shared_item(const KvAttnParams& p, int i, int* l
     if (!group_rows(p, g, r0, r1)) return;
     const int col0 = ct * NT * 8, ncol = (r1 - r0) * p.G;
     if (col0 >= ncol) return;
-    const int shared = group_shared(p, g, r0);
+    const int shared = group_shared(p, g);
     if (tid < 32) {
-        const int from = p.nbs ? pair_bulk(p, r0, r1, col0 / kBulkCols, shared, tid) : 0;
         int n = 0;
         if (tid < NT * 8) {
             const int col = col0 + tid;
@@ -534,21 +516,22 @@ __device__ __forceinline__ void shared_item(const KvAttnParams& p, int i, int* l
         }
         const int mx = __reduce_max_sync(0xffffffffu, n);
         const int mn = __reduce_min_sync(0xffffffffu, tid < NT * 8 && col0 + tid < ncol ? n : 0x7fffffff);
-        if (tid == 0) { range[0] = from; range[1] = mx; range[2] = mn; }
+        if (tid == 0) { range[0] = mx; range[1] = mn; }
     }
     __syncthreads();
-    const int t0 = range[0] + split * p.ls, t1 = min(range[1], t0 + p.ls);
+    const int t0 = split * p.ls, t1 = min(range[0], t0 + p.ls);
     if (t0 >= t1) return;  // no row of the tile sees this far
-    pa_item<D, NT, T, false>(p, r0, col0, ncol, kvh, row_seq(p, r0), t0, t1, p.nbs + split, lim, range[2], page_ids, cmul, smem);
+    const int seq = max(0, row_seq(p, r0));  // (a bad one is recorded, and reads some sequence's pages)
+    pa_item<D, NT, T, false>(p, r0, col0, ncol, kvh, seq, t0, t1, split, lim, range[1], page_ids, cmul, smem);
 }
 
 // Grid: the shared items, then the private ones.
 template <int D, int NT, typename T>
 __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const KvAttnParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int lim[NT * 8], page_ids[kPaMaxSplit / 16 + 2], range[3];
+    __shared__ int lim[NT * 8], page_ids[kPaMaxSplit / 16 + 2], range[2];
     __shared__ float cmul[NT * 8];
-    __shared__ GroupView found;
+    __shared__ int found;
     const int i = blockIdx.x;
     if (i < p.shared_items) shared_item<D, NT, T>(p, i, lim, page_ids, cmul, range, smem);
     else private_item<D, T>(p, i - p.shared_items, lim, page_ids, cmul, &found, smem);
@@ -561,29 +544,25 @@ constexpr int kPmWarps = 4;
 template <int D, typename T>
 __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttnParams p) {
     constexpr int E = D / 32;
-    __shared__ GroupView found[kPmWarps];
+    __shared__ int found[kPmWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int pair = blockIdx.x * kPmWarps + warp;
     const bool in = pair < p.rows * p.heads;
     const int r = in ? pair / p.heads : 0, h = in ? pair % p.heads : 0;
-    if (lane == 0) found[warp] = GroupView{0, 0, 0};
+    if (lane == 0) found[warp] = 0;
     __syncwarp();
     find_group(p, r, lane, 32, &found[warp]);
     __syncwarp();
-    const GroupView gv = found[warp];
-    const RowView v = row_view(p, r, gv.shared);
-    int bulk = 0;
-    if (p.nbs && v.shared > 0)
-        bulk = pair_bulk(p, gv.r0, gv.r1, ((r - gv.r0) * p.G + h % p.G) / kBulkCols, gv.shared, lane);
+    const RowView v = row_view(p, r, found[warp]);
     pdl_wait();
     if (!in || v.n < 0) return;
-    const int ns = p.nbs + p.nss + p.nsp;
+    const int ns = p.nss + p.nsp;
     const int priv = min(v.n - v.shared, p.max_private);
-    const int live_b = bulk > 0 ? (bulk + p.lb - 1) / p.lb : 0;
-    const int live_s = live_b + (v.shared > bulk ? (v.shared - bulk + p.ls - 1) / p.ls : 0);
+    if (v.n - v.shared > p.max_private && lane == 0) kv_flag(p.err, kKvBadPos);
+    const int live_s = v.shared > 0 ? (v.shared + p.ls - 1) / p.ls : 0;
     const int live = live_s + (priv > 0 ? (priv + p.lp - 1) / p.lp : 0);
     const size_t base = (size_t)pair * ns;
-    auto slot = [&](int i) { return i < live_b ? i : i < live_s ? p.nbs + (i - live_b) : p.nbs + p.nss + (i - live_s); };
+    auto slot = [&](int i) { return i < live_s ? i : p.nss + (i - live_s); };
     float M = -INFINITY;
     for (int i = lane; i < live; i += 32) M = fmaxf(M, p.part_ml[base + slot(i)].x);
     M = warp_max(M);

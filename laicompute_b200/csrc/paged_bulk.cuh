@@ -1,9 +1,8 @@
-// The bulk of a shared prefix on the 5th-generation tensor cores.
+// Shared positions of wide groups on the 5th-generation tensor cores.
 //
 // A group with many columns (rows x query heads of one KV head) makes its attention a pair of dense
-// products: S = Q K^T and O += P V over 256 columns per CTA, two tiles of M = 128. Only positions
-// that every column of the CTA sees come here, in whole tiles of kBulkKeys, so no mask enters; the
-// rest of each column's positions is left to the items of paged_attn.cuh, and the merge joins all.
+// products: S = Q K^T and O += P V over 256 columns per CTA, two tiles of M = 128, and a split of the
+// group's positions in tiles of bulk_keys.
 //
 // Roles: warp 8 loads (one lane: TMA boxes of up to a page, 128-byte swizzle, a ring of K + V
 // stages); warp 9 multiplies (one lane: tcgen05.mma, S and O in tensor memory, P read from tensor
@@ -12,6 +11,11 @@
 // one tile's products run under the other's exponentials. O is rescaled only when a maximum grew by
 // more than 2^8 since the last time (weights stay below 2^15 in binary16 with the factor 2^7 they
 // carry); both tiles' accumulators fill the 512 columns of tensor memory.
+//
+// Tiles that some column does not see to their end are masked. There 0 * V must not be 0 * inf: the
+// softmax threads clear what is not finite in V before the product (all of it past the positions any
+// column sees), note the positions, and the columns that do see one take its infinities and NaN at
+// the end.
 //
 // FP32 rows: Q as binary16 hi + lo after a scaling by a power of two, P likewise, the lo products
 // first (the accumulators then start from small terms), 64 keys per tile; binary16 rows: one product
@@ -23,6 +27,7 @@
 
 namespace laic {
 
+constexpr int kBulkCols = 256;        // score columns of a CTA
 constexpr int kBulkThreads = 320;
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
 constexpr float kBulkSlack = 8.f;     // log2 of how far a maximum may outgrow its reference
@@ -83,6 +88,12 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* r) {
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                  "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // The values of a tc_ld32 once tc_wait_ld has returned: uses of them cannot move above this.
 __device__ __forceinline__ void tc_loaded(uint32_t* r) {
@@ -118,7 +129,30 @@ __device__ __forceinline__ bool bulk_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
-// Grid [group][pair][kv head][split].
+// Packed pairs of FP32 operations.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Grid [group][pair of column tiles][kv head][split].
 template <int D, typename T>
 __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAttnParams p, const __grid_constant__ CUtensorMap mk,
                                                                      const __grid_constant__ CUtensorMap mv) {
@@ -133,104 +167,117 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     __shared__ uint64_t kv_full[NS], kv_free[NS], s_full[2], p_ready[2], o_done;
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;
-    __shared__ int s_bulk;
+    __shared__ int lim_max, lim_min;
+    __shared__ float cmul[kBulkCols];
+    __shared__ uint32_t odd[kBulkMaxSplit / 32];  // positions of the split whose V was not finite in a masked tile
+    __shared__ int any_odd;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     int i = blockIdx.x;
-    const int split = i % p.nbs;
-    i /= p.nbs;
+    const int split = i % p.nss;
+    i /= p.nss;
     const int kvh = i % p.kv_heads;
     i /= p.kv_heads;
-    const int pair = i % p.pairs, g = i / p.pairs;
+    const int pair = i % p.ctiles, g = i / p.ctiles;
     int r0, r1;
+    const int glen = p.group_len[g];
     if (!group_rows(p, g, r0, r1)) return;
     const int ncol = (r1 - r0) * p.G, col0 = pair * kBulkCols;
     if (col0 >= ncol) return;
-    if (warp == 0) {
-        const int n = pair_bulk(p, r0, r1, pair, group_shared(p, g, r0), lane);
-        if (lane == 0) s_bulk = n;
-    }
-    if (tid == 0) dead = 0;
-    __syncthreads();
-    const int t0 = split * p.lb, t1 = min(s_bulk, t0 + p.lb);
-    if (t0 >= t1) return;
-    const int seq = row_seq(p, r0);
-    const int nt = (t1 - t0) / NK;
+    const int t0 = split * p.ls;
+    const int shared = max(0, kv_clamp_len(p, glen, p.max_shared));
+    if (t0 >= shared) return;
     const int tiles = ncol - col0 > 128 ? 2 : 1;  // M tiles with columns
 
-    // ---- set-up: page ids, barriers, tensor memory, Q
-    const int first_page = t0 >> p.page_shift, npages = ((t1 - 1) >> p.page_shift) - first_page + 1;
-    for (int k = tid; k < npages; k += kBulkThreads) {
-        int id = p.table[(size_t)seq * p.pages_per_seq + first_page + k];
-        if (id < 0 || id >= p.num_pages) {
-            kv_flag(p.err, kKvBadPage);
-            id = 0;
+    // ---- a softmax thread's column and how far it sees
+    const int wg = warp >> 2, col = col0 + tid;
+    const bool live = tid < kBulkCols && col < ncol;
+    const int rr = r0 + (live ? col / p.G : 0), hh = kvh * p.G + (live ? col % p.G : 0);
+    const RowView view = row_view(p, rr, shared);
+    const int lim = live ? max(0, view.shared) : 0;
+    int seq = row_seq(p, r0);
+    if (seq < 0) seq = 0;  // (recorded) reads some sequence's pages
+    const int first_page = t0 >> p.page_shift;
+    const int npages = min(((t0 + p.ls - 1) >> p.page_shift) + 1, p.pages_per_seq) - first_page;
+    for (int k = tid; k < npages; k += kBulkThreads) page_ids[k] = p.table[(size_t)seq * p.pages_per_seq + first_page + k];
+
+    // ---- Q: a warp takes 32 columns, a lane four elements of one, with 128-byte swizzled rows
+    if (warp < 4 * tiles) {
+        constexpr int LPR = D / 4, RPI = 32 / LPR;  // lanes per row, rows per step
+        const int sub = lane / LPR, e0 = (lane % LPR) * 4;
+        const float sgn = p.scale_log2 < 0.f ? -1.f : 1.f;  // (the maximum is taken of S itself)
+#pragma unroll 8
+        for (int it = 0; it < 32 / RPI; ++it) {
+            const int cw = warp * 32 + it * RPI + sub, c = col0 + cw;  // column within the pair; of the group
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (c < ncol) {
+                const T* q = static_cast<const T*>(p.q) + (size_t)(r0 + c / p.G) * p.ldq + (size_t)(kvh * p.G + c % p.G) * D + e0;
+                if (p.q_vec) {
+                    if constexpr (F32) {
+                        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(q);
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(q);
+                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+                        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+                        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) x[k] = kv_in<T>(q[k]);
+                }
+            }
+            float fac = sgn, inv = 1.f;
+            if constexpr (F32) {
+                float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
+                fac = sgn * __uint_as_float((uint32_t)(127 - e) << 23);
+                inv = __uint_as_float((uint32_t)(127 + e) << 23);
+            }
+            if (e0 == 0) cmul[cw] = fabsf(p.scale_log2) * inv;
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float a = x[2 * k] * fac, b = x[2 * k + 1] * fac;
+                const __half ha = __float2half_rn(a), hb = __float2half_rn(b);
+                hi[k] = pack_h2(ha, hb);
+                lo[k] = pack_h2(__float2half_rn(a - __half2float(ha)), __float2half_rn(b - __half2float(hb)));
+            }
+            const int row = cw & 127, ch = e0 >> 3;
+            uint8_t* dst = base + (size_t)(cw >> 7) * HN * QPART + (ch >> 3) * (128 * 128) + row * 128 +
+                           (((ch & 7) ^ (row & 7)) << 4) + (e0 & 4) * 2;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+            if constexpr (F32) *reinterpret_cast<uint2*>(dst + QPART) = make_uint2(lo[0], lo[1]);
         }
-        page_ids[k] = id;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (tid == 0) {
         for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
         for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 1); mbar_init(&p_ready[w], 128); }
         mbar_init(&o_done, 1);
         mbar_fence_init();
+        dead = 0;
+        any_odd = 0;
+        lim_max = 0;
+        lim_min = 0x7fffffff;
     }
+    if (tid < kBulkMaxSplit / 32) odd[tid] = 0;
+    __syncthreads();
+    if (warp < 8) {  // (rows that see nothing do not keep the others' tiles from being whole)
+        const int hi = __reduce_max_sync(0xffffffffu, lim);
+        const int lo = __reduce_min_sync(0xffffffffu, lim > 0 ? lim : 0x7fffffff);
+        if (lane == 0) { atomicMax(&lim_max, hi); atomicMin(&lim_min, lo); }
+    }
+    __syncthreads();
+    const int t1 = min(lim_max, t0 + p.ls), seen_by_all = lim_min;
+    if (t0 >= t1) return;  // no column sees this far
+    const int nt = (t1 - t0 + NK - 1) / NK;
     if (warp == 9) tc_alloc(smem_u32(&tmem_at), 512);
-    const int wg = warp >> 2, row = tid & 127, col = col0 + tid;  // a softmax thread's column (tid < 256)
-    const bool live = tid < 256 && col < ncol;
-    const int rr = r0 + (live ? col / p.G : 0), hh = kvh * p.G + (live ? col % p.G : 0);
-    float cm = 0.f;
-    if (tid < 256 && wg < tiles) {
-        const T* q = static_cast<const T*>(p.q) + (size_t)rr * p.ldq + (size_t)hh * D;
-        uint8_t* qs = base + (size_t)wg * HN * QPART;
-        const float sgn = p.scale_log2 < 0.f ? -1.f : 1.f;  // (the maximum is taken of S itself)
-        float fac = sgn, inv = 1.f;
-        if constexpr (F32) {
-            float mx = 0.f;
-            for (int d = 0; live && d < D; d += 4) {
-                float4 x;
-                if (p.q_vec) x = *reinterpret_cast<const float4*>(q + d);
-                else x = make_float4(q[d], q[d + 1], q[d + 2], q[d + 3]);
-                mx = fmaxf(fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-            }
-            const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
-            fac = sgn * __uint_as_float((uint32_t)(127 - e) << 23);
-            inv = __uint_as_float((uint32_t)(127 + e) << 23);
-        }
-        cm = fabsf(p.scale_log2) * inv;
-#pragma unroll
-        for (int ch = 0; ch < D / 8; ++ch) {  // 16-byte chunks of the row
-            float x[8];
-            if (live) {
-                if (p.q_vec) {
-                    Raw8<T> raw;
-                    load8<T, true>(q + ch * 8, raw);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = raw.at(k) * fac;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[k] = kv_in<T>(q[ch * 8 + k]) * fac;
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = 0.f;
-            }
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const __half a = __float2half_rn(x[2 * k]), b = __float2half_rn(x[2 * k + 1]);
-                hi[k] = pack_h2(a, b);
-                lo[k] = pack_h2(__float2half_rn(x[2 * k] - __half2float(a)), __float2half_rn(x[2 * k + 1] - __half2float(b)));
-            }
-            const int at = (ch >> 3) * (128 * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
-            *reinterpret_cast<uint4*>(qs + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if constexpr (F32) *reinterpret_cast<uint4*>(qs + QPART + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    pdl_launch_dependents();  // the items kernel needs nothing of this one
+    pdl_launch_dependents();  // the private items need nothing of this kernel
     const uint32_t tmem = tmem_at;
     auto s_at = [&](int w) { return tmem + (uint32_t)(w * NK); };        // S, then P hi | P lo in its place
     auto o_at = [&](int w) { return tmem + 256u + (uint32_t)(w * D); };
@@ -246,8 +293,15 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 const uint32_t ks = smem_u32(stages) + (uint32_t)(s * STAGE);
                 for (int k = 0; k < NK; k += box) {
                     const int t = t0 + j * NK + k;
-                    const int y = ((page_ids[(t >> p.page_shift) - first_page] * p.kv_heads + kvh) << p.page_shift) +
-                                  (t & ((1 << p.page_shift) - 1));
+                    int id = 0;  // past the last position seen: any page (masked, and cleared in V)
+                    if (t < t1) {
+                        id = page_ids[(t >> p.page_shift) - first_page];
+                        if (id < 0 || id >= p.num_pages) {
+                            kv_flag(p.err, kKvBadPage);
+                            id = 0;
+                        }
+                    }
+                    const int y = ((id * p.kv_heads + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
 #pragma unroll
                     for (int h = 0; h < HALVES; ++h) {
                         tma_2d(ks + h * (NK * 128) + k * 128, &mk, h * 64, y, &kv_full[s]);
@@ -309,31 +363,48 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     } else if (wg < tiles) {
         const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
         const uint32_t S = s_at(wg) + lane_at, O = o_at(wg) + lane_at;
+        const float cm = cmul[tid];
+        const int wtid = tid & 127;
         float mref = 0.f, l = 0.f;
         bool ok = true;
         for (int j = 0; j < nt; ++j) {
+            const int c0 = t0 + j * NK;
+            const bool masked = c0 + NK > min(seen_by_all, t1);
             ok = __all_sync(0xffffffffu, bulk_wait(&s_full[wg], (uint32_t)j & 1, &dead, p.err));
             if (!ok) break;
             tc_fence_after();
-            uint32_t s[NK];
+            uint32_t s[2][32];
+            // ---- the maximum
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tc_ld32(S, s[0]);
 #pragma unroll
-            for (int k = 0; k < NK; k += 32) tc_ld32(S + k, s + k);
-            tc_wait_ld();
+            for (int k = 0; k < NK; k += 32) {
+                uint32_t* cur = s[(k >> 5) & 1];
+                tc_wait_ld();
+                tc_loaded(cur);
+                if (k + 32 < NK) tc_ld32(S + k + 32, s[((k >> 5) + 1) & 1]);
+                if (masked) {
 #pragma unroll
-            for (int k = 0; k < NK; k += 32) tc_loaded(s + k);
-            float mx = __uint_as_float(s[0]);
+                    for (int e = 0; e < 32; ++e)
+                        if (c0 + k + e < lim) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(cur[e]));
+                } else {
 #pragma unroll
-            for (int k = 1; k < NK; ++k) mx = fmaxf(mx, __uint_as_float(s[k]));
-            mx *= cm;
+                    for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(cur[e]));
+                }
+            }
+            tc_ld32(S, s[0]);
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * cm;
             if (j == 0) {
-                mref = mx == -INFINITY ? 0.f : mx;
+                mref = mx > -INFINITY ? mx : 0.f;
             } else if (__any_sync(0xffffffffu, mx > mref + kBulkSlack)) {
                 const float next = fmaxf(mref, mx), corr = ex2(mref - next);
                 mref = next;
                 l *= corr;
+                tc_wait_ld();
+                tc_loaded(s[0]);
 #pragma unroll 1
                 for (int k = 0; k < D; k += 32) {
-                    uint32_t o[32];
+                    uint32_t* o = s[1];
                     tc_ld32(O + k, o);
                     tc_wait_ld();
                     tc_loaded(o);
@@ -342,38 +413,81 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                     tc_st32(O + k, o);
                 }
             }
-            float sum0 = 0.f, sum1 = 0.f;
+            // ---- the weights: binary16 rows carry the factor in the exponent (their rounding is 2^-11 anyway)
+            const float shift = F32 ? -mref : 7.f - mref;
+            const uint64_t cm2 = f2_pack(cm, cm), sh2 = f2_pack(shift, shift), gain2 = f2_pack(kPaGain, kPaGain);
+            uint64_t sum2[2] = {0, 0};
+            uint32_t lo_keep[F32 ? NK / 2 : 1];
 #pragma unroll
-            for (int k = 0; k < NK; k += 64) {  // 64 positions: 32 words of hi, 32 of lo
-                uint32_t hi[32], lo[F32 ? 32 : 1];
+            for (int k = 0; k < NK; k += 32) {
+                uint32_t* cur = s[(k >> 5) & 1];
+                tc_wait_ld();
+                tc_loaded(cur);
+                if (k + 32 < NK) tc_ld32(S + k + 32, s[((k >> 5) + 1) & 1]);
+                uint32_t hi[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    float a = ex2(fmaf(__uint_as_float(s[k + 2 * e]), cm, -mref));
-                    float b = ex2(fmaf(__uint_as_float(s[k + 2 * e + 1]), cm, -mref));
-                    sum0 += a;
-                    sum1 += b;
-                    a *= kPaGain;
-                    b *= kPaGain;
+                for (int e = 0; e < 16; ++e) {
+                    float a, b;
+                    f2_unpack(f2_fma(f2_pack(__uint_as_float(cur[2 * e]), __uint_as_float(cur[2 * e + 1])), cm2, sh2), a, b);
+                    a = ex2(a);
+                    b = ex2(b);
+                    if (masked) {
+                        if (c0 + k + 2 * e >= lim) a = 0.f;
+                        if (c0 + k + 2 * e + 1 >= lim) b = 0.f;
+                    }
+                    uint64_t ab = f2_pack(a, b);
+                    sum2[e & 1] = f2_add(sum2[e & 1], ab);
+                    if constexpr (F32) {
+                        ab = f2_mul(ab, gain2);
+                        f2_unpack(ab, a, b);
+                    }
                     const __half2 h = __floats2half2_rn(a, b);
                     hi[e] = *reinterpret_cast<const uint32_t*>(&h);
                     if constexpr (F32) {
                         const float2 f = __half22float2(h);
                         const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
-                        lo[e] = *reinterpret_cast<const uint32_t*>(&r);
+                        lo_keep[k / 2 + e] = *reinterpret_cast<const uint32_t*>(&r);
                     }
                 }
-                tc_st32(S + k / 2, hi);
-                if constexpr (F32) tc_st32(S + NK / 2 + k / 2, lo);
+                tc_st16(S + k / 2, hi);  // (columns of S already read: k / 2 + 16 <= k + 32)
             }
-            l += sum0 + sum1;
+            if constexpr (F32) tc_st32(S + NK / 2, lo_keep);
+            float a, b;
+            f2_unpack(f2_add(sum2[0], sum2[1]), a, b);
+            l += a + b;
+            if (masked) {  // V where not every column sees: nothing but finite values may meet a zero weight
+                bulk_wait(&kv_full[j % NS], (uint32_t)(j / NS) & 1, &dead, p.err);
+                uint8_t* V = stages + (size_t)(j % NS) * STAGE + VOFF;
+                for (int k = wtid; k < NK * (D / 8); k += 128) {
+                    const int r = k / (D / 8), ch = k % (D / 8), t = c0 + r;
+                    if (t < seen_by_all && t < t1) continue;
+                    uint4* w = reinterpret_cast<uint4*>(V + (ch >> 3) * (NK * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                    uint4 x = *w;
+                    uint32_t* xs = reinterpret_cast<uint32_t*>(&x);
+                    bool bad = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if ((xs[e] & 0x7c00u) == 0x7c00u) { xs[e] &= 0xffff0000u; bad = true; }
+                        if ((xs[e] & 0x7c000000u) == 0x7c000000u) { xs[e] &= 0xffffu; bad = true; }
+                    }
+                    if (t >= t1) x = make_uint4(0, 0, 0, 0);
+                    if (t >= t1 || bad) *w = x;
+                    if (t < t1 && bad) {
+                        atomicOr(&odd[(t - t0) >> 5], 1u << ((t - t0) & 31));
+                        any_odd = 1;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
             tc_wait_st();
             tc_fence_before();
             mbar_arrive(&p_ready[wg]);
         }
         ok = __all_sync(0xffffffffu, bulk_wait(&o_done, 0, &dead, p.err)) && ok;
         tc_fence_after();
+        named_sync(1, 128 * tiles);  // both tiles' notes of odd positions (every softmax warp comes here)
         if (ok) {
-            const int ns = p.nbs + p.nss + p.nsp;
+            const int ns = p.nss + p.nsp;
             const size_t at = ((size_t)rr * p.heads + hh) * ns + split;
 #pragma unroll 1
             for (int k = 0; k < D; k += 32) {
@@ -381,13 +495,27 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 tc_ld32(O + k, o);
                 tc_wait_ld();
                 tc_loaded(o);
+                if (any_odd)
+                    for (int t = t0; t < min(t1, lim); ++t)
+                        if (odd[(t - t0) >> 5] >> ((t - t0) & 31) & 1) {
+                            int id = page_ids[(t >> p.page_shift) - first_page];
+                            if (id < 0 || id >= p.num_pages) id = 0;
+                            const __half* v = p.vp + (((((size_t)id * p.kv_heads + kvh) << p.page_shift) +
+                                                       (t & ((1 << p.page_shift) - 1))) * D + k);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float x = __half2float(v[e]);
+                                if (!(fabsf(x) <= 65504.f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                            }
+                        }
                 if (live) {
                     uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + k);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
             }
-            if (live) p.part_ml[at] = make_float2(mref, l * kPaGain);
+            // (l is zero only where the column saw nothing: its largest weight is at least 2^-8)
+            if (live) p.part_ml[at] = make_float2(l == 0.f ? -INFINITY : mref, F32 ? l * kPaGain : l);
         }
         tc_fence_before();
     }

@@ -99,8 +99,8 @@ struct AttnPlan {
     int nt = 1;            // column tiles of 8 of a shared item
     int lp = 64, nsp = 1;  // private splits
     int ls = 64, nss = 0, ctiles = 0;
-    int lb = 64, nbs = 0, pairs = 0;  // bulk splits of the shared part
-    int shared_items = 0, private_items = 0, bulk_items = 0;
+    int shared_items = 0, private_items = 0;
+    bool bulk = false;     // the shared items run in paged_bulk.cuh
     bool direct = false;
     size_t ml_off = 0, bytes = 0;
 };
@@ -140,33 +140,32 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
     pl.lp = split((long long)a.rows * g.kv_heads, max_private);
     pl.nsp = std::max(1, (max_private + pl.lp - 1) / pl.lp);
     if (a.groups) {
+        if (max_private == 0) pl.nsp = 0;
         const int cols = a.max_group_rows * G;
-        pl.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-        pl.ctiles = (cols + 8 * pl.nt - 1) / (8 * pl.nt);
-        pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared);
-        pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
-        if (!max_private) pl.nsp = 1;
         const long long pool_rows = (long long)g.num_pages * g.kv_heads * g.page_size;
-        if (g.head_dim >= 64 && cols >= kBulkMinCols && a.max_shared >= kBulkMinShared && pool_rows <= INT_MAX) {
+        pl.bulk = g.head_dim >= 64 && cols >= kBulkMinCols && a.max_shared >= kBulkMinShared && pool_rows <= INT_MAX;
+        if (pl.bulk) {
             // about one item per SM (a bulk CTA fills one), in whole tiles
-            pl.pairs = (cols + kBulkCols - 1) / kBulkCols;
+            pl.ctiles = (cols + kBulkCols - 1) / kBulkCols;
             const int tile = bulk_keys(a.type == LAIC_GGML_F32);
-            const long long sets = (long long)a.groups * pl.pairs * g.kv_heads;
+            const long long sets = (long long)a.groups * pl.ctiles * g.kv_heads;
             const int splits = (int)std::max<long long>(1, device_sms(g.device) / sets);
-            pl.lb = std::min(kBulkMaxSplit, std::max(2 * tile, round_up((a.max_shared + splits - 1) / splits, tile)));
-            pl.nbs = (a.max_shared + pl.lb - 1) / pl.lb;
-            if (sets * pl.nbs > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
-            pl.bulk_items = (int)(sets * pl.nbs);
+            pl.ls = std::min(kBulkMaxSplit, std::max(2 * tile, round_up((a.max_shared + splits - 1) / splits, tile)));
+        } else {
+            pl.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+            pl.ctiles = (cols + 8 * pl.nt - 1) / (8 * pl.nt);
+            pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared);
         }
+        pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
     }
     const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss;
     const long long pi = (long long)a.rows * g.kv_heads * pl.nsp;
     if (si + pi > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
     pl.shared_items = (int)si;
     pl.private_items = (int)pi;
-    pl.direct = pl.nss == 0 && pl.nsp == 1;
+    pl.direct = a.groups == 0 && pl.nsp == 1;
     if (!pl.direct) {
-        const size_t parts = (size_t)a.rows * a.heads * (pl.nbs + pl.nss + pl.nsp);
+        const size_t parts = (size_t)a.rows * a.heads * (pl.nss + pl.nsp);
         pl.ml_off = parts * g.head_dim * 4;
         pl.bytes = pl.ml_off + parts * 8;
     }
@@ -344,9 +343,9 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     p.group_rows = a.group_rows_dev; p.group_len = a.group_len_dev;
     const float scale = a.scale != 0.f ? a.scale : 1.f / sqrtf((float)g.head_dim);
     p.scale_log2 = scale * 1.44269504f;
-    p.lp = pl.lp; p.nsp = pl.nsp; p.ls = pl.ls; p.nss = pl.nss; p.ctiles = pl.ctiles; p.shared_items = pl.shared_items;
+    p.lp = pl.lp; p.nsp = pl.nsp; p.ls = pl.ls; p.nss = pl.nss; p.ctiles = pl.ctiles;
+    p.shared_items = pl.bulk ? 0 : pl.shared_items;
     p.direct = pl.direct;
-    p.lb = pl.lb; p.nbs = pl.nbs; p.pairs = pl.pairs; p.bulk_tile = bulk_keys(a.type == LAIC_GGML_F32);
     p.q_vec = aligned16(a.q_dev) && (a.rows == 1 || a.ldq * type_size(a.type) % 16 == 0);
     if (!pl.direct) {
         p.part_o = static_cast<float*>(a.workspace_dev);
@@ -356,20 +355,22 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     const bool f32 = a.type == LAIC_GGML_F32;
     return on_device(g.device, [&]() -> int {
         cudaError_t e = serving_set_attributes();
-        if (e == cudaSuccess && pl.bulk_items) {
+        if (e == cudaSuccess && pl.bulk && pl.shared_items) {
             CUtensorMap mk, mv;
-            if (!encode_pages(g, g.k_dev, p.bulk_tile, &mk) || !encode_pages(g, g.v_dev, p.bulk_tile, &mv))
+            if (!encode_pages(g, g.k_dev, bulk_keys(f32), &mk) || !encode_pages(g, g.v_dev, bulk_keys(f32), &mv))
                 return api_fail(LAIC_E_CUDA, "kv_attention: tensor map");
-            e = launch_k(bulk_pick(g.head_dim, f32), dim3(pl.bulk_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32), st,
+            e = launch_k(bulk_pick(g.head_dim, f32), dim3(pl.shared_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32), st,
                          false, p, mk, mv);
         }
-        if (e == cudaSuccess)
-            e = launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(pl.shared_items + pl.private_items), dim3(kPaWarps * 32),
-                         pa_smem(g.head_dim, pl.nt, f32), st, pl.bulk_items > 0, p);
+        const int items = p.shared_items + pl.private_items;
+        const bool before = pl.bulk && pl.shared_items;  // (a kernel of this call, which nothing earlier runs beside)
+        if (e == cudaSuccess && items)
+            e = launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(items), dim3(kPaWarps * 32),
+                         pa_smem(g.head_dim, pl.nt, f32), st, before, p);
         if (e == cudaSuccess && !pl.direct)
             e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
                          dim3((unsigned)(((long long)a.rows * a.heads + kPmWarps - 1) / kPmWarps)), dim3(kPmWarps * 32), 0,
-                         st, true, p);
+                         st, before || items, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "kv_attention");
     });
 }

@@ -48,7 +48,7 @@ int main() {
             p.group_rows = start.data(); p.group_len = len.data();
             int r0 = 0, r1 = 0;
             const bool ok = laic::group_rows(p, a[0], r0, r1);
-            const int sh = ok && r1 > r0 ? laic::group_shared(p, a[0], r0) : 0;
+            const int sh = ok && r1 > r0 ? laic::group_shared(p, a[0]) : 0;
             std::printf("%d %d %d %d %d\n", ok ? 1 : 0, r0, r1, sh, err);
         }
     }

@@ -107,6 +107,7 @@ def reference(cache, q, lens, seqs=None, scale=0.0):
     qd = q.double().cpu().view(len(lens), heads, d)
     out = torch.zeros(len(lens), heads, d, dtype=torch.float64)
     tol = torch.zeros(len(lens), heads, d, dtype=torch.float64)
+    asc = abs(sc)
     hs = HALF_STEP[F32 if q.dtype == torch.float32 else F16]
     for r, n in enumerate(lens):
         if n <= 0:
@@ -121,7 +122,7 @@ def reference(cache, q, lens, seqs=None, scale=0.0):
             # Score error: q to 2^-22 of its row's maximum; the FP32 sum of d products in d / 16 steps of
             # the tensor cores, which may truncate (2^-23 of the magnitudes each), taken as d / 8 roundings;
             # the scaling to base 2, the difference to the maximum and 2^x of it, 2^-22 relative each.
-            mag = (k.abs().sum(dim=1) * qd[r, h].abs().max()).max().item() * sc
+            mag = (k.abs().sum(dim=1) * qd[r, h].abs().max()).max().item() * asc
             ds = mag * (2.0 ** -22 + (d / 8) * 2.0 ** -23) + 3 * x.abs().max().item() * 2.0 ** -23
             # Weights relative to their sum: the score error twice (numerator and sum), the exponential, the
             # hi + lo split, and sums of n / 16 steps plus the joins of 4 warps and up to 64 items.

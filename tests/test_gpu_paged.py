@@ -327,12 +327,13 @@ def test_attention_causal_rows(heads, hkv, d, start, rows, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("heads,hkv,d,rows", [(4, 2, 64, 30), (32, 8, 128, 12), (2, 2, 32, 9), (8, 1, 128, 40)])
-def test_masked_infinities_stay_out(heads, hkv, d, rows, dtype):
+@pytest.mark.parametrize("heads,hkv,d,rows,start", [(4, 2, 64, 30, 150), (32, 8, 128, 12, 150), (2, 2, 32, 9, 150),
+                                                    (8, 1, 128, 40, 150), (8, 1, 128, 40, 300), (4, 1, 64, 80, 490)])
+def test_masked_infinities_stay_out(heads, hkv, d, rows, start, dtype):
     """Keys and values of a later row that are infinite or NaN reach only the rows that see them."""
-    total = 150 + rows
+    total = start + rows
     cache = Cache([total], hkv, d, 16, seed=2)
-    lens = [150 + j + 1 for j in range(rows)]
+    lens = [start + j + 1 for j in range(rows)]
     q = _q(rows, heads, d, dtype, seed=4)
     bad = total - 4  # position seen by the last four rows only
     p, off = cache.rows[0][bad // 16], bad % 16
