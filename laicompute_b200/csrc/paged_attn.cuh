@@ -43,6 +43,7 @@ struct KvAttnParams {
     int ls, nss, ctiles;          // shared splits, column tiles per group
     int shared_items;
     bool q_vec;                   // rows of q are 16-byte aligned
+    uint32_t g_inv;               // 2^16 / G rounded up
     float* part_o;                // [rows][heads][nss + nsp][head_dim]
     float2* part_ml;              // [rows][heads][nss + nsp] (m, l)
     int direct;                   // one item per row: it writes the output

@@ -4,13 +4,15 @@
 // products: S = Q K^T and O += P V over 256 columns per CTA, two tiles of M = 128, and a split of the
 // group's positions in tiles of bulk_keys.
 //
-// Roles: warp 8 loads (one lane: TMA boxes of up to a page, 128-byte swizzle, a ring of K + V
-// stages); warp 9 multiplies (one lane: tcgen05.mma, S and O in tensor memory, P read from tensor
-// memory, where it takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read
-// S, keep the running maximum and sum, and write P. The issue order PV(j), QK(j + 1) per tile lets
-// one tile's products run under the other's exponentials. O is rescaled only when a maximum grew by
-// more than 2^8 since the last time (weights stay below 2^15 in binary16 with the factor 2^7 they
-// carry); both tiles' accumulators fill the 512 columns of tensor memory.
+// Roles: warp 8 loads (TMA boxes of up to a page, 128-byte swizzle, a lane per box: one lane alone
+// took 125 cycles a box, 4,000 for a tile of 16-position pages; a ring of K + V stages); warp 9
+// multiplies (one lane: tcgen05.mma, S and O in tensor memory, P read from tensor memory, where it
+// takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S, keep the
+// running maximum and sum, and write P. S has two buffers per tile, and QK(j + 2) follows PV(j), so
+// the scores of the next positions are ready when a softmax warp turns to them; it waits for a
+// product only to rescale O, which it does when a maximum grew by more than 2^8 since the last time
+// (weights stay below 2^15 in binary16 with the factor 2^7 they carry). Both tiles' S and O fill the
+// 512 columns of tensor memory.
 //
 // Tiles that some column does not see to their end are masked. There 0 * V must not be 0 * inf: the
 // softmax threads clear what is not finite in V before the product (all of it past the positions any
@@ -18,8 +20,8 @@
 // the end.
 //
 // FP32 rows: Q as binary16 hi + lo after a scaling by a power of two, P likewise, the lo products
-// first (the accumulators then start from small terms), 64 keys per tile; binary16 rows: one product
-// each, P rounded to binary16, 128 keys per tile.
+// first (the accumulators then start from small terms); binary16 rows: one product each, P rounded to
+// binary16.
 #pragma once
 #include <cuda.h>
 
@@ -32,13 +34,16 @@ constexpr int kBulkThreads = 320;
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
 constexpr float kBulkSlack = 8.f;     // log2 of how far a maximum may outgrow its reference
 
-__host__ __device__ constexpr int bulk_keys(bool f32) { return f32 ? 64 : 128; }
-__host__ __device__ constexpr int bulk_stage_bytes(int D, bool f32) { return 2 * bulk_keys(f32) * D * 2; }
+constexpr int kBulkKeys = 64;         // positions per tile
+__host__ __device__ constexpr int bulk_stage_bytes(int D) { return 2 * kBulkKeys * D * 2; }
 __host__ __device__ constexpr int bulk_q_bytes(int D, bool f32) { return kBulkCols * D * 2 * (f32 ? 2 : 1); }
-__host__ __device__ constexpr int bulk_stages(int D, bool f32) { return D == 64 ? 4 : f32 ? 3 : 2; }
+// Stages: tile j's V, j + 1's and j + 2's K are in use at once; at the end the ring and Q hold O's rows.
+__host__ __device__ constexpr int bulk_stages(int D, bool f32) { return D == 128 && f32 ? 3 : 4; }
 __host__ __device__ constexpr int bulk_smem(int D, bool f32) {
-    return bulk_q_bytes(D, f32) + bulk_stages(D, f32) * bulk_stage_bytes(D, f32) + 1024;  // (aligned to 1024)
+    return bulk_q_bytes(D, f32) + bulk_stages(D, f32) * bulk_stage_bytes(D) + 1024;  // (aligned to 1024)
 }
+static_assert(bulk_smem(64, false) - 1024 >= kBulkCols * (64 + 4) * 4 && bulk_smem(128, false) - 1024 >= kBulkCols * (128 + 4) * 4,
+              "O's rows fit");
 
 // ---- PTX
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -87,6 +92,15 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* r) {
         "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+// 16 columns, waited for
+__device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                    "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr)
+                 : "memory");
 }
 __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -157,14 +171,14 @@ template <int D, typename T>
 __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAttnParams p, const __grid_constant__ CUtensorMap mk,
                                                                      const __grid_constant__ CUtensorMap mv) {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int HN = F32 ? 2 : 1, NK = bulk_keys(F32), NS = bulk_stages(D, F32), HALVES = D / 64;
-    constexpr int STAGE = bulk_stage_bytes(D, F32), VOFF = STAGE / 2;
+    constexpr int HN = F32 ? 2 : 1, NK = kBulkKeys, NS = bulk_stages(D, F32), HALVES = D / 64;
+    constexpr int STAGE = bulk_stage_bytes(D), VOFF = STAGE / 2;
     constexpr int QPART = 128 * D * 2;  // one tile's hi or lo part
     extern __shared__ uint8_t dyn[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
     uint8_t* stages = base + bulk_q_bytes(D, F32);
     __shared__ int page_ids[kBulkMaxSplit / 16 + 2];
-    __shared__ uint64_t kv_full[NS], kv_free[NS], s_full[2], p_ready[2], o_done;
+    __shared__ uint64_t kv_full[NS], kv_free[NS], s_full[2][2], p_ready[2][2], pv_done[2], o_done;
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;
     __shared__ int lim_max, lim_min;
@@ -192,7 +206,11 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     // ---- a softmax thread's column and how far it sees
     const int wg = warp >> 2, col = col0 + tid;
     const bool live = tid < kBulkCols && col < ncol;
-    const int rr = r0 + (live ? col / p.G : 0), hh = kvh * p.G + (live ? col % p.G : 0);
+    const int base_row = col0 / p.G, base_head = col0 - base_row * p.G;  // of the pair's first column
+    // column cw of the pair: its row and query head (cw + base_head < 2^9: the product by 2^16 / G rounds right)
+    auto row_of = [&](int cw) { return (int)((uint32_t)(cw + base_head) * p.g_inv >> 16); };
+    const int my_row = row_of(live ? tid : 0);
+    const int rr = r0 + base_row + my_row, hh = kvh * p.G + (live ? tid : 0) + base_head - my_row * p.G;
     const RowView view = row_view(p, rr, shared);
     const int lim = live ? max(0, view.shared) : 0;
     int seq = row_seq(p, r0);
@@ -206,26 +224,37 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         constexpr int LPR = D / 4, RPI = 32 / LPR;  // lanes per row, rows per step
         const int sub = lane / LPR, e0 = (lane % LPR) * 4;
         const float sgn = p.scale_log2 < 0.f ? -1.f : 1.f;  // (the maximum is taken of S itself)
-#pragma unroll 8
-        for (int it = 0; it < 32 / RPI; ++it) {
-            const int cw = warp * 32 + it * RPI + sub, c = col0 + cw;  // column within the pair; of the group
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            if (c < ncol) {
-                const T* q = static_cast<const T*>(p.q) + (size_t)(r0 + c / p.G) * p.ldq + (size_t)(kvh * p.G + c % p.G) * D + e0;
+        constexpr int B = 8;  // steps whose loads are in flight together
+#pragma unroll 1
+        for (int it0 = 0; it0 < 32 / RPI; it0 += B) {
+        float xs[B][4];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int cw = warp * 32 + (it0 + b) * RPI + sub;  // column within the pair
+            float* x = xs[b];
+            x[0] = x[1] = x[2] = x[3] = 0.f;
+            if (col0 + cw < ncol) {
+                const int qr = row_of(cw), qh = kvh * p.G + cw + base_head - qr * p.G;
+                const T* q = static_cast<const T*>(p.q) + (size_t)(r0 + base_row + qr) * p.ldq + (size_t)qh * D + e0;
                 if (p.q_vec) {
                     if constexpr (F32) {
                         *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(q);
                     } else {
                         const uint2 w = *reinterpret_cast<const uint2*>(q);
                         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-                        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-                        x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+                        const float2 b2 = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+                        x[0] = a.x; x[1] = a.y; x[2] = b2.x; x[3] = b2.y;
                     }
                 } else {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) x[k] = kv_in<T>(q[k]);
                 }
             }
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int cw = warp * 32 + (it0 + b) * RPI + sub;
+            const float* x = xs[b];
             float fac = sgn, inv = 1.f;
             if constexpr (F32) {
                 float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
@@ -250,11 +279,15 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
             if constexpr (F32) *reinterpret_cast<uint2*>(dst + QPART) = make_uint2(lo[0], lo[1]);
         }
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (tid == 0) {
         for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
-        for (int w = 0; w < 2; ++w) { mbar_init(&s_full[w], 1); mbar_init(&p_ready[w], 128); }
+        for (int w = 0; w < 2; ++w) {
+            for (int b = 0; b < 2; ++b) { mbar_init(&s_full[w][b], 1); mbar_init(&p_ready[w][b], 128); }
+            mbar_init(&pv_done[w], 1);
+        }
         mbar_init(&o_done, 1);
         mbar_fence_init();
         dead = 0;
@@ -279,42 +312,40 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     tc_fence_after();
     pdl_launch_dependents();  // the private items need nothing of this kernel
     const uint32_t tmem = tmem_at;
-    auto s_at = [&](int w) { return tmem + (uint32_t)(w * NK); };        // S, then P hi | P lo in its place
+    auto s_at = [&](int w, int j) { return tmem + (uint32_t)(w * 2 * NK + (j & 1) * NK); };  // S(j), then P hi | P lo in its place
     auto o_at = [&](int w) { return tmem + 256u + (uint32_t)(w * D); };
 
     if (warp == 8) {
-        if (lane == 0) {
-            const int box = min(1 << p.page_shift, NK);  // rows of a TMA box
-            int j = 0;
-            for (; j < nt; ++j) {
-                const int s = j % NS;
-                if (j >= NS && !bulk_wait(&kv_free[s], (uint32_t)(j / NS - 1) & 1, &dead, p.err)) break;
-                mbar_expect_tx(&kv_full[s], STAGE);
-                const uint32_t ks = smem_u32(stages) + (uint32_t)(s * STAGE);
-                for (int k = 0; k < NK; k += box) {
-                    const int t = t0 + j * NK + k;
-                    int id = 0;  // past the last position seen: any page (masked, and cleared in V)
-                    if (t < t1) {
-                        id = page_ids[(t >> p.page_shift) - first_page];
-                        if (id < 0 || id >= p.num_pages) {
-                            kv_flag(p.err, kKvBadPage);
-                            id = 0;
-                        }
-                    }
-                    const int y = ((id * p.kv_heads + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-#pragma unroll
-                    for (int h = 0; h < HALVES; ++h) {
-                        tma_2d(ks + h * (NK * 128) + k * 128, &mk, h * 64, y, &kv_full[s]);
-                        tma_2d(ks + VOFF + h * (NK * 128) + k * 128, &mv, h * 64, y, &kv_full[s]);
+        // a lane per box: (piece of the tile, K or V, half of the row)
+        const int box = min(1 << p.page_shift, NK), boxes = NK / box * 2 * HALVES;
+        const int half = lane % HALVES, which = lane / HALVES & 1, k = lane / (2 * HALVES) * box;
+        int j = 0;
+        for (; j < nt; ++j) {
+            const int s = j % NS;
+            const bool ok = j < NS || bulk_wait(&kv_free[s], (uint32_t)(j / NS - 1) & 1, &dead, p.err);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            if (lane == 0) mbar_expect_tx(&kv_full[s], STAGE);
+            __syncwarp();
+            if (lane < boxes) {
+                const int t = t0 + j * NK + k;
+                int id = 0;  // past the last position seen: any page (masked, and cleared in V)
+                if (t < t1) {
+                    id = page_ids[(t >> p.page_shift) - first_page];
+                    if (id < 0 || id >= p.num_pages) {
+                        kv_flag(p.err, kKvBadPage);
+                        id = 0;
                     }
                 }
+                const int y = ((id * p.kv_heads + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+                tma_2d(smem_u32(stages) + (uint32_t)(s * STAGE + which * VOFF + half * (NK * 128) + k * 128), which ? &mv : &mk,
+                       half * 64, y, &kv_full[s]);
             }
-            if (dead)  // copies still in flight land before the CTA's memory is given up
-                for (int k = max(0, j - NS); k < j; ++k) {
-                    const long long since = clock64();
-                    while (!mbar_try_wait(&kv_full[k % NS], (uint32_t)(k / NS) & 1) && clock64() - since < 200000000LL) {}
-                }
         }
+        if (lane == 0 && dead)  // copies still in flight land before the CTA's memory is given up
+            for (int q = max(0, j - NS); q < j; ++q) {
+                const long long since = clock64();
+                while (!mbar_try_wait(&kv_full[q % NS], (uint32_t)(q / NS) & 1) && clock64() - since < 200000000LL) {}
+            }
     } else if (warp == 9) {
         if (lane == 0) {
             constexpr uint32_t iqk = umma_idesc(NK, false), ipv = umma_idesc(D, true);
@@ -327,10 +358,10 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
                         const uint32_t off = (uint32_t)(k & 3) * 32;
-                        tc_mma_ss(s_at(w), umma_desc(qa + part * QPART + (k >> 2) * (128 * 128) + off, 16, 1024),
+                        tc_mma_ss(s_at(w, j), umma_desc(qa + part * QPART + (k >> 2) * (128 * 128) + off, 16, 1024),
                                   umma_desc(ks + (k >> 2) * (NK * 128) + off, 16, 1024), iqk, part != HN - 1 || k > 0);
                     }
-                tc_commit(&s_full[w]);
+                tc_commit(&s_full[w][j & 1]);
             };
             auto pv = [&](int w, int j) {
                 const uint32_t vs = smem_u32(stages) + (uint32_t)(j % NS * STAGE) + VOFF;
@@ -338,31 +369,35 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 for (int part = HN - 1; part >= 0; --part)
 #pragma unroll
                     for (int k = 0; k < NK / 16; ++k)
-                        tc_mma_ts(o_at(w), s_at(w) + part * (NK / 2) + k * 8, umma_desc(vs + k * 2048, NK * 128, 1024), ipv,
+                        tc_mma_ts(o_at(w), s_at(w, j) + part * (NK / 2) + k * 8, umma_desc(vs + k * 2048, NK * 128, 1024), ipv,
                                   j > 0 || part != HN - 1 || k > 0);
+                tc_commit(&pv_done[w]);
             };
-            ok = bulk_wait(&kv_full[0], 0, &dead, p.err);
-            if (ok) {
+            auto full = [&](int j) {
+                const bool got = bulk_wait(&kv_full[j % NS], (uint32_t)(j / NS) & 1, &dead, p.err);
                 tc_fence_after();
-                for (int w = 0; w < tiles; ++w) qk(w, 0);
+                return got;
+            };
+            for (int j = 0; j < min(nt, 2) && ok; ++j) {
+                if (!(ok = full(j))) break;
+                for (int w = 0; w < tiles; ++w) qk(w, j);
             }
             for (int j = 0; j < nt && ok; ++j)
                 for (int w = 0; w < tiles && ok; ++w) {
-                    if (!(ok = bulk_wait(&p_ready[w], (uint32_t)j & 1, &dead, p.err))) break;
+                    if (!(ok = bulk_wait(&p_ready[w][j & 1], (uint32_t)(j >> 1) & 1, &dead, p.err))) break;
                     tc_fence_after();
                     pv(w, j);
                     if (w == tiles - 1) tc_commit(&kv_free[j % NS]);
-                    if (j + 1 < nt) {
-                        if (w == 0 && !(ok = bulk_wait(&kv_full[(j + 1) % NS], (uint32_t)((j + 1) / NS) & 1, &dead, p.err))) break;
-                        tc_fence_after();
-                        qk(w, j + 1);
+                    if (j + 2 < nt) {
+                        if (w == 0 && !(ok = full(j + 2))) break;
+                        qk(w, j + 2);
                     }
                 }
             tc_commit(&o_done);  // after a failed wait too: whatever was issued ends before tensor memory is freed
         }
     } else if (wg < tiles) {
         const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
-        const uint32_t S = s_at(wg) + lane_at, O = o_at(wg) + lane_at;
+        const uint32_t O = o_at(wg) + lane_at;
         const float cm = cmul[tid];
         const int wtid = tid & 127;
         float mref = 0.f, l = 0.f;
@@ -370,29 +405,26 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         for (int j = 0; j < nt; ++j) {
             const int c0 = t0 + j * NK;
             const bool masked = c0 + NK > min(seen_by_all, t1);
-            ok = __all_sync(0xffffffffu, bulk_wait(&s_full[wg], (uint32_t)j & 1, &dead, p.err));
+            const uint32_t S = s_at(wg, j) + lane_at;
+            ok = __all_sync(0xffffffffu, bulk_wait(&s_full[wg][j & 1], (uint32_t)(j >> 1) & 1, &dead, p.err));
             if (!ok) break;
             tc_fence_after();
-            uint32_t s[2][32];
+            uint32_t s[NK];
+            tc_ld32(S, s);
+            tc_ld32(S + 32, s + 32);
+            tc_wait_ld();
+            tc_loaded(s);
+            tc_loaded(s + 32);
             // ---- the maximum
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tc_ld32(S, s[0]);
+            if (masked) {
 #pragma unroll
-            for (int k = 0; k < NK; k += 32) {
-                uint32_t* cur = s[(k >> 5) & 1];
-                tc_wait_ld();
-                tc_loaded(cur);
-                if (k + 32 < NK) tc_ld32(S + k + 32, s[((k >> 5) + 1) & 1]);
-                if (masked) {
+                for (int e = 0; e < NK; ++e)
+                    if (c0 + e < lim) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (c0 + k + e < lim) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(cur[e]));
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(cur[e]));
-                }
+                for (int e = 0; e < NK; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
             }
-            tc_ld32(S, s[0]);
             const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * cm;
             if (j == 0) {
                 mref = mx > -INFINITY ? mx : 0.f;
@@ -400,35 +432,29 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 const float next = fmaxf(mref, mx), corr = ex2(mref - next);
                 mref = next;
                 l *= corr;
-                tc_wait_ld();
-                tc_loaded(s[0]);
+                ok = __all_sync(0xffffffffu, bulk_wait(&pv_done[wg], (uint32_t)(j - 1) & 1, &dead, p.err));
+                if (!ok) break;
+                tc_fence_after();
 #pragma unroll 1
-                for (int k = 0; k < D; k += 32) {
-                    uint32_t* o = s[1];
-                    tc_ld32(O + k, o);
-                    tc_wait_ld();
-                    tc_loaded(o);
+                for (int k = 0; k < D; k += 16) {
+                    uint32_t o[16];
+                    tc_ld16(O + k, o);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                    tc_st32(O + k, o);
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                    tc_st16(O + k, o);
                 }
             }
             // ---- the weights: binary16 rows carry the factor in the exponent (their rounding is 2^-11 anyway)
             const float shift = F32 ? -mref : 7.f - mref;
             const uint64_t cm2 = f2_pack(cm, cm), sh2 = f2_pack(shift, shift), gain2 = f2_pack(kPaGain, kPaGain);
             uint64_t sum2[2] = {0, 0};
-            uint32_t lo_keep[F32 ? NK / 2 : 1];
 #pragma unroll
             for (int k = 0; k < NK; k += 32) {
-                uint32_t* cur = s[(k >> 5) & 1];
-                tc_wait_ld();
-                tc_loaded(cur);
-                if (k + 32 < NK) tc_ld32(S + k + 32, s[((k >> 5) + 1) & 1]);
-                uint32_t hi[16];
+                uint32_t hi[16], lo[F32 ? 16 : 1];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     float a, b;
-                    f2_unpack(f2_fma(f2_pack(__uint_as_float(cur[2 * e]), __uint_as_float(cur[2 * e + 1])), cm2, sh2), a, b);
+                    f2_unpack(f2_fma(f2_pack(__uint_as_float(s[k + 2 * e]), __uint_as_float(s[k + 2 * e + 1])), cm2, sh2), a, b);
                     a = ex2(a);
                     b = ex2(b);
                     if (masked) {
@@ -446,12 +472,12 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                     if constexpr (F32) {
                         const float2 f = __half22float2(h);
                         const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
-                        lo_keep[k / 2 + e] = *reinterpret_cast<const uint32_t*>(&r);
+                        lo[e] = *reinterpret_cast<const uint32_t*>(&r);
                     }
                 }
-                tc_st16(S + k / 2, hi);  // (columns of S already read: k / 2 + 16 <= k + 32)
+                tc_st16(S + k / 2, hi);
+                if constexpr (F32) tc_st16(S + NK / 2 + k / 2, lo);
             }
-            if constexpr (F32) tc_st32(S + NK / 2, lo_keep);
             float a, b;
             f2_unpack(f2_add(sum2[0], sum2[1]), a, b);
             l += a + b;
@@ -481,14 +507,16 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             }
             tc_wait_st();
             tc_fence_before();
-            mbar_arrive(&p_ready[wg]);
+            mbar_arrive(&p_ready[wg][j & 1]);
         }
         ok = __all_sync(0xffffffffu, bulk_wait(&o_done, 0, &dead, p.err)) && ok;
         tc_fence_after();
         named_sync(1, 128 * tiles);  // both tiles' notes of odd positions (every softmax warp comes here)
         if (ok) {
+            // O's rows through shared memory (nothing reads it any more): a thread's own stores to global
+            // memory would touch 32 lines per instruction (13,000 cycles measured, against 1,500)
             const int ns = p.nss + p.nsp;
-            const size_t at = ((size_t)rr * p.heads + hh) * ns + split;
+            float* rows = reinterpret_cast<float*>(base) + (size_t)warp * 32 * (D + 4);
 #pragma unroll 1
             for (int k = 0; k < D; k += 32) {
                 uint32_t o[32];
@@ -508,14 +536,23 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                                 if (!(fabsf(x) <= 65504.f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
                             }
                         }
-                if (live) {
-                    uint4* dst = reinterpret_cast<uint4*>(p.part_o + at * D + k);
+                uint4* dst = reinterpret_cast<uint4*>(rows + (size_t)lane * (D + 4) + k);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                }
+                for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
+            const size_t at = ((size_t)rr * p.heads + hh) * ns + split;
             // (l is zero only where the column saw nothing: its largest weight is at least 2^-8)
             if (live) p.part_ml[at] = make_float2(l == 0.f ? -INFINITY : mref, F32 ? l * kPaGain : l);
+            __syncwarp();
+            constexpr int LPR = D / 4;  // lanes per row
+#pragma unroll 4
+            for (int q = 0; q < 32; q += 32 / LPR) {
+                const int c = q + lane / LPR;
+                const size_t to = __shfl_sync(0xffffffffu, (unsigned long long)at, c);
+                if (col0 + warp * 32 + c < ncol)
+                    *reinterpret_cast<float4*>(p.part_o + to * D + lane % LPR * 4) =
+                        *reinterpret_cast<const float4*>(rows + (size_t)c * (D + 4) + lane % LPR * 4);
+            }
         }
         tc_fence_before();
     }

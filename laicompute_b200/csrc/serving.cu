@@ -147,10 +147,9 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
         if (pl.bulk) {
             // about one item per SM (a bulk CTA fills one), in whole tiles
             pl.ctiles = (cols + kBulkCols - 1) / kBulkCols;
-            const int tile = bulk_keys(a.type == LAIC_GGML_F32);
             const long long sets = (long long)a.groups * pl.ctiles * g.kv_heads;
             const int splits = (int)std::max<long long>(1, device_sms(g.device) / sets);
-            pl.ls = std::min(kBulkMaxSplit, std::max(2 * tile, round_up((a.max_shared + splits - 1) / splits, tile)));
+            pl.ls = std::min(kBulkMaxSplit, std::max(2 * kBulkKeys, round_up((a.max_shared + splits - 1) / splits, kBulkKeys)));
         } else {
             pl.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
             pl.ctiles = (cols + 8 * pl.nt - 1) / (8 * pl.nt);
@@ -208,12 +207,12 @@ EncodeFn tensor_map_encode() {
 }
 // One pool as rows of head_dim binary16 values; a box is 64 columns (x 0 or 64: whole 128-byte lines) of
 // up to a page's positions, so it never leaves a (page, head) run.
-bool encode_pages(const laic_kv_pages& g, void* pool, int tile, CUtensorMap* map) {
+bool encode_pages(const laic_kv_pages& g, void* pool, CUtensorMap* map) {
     const EncodeFn f = tensor_map_encode();
     if (!f) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_pages * g.kv_heads * g.page_size};
     const cuuint64_t strides[1] = {(cuuint64_t)g.head_dim * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)std::min(g.page_size, tile)}, step[2] = {1, 1};
+    const cuuint32_t box[2] = {64, (cuuint32_t)std::min(g.page_size, kBulkKeys)}, step[2] = {1, 1};
     return f(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, pool, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -336,6 +335,7 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     p.kp = static_cast<const __half*>(g.k_dev); p.vp = static_cast<const __half*>(g.v_dev);
     p.num_pages = g.num_pages; p.page_shift = log2i(g.page_size);
     p.kv_heads = g.kv_heads; p.heads = a.heads; p.G = a.heads / g.kv_heads;
+    p.g_inv = (65536 + p.G - 1) / p.G;
     p.len = a.len_dev; p.seq = a.seq_dev; p.table = a.page_table_dev;
     p.nseq = a.nseq; p.pages_per_seq = a.pages_per_seq; p.rows = a.rows; p.max_len = a.max_len;
     p.groups = a.groups; p.max_group_rows = a.max_group_rows; p.max_shared = a.max_shared;
@@ -357,7 +357,7 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
         cudaError_t e = serving_set_attributes();
         if (e == cudaSuccess && pl.bulk && pl.shared_items) {
             CUtensorMap mk, mv;
-            if (!encode_pages(g, g.k_dev, bulk_keys(f32), &mk) || !encode_pages(g, g.v_dev, bulk_keys(f32), &mv))
+            if (!encode_pages(g, g.k_dev, &mk) || !encode_pages(g, g.v_dev, &mv))
                 return api_fail(LAIC_E_CUDA, "kv_attention: tensor map");
             e = launch_k(bulk_pick(g.head_dim, f32), dim3(pl.shared_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32), st,
                          false, p, mk, mv);
