@@ -326,7 +326,7 @@ typedef struct laic_kv_attention_args {
     int32_t groups;           /* groups of rows that share their first positions (0: none) */
     int32_t max_group_rows, max_shared; /* bounds on the groups' rows and shared lengths */
     int32_t max_private;      /* bound on a row's positions beyond its group's shared ones (-1: max_len) */
-    float scale;              /* of the scores; 0: 1 / sqrt(head_dim) */
+    float scale;              /* of the scores, positive; 0: 1 / sqrt(head_dim) */
     int64_t ldq, ldo;
     const void* q_dev;
     void* out_dev;

@@ -5,14 +5,15 @@
 // group's positions in tiles of bulk_keys.
 //
 // Roles: warp 8 loads (TMA boxes of up to a page, 128-byte swizzle, a lane per box: one lane alone
-// took 125 cycles a box, 4,000 for a tile of 16-position pages; a ring of K + V stages); warp 9
+// took 125 cycles a box, 4,000 for a tile of 16-position pages; a ring of K and V tiles); warp 9
 // multiplies (one lane: tcgen05.mma, S and O in tensor memory, P read from tensor memory, where it
-// takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S, keep the
-// running maximum and sum, and write P. S has two buffers per tile, and QK(j + 2) follows PV(j), so
-// the scores of the next positions are ready when a softmax warp turns to them; it waits for a
-// product only to rescale O, which it does when a maximum grew by more than 2^8 since the last time
-// (weights stay below 2^15 in binary16 with the factor 2^7 they carry). Both tiles' S and O fill the
-// 512 columns of tensor memory.
+// takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S (twice, 32
+// columns at a time: a column's 128 scores do not fit the registers beside the rest), keep the
+// running maximum and sum, and write P in two halves, so that PV starts on the first. One tile's products run under the other's exponentials. 128 positions
+// per tile: a product of N = 64 takes about as long as one of N = 128 (100 against 85 cycles
+// measured), and two score buffers of 64 ran slower than one of 128. O is rescaled only when a
+// maximum grew by more than 2^8 since the last time (weights stay below 2^15 in binary16 with the
+// factor 2^7 they carry). Both tiles' S and O fill the 512 columns of tensor memory.
 //
 // Tiles that some column does not see to their end are masked. There 0 * V must not be 0 * inf: the
 // softmax threads clear what is not finite in V before the product (all of it past the positions any
@@ -34,14 +35,14 @@ constexpr int kBulkThreads = 320;
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
 constexpr float kBulkSlack = 8.f;     // log2 of how far a maximum may outgrow its reference
 
-constexpr int kBulkKeys = 64;         // positions per tile
-__host__ __device__ constexpr int bulk_stage_bytes(int D) { return 2 * kBulkKeys * D * 2; }
+constexpr int kBulkKeys = 128;        // positions per tile
+__host__ __device__ constexpr int bulk_slot_bytes(int D) { return kBulkKeys * D * 2; }  // a tile of K or of V
 __host__ __device__ constexpr int bulk_q_bytes(int D, bool f32) { return kBulkCols * D * 2 * (f32 ? 2 : 1); }
-// Stages: tile j's V, j + 1's and j + 2's K are in use at once; at the end the ring and Q hold O's rows.
-__host__ __device__ constexpr int bulk_stages(int D, bool f32) { return D == 128 && f32 ? 3 : 4; }
+__host__ __device__ constexpr int bulk_slots(int D, bool f32) { return D == 64 ? 6 : f32 ? 3 : 5; }
 __host__ __device__ constexpr int bulk_smem(int D, bool f32) {
-    return bulk_q_bytes(D, f32) + bulk_stages(D, f32) * bulk_stage_bytes(D) + 1024;  // (aligned to 1024)
+    return bulk_q_bytes(D, f32) + bulk_slots(D, f32) * bulk_slot_bytes(D) + 1024;  // (aligned to 1024)
 }
+// (at the end the ring and Q hold O's rows)
 static_assert(bulk_smem(64, false) - 1024 >= kBulkCols * (64 + 4) * 4 && bulk_smem(128, false) - 1024 >= kBulkCols * (128 + 4) * 4,
               "O's rows fit");
 
@@ -171,14 +172,14 @@ template <int D, typename T>
 __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAttnParams p, const __grid_constant__ CUtensorMap mk,
                                                                      const __grid_constant__ CUtensorMap mv) {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int HN = F32 ? 2 : 1, NK = kBulkKeys, NS = bulk_stages(D, F32), HALVES = D / 64;
-    constexpr int STAGE = bulk_stage_bytes(D), VOFF = STAGE / 2;
+    constexpr int HN = F32 ? 2 : 1, NK = kBulkKeys, NS = bulk_slots(D, F32), HALVES = D / 64;
+    constexpr int SLOT = bulk_slot_bytes(D);
     constexpr int QPART = 128 * D * 2;  // one tile's hi or lo part
     extern __shared__ uint8_t dyn[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    uint8_t* stages = base + bulk_q_bytes(D, F32);
+    uint8_t* ring = base + bulk_q_bytes(D, F32);
     __shared__ int page_ids[kBulkMaxSplit / 16 + 2];
-    __shared__ uint64_t kv_full[NS], kv_free[NS], s_full[2][2], p_ready[2][2], pv_done[2], o_done;
+    __shared__ uint64_t kv_full[NS], kv_free[NS], s_full[2], p_ready[2][2], o_done;
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;
     __shared__ int lim_max, lim_min;
@@ -219,74 +220,89 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     const int npages = min(((t0 + p.ls - 1) >> p.page_shift) + 1, p.pages_per_seq) - first_page;
     for (int k = tid; k < npages; k += kBulkThreads) page_ids[k] = p.table[(size_t)seq * p.pages_per_seq + first_page + k];
 
-    // ---- Q: a warp takes 32 columns, a lane four elements of one, with 128-byte swizzled rows
-    if (warp < 4 * tiles) {
-        constexpr int LPR = D / 4, RPI = 32 / LPR;  // lanes per row, rows per step
-        const int sub = lane / LPR, e0 = (lane % LPR) * 4;
-        const float sgn = p.scale_log2 < 0.f ? -1.f : 1.f;  // (the maximum is taken of S itself)
-        constexpr int B = 8;  // steps whose loads are in flight together
+    // ---- Q in 128-byte swizzled rows
+    auto q_at = [&](int cw) {  // row of q of the pair's column cw
+        const int qr = row_of(cw);
+        return static_cast<const T*>(p.q) + (size_t)(r0 + base_row + qr) * p.ldq + (size_t)(kvh * p.G + cw + base_head - qr * p.G) * D;
+    };
+    auto q_dst = [&](int cw, int ch) {  // 16-byte chunk ch of its binary16 row
+        const int row = cw & 127;
+        return base + (size_t)(cw >> 7) * HN * QPART + (ch >> 3) * (128 * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+    };
+    constexpr int CH = D / 8;  // chunks per row
+    if constexpr (!F32) {
+        for (int k = tid; k < tiles * 128 * CH; k += kBulkThreads) {
+            const int cw = k / CH, ch = k % CH;
+            const bool in = col0 + cw < ncol;
+            if (p.q_vec) {
+                cp_async16_z(smem_u32(q_dst(cw, ch)), in ? q_at(cw) + ch * 8 : static_cast<const T*>(p.q), in);
+            } else {
+                __half x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = in ? q_at(cw)[ch * 8 + e] : __float2half_rn(0.f);
+                *reinterpret_cast<uint4*>(q_dst(cw, ch)) = *reinterpret_cast<const uint4*>(x);
+            }
+        }
+        if (tid < kBulkCols) cmul[tid] = p.scale_log2;
+        cp_async_commit();
+        cp_async_wait_all();
+    } else if (warp < 4 * tiles) {
+        // a warp takes 32 columns, CH lanes a row; four steps' loads in flight
+        constexpr int RPI = 32 / CH, STEPS = 32 / RPI, B = 4;
+        const int sub = lane / CH, ch = lane % CH;
 #pragma unroll 1
-        for (int it0 = 0; it0 < 32 / RPI; it0 += B) {
-        float xs[B][4];
+        for (int it0 = 0; it0 < STEPS; it0 += B) {
+            float xs[B][8];
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const int cw = warp * 32 + (it0 + b) * RPI + sub;  // column within the pair
-            float* x = xs[b];
-            x[0] = x[1] = x[2] = x[3] = 0.f;
-            if (col0 + cw < ncol) {
-                const int qr = row_of(cw), qh = kvh * p.G + cw + base_head - qr * p.G;
-                const T* q = static_cast<const T*>(p.q) + (size_t)(r0 + base_row + qr) * p.ldq + (size_t)qh * D + e0;
-                if (p.q_vec) {
-                    if constexpr (F32) {
+            for (int b = 0; b < B; ++b) {
+                const int cw = warp * 32 + (it0 + b) * RPI + sub;
+                float* x = xs[b];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = 0.f;
+                if (col0 + cw < ncol) {
+                    const float* q = reinterpret_cast<const float*>(q_at(cw)) + ch * 8;
+                    if (p.q_vec) {
                         *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(q);
+                        *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(q + 4);
                     } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(q);
-                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-                        const float2 b2 = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-                        x[0] = a.x; x[1] = a.y; x[2] = b2.x; x[3] = b2.y;
-                    }
-                } else {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) x[k] = kv_in<T>(q[k]);
+                        for (int e = 0; e < 8; ++e) x[e] = q[e];
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const int cw = warp * 32 + (it0 + b) * RPI + sub;
-            const float* x = xs[b];
-            float fac = sgn, inv = 1.f;
-            if constexpr (F32) {
-                float mx = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+            for (int b = 0; b < B; ++b) {
+                const int cw = warp * 32 + (it0 + b) * RPI + sub;
+                const float* x = xs[b];
+                float mx = 0.f;
 #pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
-                fac = sgn * __uint_as_float((uint32_t)(127 - e) << 23);
-                inv = __uint_as_float((uint32_t)(127 + e) << 23);
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+#pragma unroll
+                for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
+                const float fac = __uint_as_float((uint32_t)(127 - ex) << 23);
+                if (ch == 0) cmul[cw] = p.scale_log2 * __uint_as_float((uint32_t)(127 + ex) << 23);
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float a = x[2 * k] * fac, c = x[2 * k + 1] * fac;
+                    const __half2 h = __floats2half2_rn(a, c);
+                    const float2 f = __half22float2(h);
+                    const __half2 r = __floats2half2_rn(a - f.x, c - f.y);
+                    hi[k] = *reinterpret_cast<const uint32_t*>(&h);
+                    lo[k] = *reinterpret_cast<const uint32_t*>(&r);
+                }
+                *reinterpret_cast<uint4*>(q_dst(cw, ch)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(q_dst(cw, ch) + QPART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
-            if (e0 == 0) cmul[cw] = fabsf(p.scale_log2) * inv;
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const float a = x[2 * k] * fac, b = x[2 * k + 1] * fac;
-                const __half ha = __float2half_rn(a), hb = __float2half_rn(b);
-                hi[k] = pack_h2(ha, hb);
-                lo[k] = pack_h2(__float2half_rn(a - __half2float(ha)), __float2half_rn(b - __half2float(hb)));
-            }
-            const int row = cw & 127, ch = e0 >> 3;
-            uint8_t* dst = base + (size_t)(cw >> 7) * HN * QPART + (ch >> 3) * (128 * 128) + row * 128 +
-                           (((ch & 7) ^ (row & 7)) << 4) + (e0 & 4) * 2;
-            *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-            if constexpr (F32) *reinterpret_cast<uint2*>(dst + QPART) = make_uint2(lo[0], lo[1]);
         }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (tid == 0) {
         for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
         for (int w = 0; w < 2; ++w) {
-            for (int b = 0; b < 2; ++b) { mbar_init(&s_full[w][b], 1); mbar_init(&p_ready[w][b], 128); }
-            mbar_init(&pv_done[w], 1);
+            mbar_init(&s_full[w], 1);
+            for (int h = 0; h < 2; ++h) mbar_init(&p_ready[w][h], 128);
         }
         mbar_init(&o_done, 1);
         mbar_fence_init();
@@ -312,22 +328,27 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     tc_fence_after();
     pdl_launch_dependents();  // the private items need nothing of this kernel
     const uint32_t tmem = tmem_at;
-    auto s_at = [&](int w, int j) { return tmem + (uint32_t)(w * 2 * NK + (j & 1) * NK); };  // S(j), then P hi | P lo in its place
+    // S; then, in the place of each half of its positions, P hi (32 columns) and P lo (32)
+    auto s_at = [&](int w) { return tmem + (uint32_t)(w * NK); };
     auto o_at = [&](int w) { return tmem + 256u + (uint32_t)(w * D); };
 
+    // ring item m: K of tile m / 2, then its V
+    auto slot = [&](int m) { return smem_u32(ring) + (uint32_t)(m % NS * SLOT); };
+    auto full = [&](int m) { return bulk_wait(&kv_full[m % NS], (uint32_t)(m / NS) & 1, &dead, p.err); };
+
     if (warp == 8) {
-        // a lane per box: (piece of the tile, K or V, half of the row)
-        const int box = min(1 << p.page_shift, NK), boxes = NK / box * 2 * HALVES;
-        const int half = lane % HALVES, which = lane / HALVES & 1, k = lane / (2 * HALVES) * box;
-        int j = 0;
-        for (; j < nt; ++j) {
-            const int s = j % NS;
-            const bool ok = j < NS || bulk_wait(&kv_free[s], (uint32_t)(j / NS - 1) & 1, &dead, p.err);
+        // a lane per box: (piece of the tile, half of the row)
+        const int box = min(1 << p.page_shift, NK), boxes = NK / box * HALVES;
+        const int half = lane % HALVES, k = lane / HALVES * box;
+        int m = 0;
+        for (; m < 2 * nt; ++m) {
+            const int s = m % NS;
+            const bool ok = m < NS || bulk_wait(&kv_free[s], (uint32_t)(m / NS - 1) & 1, &dead, p.err);
             if (!__all_sync(0xffffffffu, ok)) break;
-            if (lane == 0) mbar_expect_tx(&kv_full[s], STAGE);
+            if (lane == 0) mbar_expect_tx(&kv_full[s], SLOT);
             __syncwarp();
             if (lane < boxes) {
-                const int t = t0 + j * NK + k;
+                const int t = t0 + (m >> 1) * NK + k;
                 int id = 0;  // past the last position seen: any page (masked, and cleared in V)
                 if (t < t1) {
                     id = page_ids[(t >> p.page_shift) - first_page];
@@ -337,104 +358,107 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                     }
                 }
                 const int y = ((id * p.kv_heads + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-                tma_2d(smem_u32(stages) + (uint32_t)(s * STAGE + which * VOFF + half * (NK * 128) + k * 128), which ? &mv : &mk,
-                       half * 64, y, &kv_full[s]);
+                tma_2d(slot(m) + half * (NK * 128) + k * 128, m & 1 ? &mv : &mk, half * 64, y, &kv_full[s]);
             }
         }
         if (lane == 0 && dead)  // copies still in flight land before the CTA's memory is given up
-            for (int q = max(0, j - NS); q < j; ++q) {
+            for (int q = max(0, m - NS); q < m; ++q) {
                 const long long since = clock64();
                 while (!mbar_try_wait(&kv_full[q % NS], (uint32_t)(q / NS) & 1) && clock64() - since < 200000000LL) {}
             }
     } else if (warp == 9) {
         if (lane == 0) {
             constexpr uint32_t iqk = umma_idesc(NK, false), ipv = umma_idesc(D, true);
-            bool ok = true;
             auto qk = [&](int w, int j) {
-                const uint32_t ks = smem_u32(stages) + (uint32_t)(j % NS * STAGE);
-                const uint32_t qa = smem_u32(base) + (uint32_t)(w * HN * QPART);
+                uint32_t ks = slot(2 * j), qa = smem_u32(base) + (uint32_t)(w * HN * QPART);
+                asm volatile("" : "+r"(ks), "+r"(qa));  // (descriptors are formed here, not kept over the loop)
 #pragma unroll
                 for (int part = HN - 1; part >= 0; --part)  // lo, then hi
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
                         const uint32_t off = (uint32_t)(k & 3) * 32;
-                        tc_mma_ss(s_at(w, j), umma_desc(qa + part * QPART + (k >> 2) * (128 * 128) + off, 16, 1024),
+                        tc_mma_ss(s_at(w), umma_desc(qa + part * QPART + (k >> 2) * (128 * 128) + off, 16, 1024),
                                   umma_desc(ks + (k >> 2) * (NK * 128) + off, 16, 1024), iqk, part != HN - 1 || k > 0);
                     }
-                tc_commit(&s_full[w][j & 1]);
+                tc_commit(&s_full[w]);
+                if (w == tiles - 1) tc_commit(&kv_free[2 * j % NS]);
             };
-            auto pv = [&](int w, int j) {
-                const uint32_t vs = smem_u32(stages) + (uint32_t)(j % NS * STAGE) + VOFF;
+            auto pv = [&](int w, int j, int h) {
+                uint32_t vs = slot(2 * j + 1);
+                asm volatile("" : "+r"(vs));
 #pragma unroll
                 for (int part = HN - 1; part >= 0; --part)
 #pragma unroll
-                    for (int k = 0; k < NK / 16; ++k)
-                        tc_mma_ts(o_at(w), s_at(w, j) + part * (NK / 2) + k * 8, umma_desc(vs + k * 2048, NK * 128, 1024), ipv,
-                                  j > 0 || part != HN - 1 || k > 0);
-                tc_commit(&pv_done[w]);
+                    for (int k = 0; k < NK / 32; ++k)
+                        tc_mma_ts(o_at(w), s_at(w) + h * (NK / 2) + part * (NK / 4) + k * 8,
+                                  umma_desc(vs + (h * (NK / 32) + k) * 2048, NK * 128, 1024), ipv,
+                                  j > 0 || h > 0 || part != HN - 1 || k > 0);
             };
-            auto full = [&](int j) {
-                const bool got = bulk_wait(&kv_full[j % NS], (uint32_t)(j / NS) & 1, &dead, p.err);
-                tc_fence_after();
-                return got;
-            };
-            for (int j = 0; j < min(nt, 2) && ok; ++j) {
-                if (!(ok = full(j))) break;
-                for (int w = 0; w < tiles; ++w) qk(w, j);
-            }
+            bool ok = full(0);
+            tc_fence_after();
+            for (int w = 0; w < tiles && ok; ++w) qk(w, 0);
             for (int j = 0; j < nt && ok; ++j)
                 for (int w = 0; w < tiles && ok; ++w) {
-                    if (!(ok = bulk_wait(&p_ready[w][j & 1], (uint32_t)(j >> 1) & 1, &dead, p.err))) break;
-                    tc_fence_after();
-                    pv(w, j);
-                    if (w == tiles - 1) tc_commit(&kv_free[j % NS]);
-                    if (j + 2 < nt) {
-                        if (w == 0 && !(ok = full(j + 2))) break;
-                        qk(w, j + 2);
+                    if (w == 0 && !(ok = full(2 * j + 1))) break;
+                    for (int h = 0; h < 2 && ok; ++h) {
+                        if (!(ok = bulk_wait(&p_ready[w][h], (uint32_t)j & 1, &dead, p.err))) break;
+                        tc_fence_after();
+                        pv(w, j, h);
+                    }
+                    if (!ok) break;
+                    if (w == tiles - 1) tc_commit(&kv_free[(2 * j + 1) % NS]);
+                    if (j + 1 < nt) {
+                        if (w == 0 && !(ok = full(2 * j + 2))) break;
+                        tc_fence_after();
+                        qk(w, j + 1);
                     }
                 }
             tc_commit(&o_done);  // after a failed wait too: whatever was issued ends before tensor memory is freed
         }
     } else if (wg < tiles) {
         const uint32_t lane_at = (uint32_t)(warp & 3) * 32u << 16;
-        const uint32_t O = o_at(wg) + lane_at;
-        const float cm = cmul[tid];
+        const uint32_t S = s_at(wg) + lane_at, O = o_at(wg) + lane_at;
+        const float cm = fmaxf(cmul[tid], 1e-36f);  // (-inf * 0 would be NaN; below this every score is 0)
         const int wtid = tid & 127;
         float mref = 0.f, l = 0.f;
         bool ok = true;
         for (int j = 0; j < nt; ++j) {
             const int c0 = t0 + j * NK;
             const bool masked = c0 + NK > min(seen_by_all, t1);
-            const uint32_t S = s_at(wg, j) + lane_at;
-            ok = __all_sync(0xffffffffu, bulk_wait(&s_full[wg][j & 1], (uint32_t)(j >> 1) & 1, &dead, p.err));
+            ok = __all_sync(0xffffffffu, bulk_wait(&s_full[wg], (uint32_t)j & 1, &dead, p.err));
             if (!ok) break;
             tc_fence_after();
-            uint32_t s[NK];
-            tc_ld32(S, s);
-            tc_ld32(S + 32, s + 32);
-            tc_wait_ld();
-            tc_loaded(s);
-            tc_loaded(s + 32);
+            // S in blocks of 32 columns, the next one on its way: f(block, its first column)
+            auto each_block = [&](auto&& f) {
+                uint32_t s[2][32];
+                tc_ld32(S, s[0]);
+#pragma unroll
+                for (int k = 0; k < NK; k += 32) {
+                    uint32_t* cur = s[k >> 5 & 1];
+                    tc_wait_ld();
+                    tc_loaded(cur);
+                    if (k + 32 < NK) tc_ld32(S + k + 32, s[(k >> 5 & 1) ^ 1]);
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (c0 + k + e >= lim) cur[e] = 0xff800000u;  // -inf
+                    }
+                    f(cur, k);
+                }
+            };
             // ---- the maximum
             float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (masked) {
+            each_block([&](const uint32_t* s, int) {
 #pragma unroll
-                for (int e = 0; e < NK; ++e)
-                    if (c0 + e < lim) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
-            } else {
-#pragma unroll
-                for (int e = 0; e < NK; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
-            }
+                for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
+            });
             const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * cm;
             if (j == 0) {
                 mref = mx > -INFINITY ? mx : 0.f;
             } else if (__any_sync(0xffffffffu, mx > mref + kBulkSlack)) {
                 const float next = fmaxf(mref, mx), corr = ex2(mref - next);
                 mref = next;
-                l *= corr;
-                ok = __all_sync(0xffffffffu, bulk_wait(&pv_done[wg], (uint32_t)(j - 1) & 1, &dead, p.err));
-                if (!ok) break;
-                tc_fence_after();
+                l *= corr;  // (PV(j - 1) is complete: QK(j), which S is of, was issued behind it)
 #pragma unroll 1
                 for (int k = 0; k < D; k += 16) {
                     uint32_t o[16];
@@ -448,42 +472,9 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             const float shift = F32 ? -mref : 7.f - mref;
             const uint64_t cm2 = f2_pack(cm, cm), sh2 = f2_pack(shift, shift), gain2 = f2_pack(kPaGain, kPaGain);
             uint64_t sum2[2] = {0, 0};
-#pragma unroll
-            for (int k = 0; k < NK; k += 32) {
-                uint32_t hi[16], lo[F32 ? 16 : 1];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float a, b;
-                    f2_unpack(f2_fma(f2_pack(__uint_as_float(s[k + 2 * e]), __uint_as_float(s[k + 2 * e + 1])), cm2, sh2), a, b);
-                    a = ex2(a);
-                    b = ex2(b);
-                    if (masked) {
-                        if (c0 + k + 2 * e >= lim) a = 0.f;
-                        if (c0 + k + 2 * e + 1 >= lim) b = 0.f;
-                    }
-                    uint64_t ab = f2_pack(a, b);
-                    sum2[e & 1] = f2_add(sum2[e & 1], ab);
-                    if constexpr (F32) {
-                        ab = f2_mul(ab, gain2);
-                        f2_unpack(ab, a, b);
-                    }
-                    const __half2 h = __floats2half2_rn(a, b);
-                    hi[e] = *reinterpret_cast<const uint32_t*>(&h);
-                    if constexpr (F32) {
-                        const float2 f = __half22float2(h);
-                        const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
-                        lo[e] = *reinterpret_cast<const uint32_t*>(&r);
-                    }
-                }
-                tc_st16(S + k / 2, hi);
-                if constexpr (F32) tc_st16(S + NK / 2 + k / 2, lo);
-            }
-            float a, b;
-            f2_unpack(f2_add(sum2[0], sum2[1]), a, b);
-            l += a + b;
             if (masked) {  // V where not every column sees: nothing but finite values may meet a zero weight
-                bulk_wait(&kv_full[j % NS], (uint32_t)(j / NS) & 1, &dead, p.err);
-                uint8_t* V = stages + (size_t)(j % NS) * STAGE + VOFF;
+                full(2 * j + 1);
+                uint8_t* V = ring + (size_t)((2 * j + 1) % NS) * SLOT;
                 for (int k = wtid; k < NK * (D / 8); k += 128) {
                     const int r = k / (D / 8), ch = k % (D / 8), t = c0 + r;
                     if (t < seen_by_all && t < t1) continue;
@@ -505,9 +496,40 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_ready[wg][j & 1]);
+            uint32_t lo[F32 ? 32 : 1];  // of a half: stored once both its blocks of S are read
+            each_block([&](const uint32_t* s, int k) {
+                uint32_t hi[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float a, b;
+                    f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), cm2, sh2), a, b);
+                    a = ex2(a);
+                    b = ex2(b);
+                    uint64_t ab = f2_pack(a, b);
+                    sum2[e & 1] = f2_add(sum2[e & 1], ab);
+                    if constexpr (F32) {
+                        ab = f2_mul(ab, gain2);
+                        f2_unpack(ab, a, b);
+                    }
+                    const __half2 h = __floats2half2_rn(a, b);
+                    hi[e] = *reinterpret_cast<const uint32_t*>(&h);
+                    if constexpr (F32) {
+                        const float2 f = __half22float2(h);
+                        const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+                        lo[(k >> 1 & 16) + e] = *reinterpret_cast<const uint32_t*>(&r);
+                    }
+                }
+                tc_st16(S + (k >> 6) * 64 + (k >> 1 & 16), hi);
+                if (k & 32) {  // a half is written
+                    if constexpr (F32) tc_st32(S + (k >> 6) * 64 + 32, lo);
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&p_ready[wg][k >> 6]);
+                }
+            });
+            float a, b;
+            f2_unpack(f2_add(sum2[0], sum2[1]), a, b);
+            l += a + b;
         }
         ok = __all_sync(0xffffffffu, bulk_wait(&o_done, 0, &dead, p.err)) && ok;
         tc_fence_after();

@@ -116,6 +116,7 @@ int check_attention(const laic_kv_pages& g, const laic_kv_attention_args& a) {
     if (a.heads < 1 || a.heads % g.kv_heads) return api_fail(LAIC_E_INVALID, "heads must be a multiple of kv_heads");
     if (a.heads / g.kv_heads > 8) return api_fail(LAIC_E_UNSUPPORTED, "at most 8 query heads per kv head");
     if (!type_ok(a.type)) return api_fail(LAIC_E_UNSUPPORTED, "query and output type must be F32 or F16");
+    if (!(a.scale >= 0.f)) return api_fail(LAIC_E_INVALID, "scale must not be negative");
     if (a.max_len < 0 || a.groups < 0 || a.max_private < -1) return api_fail(LAIC_E_INVALID, "negative bound");
     if (a.groups && (a.max_group_rows < 1 || a.max_shared < 0 || a.max_group_rows > a.rows))
         return api_fail(LAIC_E_INVALID, "groups need max_group_rows in [1, rows] and max_shared >= 0");

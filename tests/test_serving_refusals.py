@@ -71,7 +71,8 @@ def test_append_null_and_in_place_refused():
     (dict(type=8), UNSUPPORTED, "F32 or F16"), (dict(max_len=33), INVALID, "must not exceed"),
     (dict(max_len=-1), INVALID, "negative"), (dict(max_private=-2), INVALID, "negative"),
     (dict(groups=1), INVALID, "max_group_rows"), (dict(groups=1, max_group_rows=2), INVALID, "max_group_rows"),
-    (dict(groups=1, max_group_rows=1, max_shared=33), INVALID, "must not exceed"), (dict(rows=-1), INVALID, "rows")])
+    (dict(groups=1, max_group_rows=1, max_shared=33), INVALID, "must not exceed"), (dict(rows=-1), INVALID, "rows"),
+    (dict(scale=-0.5), INVALID, "scale"), (dict(scale=float("nan")), INVALID, "scale")])
 def test_attention_bounds_refused(kw, code, text):
     a = dict(rows=1, heads=4, nseq=1, pages_per_seq=2, max_len=32)
     a.update(kw)
