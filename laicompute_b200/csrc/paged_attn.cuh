@@ -124,9 +124,8 @@ __device__ __forceinline__ void find_group(const KvAttnParams& p, int r, int tid
         if (group_rows(p, g, r0, r1) && r >= r0 && r < r1) *found = group_shared(p, g);
     }
 }
-__host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int shared) {
+__host__ __device__ inline RowView row_view(const KvAttnParams& p, int n, int s, int shared) {  // n, s: len[r], seq[r]
     RowView v;
-    const int n = p.len[r], s = p.seq ? p.seq[r] : r;  // (both loads at once)
     v.n = -1;
     v.seq = -1;
     v.shared = 0;
@@ -140,6 +139,9 @@ __host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int sh
     }
     v.shared = v.n < shared ? v.n : shared;
     return v;
+}
+__host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int shared) {
+    return row_view(p, p.len[r], p.seq ? p.seq[r] : r, shared);
 }
 
 template <typename T>
@@ -178,22 +180,33 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
     }
     __syncthreads();
 
-    const int nch = (t1 - t0 + kPaChunk - 1) / kPaChunk;
+    // chunks start at a multiple of 16, so that 16 positions lie in one page (positions before t0 are masked)
+    const int a0 = t0 & ~15;
+    const int nch = (t1 - a0 + kPaChunk - 1) / kPaChunk;
     const uint32_t ring = smem_u32(smem);
-    const size_t head_run = (size_t)D << p.page_shift;  // elements of a (page, head) pair
+    constexpr uint32_t STAGE = 2 * kPaChunk * D * 2;
+    constexpr int RPP = NTH / CPR;  // rows a pass of the CTA covers; a thread's row within 8 stays the same
+    const int lrow = tid / CPR, lcc = tid % CPR;
+    const uint32_t dst0 = ring + 2 * attn_swz<D>(lrow, lcc);
+    const size_t src0 = (size_t)(lrow & 15) * D + lcc * 8;
+    const int page_mask = (1 << p.page_shift) - 1;
     auto load = [&](int ch) {
         if (ch < nch) {
-            const uint32_t ks = ring + (uint32_t)(ch % NST) * (2 * kPaChunk * D * 2);
-            const uint32_t vs = ks + kPaChunk * D * 2;
+            const int c0 = a0 + ch * kPaChunk;
+            const uint32_t kd = dst0 + (uint32_t)(ch % NST) * STAGE;
+            size_t off = 0;
 #pragma unroll
-            for (int i = tid; i < kPaChunk * CPR; i += NTH) {
-                const int r = i / CPR, cc = i % CPR, t = t0 + ch * kPaChunk + r;
-                const bool live = t < t1;
-                const int tt = live ? t : t0;
-                const size_t off = ((size_t)page_ids[(tt >> p.page_shift) - first_page] * p.kv_heads + kvh) * head_run +
-                                   (size_t)(tt & ((1 << p.page_shift) - 1)) * D + cc * 8;
-                cp_async16_z(ks + 2 * attn_swz<D>(r, cc), p.kp + off, live);
-                cp_async16_z(vs + 2 * attn_swz<D>(r, cc), p.vp + off, live);  // rows past the end: zeros
+            for (int i = 0; i < kPaChunk / RPP; ++i) {
+                const int r = lrow + i * RPP;
+                if (RPP >= 16 || i % (16 / RPP) == 0) {  // a new block of 16 positions
+                    const int tb = c0 + (r & ~15);
+                    const int page = tb < t1 ? page_ids[(tb >> p.page_shift) - first_page] : 0;
+                    off = ((((size_t)page * p.kv_heads + kvh) << p.page_shift) + (tb & page_mask)) * D + src0;
+                }
+                const size_t at = off + (RPP < 16 ? (i % (16 / RPP)) * RPP * D : 0);
+                const bool live = c0 + r < t1;  // rows past the end: zeros
+                cp_async16_z(kd + i * RPP * D * 2, p.kp + at, live);
+                cp_async16_z(kd + kPaChunk * D * 2 + i * RPP * D * 2, p.vp + at, live);
             }
         }
         cp_async_commit();
@@ -250,12 +263,19 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
     const int li = lane >> 3, lr = lane & 7;  // ldmatrix: this lane addresses row lr of matrix li
     const int wp = warp * 16;                 // this warp's first position of a chunk
 
+    uint2 qr[NT == 1 ? KS : 1][HN];  // one tile: the query fragments stay in registers
     for (int ch = 0; ch < nch; ++ch) {
         cp_async_wait<NST - 2>();
         __syncthreads();  // chunk ch is in shared memory, and chunk ch - 1 consumed
+        if (NT == 1 && ch == 0) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int hl = 0; hl < HN; ++hl) qr[ks][hl] = *reinterpret_cast<const uint2*>(qf + ((ks * HN + hl) * 32 + lane) * 2);
+        }
         load(ch + NST - 1);
-        const int c0 = t0 + ch * kPaChunk;
-        if (c0 + wp < t1) {
+        const int c0 = a0 + ch * kPaChunk;
+        if (c0 + wp < t1 && c0 + wp + 16 > t0) {
             const uint32_t ks_a = ring + (uint32_t)(ch % NST) * (2 * kPaChunk * D * 2), vs_a = ks_a + kPaChunk * D * 2;
             float s[NT][4], sl[NT][4];
 #pragma unroll
@@ -270,16 +290,16 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const uint32_t* qa = qf + (((ks * NT + nt) * HN) * 32 + lane) * 2;
-                    const uint2 b = *reinterpret_cast<const uint2*>(qa);
+                    const uint2 b = NT == 1 ? qr[NT == 1 ? ks : 0][0] : *reinterpret_cast<const uint2*>(qa);
                     mma16816_acc(s[nt], a[0], a[1], a[2], a[3], b.x, b.y);
                     if (HL) {
-                        const uint2 bl = *reinterpret_cast<const uint2*>(qa + 64);
+                        const uint2 bl = NT == 1 ? qr[NT == 1 ? ks : 0][HN - 1] : *reinterpret_cast<const uint2*>(qa + 64);
                         mma16816_acc(sl[nt], a[0], a[1], a[2], a[3], bl.x, bl.y);
                     }
                 }
             }
             const int pos = c0 + wp + gq;
-            const bool full = c0 + wp + 16 <= min(t1, minlim);  // every live column sees all 16 positions
+            const bool full = c0 + wp >= t0 && c0 + wp + 16 <= min(t1, minlim);  // every live column sees all 16 positions
             uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -296,7 +316,8 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                     if (HL) s[nt][e] += sl[nt][e];
                     if (PK) s[nt][e] += __shfl_xor_sync(0xffffffffu, s[nt][e], 2);
                     const float x = s[nt][e] * cm2[e & 1];
-                    if (full || pos + (e >> 1) * 8 < lm[e & 1]) mx[e & 1] = fmaxf(mx[e & 1], x);
+                    const int at = pos + (e >> 1) * 8;
+                    if (full || (at < lm[e & 1] && at >= t0)) mx[e & 1] = fmaxf(mx[e & 1], x);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -313,7 +334,8 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     pv[e] = ex2(fmaf(s[nt][e], cm2[e & 1], -mx[e & 1]));
-                    if (!full && pos + (e >> 1) * 8 >= lm[e & 1]) pv[e] = 0.f;
+                    const int at = pos + (e >> 1) * 8;
+                    if (!full && (at >= lm[e & 1] || at < t0)) pv[e] = 0.f;
                     sum[e & 1] += pv[e];
                     pv[e] *= kPaGain;
                 }
@@ -330,10 +352,12 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                     }
                     ph[nt][j] = movm_t(pack_h2(h0, h1));
                 }
+                if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
-                for (int mt = 0; mt < KS; ++mt) {
-                    o[mt][nt][0] *= corr[0]; o[mt][nt][1] *= corr[1];
-                    o[mt][nt][2] *= corr[0]; o[mt][nt][3] *= corr[1];
+                    for (int mt = 0; mt < KS; ++mt) {
+                        o[mt][nt][0] *= corr[0]; o[mt][nt][1] *= corr[1];
+                        o[mt][nt][2] *= corr[0]; o[mt][nt][3] *= corr[1];
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[nt][e] = PK && c >= 2 ? 0.f : pv[e];
@@ -341,7 +365,7 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             // a position that some columns see and others do not: where its value is not finite,
             // 0 * inf would reach the others, so those products are summed one by one
             bool odd = false;
-            if (!full && min(c0 + wp + 16, t1) > minlim) {
+            if (!full && min(c0 + wp + 16, t1) > minlim) {  // (positions before t0 are seen too, by other items)
 #pragma unroll
                 for (int i = lane; i < 16 * CPR; i += 32) {
                     const uint4 w = lds128(vs_a + 2 * attn_swz<D>(wp + i / CPR, i % CPR));
@@ -463,6 +487,7 @@ __device__ __forceinline__ void private_item(const KvAttnParams& p, int i, int* 
     const int tid = threadIdx.x, split = i % p.nsp;
     i /= p.nsp;
     const int kvh = i % p.kv_heads, r = i / p.kv_heads;
+    const int len = p.len[r], sq = p.seq ? p.seq[r] : r;  // under way while the groups are searched
     int shared = 0;
     if (p.groups) {
         if (tid == 0) *found = 0;
@@ -471,7 +496,7 @@ __device__ __forceinline__ void private_item(const KvAttnParams& p, int i, int* 
         __syncthreads();
         shared = *found;
     }
-    const RowView v = row_view(p, r, shared);
+    const RowView v = row_view(p, len, sq, shared);
     if (v.n < 0) return;
     if (v.n - v.shared > p.max_private && tid == 0) kv_flag(p.err, kKvBadPos);
     const int t0 = v.shared + split * p.lp, t1 = min(min(v.n, v.shared + p.max_private), t0 + p.lp);
@@ -550,11 +575,12 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
     const int pair = blockIdx.x * kPmWarps + warp;
     const bool in = pair < p.rows * p.heads;
     const int r = in ? pair / p.heads : 0, h = in ? pair % p.heads : 0;
+    const int len = p.len[r], sq = p.seq ? p.seq[r] : r;
     if (lane == 0) found[warp] = 0;
     __syncwarp();
     find_group(p, r, lane, 32, &found[warp]);
     __syncwarp();
-    const RowView v = row_view(p, r, found[warp]);
+    const RowView v = row_view(p, len, sq, found[warp]);
     pdl_wait();
     if (!in || v.n < 0) return;
     const int ns = p.nss + p.nsp;
@@ -576,7 +602,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
             L = fmaf(ml.y, w, L);
         }
         const int n = min(32, live - i0);
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < n; ++i) {
             const float wi = __shfl_sync(0xffffffffu, w, i);
             const float* src = p.part_o + (base + slot(i0 + i)) * D + lane * E;

@@ -236,12 +236,39 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     double total = 0.0, before = 0.0;
     int owner = -1;
     for (int pass = 0; pass < 2; ++pass) {
-        double a = 0.0;
-#pragma unroll 8
-        for (int i = v0 + lane * 4; i < v1; i += 128) {
+        double a = 0.0, a2 = 0.0;
+        const bool sub = mode && Q;
+        int i = v0 + lane * 4;
+        constexpr int U = 4;  // steps whose loads are in flight together
+        for (; VEC && i - lane * 4 + U * 128 <= v1; i += U * 128) {
+            float4 x[U], q[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[u] = __ldcs(reinterpret_cast<const float4*>(P + i + u * 128));
+            if (sub) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) q[u] = __ldcs(reinterpret_cast<const float4*>(Q + i + u * 128));
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float xs[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+                const float qs[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // (p - q where p > q: exact in 64 bits; NaN compares false)
+                    if (sub) {
+                        const float qv = prob_in(qs[e]);
+                        if (xs[e] > qv) { a += (double)xs[e]; a2 += (double)qv; }
+                    } else if (xs[e] > 0.f && (mode == 0 || (unsigned)(i + u * 128 + e) != hole)) {
+                        a += (double)xs[e];
+                    }
+                }
+            }
+        }
+        a -= a2;
+        for (; i < v1; i += 128) {
             float x[4], q[4] = {};
             four(P, i, x);
-            if (mode && Q) four(Q, i, q);
+            if (sub) four(Q, i, q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) a += value(x[e], q[e], i + e);
         }
