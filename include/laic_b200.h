@@ -76,6 +76,10 @@ typedef struct laic_dev_desc {
                                      decode-step kernel where it applies (off by default: per-projection launches
                                      measured faster) */
 
+#define LAIC_FLAG_PAGED_KV 512u /* the KV cache in pages of 64 positions: slots may share a prompt's pages
+                                   (laic_dev_fork_slot) and several tokens per slot may be checked in one step
+                                   (laic_dev_verify). FP16 KV, one GPU; laic_dev_step runs no step ahead */
+
 /* Device-side options (no counterpart in the reference, which is CPU-only). */
 typedef struct laic_dev_opts {
     int32_t device;       /* CUDA device ordinal */
@@ -147,6 +151,23 @@ LAIC_API int laic_dev_prefill_batch(laic_dev* dev, int32_t slot, const uint32_t*
  * LAIC_FLAG_NO_SPECULATION turns it off. */
 LAIC_API int laic_dev_step(laic_dev* dev, int32_t nseq, const uint32_t* tokens, const int32_t* slots,
                   const laic_sample_params* params, int32_t nparams, uint32_t* out_ids, float* out_logits);
+
+/* Engines with LAIC_FLAG_PAGED_KV: slot dst becomes a copy of slot src (cache, position, history). Whole pages
+ * are shared, the partly filled one is copied. Slots that share pages and stand next to each other in a step's
+ * list have their shared positions read once for all. No counterpart in the reference. */
+LAIC_API int laic_dev_fork_slot(laic_dev* dev, int32_t src, int32_t dst);
+
+/* Engines with LAIC_FLAG_PAGED_KV: speculative decoding's step. tokens [nseq][max_draft + 1] holds for each
+ * sequence the token laic_dev_step would take next and n_draft drafted ones; all go through the model together
+ * (nseq * (max_draft + 1) <= 64), and laic_verify_drafts decides on the drafted ones with the target's
+ * probabilities softmax(logits / temperature) (temperature <= 0: the first maximum) and numbers from
+ * mt19937_64(seed). draft_probs_dev: device memory [nseq][max_draft][vocab] the drafts were drawn from, or NULL
+ * (drafted with certainty). out_ids [nseq][max_draft + 1] receives the tokens that follow, out_n how many; the
+ * last one is not in the cache yet. Positions advance by out_n. top_k, top_p and repeat_penalty must be off. No
+ * counterpart in the reference. */
+LAIC_API int laic_dev_verify(laic_dev* dev, int32_t nseq, const int32_t* slots, int32_t max_draft, const uint32_t* tokens,
+                             const int32_t* n_draft, const float* draft_probs_dev, const laic_sample_params* params,
+                             int32_t nparams, uint32_t* out_ids, int32_t* out_n);
 
 /* Forget a slot's KV cache and token history (generate_ids' cache reset). */
 LAIC_API int laic_dev_reset_slot(laic_dev* dev, int32_t slot);

@@ -15,6 +15,7 @@ LAIC_E_INVALID, LAIC_E_CUDA, LAIC_E_NCCL, LAIC_E_CONTEXT, LAIC_E_UNSUPPORTED, LA
 FLAG_NO_GRAPH, FLAG_NO_PDL, FLAG_KV_F32, FLAG_LAYER_LAUNCHES, FLAG_TRACE, FLAG_STEP_KERNEL = 1, 2, 4, 8, 16, 32
 FLAG_Q4_0_UPSTREAM = 128
 FLAG_NO_SPECULATION = 256
+FLAG_PAGED_KV = 512
 
 # Every entry point include/laic_b200.h declares (checked by the tests).
 EXPORTS = (
@@ -25,7 +26,7 @@ EXPORTS = (
     "laic_dev_prefill_batch", "laic_tensor_check", "laic_selftest_peer_timeout",
     "laic_dev_step_trace", "laic_blocks_convert",
     "laic_kv_append", "laic_kv_attention", "laic_kv_attention_workspace", "laic_kv_check", "laic_logits_probs",
-    "laic_verify_drafts",
+    "laic_verify_drafts", "laic_dev_fork_slot", "laic_dev_verify",
 )
 
 
@@ -139,6 +140,8 @@ def lib() -> ctypes.CDLL:
                                       ctypes.POINTER(I32)]
     L.laic_selftest_peer_timeout.argtypes = [I32, ctypes.c_int64, ctypes.POINTER(I32)]
     L.laic_blocks_convert.argtypes = [I32, P, U64, ctypes.c_uint32, ctypes.POINTER(I32), P, U64, ctypes.POINTER(U64)]
+    L.laic_dev_fork_slot.argtypes = [P, I32, I32]
+    L.laic_dev_verify.argtypes = [P, I32, P, I32, P, P, P, ctypes.POINTER(SampleParams), I32, P, P]
     KP = ctypes.POINTER(KvPagesDesc)
     I64 = ctypes.c_int64
     L.laic_kv_append.argtypes = [KP, ctypes.POINTER(KvAppendArgs), P]
@@ -148,7 +151,7 @@ def lib() -> ctypes.CDLL:
     L.laic_logits_probs.argtypes = [I32, I32, I32, P, I64, P, P, I64, P]
     L.laic_verify_drafts.argtypes = [I32, ctypes.POINTER(VerifyArgs), P]
     for name in ("laic_kv_append", "laic_kv_attention", "laic_kv_attention_workspace", "laic_kv_check",
-                 "laic_logits_probs", "laic_verify_drafts", "laic_dev_create", "laic_dev_upload", "laic_dev_prefill", "laic_dev_step", "laic_dev_reset_slot",
+                 "laic_logits_probs", "laic_verify_drafts", "laic_dev_fork_slot", "laic_dev_verify", "laic_dev_create", "laic_dev_upload", "laic_dev_prefill", "laic_dev_step", "laic_dev_reset_slot",
                  "laic_dev_slot_pos", "laic_dev_fill_kv", "laic_dev_sync", "laic_dev_stats_get",
                  "laic_dev_decode", "laic_dev_profile", "laic_nccl_unique_id", "laic_tensor_create", "laic_tensor_matvec",
                  "laic_tensor_dequant", "laic_tensor_matvec_noalloc", "laic_dev_prefill_batch", "laic_tensor_check",

@@ -26,6 +26,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
@@ -503,7 +504,12 @@ enum : unsigned { H_ANORM = 1, H_Q = 2, H_K = 4, H_V = 8, H_O = 16, H_FNORM = 32
 // previous step's sampled ids, slots and parameters already on the device), outputs like
 // MODE_STEP (ids and error words copied to pinned host memory: buffer 0 or 1, so that the
 // next guess can be queued before this one's outputs are read).
-enum StepMode : int { MODE_PREFILL = 0, MODE_STEP = 1, MODE_CHAIN = 2, MODE_SPEC0 = 3, MODE_SPEC1 = 4 };
+// MODE_VERIFY: laic_dev_verify's rows (several tokens per slot), whose logits go to the check of the
+// drafted tokens instead of the sampler.
+enum StepMode : int { MODE_PREFILL = 0, MODE_STEP = 1, MODE_CHAIN = 2, MODE_SPEC0 = 3, MODE_SPEC1 = 4, MODE_VERIFY = 5 };
+
+constexpr int kKvPage = 64;      // positions per page of an engine's paged cache
+constexpr int kMaxRows = 64;     // rows of one step (the matvec kernels' largest batch)
 
 }  // namespace
 
@@ -588,7 +594,7 @@ struct laic_dev {
     static constexpr int kPfRows = 512;  // tokens per pass
     float *pf_x = nullptr, *pf_c = nullptr, *pf_q = nullptr, *pf_attn = nullptr;
     __half *pf_a = nullptr, *pf_w = nullptr;
-    int *pf_slots = nullptr, *pf_npos = nullptr;
+    int *pf_slots = nullptr, *pf_npos = nullptr, *pf_len = nullptr, *pf_group = nullptr;
     unsigned* pf_tokens = nullptr;
     void* pf_ws = nullptr;
     size_t pf_ws_bytes = 0;
@@ -622,7 +628,146 @@ struct laic_dev {
     laic::SampleDev* h_params = nullptr;
     std::vector<long long> h_pos;
 
+    // LAIC_FLAG_PAGED_KV: the cache in pages (serving.cuh), its page table on the host and the device
+    bool paged = false;
+    int RB = 0;                  // rows the activation buffers hold
+    int pps = 0, npages = 0;     // pages per slot, pages in the pool
+    __half *pk = nullptr, *pv = nullptr;  // [layer][page][kv head][position][dim]
+    std::vector<int> ptab, pref, pfree;   // page table [slot][pps] (-1: none), references per page, free pages
+    int *d_table = nullptr, *h_table = nullptr;
+    int *d_rpos = nullptr, *d_rlen = nullptr, *d_groups = nullptr;  // per row; groups: [RB + 1] first rows, [RB] lengths
+    int* h_rows = nullptr;       // pinned staging: [RB] positions, [RB] lengths, [2 RB + 1] groups
+    float* qkv = nullptr;        // [RB][hq + 2 kv]
+    void* attn_ws = nullptr;
+    size_t attn_ws_cap = 0;
+    struct KvBounds {            // what a captured step's attention is launched for
+        int groups = 0, group_rows = 0, shared = 0, priv = 0, len = 0;
+    } kb;
+    // laic_dev_verify
+    float *vf_probs = nullptr, *vf_temp = nullptr, *vf_u = nullptr;  // u: [RB] accept, [RB] sample
+    unsigned* vf_ids = nullptr;  // drafted ids [nseq][max_draft], then out ids [nseq][max_draft + 1]
+    int* vf_n = nullptr;         // drafted counts, then out counts
+    const float* vf_draft = nullptr;
+    int vf_nseq = 0, vf_max = 0;
+
+    // The whole-page prefix that two slots' page tables share, in pages.
+    int common_pages(int a, int b) const {
+        int n = 0;
+        while (n < pps && ptab[(size_t)a * pps + n] >= 0 && ptab[(size_t)a * pps + n] == ptab[(size_t)b * pps + n]) ++n;
+        return n;
+    }
+    // Pages for positions below `end` of a slot. The pool holds every slot's capacity, so there is always a free one.
+    void grow_slot(int slot, long long end) {
+        for (long long i = 0; i * kKvPage < end; ++i) {
+            int& e = ptab[(size_t)slot * pps + i];
+            if (e >= 0) continue;
+            e = pfree.back();
+            pfree.pop_back();
+            pref[e] = 1;
+        }
+    }
+    void drop_slot(int slot) {
+        for (int i = 0; i < pps; ++i) {
+            int& e = ptab[(size_t)slot * pps + i];
+            if (e >= 0 && --pref[e] == 0) pfree.push_back(e);
+            e = -1;
+        }
+    }
+    laic_kv_pages layer_pages(int l) const {
+        const size_t off = (size_t)l * npages * Hkv * kKvPage * D;
+        return laic_kv_pages{device, Hkv, D, kKvPage, npages, pk + off, pv + off, mvs.err};
+    }
+    laic_kv_append_args append_args(int rows, const float* c, float* qout) const {
+        laic_kv_append_args a{};
+        a.rows = rows; a.heads = H; a.in_type = a.q_type = LAIC_GGML_F32;
+        a.rope_dim = 2 * rope_pairs; a.rope_positions = cap;
+        a.nseq = S; a.pages_per_seq = pps;
+        a.ldq = a.ldk = a.ldv = hq + 2 * kv; a.ldqo = hq;
+        a.q_dev = c; a.k_dev = c + hq; a.v_dev = c + hq + kv; a.q_out_dev = qout;
+        a.page_table_dev = d_table; a.rope_dev = reinterpret_cast<const float*>(rope_cs);
+        return a;
+    }
+    laic_kv_attention_args attention_args(int rows, const KvBounds& b) const {
+        laic_kv_attention_args a{};
+        a.rows = rows; a.heads = H; a.type = LAIC_GGML_F32; a.nseq = S; a.pages_per_seq = pps;
+        a.max_len = b.len; a.groups = b.groups; a.max_group_rows = b.group_rows; a.max_shared = b.shared; a.max_private = b.priv;
+        a.ldq = a.ldo = hq;
+        a.page_table_dev = d_table;
+        a.group_rows_dev = d_groups; a.group_len_dev = d_groups + RB + 1;
+        a.workspace_dev = attn_ws; a.workspace_bytes = attn_ws_cap;
+        return a;
+    }
+    // A bound for a captured step: the next power of two, so that a growing context recaptures seldom.
+    int bucket(long long n) const {
+        long long b = 256;
+        while (b < n) b *= 2;
+        return (int)std::min<long long>(n ? b : 0, (long long)pps * kKvPage);
+    }
+    int reserve_attn_ws(int rows, const KvBounds& b) {
+        uint64_t need = 0;
+        if (int rc = laic::kv_attention_bytes(layer_pages(0), attention_args(rows, b), &need)) return rc;
+        if (need <= attn_ws_cap) return LAIC_OK;
+        if (attn_ws) cudaFree(attn_ws);
+        attn_ws = nullptr;
+        attn_ws_cap = 0;
+        CK(cudaMalloc(&attn_ws, need));
+        attn_ws_cap = need;
+        drop_graphs();
+        return LAIC_OK;
+    }
+    void drop_graphs() {
+        for (auto& kv : graphs) cudaGraphExecDestroy(kv.second);
+        graphs.clear();
+        for (auto& kv : paged_graphs) cudaGraphExecDestroy(kv.second);
+        paged_graphs.clear();
+    }
+    int upload_table() {
+        std::copy(ptab.begin(), ptab.end(), h_table);
+        CK(cudaMemcpyAsync(d_table, h_table, ptab.size() * sizeof(int), cudaMemcpyHostToDevice, st));
+        return LAIC_OK;
+    }
+    // Before `steps` steps of the listed slots (the stream is idle): pages for their new positions, and
+    // the groups: consecutive listed slots whose page tables start with the same pages.
+    int paged_prepare(int nseq, const int* slots, int steps) {
+        for (int i = 0; i < nseq; ++i) grow_slot(slots[i], h_pos[slots[i]] + steps);
+        if (int rc = upload_table()) return rc;
+        int* starts = h_rows + 2 * RB;
+        int* lens = starts + RB + 1;
+        KvBounds b;
+        long long len = 0, priv = 0, shared = 0;
+        for (int i = 0; i < nseq;) {
+            int j = i + 1, pages = pps;
+            for (; j < nseq; ++j) {
+                const int c = std::min(pages, common_pages(slots[i], slots[j]));
+                if (c < 1) break;
+                pages = c;
+            }
+            long long common = j - i > 1 ? (long long)pages * kKvPage : 0;  // (a row alone: a group that shares nothing)
+            for (int k = i; k < j; ++k) common = std::min(common, h_pos[slots[k]]);
+            if (common == 0) j = i + 1;
+            starts[b.groups] = i;
+            lens[b.groups++] = (int)common;
+            b.group_rows = std::max(b.group_rows, j - i);
+            shared = std::max(shared, common);
+            for (int k = i; k < j; ++k) {
+                len = std::max(len, h_pos[slots[k]] + steps);
+                priv = std::max(priv, h_pos[slots[k]] + steps - common);
+            }
+            i = j;
+        }
+        starts[b.groups] = nseq;
+        if (shared == 0) b.groups = b.group_rows = 0;
+        b.len = bucket(len);
+        b.priv = bucket(priv);
+        b.shared = bucket(shared);
+        kb = b;
+        if (b.groups)
+            CK(cudaMemcpyAsync(d_groups, starts, (2 * RB + 1) * sizeof(int), cudaMemcpyHostToDevice, st));
+        return reserve_attn_ws(nseq, b);
+    }
+
     std::map<std::pair<int, int>, cudaGraphExec_t> graphs;  // (nseq, mode) -> graph
+    std::map<std::array<int, 7>, cudaGraphExec_t> paged_graphs;  // (rows, mode, KvBounds) -> graph
     MvScratch mvs;  // split-K partials and tickets of the matvec launches
     int last_split = 1;
 
@@ -760,10 +905,10 @@ struct laic_dev {
         auto t_end = [&]() {
             if (timer) cudaEventRecord(timer->ev.back().second.second, s);
         };
-        if (mode == MODE_PREFILL || mode == MODE_STEP) {  // chained / speculative steps read the ids the previous step sampled
+        if (mode == MODE_PREFILL || mode == MODE_STEP || mode == MODE_VERIFY) {  // chained / speculative steps read the ids the previous step sampled
             CK(cudaMemcpyAsync(d_tokens, h_tokens, nseq * sizeof(unsigned), cudaMemcpyHostToDevice, s));
             CK(cudaMemcpyAsync(d_slots, h_slots, nseq * sizeof(int), cudaMemcpyHostToDevice, s));
-            if (full) CK(cudaMemcpyAsync(d_params, h_params, nseq * sizeof(laic::SampleDev), cudaMemcpyHostToDevice, s));
+            if (full && mode != MODE_VERIFY) CK(cudaMemcpyAsync(d_params, h_params, nseq * sizeof(laic::SampleDev), cudaMemcpyHostToDevice, s));
         }
 
         const bool step_path = nseq == 1 && ls_ready;
@@ -792,6 +937,11 @@ struct laic_dev {
             CK(launch_k(laic::embed_kernel, dim3(nseq, ecta), dim3(256), 0, s, pdl, ep));
             ++nl;
             t_end();
+        }
+        if (paged && mode != MODE_VERIFY) {  // (a verification's rows come from the host)
+            CK(launch_k(laic::paged_rows_kernel, dim3(1), dim3(64), 0, s, pdl, (const int*)d_slots, (const int*)pos, nseq, d_rpos,
+                        d_rlen));
+            ++nl;
         }
 
         const int nsplit = nsplit_for(nseq);
@@ -825,14 +975,29 @@ struct laic_dev {
             p.kc = (char*)kc + (size_t)l * kv_layer_stride * kvb;
             p.vc = (char*)vc + (size_t)l * kv_layer_stride * kvb;
             p.kv_slot_stride = kv_slot_stride; p.kv_cap = cap;
+            if (paged) { p.out = qkv; p.ldo = hq + 2 * kv; }
             t_begin("qkv", (double)ly.qkv.bytes() + 4.0 * nseq * (h + ly.qkv.rows));
             RecIn r_qkv;
             if (recs || dprecs) {
                 r_qkv.xg = rec_x; r_qkv.mode = 1; r_qkv.ss = rec_ss; r_qkv.ss_tiles = l == 0 ? ecta : ntiles_h;
                 r_qkv.dp = dprecs;
             }
-            CK(launch_matvec(ly.qkv, p, laic::EPI_QKV, kv32, mvs, s, pdl, &nl, &r_qkv, !recs));
+            CK(launch_matvec(ly.qkv, p, paged ? laic::EPI_STORE : laic::EPI_QKV, kv32, mvs, s, pdl, &nl, &r_qkv, !recs));
             t_end();
+            if (paged) {  // into the pages, then attention over them
+                const laic_kv_pages pg = layer_pages(l);
+                laic_kv_append_args aa = append_args(nseq, qkv, q);
+                aa.pos_dev = d_rpos; aa.seq_dev = d_slots;
+                t_begin("kv_append", 4.0 * nseq * (2 * hq + 2 * kv) + 4.0 * nseq * kv);
+                if (int rc = laic::kv_append(pg, aa, s)) return rc;
+                t_end();
+                laic_kv_attention_args at = attention_args(nseq, kb);
+                at.q_dev = q; at.out_dev = attn; at.len_dev = d_rlen; at.seq_dev = d_slots;
+                t_begin("attention", attn_bytes);
+                if (int rc = laic::kv_attention(pg, at, s)) return rc;
+                t_end();
+                nl += 2;
+            }
             // attention
             laic::AttnParams ap{};
             ap.q = q; ap.ldq = hq; ap.out = attn; ap.ldo = hq;
@@ -840,6 +1005,7 @@ struct laic_dev {
             ap.heads = H; ap.kv_heads = Hkv; ap.slots = d_slots; ap.pos = pos; ap.nsplit = nsplit;
             ap.part = attn_part; ap.counters = attn_cnt; ap.sqrt_d = sqrtf((float)D); ap.err = mvs.err;
             ap.nseq = nseq; ap.rec_out = recs ? rec_attn : nullptr; ap.nbuf = attn_nbuf(nseq);
+            if (!paged) {
             t_begin("attention", attn_bytes);
             if (attn_cluster(nsplit, kv32))
                 CK(laic::launch_cluster_k(attn_pick(D, G, kv32, true), dim3(nsplit, Hkv, nseq), dim3(laic::kAttnWarps * 32),
@@ -849,12 +1015,14 @@ struct laic_dev {
                             pdl, ap));
             ++nl;
             t_end();
+            }
             // o + residual
             laic::MvParams po{};
             po.nseq = nseq; po.x = attn; po.ldx = hq; po.out = x; po.ldo = h;
             RecIn r_o;
             if (recs) {
-                po.rec_out = rec_x; po.rec_w = ly.ffn_norm; po.ss_out = rec_ss; r_o.xg = rec_attn; r_o.mode = 2;
+                po.rec_out = rec_x; po.rec_w = ly.ffn_norm; po.ss_out = rec_ss;
+                if (!paged) { r_o.xg = rec_attn; r_o.mode = 2; }  // (the paged attention writes no records)
             } else if (dprecs) {
                 po.ss_out = rec_ss; r_o.mode = 2; r_o.dp = true;
             }
@@ -916,6 +1084,21 @@ struct laic_dev {
                     ++nl;
                 }
                 t_end();
+            }
+            if (mode == MODE_VERIFY) {
+                t_begin("verify", 0);
+                if (int rc = laic::logits_probs(device, nseq, V, logits, V, vf_temp, vf_probs, V, s)) return rc;
+                laic_verify_args va{};
+                va.nseq = vf_nseq; va.max_draft = vf_max; va.vocab = V; va.ld_target = va.ld_draft = V;
+                va.target_dev = vf_probs; va.draft_dev = vf_draft;
+                va.draft_ids_dev = vf_ids; va.n_draft_dev = vf_n;
+                va.accept_u_dev = vf_u; va.sample_u_dev = vf_u + RB;
+                va.out_ids_dev = vf_ids + RB; va.out_n_dev = vf_n + RB;
+                if (int rc = laic::verify_drafts(device, va, s)) return rc;
+                nl += 2;
+                t_end();
+                launches_step = nl;
+                return LAIC_OK;
             }
             laic::SamplerParams sp{logits, V, V, d_slots, counts, d_params, nseq, d_out_ids, d_tokens, pos, d_err,
                                    samp_v, samp_i, samp_cnt};
@@ -1075,6 +1258,8 @@ struct laic_dev {
         CK(cudaMalloc(&pf_slots, T * 4));
         CK(cudaMalloc(&pf_npos, T * 4));
         CK(cudaMalloc(&pf_tokens, T * 4));
+        CK(cudaMalloc(&pf_len, T * 4));
+        CK(cudaMalloc(&pf_group, 3 * 4));
         for (auto& l : layers)
             for (const Mat* m : {&l.qkv, &l.o, &l.gu, &l.down})
                 pf_ws_bytes = std::max(pf_ws_bytes, laic::gemm_f16_workspace((int)T, m->rows, m->in));
@@ -1104,16 +1289,36 @@ struct laic_dev {
             const int p0 = (int)h_pos[slot];
             CK(cudaMemcpyAsync(pf_tokens, tokens + t0, (size_t)T * 4, cudaMemcpyHostToDevice, s));
             laic::prefill_rows_kernel<<<(T + 255) / 256, 256, 0, s>>>(slot, p0, T, pf_slots, pf_npos);
+            KvBounds fb;  // this pass's attention
+            if (paged) {
+                grow_slot(slot, p0 + T);
+                if (int rc = upload_table()) return rc;
+                fb.groups = 1; fb.group_rows = T; fb.shared = fb.len = p0 + T; fb.priv = 0;
+                if (int rc = reserve_attn_ws(T, fb)) return rc;
+                laic::prefill_group_kernel<<<(T + 255) / 256, 256, 0, s>>>(p0, T, pf_len, pf_group);
+                CK(cudaGetLastError());
+            }
             laic::EmbedParams ep{embd.type, embd.q, embd.s, h, embd.nb, pf_tokens, pf_slots, pf_x, counts, V};
             laic::embed_kernel<<<T, 256, 0, s>>>(ep);
             CK(cudaGetLastError());
             for (int l = 0; l < L; ++l) {
                 Layer& ly = layers[l];
-                __half* kcl = (__half*)((char*)kc + ((size_t)l * kv_layer_stride + (size_t)slot * kv_slot_stride) * kvb);
-                __half* vcl = (__half*)((char*)vc + ((size_t)l * kv_layer_stride + (size_t)slot * kv_slot_stride) * kvb);
+                __half* kcl = paged ? nullptr : (__half*)((char*)kc + ((size_t)l * kv_layer_stride + (size_t)slot * kv_slot_stride) * kvb);
+                __half* vcl = paged ? nullptr : (__half*)((char*)vc + ((size_t)l * kv_layer_stride + (size_t)slot * kv_slot_stride) * kvb);
                 // qkv
                 laic::rmsnorm_f16_kernel<<<T, 256, 0, s>>>(pf_x, h, ly.attn_norm, a.rms_eps, h, pf_a, h);
                 if (int rc = prefill_gemm(ly.qkv, T, s)) return rc;
+                if (paged) {
+                    const laic_kv_pages pg = layer_pages(l);
+                    laic_kv_append_args aa = append_args(T, pf_c, pf_q);
+                    aa.pos_dev = pf_npos; aa.seq_dev = pf_slots;
+                    if (int rc = laic::kv_append(pg, aa, s)) return rc;
+                    // the rows of the pass are one group: causal lengths over the sequence's positions
+                    laic_kv_attention_args at = attention_args(T, fb);
+                    at.q_dev = pf_q; at.out_dev = pf_attn; at.len_dev = pf_len; at.seq_dev = pf_slots;
+                    at.group_rows_dev = pf_group; at.group_len_dev = pf_group + 2;
+                    if (int rc = laic::kv_attention(pg, at, s)) return rc;
+                } else {
                 laic::QkvPostParams qp{pf_c, T, hq, kv, D, rope_pairs, p0, rope_cs, pf_q, kcl, vcl, cap};
                 laic::qkv_post_kernel<<<grid, 256, 0, s>>>(qp);
                 // attention: one query row per token, causal through its own position
@@ -1125,6 +1330,7 @@ struct laic_dev {
                 ap.part = attn_part; ap.counters = attn_cnt; ap.sqrt_d = sqrtf((float)D); ap.err = mvs.err; ap.nseq = T;
                 CK(laic::launch_k(attn_pick(D, G, false), dim3(1, Hkv, T), dim3(laic::kAttnWarps * 32), attn_smem(D, false),
                                   s, false, ap));
+                }
                 // o + residual
                 laic::to_f16_kernel<<<grid, 256, 0, s>>>(pf_attn, pf_a, (size_t)T * hq);
                 if (int rc = prefill_gemm(ly.o, T, s)) return rc;
@@ -1156,19 +1362,25 @@ struct laic_dev {
         see(lm_head());
         bool moved = false;
         int rc = mv_scratch_reserve(mvs, need, &moved);
-        if (!rc && moved) {  // graphs captured the old buffers
-            for (auto& kv : graphs) cudaGraphExecDestroy(kv.second);
-            graphs.clear();
-        }
+        if (!rc && moved) drop_graphs();  // graphs captured the old buffers
         return rc;
     }
 
     int run(int nseq, int mode) {
         int rc0 = reserve_scratch(nseq);
         if (rc0) return rc0;
-        if (!use_graph) return enqueue(nseq, mode, st, nullptr);
+        if (!use_graph || mode == MODE_VERIFY) return enqueue(nseq, mode, st, nullptr);
+        const std::array<int, 7> pkey{nseq, mode, kb.groups, kb.group_rows, kb.shared, kb.priv, kb.len};
+        if (paged) {
+            auto it = paged_graphs.find(pkey);
+            if (it != paged_graphs.end()) {
+                CK(cudaGraphLaunch(it->second, st));
+                return LAIC_OK;
+            }
+            if (paged_graphs.size() >= 64) drop_graphs();
+        }
         auto key = std::make_pair(nseq, mode);
-        auto it = graphs.find(key);
+        auto it = paged ? graphs.end() : graphs.find(key);
         if (it == graphs.end()) {
             cudaGraph_t g = nullptr;
             CK(cudaStreamBeginCapture(st, cudaStreamCaptureModeThreadLocal));
@@ -1180,6 +1392,11 @@ struct laic_dev {
             ce = cudaGraphInstantiate(&ex, g, 0);
             cudaGraphDestroy(g);
             if (ce != cudaSuccess) return fail(LAIC_E_CUDA, std::string("graph instantiate: ") + cudaGetErrorString(ce));
+            if (paged) {
+                paged_graphs.emplace(pkey, ex);
+                CK(cudaGraphLaunch(ex, st));
+                return LAIC_OK;
+            }
             it = graphs.emplace(key, ex).first;
         }
         CK(cudaGraphLaunch(it->second, st));
@@ -1267,6 +1484,8 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     if (a.hidden % 32 || a.ffn % 32) return fail(LAIC_E_UNSUPPORTED, "hidden and ffn must be multiples of 32");
     if (o.max_seqs < 1) return fail(LAIC_E_INVALID, "max_seqs must be >= 1");
     if (o.max_seqs > 64) return fail(LAIC_E_UNSUPPORTED, "at most 64 sequence slots per device");
+    if ((o.flags & LAIC_FLAG_PAGED_KV) && (tp > 1 || (o.flags & (LAIC_FLAG_KV_F32 | LAIC_FLAG_STEP_KERNEL))))
+        return fail(LAIC_E_UNSUPPORTED, "a paged cache needs FP16 KV, one GPU and per-projection launches");
     const uint32_t ctx = a.ctx ? a.ctx : 2048;
     int cap = o.kv_capacity > 0 ? std::min<int>(o.kv_capacity, (int)ctx) : (int)ctx;
 
@@ -1287,6 +1506,9 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     d->q4_upstream = (o.flags & LAIC_FLAG_Q4_0_UPSTREAM) != 0;
     d->use_spec = (o.flags & LAIC_FLAG_NO_SPECULATION) == 0;
     d->trace_on = (o.flags & LAIC_FLAG_TRACE) != 0;
+    d->paged = (o.flags & LAIC_FLAG_PAGED_KV) != 0;
+    if (d->paged) d->use_ls = d->use_spec = false;
+    d->RB = d->paged ? kMaxRows : o.max_seqs;
     d->layers.resize(a.layers);
     d->h_pos.assign(o.max_seqs, 0);
     CK(cudaStreamCreateWithFlags(&d->st, cudaStreamNonBlocking));
@@ -1297,12 +1519,12 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
             CK(cudaFuncSetAttribute(attn_pick(D, d->G, false, cl), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     (int)attn_smem(D, false, attn_max_nbuf(D))));
 
-    const size_t S = o.max_seqs, kvb = d->kv32 ? 4 : 2;
-    CK(cudaMalloc(&d->x, S * d->h * 4));
-    CK(cudaMalloc(&d->q, S * d->hq * 4));
-    CK(cudaMalloc(&d->attn, S * d->hq * 4));
-    CK(cudaMalloc(&d->act, S * d->F * 4));
-    CK(cudaMalloc(&d->logits, S * d->V * 4));
+    const size_t S = o.max_seqs, kvb = d->kv32 ? 4 : 2, RB = d->RB;
+    CK(cudaMalloc(&d->x, RB * d->h * 4));
+    CK(cudaMalloc(&d->q, RB * d->hq * 4));
+    CK(cudaMalloc(&d->attn, RB * d->hq * 4));
+    CK(cudaMalloc(&d->act, RB * d->F * 4));
+    CK(cudaMalloc(&d->logits, RB * d->V * 4));
     if (tp > 1) {
         CK(cudaMalloc(&d->logits_l, S * d->Vl * 4));
         CK(cudaMalloc(&d->logits_g, S * d->V * 4));
@@ -1318,17 +1540,37 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     d->kv_slot_stride = (long long)d->Hkv * cap * D;
     d->kv_layer_stride = d->kv_slot_stride * (long long)S;
     const size_t kv_bytes = (size_t)d->kv_layer_stride * d->L * kvb;
-    CK(cudaMalloc(&d->kc, kv_bytes));
-    CK(cudaMalloc(&d->vc, kv_bytes));
-    CK(cudaMemset(d->kc, 0, kv_bytes));
-    CK(cudaMemset(d->vc, 0, kv_bytes));
+    if (!d->paged) {
+        CK(cudaMalloc(&d->kc, kv_bytes));
+        CK(cudaMalloc(&d->vc, kv_bytes));
+        CK(cudaMemset(d->kc, 0, kv_bytes));
+        CK(cudaMemset(d->vc, 0, kv_bytes));
+    } else {
+        CK(laic::serving_set_attributes());
+        if (int rc = mv_scratch_reserve(d->mvs, MvNeed{})) return rc;  // the error word, which the pages' kernels share
+        d->pps = (cap + kKvPage - 1) / kKvPage;
+        d->npages = d->pps * (int)S;
+        const size_t pool = (size_t)d->L * d->npages * d->Hkv * kKvPage * D * 2;
+        CK(cudaMalloc(&d->pk, pool));
+        CK(cudaMalloc(&d->pv, pool));
+        d->ptab.assign((size_t)d->pps * S, -1);
+        d->pref.assign(d->npages, 0);
+        for (int i = d->npages - 1; i >= 0; --i) d->pfree.push_back(i);
+        CK(cudaMalloc(&d->d_table, d->ptab.size() * 4));
+        CK(cudaMallocHost(&d->h_table, d->ptab.size() * 4));
+        CK(cudaMalloc(&d->d_rpos, RB * 4));
+        CK(cudaMalloc(&d->d_rlen, RB * 4));
+        CK(cudaMalloc(&d->d_groups, (2 * RB + 1) * 4));
+        CK(cudaMallocHost(&d->h_rows, (4 * RB + 1) * 4));
+        CK(cudaMalloc(&d->qkv, RB * (d->hq + 2 * d->kv) * 4));
+    }
     CK(cudaMalloc(&d->pos, S * 4));
     CK(cudaMemset(d->pos, 0, S * 4));
     if (d->tile_step(S) || d->tp == 1) {  // activation records between the projections
-        CK(cudaMalloc(&d->rec_x, S * d->h * 4));
-        CK(cudaMalloc(&d->rec_act, S * d->F * 4));
-        CK(cudaMalloc(&d->rec_attn, S * d->hq * 4));
-        CK(cudaMalloc(&d->rec_ss, S * ((d->h + 15) / 16) * 4));
+        CK(cudaMalloc(&d->rec_x, RB * d->h * 4));
+        CK(cudaMalloc(&d->rec_act, RB * d->F * 4));
+        CK(cudaMalloc(&d->rec_attn, RB * d->hq * 4));
+        CK(cudaMalloc(&d->rec_ss, RB * ((d->h + 15) / 16) * 4));
     }
     CK(cudaMalloc(&d->counts, S * d->V * 4));
     CK(cudaMemset(d->counts, 0, S * d->V * 4));
@@ -1351,9 +1593,9 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     CK(cudaMalloc(&d->attn_cnt, S * d->Hkv * 4));
     CK(cudaMemset(d->attn_cnt, 0, S * d->Hkv * 4));
 
-    CK(cudaMalloc(&d->d_tokens, S * 4));
+    CK(cudaMalloc(&d->d_tokens, RB * 4));
     CK(cudaMalloc(&d->d_out_ids, S * 4));
-    CK(cudaMalloc(&d->d_slots, S * 4));
+    CK(cudaMalloc(&d->d_slots, RB * 4));
     CK(cudaMalloc(&d->d_err, 4));
     CK(cudaMemset(d->d_err, 0, 4));
     CK(cudaMalloc(&d->samp_v, S * laic::kSampleSlices * 4));
@@ -1362,7 +1604,7 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     CK(cudaMemset(d->samp_cnt, 0, S * 4));
     CK(cudaMalloc(&d->d_hist_count, 4));
     CK(cudaMalloc(&d->d_params, S * sizeof(laic::SampleDev)));
-    CK(cudaMallocHost(&d->h_tokens, S * 4));
+    CK(cudaMallocHost(&d->h_tokens, RB * 4));
     CK(cudaMallocHost(&d->h_out_ids, 2 * S * 4));
     CK(cudaMallocHost(&d->h_err, 4 * sizeof(int)));
     CK(cudaEventCreateWithFlags(&d->spec_ev[0], cudaEventDisableTiming));
@@ -1370,7 +1612,7 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     CK(cudaMallocHost(&d->h_spec, 2 * (size_t)o.max_seqs * sizeof(int)));
     CK(cudaMalloc(&d->d_spec, 2 * (size_t)o.max_seqs * sizeof(int)));
     d->h_err[0] = d->h_err[1] = d->h_err[2] = d->h_err[3] = 0;
-    CK(cudaMallocHost(&d->h_slots, S * 4));
+    CK(cudaMallocHost(&d->h_slots, RB * 4));
     CK(cudaMallocHost(&d->h_params, S * sizeof(laic::SampleDev)));
     if (tp > 1) {
         // the residual allreduce through peer memory unless LAIC_TP_NCCL_ALLREDUCE=1 asks for NCCL
@@ -1391,8 +1633,7 @@ void laic_dev_destroy(laic_dev* d) {
     cudaSetDevice(d->device);
     cudaStreamSynchronize(d->st);
     for (cudaEvent_t ev : d->spec_ev) if (ev) cudaEventDestroy(ev);
-    for (auto& kv : d->graphs) cudaGraphExecDestroy(kv.second);  // graphs holding NCCL calls go first
-    d->graphs.clear();
+    d->drop_graphs();  // graphs holding NCCL calls go first
     for (int q = 0; q < d->tp && d->ar_p2p; ++q) {
         if (q == d->tr) continue;
         if (d->ar.box[q]) cudaIpcCloseMemHandle(d->ar.box[q]);
@@ -1412,9 +1653,12 @@ void laic_dev_destroy(laic_dev* d) {
                     d->d_hist, d->d_hist_count, d->logits_l, d->logits_g, d->rec_x, d->rec_act, d->rec_ss, d->rec_attn,
                     d->ar_box, d->ar_flags, d->ar_ctr,
                     d->pf_x, d->pf_c, d->pf_q, d->pf_attn, d->pf_a, d->pf_w, d->pf_slots, d->pf_npos, d->pf_tokens,
-                    d->pf_ws, d->samp_v, d->samp_i, d->samp_cnt, d->d_spec};
+                    d->pf_ws, d->samp_v, d->samp_i, d->samp_cnt, d->d_spec, d->pf_len, d->pf_group, d->pk, d->pv, d->d_table,
+                    d->d_rpos, d->d_rlen, d->d_groups, d->qkv, d->attn_ws, d->vf_probs, d->vf_temp, d->vf_u, d->vf_ids, d->vf_n};
     for (void* b : bufs) if (b) cudaFree(b);
     if (d->h_spec) cudaFreeHost(d->h_spec);
+    if (d->h_table) cudaFreeHost(d->h_table);
+    if (d->h_rows) cudaFreeHost(d->h_rows);
     void* hb[] = {d->h_tokens, d->h_out_ids, d->h_slots, d->h_params, d->h_err};
     for (void* b : hb) if (b) cudaFreeHost(b);
     if (d->st) cudaStreamDestroy(d->st);
@@ -1438,9 +1682,7 @@ int laic_dev_upload(laic_dev* d, const char* cname, int32_t type, const uint64_t
         nbytes = conv.size();
     }
     auto shape_is = [&](uint64_t in, uint64_t out) { return ndim == 2 && shape[0] == in && shape[1] == out; };
-    // any graph captured before this upload points at old buffers
-    for (auto& kv : d->graphs) cudaGraphExecDestroy(kv.second);
-    d->graphs.clear();
+    d->drop_graphs();  // any graph captured before this upload points at old buffers
     d->ls_checked = false;
 
     if (name == "output_norm.weight") {
@@ -1568,6 +1810,7 @@ int laic_dev_prefill(laic_dev* d, int32_t nseq, const uint32_t* tokens, const in
     if (int rc_ = d->spec_cancel()) return rc_;  // (a pending speculative step assumed the old state)
     int rc = fill_inputs(d, nseq, tokens, slots);
     if (rc) return rc;
+    if (d->paged && (rc = d->paged_prepare(nseq, slots, 1))) return rc;
     if ((rc = d->run(nseq, MODE_PREFILL))) return rc;
     CK(cudaStreamSynchronize(d->st));
     for (int i = 0; i < nseq; ++i) d->h_pos[slots[i]] += 1;
@@ -1600,6 +1843,7 @@ static std::string wait_error_text(int code) {
     case laic::kErrTeamMerge: return "device wait timed out: a matvec warp team's partial-sum slot was never released";
     case laic::kErrGridBarrier: return "device wait timed out: a decode-step grid barrier was not reached by every CTA";
     case laic::kErrPeerFlag: return "device wait timed out: a tensor-parallel peer never published its allreduce slice";
+    case laic::kKvWait: return "device wait timed out: a tile of the paged attention was never loaded or multiplied";
     case laic::kErrDepCounter: return "device wait timed out: a decode-step dependency counter never reached its target";
     }
     return "device wait timed out (code " + std::to_string(code) + ")";
@@ -1679,6 +1923,7 @@ int laic_dev_step(laic_dev* d, int32_t nseq, const uint32_t* tokens, const int32
         d->spec_buf = buf ^ 1;
     } else {
         if ((rc = d->spec_cancel())) return rc;
+        if (d->paged && (rc = d->paged_prepare(nseq, slots, 1))) return rc;
         if ((rc = d->run(nseq, MODE_STEP))) return rc;
         if (out_logits)
             CK(cudaMemcpyAsync(out_logits, d->logits, (size_t)nseq * d->V * 4, cudaMemcpyDeviceToHost, d->st));
@@ -1710,10 +1955,154 @@ int laic_dev_reset_slot(laic_dev* d, int32_t slot) {
     CK(cudaSetDevice(d->device));
     if (int rc_ = d->spec_cancel()) return rc_;  // (a pending speculative step assumed the old state)
     CK(cudaStreamSynchronize(d->st));
+    if (d->paged) d->drop_slot(slot);
     CK(cudaMemset(d->pos + slot, 0, 4));
     CK(cudaMemset(d->counts + (size_t)slot * d->V, 0, (size_t)d->V * 4));
     d->h_pos[slot] = 0;
     return LAIC_OK;
+}
+
+int laic_dev_fork_slot(laic_dev* d, int32_t src, int32_t dst) {
+    if (!d || src < 0 || src >= d->S || dst < 0 || dst >= d->S) return fail(LAIC_E_INVALID, "slot out of range");
+    if (!d->paged) return fail(LAIC_E_UNSUPPORTED, "forking a slot needs a paged cache (LAIC_FLAG_PAGED_KV)");
+    if (src == dst) return LAIC_OK;
+    CK(cudaSetDevice(d->device));
+    CK(cudaStreamSynchronize(d->st));
+    d->drop_slot(dst);
+    const long long n = d->h_pos[src];
+    int* from = d->ptab.data() + (size_t)src * d->pps;
+    int* to = d->ptab.data() + (size_t)dst * d->pps;
+    const int whole = (int)(n / kKvPage);
+    for (int i = 0; i < whole; ++i) {
+        to[i] = from[i];
+        ++d->pref[to[i]];
+    }
+    if (n % kKvPage) {  // the partly filled page is copied: each slot goes on in its own
+        d->grow_slot(dst, n);
+        const size_t page = (size_t)d->Hkv * kKvPage * d->D;
+        for (int l = 0; l < d->L; ++l)
+            for (__half* pool : {d->pk, d->pv}) {
+                __half* layer = pool + (size_t)l * d->npages * page;
+                CK(cudaMemcpyAsync(layer + to[whole] * page, layer + from[whole] * page, page * 2, cudaMemcpyDeviceToDevice, d->st));
+            }
+    }
+    CK(cudaMemcpyAsync(d->pos + dst, d->pos + src, 4, cudaMemcpyDeviceToDevice, d->st));
+    CK(cudaMemcpyAsync(d->counts + (size_t)dst * d->V, d->counts + (size_t)src * d->V, (size_t)d->V * 4,
+                       cudaMemcpyDeviceToDevice, d->st));
+    CK(cudaStreamSynchronize(d->st));
+    d->h_pos[dst] = n;
+    return LAIC_OK;
+}
+
+int laic_dev_verify(laic_dev* d, int32_t nseq, const int32_t* slots, int32_t max_draft, const uint32_t* tokens,
+                    const int32_t* n_draft, const float* draft_probs_dev, const laic_sample_params* params, int32_t nparams,
+                    uint32_t* out_ids, int32_t* out_n) {
+    if (!d) return fail(LAIC_E_INVALID, "null device");
+    if (!d->paged) return fail(LAIC_E_UNSUPPORTED, "verifying drafted tokens needs a paged cache (LAIC_FLAG_PAGED_KV)");
+    if (!slots || !tokens || !n_draft || !out_ids || !out_n) return fail(LAIC_E_INVALID, "null argument");
+    if (nseq < 1 || nseq > d->S) return fail(LAIC_E_INVALID, "nseq must be in [1, max_seqs]");
+    if (max_draft < 0 || (long long)nseq * (max_draft + 1) > kMaxRows)
+        return fail(LAIC_E_UNSUPPORTED, "nseq * (max_draft + 1) must be at most 64");
+    if (params && nparams != 1 && nparams != nseq) return fail(LAIC_E_INVALID, "nparams must be 1 or nseq");
+    std::string missing;
+    if (!d->ready(missing)) return fail(LAIC_E_MISSING, "missing tensor: " + missing);
+    const int m1 = max_draft + 1, rows = nseq * m1;
+    std::vector<char> seen(d->S, 0);
+    for (int i = 0; i < nseq; ++i) {
+        if (slots[i] < 0 || slots[i] >= d->S) return fail(LAIC_E_INVALID, "slot out of range");
+        if (seen[slots[i]]) return fail(LAIC_E_INVALID, "slot listed twice in one step");
+        seen[slots[i]] = 1;
+        if (n_draft[i] < 0 || n_draft[i] > max_draft) return fail(LAIC_E_INVALID, "n_draft must be in [0, max_draft]");
+        for (int j = 0; j <= n_draft[i]; ++j)
+            if (tokens[i * m1 + j] >= (uint32_t)d->V || tokens[i * m1 + j] >= (uint32_t)d->embd.rows)
+                return fail(LAIC_E_INVALID, "invalid embedding tensor");
+        if (d->h_pos[slots[i]] + n_draft[i] + 1 > d->cap) return fail(LAIC_E_CONTEXT, "context length exceeded");
+        if (params) {
+            const laic_sample_params& sp = params[nparams == 1 ? 0 : i];
+            if (sp.temperature > 0.f && (sp.top_k || sp.top_p != 1.f || sp.repeat_penalty != 1.f))
+                return fail(LAIC_E_UNSUPPORTED, "verification samples from the whole vocabulary (top_k, top_p and repeat_penalty off)");
+            if (!(sp.temperature > 0.f) && sp.repeat_penalty != 1.f)
+                return fail(LAIC_E_UNSUPPORTED, "verification applies no repeat penalty");
+        }
+    }
+    CK(cudaSetDevice(d->device));
+    const size_t RB = d->RB;
+    if (!d->vf_probs) {
+        CK(cudaMalloc(&d->vf_temp, RB * 4));
+        CK(cudaMalloc(&d->vf_u, 2 * RB * 4));
+        CK(cudaMalloc(&d->vf_ids, 2 * RB * 4));
+        CK(cudaMalloc(&d->vf_n, 2 * RB * 4));
+        CK(cudaMalloc(&d->vf_probs, RB * d->V * 4));
+    }
+    // rows: per sequence its token and the drafted ones, then padding (in no page, seen by nothing)
+    std::vector<float> temp(rows, 0.f), u(2 * RB, 0.f);
+    std::vector<uint32_t> ids(RB, 0);
+    std::vector<int> nd(n_draft, n_draft + nseq);
+    int *rpos = d->h_rows, *rlen = rpos + RB, *starts = rlen + RB, *lens = starts + RB + 1;
+    laic_dev::KvBounds b;
+    b.groups = nseq;
+    b.group_rows = m1;
+    for (int i = 0; i < nseq; ++i) {
+        const laic_sample_params greedy{0.f, 0, 1.f, 1.f, 0};
+        const laic_sample_params& sp = params ? params[nparams == 1 ? 0 : i] : greedy;
+        const long long p0 = d->h_pos[slots[i]];
+        std::mt19937_64 rng(sp.temperature > 0.f ? (sp.seed ? sp.seed : std::random_device{}()) : 0);
+        auto draw = [&] { return (float)((rng() >> 40) * 0x1p-24); };  // [0, 1), 24 bits
+        for (int j = 0; j < m1; ++j) {
+            const bool live = j <= n_draft[i];
+            const int r = i * m1 + j;
+            d->h_tokens[r] = live ? tokens[r] : 0;
+            d->h_slots[r] = slots[i];
+            rpos[r] = live ? (int)(p0 + j) : -1;
+            rlen[r] = live ? (int)(p0 + j + 1) : -1;
+            temp[r] = sp.temperature;
+            if (j) ids[i * max_draft + j - 1] = live ? tokens[r] : LAIC_NO_TOKEN;
+            if (j) u[i * max_draft + j - 1] = draw();
+        }
+        u[RB + i] = draw();
+        starts[i] = i * m1;
+        lens[i] = (int)(p0 + n_draft[i] + 1);
+        b.len = std::max(b.len, lens[i]);
+        d->grow_slot(slots[i], lens[i]);
+    }
+    starts[nseq] = rows;
+    b.shared = b.len;
+    if (int rc = d->upload_table()) return rc;
+    const cudaStream_t st = d->st;
+    CK(cudaMemcpyAsync(d->d_rpos, rpos, rows * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(d->d_rlen, rlen, rows * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(d->d_groups, starts, (2 * RB + 1) * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(d->vf_temp, temp.data(), rows * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(d->vf_u, u.data(), 2 * RB * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(d->vf_ids, ids.data(), RB * 4, cudaMemcpyHostToDevice, st));
+    CK(cudaMemcpyAsync(d->vf_n, nd.data(), nseq * 4, cudaMemcpyHostToDevice, st));
+    d->kb = b;
+    d->vf_nseq = nseq; d->vf_max = max_draft; d->vf_draft = draft_probs_dev;
+    int rc = d->reserve_attn_ws(rows, b);
+    if (!rc) rc = d->run(rows, MODE_VERIFY);
+    if (rc) { cudaStreamSynchronize(st); return rc; }
+    std::vector<uint32_t> got(rows);
+    std::vector<int> cnt(nseq);
+    CK(cudaMemcpyAsync(got.data(), d->vf_ids + RB, rows * 4, cudaMemcpyDeviceToHost, st));
+    CK(cudaMemcpyAsync(cnt.data(), d->vf_n + RB, nseq * 4, cudaMemcpyDeviceToHost, st));
+    CK(cudaStreamSynchronize(st));
+    // positions move past what was kept; the refused and padding rows leave the history again
+    for (int i = 0; i < nseq; ++i) {
+        const int kept = std::max(1, std::min(cnt[i], m1));
+        d->h_pos[slots[i]] += kept;
+        for (int j = kept; j < m1; ++j) {
+            const int k = i * m1 + j;
+            d->h_slots[k] = slots[i] | INT32_MIN;  // to be taken off
+        }
+    }
+    CK(cudaMemcpyAsync(d->d_slots, d->h_slots, rows * 4, cudaMemcpyHostToDevice, st));
+    laic::unverify_kernel<<<1, 64, 0, st>>>(d->d_slots, d->d_tokens, rows, m1, d->pos, d->counts, d->V);
+    CK(cudaGetLastError());
+    CK(cudaStreamSynchronize(st));
+    d->last_nseq = 0;
+    std::copy(got.begin(), got.end(), out_ids);
+    std::copy(cnt.begin(), cnt.end(), out_n);
+    return check_sampler_err(d);
 }
 
 int laic_dev_slot_pos(laic_dev* d, int32_t slot, int64_t* pos) {
@@ -1725,6 +2114,7 @@ int laic_dev_slot_pos(laic_dev* d, int32_t slot, int64_t* pos) {
 int laic_dev_fill_kv(laic_dev* d, int32_t slot, int32_t npos, uint64_t seed) {
     if (!d || slot < 0 || slot >= d->S) return fail(LAIC_E_INVALID, "slot out of range");
     if (npos < 0 || npos > d->cap) return fail(LAIC_E_CONTEXT, "context length exceeded");
+    if (d->paged) return fail(LAIC_E_UNSUPPORTED, "laic_dev_fill_kv fills contiguous caches only");
     CK(cudaSetDevice(d->device));
     if (int rc_ = d->spec_cancel()) return rc_;  // (a pending speculative step assumed the old state)
     if (npos > 0) {
@@ -1786,13 +2176,13 @@ int laic_dev_decode(laic_dev* d, int32_t nseq, const uint32_t* tokens, const int
         d->hist_cap = 0;
         CK(cudaMalloc(&d->d_hist, need * sizeof(unsigned)));
         d->hist_cap = need;
-        for (auto& kv : d->graphs) cudaGraphExecDestroy(kv.second);  // they captured the old buffer
-        d->graphs.clear();
+        d->drop_graphs();  // they captured the old buffer
     }
     CK(cudaMemcpyAsync(d->d_tokens, d->h_tokens, nseq * 4, cudaMemcpyHostToDevice, d->st));
     CK(cudaMemcpyAsync(d->d_slots, d->h_slots, nseq * 4, cudaMemcpyHostToDevice, d->st));
     CK(cudaMemcpyAsync(d->d_params, d->h_params, nseq * sizeof(laic::SampleDev), cudaMemcpyHostToDevice, d->st));
     CK(cudaMemsetAsync(d->d_hist_count, 0, 4, d->st));
+    if (d->paged && (rc = d->paged_prepare(nseq, slots, steps))) return rc;
     cudaEvent_t e0, e1;
     CK(cudaEventCreate(&e0));
     CK(cudaEventCreate(&e1));
@@ -1825,6 +2215,7 @@ int laic_dev_profile(laic_dev* d, int32_t nseq, const uint32_t* tokens, int32_t 
         int rc = fill_inputs(d, nseq, tokens + (size_t)it * nseq, slots.data());
         if (rc) return rc;
         if ((rc = fill_params(d, nseq, nullptr, 0))) return rc;
+        if (d->paged && (rc = d->paged_prepare(nseq, slots.data(), 1))) return rc;
         laic_dev::Timer t;
         // hold the stream while the host queues the step, so the events time the kernels, not the host
         laic::hold_kernel<<<1, 1, 0, d->st>>>(20000000LL);

@@ -92,6 +92,30 @@ __global__ void advance_pos_kernel(const int* slots, int* pos, int nseq) {
     for (int s = threadIdx.x; s < nseq; s += blockDim.x) pos[slots[s]] += 1;
 }
 
+// A paged step's rows: the position each listed slot's token takes, and what it sees (itself included).
+__global__ void paged_rows_kernel(const int* slots, const int* pos, int nseq, int* rpos, int* rlen) {
+    pdl_wait();
+    for (int s = threadIdx.x; s < nseq; s += blockDim.x) {
+        const int p = pos[slots[s]];
+        rpos[s] = p;
+        rlen[s] = p + 1;
+    }
+}
+
+// After a verification of rows [sequence][m1]: the rows whose slot carries the sign bit were refused or
+// padding, their tokens leave the slot's history; each slot's position moves by the rows kept.
+__global__ void unverify_kernel(const int* slots, const unsigned* toks, int rows, int m1, int* pos, unsigned* counts, int vocab) {
+    for (int r = threadIdx.x; r < rows; r += blockDim.x) {
+        const int s = slots[r] & 0x7fffffff;
+        if (slots[r] < 0) atomicSub(counts + (size_t)s * vocab + toks[r], 1u);
+        if (r % m1 == 0) {
+            int kept = 0;
+            while (kept < m1 && slots[r + kept] >= 0) ++kept;
+            pos[s] += kept;
+        }
+    }
+}
+
 // Chained decode: append this step's sampled ids to the history buffer.
 __global__ void record_ids_kernel(const unsigned* ids, unsigned* hist, int* counter, int nseq) {
     pdl_wait();

@@ -103,6 +103,15 @@ __global__ void prefill_rows_kernel(int slot, int p0, int T, int* slots, int* np
         npos[t] = p0 + t;
     }
 }
+// Paged cache: the pass's causal lengths, and its rows as one group over the whole sequence.
+__global__ void prefill_group_kernel(int p0, int T, int* len, int* group) {
+    for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < T; t += gridDim.x * blockDim.x) len[t] = p0 + t + 1;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        group[0] = 0;
+        group[1] = T;
+        group[2] = p0 + T;
+    }
+}
 __global__ void add_pos_kernel(int* pos, int slot, int n) {
     if (threadIdx.x == 0 && blockIdx.x == 0) pos[slot] += n;
 }

@@ -6,6 +6,8 @@
 
 #include "../../include/laic_b200.h"
 
+#include "paged.cuh"  // the error bits
+
 namespace laic {
 
 // Records the calling thread's error message (laic_last_error) and returns `code` (engine.cu).

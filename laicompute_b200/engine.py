@@ -13,7 +13,7 @@ import numpy as np
 
 from . import gguf
 from ._native import (DevDesc, DevOpts, DevStats, FLAG_KV_F32, FLAG_NO_GRAPH, FLAG_NO_PDL, FLAG_LAYER_LAUNCHES, FLAG_TRACE,
-                      FLAG_STEP_KERNEL, FLAG_Q4_0_UPSTREAM, FLAG_NO_SPECULATION, KernelRecord, SampleParams,
+                      FLAG_STEP_KERNEL, FLAG_Q4_0_UPSTREAM, FLAG_NO_SPECULATION, FLAG_PAGED_KV, KernelRecord, SampleParams,
                       check, lib)
 
 
@@ -39,11 +39,12 @@ class Engine:
                  graphs: bool = True, pdl: bool = True, tp_size: int = 1, tp_rank: int = 0,
                  nccl_id: Optional[bytes] = None, layer_launches: bool = False, trace: bool = False,
                  step_kernel: Optional[bool] = None, q4_0_upstream: bool = False,
-                 speculate: bool = True) -> None:
+                 speculate: bool = True, paged: bool = False) -> None:
         """`step_kernel`: True runs one-sequence Q4_0/Q8_0 steps as the persistent decode-step kernel, False
         (or `layer_launches`) and None (the default) launch per projection. `q4_0_upstream`: the file's Q4_0
         tensors use upstream ggml's nibble order (llama.cpp's files) rather than the reference's. `speculate`:
-        step() starts the next step on its own sampled ids while the caller decides (laic_dev_step)."""
+        step() starts the next step on its own sampled ids while the caller decides (laic_dev_step). `paged`: the
+        KV cache in pages, for fork() and verify()."""
         L = lib()
         if step_kernel is False:
             layer_launches = True
@@ -52,7 +53,7 @@ class Engine:
         flags = ((FLAG_KV_F32 if kv_f32 else 0) | (0 if graphs else FLAG_NO_GRAPH) | (0 if pdl else FLAG_NO_PDL)
                  | (FLAG_LAYER_LAUNCHES if layer_launches else 0) | (FLAG_TRACE if trace else 0)
                  | (FLAG_STEP_KERNEL if step_kernel else 0) | (FLAG_Q4_0_UPSTREAM if q4_0_upstream else 0)
-                 | (0 if speculate else FLAG_NO_SPECULATION))
+                 | (0 if speculate else FLAG_NO_SPECULATION) | (FLAG_PAGED_KV if paged else 0))
         self._nccl_id = ctypes.create_string_buffer(nccl_id, 128) if nccl_id else None
         opts = DevOpts(device=device, max_seqs=max_seqs, kv_capacity=kv_capacity, tp_size=tp_size, tp_rank=tp_rank,
                        nccl_id=ctypes.cast(self._nccl_id, ctypes.c_void_p) if self._nccl_id else None, flags=flags)
@@ -107,6 +108,26 @@ class Engine:
         check(lib().laic_dev_step(self.h, n, t.ctypes.data, s.ctypes.data, arr, len(arr), ids.ctypes.data,
                                   logits.ctypes.data if logits is not None else None))
         return ids, logits
+
+    def fork(self, src: int, dst: int) -> None:
+        """Slot dst becomes a copy of slot src, sharing its whole pages (engines with paged=True)."""
+        check(lib().laic_dev_fork_slot(self.h, src, dst))
+
+    def verify(self, tokens, n_draft, slots=None, params=None, draft_probs: int = 0):
+        """One speculative step (engines with paged=True): tokens [nseq][1 + max_draft], each row the next token
+        and then n_draft[i] drafted ones; draft_probs: device pointer [nseq][max_draft][vocab] or 0. Returns
+        (ids [nseq][1 + max_draft], counts): the tokens that follow, counts[i] of them valid."""
+        t = np.ascontiguousarray(np.atleast_2d(tokens), dtype=np.uint32)
+        n = np.ascontiguousarray(np.atleast_1d(n_draft), dtype=np.int32)
+        nseq, m1 = t.shape
+        s = np.arange(nseq, dtype=np.int32) if slots is None else np.ascontiguousarray(np.atleast_1d(slots), np.int32)
+        if len(n) != nseq or len(s) != nseq:
+            raise ValueError("one n_draft and slot per row of tokens")
+        arr = self._params(params, nseq)
+        ids, cnt = np.zeros((nseq, m1), dtype=np.uint32), np.zeros(nseq, dtype=np.int32)
+        check(lib().laic_dev_verify(self.h, nseq, s.ctypes.data, m1 - 1, t.ctypes.data, n.ctypes.data, draft_probs, arr,
+                                    len(arr), ids.ctypes.data, cnt.ctypes.data))
+        return ids, cnt
 
     def reset_slot(self, slot: int) -> None:
         check(lib().laic_dev_reset_slot(self.h, slot))
