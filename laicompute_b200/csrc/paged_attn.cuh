@@ -41,8 +41,9 @@ struct KvAttnParams {
     float scale_log2;             // scale * log2(e)
     int lp, nsp;                  // private splits: positions each, count
     int ls, nss, ctiles;          // shared splits, column tiles per group
+    int lc;                       // splits joined into one partial (the bulk kernel's clusters; else 1)
     int shared_items;
-    bool q_vec;                   // rows of q are 16-byte aligned
+    bool q_vec, out_vec;          // rows of q, of out are 16-byte aligned
     uint32_t g_inv;               // 2^16 / G rounded up
     float* part_o;                // [rows][heads][nss + nsp][head_dim]
     float2* part_ml;              // [rows][heads][nss + nsp] (m, l)
@@ -586,7 +587,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
     const int ns = p.nss + p.nsp;
     const int priv = min(v.n - v.shared, p.max_private);
     if (v.n - v.shared > p.max_private && lane == 0) kv_flag(p.err, kKvBadPos);
-    const int live_s = v.shared > 0 ? (v.shared + p.ls - 1) / p.ls : 0;
+    const int live_s = v.shared > 0 ? (v.shared + p.ls * p.lc - 1) / (p.ls * p.lc) : 0;
     const int live = live_s + (priv > 0 ? (priv + p.lp - 1) / p.lp : 0);
     const size_t base = (size_t)pair * ns;
     auto slot = [&](int i) { return i < live_s ? i : p.nss + (i - live_s); };

@@ -5,8 +5,8 @@
 // group's positions in tiles of bulk_keys.
 //
 // Roles: warp 8 loads (TMA boxes of up to a page, 128-byte swizzle, a lane per box: one lane alone
-// took 125 cycles a box, 4,000 for a tile of 16-position pages; a ring of K and V tiles); warp 9
-// multiplies (one lane: tcgen05.mma, S and O in tensor memory, P read from tensor memory, where it
+// took 125 cycles a box, 4,000 for a tile of 16-position pages; a ring of K and V tiles); warps 9 and
+// 10 multiply, one lane for each tile of columns (tcgen05.mma, S and O in tensor memory, P read from tensor memory, where it
 // takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S (twice, 32
 // columns at a time: a column's 128 scores do not fit the registers beside the rest), keep the
 // running maximum and sum, and write P in two halves, so that PV starts on the first. One tile's products run under the other's exponentials. 128 positions
@@ -14,6 +14,10 @@
 // measured), and two score buffers of 64 ran slower than one of 128. O is rescaled only when a
 // maximum grew by more than 2^8 since the last time (weights stay below 2^15 in binary16 with the
 // factor 2^7 they carry). Both tiles' S and O fill the 512 columns of tensor memory.
+//
+// The splits of a set of columns form a thread-block cluster and join through distributed shared
+// memory: one partial per cluster goes to global memory, or the output itself where the cluster holds
+// all that its rows see.
 //
 // Tiles that some column does not see to their end are masked. There 0 * V must not be 0 * inf: the
 // softmax threads clear what is not finite in V before the product (all of it past the positions any
@@ -26,12 +30,15 @@
 #pragma once
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "paged_attn.cuh"
 
 namespace laic {
 
 constexpr int kBulkCols = 256;        // score columns of a CTA
-constexpr int kBulkThreads = 320;
+constexpr int kBulkThreads = 352;
+constexpr int kBulkMaxCluster = 8;   // clusters of 1, 2, 4 or 8
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
 constexpr float kBulkSlack = 8.f;     // log2 of how far a maximum may outgrow its reference
 
@@ -42,15 +49,17 @@ __host__ __device__ constexpr int bulk_slots(int D, bool f32) { return D == 64 ?
 __host__ __device__ constexpr int bulk_smem(int D, bool f32) {
     return bulk_q_bytes(D, f32) + bulk_slots(D, f32) * bulk_slot_bytes(D) + 1024;  // (aligned to 1024)
 }
-// (at the end the ring and Q hold O's rows)
-static_assert(bulk_smem(64, false) - 1024 >= kBulkCols * (64 + 4) * 4 && bulk_smem(128, false) - 1024 >= kBulkCols * (128 + 4) * 4,
-              "O's rows fit");
+// (at the end the ring and Q hold O's rows and their maxima and sums)
+__host__ __device__ constexpr int bulk_rows_bytes(int D) { return kBulkCols * (D + 4) * 4; }
+static_assert(bulk_smem(64, false) - 1024 >= bulk_rows_bytes(64) + kBulkCols * 8 &&
+              bulk_smem(128, false) - 1024 >= bulk_rows_bytes(128) + kBulkCols * 8, "O's rows fit");
 
 // ---- PTX
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tc_alloc(uint32_t smem_dst, uint32_t cols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -167,7 +176,7 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
     return r;
 }
 
-// Grid [group][pair of column tiles][kv head][split].
+// Grid [group][pair of column tiles][kv head][split], clusters of bulk_cluster consecutive splits.
 template <int D, typename T>
 __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAttnParams p, const __grid_constant__ CUtensorMap mk,
                                                                      const __grid_constant__ CUtensorMap mv) {
@@ -188,9 +197,13 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     __shared__ int any_odd;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    if (tid == 0) { tma_prefetch(&mk); tma_prefetch(&mv); }
     int i = blockIdx.x;
-    const int split = i % p.nss;
-    i /= p.nss;
+    const int nsplit = p.nss * C, split = i % nsplit;
+    i /= nsplit;
     const int kvh = i % p.kv_heads;
     i /= p.kv_heads;
     const int pair = i % p.ctiles, g = i / p.ctiles;
@@ -201,7 +214,6 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     if (col0 >= ncol) return;
     const int t0 = split * p.ls;
     const int shared = max(0, kv_clamp_len(p, glen, p.max_shared));
-    if (t0 >= shared) return;
     const int tiles = ncol - col0 > 128 ? 2 : 1;  // M tiles with columns
 
     // ---- a softmax thread's column and how far it sees
@@ -213,6 +225,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     const int my_row = row_of(live ? tid : 0);
     const int rr = r0 + base_row + my_row, hh = kvh * p.G + (live ? tid : 0) + base_head - my_row * p.G;
     const RowView view = row_view(p, rr, shared);
+    if (live && split == 0 && view.n - view.shared > p.max_private) kv_flag(p.err, kKvBadPos);
     const int lim = live ? max(0, view.shared) : 0;
     int seq = row_seq(p, r0);
     if (seq < 0) seq = 0;  // (recorded) reads some sequence's pages
@@ -299,12 +312,12 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (tid == 0) {
-        for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], 1); }
+        for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], tiles); }
         for (int w = 0; w < 2; ++w) {
             mbar_init(&s_full[w], 1);
             for (int h = 0; h < 2; ++h) mbar_init(&p_ready[w][h], 128);
         }
-        mbar_init(&o_done, 1);
+        mbar_init(&o_done, tiles);
         mbar_fence_init();
         dead = 0;
         any_odd = 0;
@@ -320,8 +333,10 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     }
     __syncthreads();
     const int t1 = min(lim_max, t0 + p.ls), seen_by_all = lim_min;
-    if (t0 >= t1) return;  // no column sees this far
-    const int nt = (t1 - t0 + NK - 1) / NK;
+    const int nt = t0 < t1 ? (t1 - t0 + NK - 1) / NK : 0;  // 0: no column sees this far
+    float* rows = reinterpret_cast<float*>(base);           // at the end: O's rows, [column][D + 4]
+    float2* row_ml = reinterpret_cast<float2*>(base + bulk_rows_bytes(D));  // (m, l); l -1: padding
+    if (nt > 0) {
     if (warp == 9) tc_alloc(smem_u32(&tmem_at), 512);
     tc_fence_before();
     __syncthreads();
@@ -366,10 +381,11 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 const long long since = clock64();
                 while (!mbar_try_wait(&kv_full[q % NS], (uint32_t)(q / NS) & 1) && clock64() - since < 200000000LL) {}
             }
-    } else if (warp == 9) {
-        if (lane == 0) {
+    } else if (warp >= 9) {
+        const int w = warp - 9;
+        if (lane == 0 && w < tiles) {
             constexpr uint32_t iqk = umma_idesc(NK, false), ipv = umma_idesc(D, true);
-            auto qk = [&](int w, int j) {
+            auto qk = [&](int j) {
                 uint32_t ks = slot(2 * j), qa = smem_u32(base) + (uint32_t)(w * HN * QPART);
                 asm volatile("" : "+r"(ks), "+r"(qa));  // (descriptors are formed here, not kept over the loop)
 #pragma unroll
@@ -381,9 +397,9 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                                   umma_desc(ks + (k >> 2) * (NK * 128) + off, 16, 1024), iqk, part != HN - 1 || k > 0);
                     }
                 tc_commit(&s_full[w]);
-                if (w == tiles - 1) tc_commit(&kv_free[2 * j % NS]);
+                tc_commit(&kv_free[2 * j % NS]);
             };
-            auto pv = [&](int w, int j, int h) {
+            auto pv = [&](int j, int h) {
                 uint32_t vs = slot(2 * j + 1);
                 asm volatile("" : "+r"(vs));
 #pragma unroll
@@ -396,23 +412,22 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             };
             bool ok = full(0);
             tc_fence_after();
-            for (int w = 0; w < tiles && ok; ++w) qk(w, 0);
-            for (int j = 0; j < nt && ok; ++j)
-                for (int w = 0; w < tiles && ok; ++w) {
-                    if (w == 0 && !(ok = full(2 * j + 1))) break;
-                    for (int h = 0; h < 2 && ok; ++h) {
-                        if (!(ok = bulk_wait(&p_ready[w][h], (uint32_t)j & 1, &dead, p.err))) break;
-                        tc_fence_after();
-                        pv(w, j, h);
-                    }
-                    if (!ok) break;
-                    if (w == tiles - 1) tc_commit(&kv_free[(2 * j + 1) % NS]);
-                    if (j + 1 < nt) {
-                        if (w == 0 && !(ok = full(2 * j + 2))) break;
-                        tc_fence_after();
-                        qk(w, j + 1);
-                    }
+            if (ok) qk(0);
+            for (int j = 0; j < nt && ok; ++j) {
+                ok = full(2 * j + 1);
+                for (int h = 0; h < 2 && ok; ++h) {
+                    if (!(ok = bulk_wait(&p_ready[w][h], (uint32_t)j & 1, &dead, p.err))) break;
+                    tc_fence_after();
+                    pv(j, h);
                 }
+                if (!ok) break;
+                tc_commit(&kv_free[(2 * j + 1) % NS]);
+                if (j + 1 < nt) {
+                    if (!(ok = full(2 * j + 2))) break;
+                    tc_fence_after();
+                    qk(j + 1);
+                }
+            }
             tc_commit(&o_done);  // after a failed wait too: whatever was issued ends before tensor memory is freed
         }
     } else if (wg < tiles) {
@@ -535,10 +550,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         tc_fence_after();
         named_sync(1, 128 * tiles);  // both tiles' notes of odd positions (every softmax warp comes here)
         if (ok) {
-            // O's rows through shared memory (nothing reads it any more): a thread's own stores to global
-            // memory would touch 32 lines per instruction (13,000 cycles measured, against 1,500)
-            const int ns = p.nss + p.nsp;
-            float* rows = reinterpret_cast<float*>(base) + (size_t)warp * 32 * (D + 4);
+            // O's rows into shared memory, where the loads and Q are done with
 #pragma unroll 1
             for (int k = 0; k < D; k += 32) {
                 uint32_t o[32];
@@ -558,23 +570,12 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                                 if (!(fabsf(x) <= 65504.f)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
                             }
                         }
-                uint4* dst = reinterpret_cast<uint4*>(rows + (size_t)lane * (D + 4) + k);
+                uint4* dst = reinterpret_cast<uint4*>(rows + (size_t)tid * (D + 4) + k);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
-            const size_t at = ((size_t)rr * p.heads + hh) * ns + split;
             // (l is zero only where the column saw nothing: its largest weight is at least 2^-8)
-            if (live) p.part_ml[at] = make_float2(l == 0.f ? -INFINITY : mref, F32 ? l * kPaGain : l);
-            __syncwarp();
-            constexpr int LPR = D / 4;  // lanes per row
-#pragma unroll 4
-            for (int q = 0; q < 32; q += 32 / LPR) {
-                const int c = q + lane / LPR;
-                const size_t to = __shfl_sync(0xffffffffu, (unsigned long long)at, c);
-                if (col0 + warp * 32 + c < ncol)
-                    *reinterpret_cast<float4*>(p.part_o + to * D + lane % LPR * 4) =
-                        *reinterpret_cast<const float4*>(rows + (size_t)c * (D + 4) + lane % LPR * 4);
-            }
+            row_ml[tid] = make_float2(l == 0.f ? -INFINITY : mref, live && view.n < 0 ? -1.f : F32 ? l * kPaGain : l);
         }
         tc_fence_before();
     }
@@ -585,6 +586,97 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         __syncwarp();
         tc_fence_after();
         tc_dealloc(tmem, 512);
+    }
+    } else {
+        pdl_launch_dependents();
+        if (tid < 128 * tiles) row_ml[tid] = make_float2(-INFINITY, live && view.n < 0 ? -1.f : 0.f);
+    }
+    // ---- join the cluster's splits: CTA `rank` takes every C-th block of rows, a warp a row at a time
+    // (a lane four dimensions), the splits' rows loaded together and added in split order
+    if (C > 1) cluster.sync();
+    else __syncthreads();
+    constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp and step
+    const int ns = p.nss + p.nsp, slot_at = split / C, cols = min(kBulkCols, ncol - col0);
+    auto join = [&](auto cc) {
+        constexpr int CC = decltype(cc)::value, U = 8 / CC;  // U rows at a time: eight loads in flight
+        const float* far_rows[CC];
+        const float2* far_ml[CC];
+#pragma unroll
+        for (int c = 0; c < CC; ++c) {
+            far_rows[c] = CC > 1 ? cluster.map_shared_rank(rows, c) : rows;
+            far_ml[c] = CC > 1 ? cluster.map_shared_rank(row_ml, c) : row_ml;
+        }
+        constexpr int STEP = RPW * CC;
+        const int e0 = lane % LPR * 4;
+        for (int r = (warp * U * CC + rank) * RPW; r < cols; r += (kBulkThreads / 32) * U * STEP) {
+            float2 ml[U][CC];
+            float4 v[U][CC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int cw = min(r + u * STEP + lane / LPR, cols - 1);
+#pragma unroll
+                for (int c = 0; c < CC; ++c) {
+                    ml[u][c] = far_ml[c][cw];
+                    v[u][c] = *reinterpret_cast<const float4*>(far_rows[c] + (size_t)cw * (D + 4) + e0);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int cw = r + u * STEP + lane / LPR;
+                if (cw >= cols || ml[u][0].y < 0.f) continue;  // (negative: padding)
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int c = 0; c < CC; ++c) M = fmaxf(M, ml[u][c].x);
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < CC; ++c)
+                    if (ml[u][c].x != -INFINITY) {
+                        const float w = ex2(ml[u][c].x - M);
+                        L = fmaf(ml[u][c].y, w, L);
+                        a.x = fmaf(v[u][c].x, w, a.x); a.y = fmaf(v[u][c].y, w, a.y);
+                        a.z = fmaf(v[u][c].z, w, a.z); a.w = fmaf(v[u][c].w, w, a.w);
+                    }
+                const int qr = row_of(cw);
+                const size_t row = (size_t)(r0 + base_row + qr);
+                const int head = kvh * p.G + cw + base_head - qr * p.G;
+                if (p.direct) {
+                    const float iv = M == -INFINITY ? 0.f : 1.f / L;
+                    T* dst = static_cast<T*>(p.out) + row * p.ldo + (size_t)head * D + e0;
+                    const float o[4] = {a.x * iv, a.y * iv, a.z * iv, a.w * iv};
+                    if (p.out_vec) {
+                        if constexpr (F32) {
+                            *reinterpret_cast<float4*>(dst) = make_float4(o[0], o[1], o[2], o[3]);
+                        } else {
+                            const __half2 x = __floats2half2_rn(o[0], o[1]), y = __floats2half2_rn(o[2], o[3]);
+                            *reinterpret_cast<uint2*>(dst) =
+                                make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dst[e] = kv_out<T>(o[e]);
+                    }
+                } else {
+                    const size_t at = (row * p.heads + head) * ns + slot_at;
+                    *reinterpret_cast<float4*>(p.part_o + at * D + e0) = a;
+                    if (e0 == 0) p.part_ml[at] = make_float2(M, L);
+                }
+            }
+        }
+    };
+    if (C == 1) join(std::integral_constant<int, 1>{});
+    else if (C == 2) join(std::integral_constant<int, 2>{});
+    else if (C == 4) join(std::integral_constant<int, 4>{});
+    else join(std::integral_constant<int, 8>{});
+    if (C > 1) cluster.sync();  // no CTA leaves while another may still read its rows
+    if (p.direct && blockIdx.x == 0) {  // rows of no group see nothing here
+        const int g0 = max(0, min(p.rows, p.group_rows[0])), g1 = max(g0, min(p.rows, p.group_rows[p.groups]));
+        for (int r = warp; r < p.rows; r += kBulkThreads / 32) {
+            if (r >= g0 && r < g1) continue;
+            const RowView v = row_view(p, r, 0);
+            if (v.n < 0) continue;
+            if (v.n > 0 && lane == 0) kv_flag(p.err, kKvBadPos);
+            for (int e = lane; e < p.heads * D; e += 32) static_cast<T*>(p.out)[(size_t)r * p.ldo + e] = kv_out<T>(0.f);
+        }
     }
 }
 

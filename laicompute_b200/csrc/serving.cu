@@ -94,13 +94,50 @@ int device_sms(int dev) {
     return n;
 }
 
+using BulkFn = void (*)(KvAttnParams, CUtensorMap, CUtensorMap);
+BulkFn bulk_pick(int D, bool f32) {
+    if (D == 64) return f32 ? paged_bulk_kernel<64, float> : paged_bulk_kernel<64, __half>;
+    return f32 ? paged_bulk_kernel<128, float> : paged_bulk_kernel<128, __half>;
+}
+
+// Clusters of c bulk CTAs that are resident at once on `device` (asked once; without a device, by the SM count).
+int bulk_clusters(int device, int c) {
+    static std::atomic<int> known[64][kBulkMaxCluster + 1];
+    const int guess = device_sms(device) / c;
+    if (device < 0 || device >= 64) return guess;
+    int n = known[device][c].load();
+    if (n) return n;
+    DeviceGuard dg(device);
+    if (dg.err != cudaSuccess || serving_set_attributes() != cudaSuccess) {
+        cudaGetLastError();
+        return guess;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c * device_sms(device));
+    cfg.blockDim = dim3(kBulkThreads);
+    cfg.dynamicSmemBytes = bulk_smem(128, true);  // the largest
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)c;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, bulk_pick(128, true), &cfg) != cudaSuccess || n < 1) {
+        cudaGetLastError();
+        return guess;
+    }
+    known[device][c].store(n);
+    return n;
+}
+
 // ---- attention: how a call is cut into items
 struct AttnPlan {
     int nt = 1;            // column tiles of 8 of a shared item
     int lp = 64, nsp = 1;  // private splits
     int ls = 64, nss = 0, ctiles = 0;
     int shared_items = 0, private_items = 0;
-    bool bulk = false;     // the shared items run in paged_bulk.cuh
+    bool bulk = false;     // the shared items run in paged_bulk.cuh,
+    int cluster = 1;       // this many splits of a set of columns in a cluster (nss counts clusters)
     bool direct = false;
     size_t ml_off = 0, bytes = 0;
 };
@@ -146,24 +183,35 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
         const long long pool_rows = (long long)g.num_pages * g.kv_heads * g.page_size;
         pl.bulk = g.head_dim >= 64 && cols >= kBulkMinCols && a.max_shared >= kBulkMinShared && pool_rows <= INT_MAX;
         if (pl.bulk) {
-            // about one item per SM (a bulk CTA fills one), in whole tiles
+            // about one CTA per SM (a bulk CTA fills one), in whole tiles, as few clusters per set of columns
+            // as that allows
             pl.ctiles = (cols + kBulkCols - 1) / kBulkCols;
             const long long sets = (long long)a.groups * pl.ctiles * g.kv_heads;
-            const int splits = (int)std::max<long long>(1, device_sms(g.device) / sets);
-            pl.ls = std::min(kBulkMaxSplit, std::max(2 * kBulkKeys, round_up((a.max_shared + splits - 1) / splits, kBulkKeys)));
+            const long long most = std::max(1LL, (a.max_shared + 2LL * kBulkKeys - 1) / (2 * kBulkKeys));  // two tiles each
+            int best = 1, count = 1;
+            for (int c = kBulkMaxCluster; c >= 1; c /= 2) {
+                const long long fit = std::min(bulk_clusters(g.device, c) / sets, (most + c - 1) / c);
+                if (c <= 2 * most && fit * c > (long long)best * count) {
+                    best = c;
+                    count = (int)fit;
+                }
+            }
+            pl.cluster = best;
+            pl.ls = std::min(kBulkMaxSplit, std::max(2 * kBulkKeys, round_up((a.max_shared + best * count - 1) / (best * count), kBulkKeys)));
+            pl.nss = (int)((a.max_shared + (long long)pl.ls * best - 1) / ((long long)pl.ls * best));
         } else {
             pl.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
             pl.ctiles = (cols + 8 * pl.nt - 1) / (8 * pl.nt);
             pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared);
         }
-        pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
+        if (!pl.bulk) pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
     }
-    const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss;
+    const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss * pl.cluster;
     const long long pi = (long long)a.rows * g.kv_heads * pl.nsp;
     if (si + pi > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
     pl.shared_items = (int)si;
     pl.private_items = (int)pi;
-    pl.direct = a.groups == 0 && pl.nsp == 1;
+    pl.direct = a.groups == 0 ? pl.nsp == 1 : pl.bulk && pl.nss == 1 && pl.nsp == 0;
     if (!pl.direct) {
         const size_t parts = (size_t)a.rows * a.heads * (pl.nss + pl.nsp);
         pl.ml_off = parts * g.head_dim * 4;
@@ -185,12 +233,6 @@ PaFn pa_pick(int D, int nt, int type) { return type == LAIC_GGML_F32 ? pa_fn<flo
 template <typename T>
 PaFn pm_fn(int D) {
     return D == 32 ? paged_merge_kernel<32, T> : D == 64 ? paged_merge_kernel<64, T> : paged_merge_kernel<128, T>;
-}
-
-using BulkFn = void (*)(KvAttnParams, CUtensorMap, CUtensorMap);
-BulkFn bulk_pick(int D, bool f32) {
-    if (D == 64) return f32 ? paged_bulk_kernel<64, float> : paged_bulk_kernel<64, __half>;
-    return f32 ? paged_bulk_kernel<128, float> : paged_bulk_kernel<128, __half>;
 }
 
 using EncodeFn = decltype(&cuTensorMapEncodeTiled);
@@ -344,9 +386,10 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     p.group_rows = a.group_rows_dev; p.group_len = a.group_len_dev;
     const float scale = a.scale != 0.f ? a.scale : 1.f / sqrtf((float)g.head_dim);
     p.scale_log2 = scale * 1.44269504f;
-    p.lp = pl.lp; p.nsp = pl.nsp; p.ls = pl.ls; p.nss = pl.nss; p.ctiles = pl.ctiles;
+    p.lp = pl.lp; p.nsp = pl.nsp; p.ls = pl.ls; p.nss = pl.nss; p.ctiles = pl.ctiles; p.lc = pl.cluster;
     p.shared_items = pl.bulk ? 0 : pl.shared_items;
     p.direct = pl.direct;
+    p.out_vec = aligned16(a.out_dev) && (a.rows == 1 || a.ldo * type_size(a.type) % 16 == 0);
     p.q_vec = aligned16(a.q_dev) && (a.rows == 1 || a.ldq * type_size(a.type) % 16 == 0);
     if (!pl.direct) {
         p.part_o = static_cast<float*>(a.workspace_dev);
@@ -360,8 +403,8 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
             CUtensorMap mk, mv;
             if (!encode_pages(g, g.k_dev, &mk) || !encode_pages(g, g.v_dev, &mv))
                 return api_fail(LAIC_E_CUDA, "kv_attention: tensor map");
-            e = launch_k(bulk_pick(g.head_dim, f32), dim3(pl.shared_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32), st,
-                         false, p, mk, mv);
+            e = launch_cluster_k(bulk_pick(g.head_dim, f32), dim3(pl.shared_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32),
+                                 st, false, pl.cluster, p, mk, mv);
         }
         const int items = p.shared_items + pl.private_items;
         const bool before = pl.bulk && pl.shared_items;  // (a kernel of this call, which nothing earlier runs beside)
