@@ -3,9 +3,10 @@
 // out[r] = sum_t p_t v_t, p = softmax_t(scale q[r] . k_t) over the positions t < n_r of row r's
 // sequence. The work is cut into items, each a set of score columns (query row, query head of one
 // KV head) over a range of positions:
-//   private item: one row's G = heads / kv_heads columns over a split of [shared, n_r);
-//   shared item: up to 8 NT columns of a group's rows over a split of [0, shared), so the keys and
-//   values of a shared position are read once for all of them.
+//   private item: one row's G = heads / kv_heads columns over [shared, n_r): a CTA's four warps where the
+//   range is short (it then joins the shared items' results and writes the output), else a warp per split;
+//   shared item (a CTA): up to 8 NT columns of a group's rows over a split of [0, shared), so the keys
+//   and values of a shared position are read once for all of them (wide groups: paged_bulk.cuh).
 // An item keeps, per column, the running maximum m of the scores (log2 domain), l = sum 2^(s - m)
 // and the unnormalised output; where a row has several items the merge kernel joins them by
 // out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
@@ -17,8 +18,8 @@
 // magnitude leaves binary16's range, and the weights carry a factor 2^7 that keeps small ones
 // out of its subnormals (both sides of the final division have it). The hi and lo products have
 // accumulators of their own: the tensor cores truncate as they accumulate, and lo parts added to a
-// large sum would only lengthen that chain. With at most four columns (a decode step of the usual
-// groups) hi and lo sit side by side in one tile's eight columns (PK), so the split costs no
+// large sum would only lengthen that chain. A private item of at most four columns (a decode step of
+// the usual groups) has hi and lo side by side in one tile's eight columns (PK), so the split costs no
 // product at all.
 #pragma once
 #include "common.cuh"
@@ -42,12 +43,12 @@ struct KvAttnParams {
     int lp, nsp;                  // private splits: positions each, count
     int ls, nss, ctiles;          // shared splits, column tiles per group
     int lc;                       // splits joined into one partial (the bulk kernel's clusters; else 1)
-    int shared_items;
+    int private_items;
     bool q_vec, out_vec;          // rows of q, of out are 16-byte aligned
     uint32_t g_inv;               // 2^16 / G rounded up
     float* part_o;                // [rows][heads][nss + nsp][head_dim]
     float2* part_ml;              // [rows][heads][nss + nsp] (m, l)
-    int direct;                   // one item per row: it writes the output
+    int direct;                   // the bulk kernel's clusters hold all that their rows see: they write the output
     int* err;
 };
 
@@ -153,14 +154,13 @@ __device__ __forceinline__ float q_at(const KvAttnParams& p, int r, int h, int d
 // One item: columns [col0, col0 + 8 NT) of rows r0.. (column = row offset * G + head), positions
 // [t0, t1) of sequence `seq`. Column c sees positions below lim[c] (shared memory; 0: no column).
 // slot: the partial's index among its row's; minlim: the smallest lim of a live column.
-template <int D, int NT, typename T, bool PK>
+template <int D, int NT, typename T>
 __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0, int ncol, int kvh, int seq, int t0,
                                         int t1, int slot, const int* lim, int minlim, int* page_ids, float* cmul,
                                         uint8_t* smem) {
-    constexpr bool HL = sizeof(T) == 4 && !PK;  // a second set of products for the lo parts
+    constexpr bool HL = sizeof(T) == 4;  // a second set of products for the lo parts
     constexpr int HN = HL ? 2 : 1;
-    static_assert(!PK || (NT == 1 && sizeof(T) == 4), "hi and lo side by side: one tile of FP32 columns");
-    constexpr int KS = D / 16, CPR = D / 8, NC = PK ? 4 : NT * 8, NW = kPaWarps, NTH = kPaWarps * 32;
+    constexpr int KS = D / 16, CPR = D / 8, NC = NT * 8, NW = kPaWarps, NTH = kPaWarps * 32;
     constexpr int NST = pa_stages(D);
     constexpr size_t kRed = (size_t)NW * NC * (D + 4) * 4;
     constexpr size_t kQoff = pa_ring_bytes(D) > kRed ? pa_ring_bytes(D) : kRed;
@@ -231,7 +231,7 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             mx = fmaxf(mx, fmaxf(fabsf(a[i]), fabsf(b[i])));
         }
         float fac = 1.f, inv = 1.f;
-        if (HL || PK) {
+        if (HL) {
             mx = warp_max(mx);
             const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
             fac = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -247,8 +247,7 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                 const float va = a[i] * fac, vb = b[i] * fac;
                 const __half ha = __float2half_rn(va), hb = __float2half_rn(vb);
                 dst[0] = pack_h2(ha, hb);
-                if (HL || PK)  // the next plane, or the column four on
-                    dst[HL ? 64 : 32] = pack_h2(__float2half_rn(va - __half2float(ha)), __float2half_rn(vb - __half2float(hb)));
+                if (HL) dst[64] = pack_h2(__float2half_rn(va - __half2float(ha)), __float2half_rn(vb - __half2float(hb)));
             }
         }
     }
@@ -308,14 +307,13 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                 int lm[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int col = PK ? (2 * c + h) & 3 : nt * 8 + 2 * c + h;
+                    const int col = nt * 8 + 2 * c + h;
                     cm2[h] = cmul[col];
                     lm[h] = min(t1, lim[col]);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (HL) s[nt][e] += sl[nt][e];
-                    if (PK) s[nt][e] += __shfl_xor_sync(0xffffffffu, s[nt][e], 2);
                     const float x = s[nt][e] * cm2[e & 1];
                     const int at = pos + (e >> 1) * 8;
                     if (full || (at < lm[e & 1] && at >= t0)) mx[e & 1] = fmaxf(mx[e & 1], x);
@@ -344,13 +342,10 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                 for (int h = 0; h < 2; ++h) l_[nt][h] = fmaf(l_[nt][h], corr[h], sum[h]);  // this lane's positions
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    __half h0 = __float2half_rn(pv[2 * j]), h1 = __float2half_rn(pv[2 * j + 1]);
-                    if (HL || PK) {
-                        const __half l0 = __float2half_rn(pv[2 * j] - __half2float(h0));
-                        const __half l1 = __float2half_rn(pv[2 * j + 1] - __half2float(h1));
-                        if (HL) pl[nt][j] = movm_t(pack_h2(l0, l1));
-                        if (PK && c >= 2) { h0 = l0; h1 = l1; }
-                    }
+                    const __half h0 = __float2half_rn(pv[2 * j]), h1 = __float2half_rn(pv[2 * j + 1]);
+                    if (HL)
+                        pl[nt][j] = movm_t(pack_h2(__float2half_rn(pv[2 * j] - __half2float(h0)),
+                                                   __float2half_rn(pv[2 * j + 1] - __half2float(h1))));
                     ph[nt][j] = movm_t(pack_h2(h0, h1));
                 }
                 if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
@@ -361,7 +356,7 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = PK && c >= 2 ? 0.f : pv[e];
+                for (int e = 0; e < 4; ++e) s[nt][e] = pv[e];
             }
             // a position that some columns see and others do not: where its value is not finite,
             // 0 * inf would reach the others, so those products are summed one by one
@@ -433,20 +428,15 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
     float* red = reinterpret_cast<float*>(smem);  // [warp][column][D + 4]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const bool mine = !PK || c < 2;  // (PK: the lo columns' outputs are added to the hi columns')
-        if (gq == 0 && mine) {
+        if (gq == 0) {
             cm[warp][nt * 8 + 2 * c] = m_[nt][0]; cm[warp][nt * 8 + 2 * c + 1] = m_[nt][1];
             cl[warp][nt * 8 + 2 * c] = l_[nt][0]; cl[warp][nt * 8 + 2 * c + 1] = l_[nt][1];
         }
 #pragma unroll
         for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float v = o[mt][nt][e];
-                if (PK) v += __shfl_xor_sync(0xffffffffu, v, 2);
-                if (mine)
-                    red[((size_t)warp * NC + nt * 8 + 2 * c + (e & 1)) * (D + 4) + mt * 16 + gq + (e >> 1) * 8] = v;
-            }
+            for (int e = 0; e < 4; ++e)
+                red[((size_t)warp * NC + nt * 8 + 2 * c + (e & 1)) * (D + 4) + mt * 16 + gq + (e >> 1) * 8] = o[mt][nt][e];
     }
     __syncthreads();
     const int ns = p.nss + p.nsp;
@@ -468,55 +458,314 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             }
         }
         const int r = r0 + cc / p.G, h = kvh * p.G + cc % p.G;
-        if (p.direct) {
-            const float iv = M == -INFINITY ? 0.f : 1.f / L;
-            T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)h * D + d;
-            dst[0] = kv_out<T>(A.x * iv); dst[1] = kv_out<T>(A.y * iv);
-            dst[2] = kv_out<T>(A.z * iv); dst[3] = kv_out<T>(A.w * iv);
-        } else {
-            const size_t at = ((size_t)r * p.heads + h) * ns + slot;
-            *reinterpret_cast<float4*>(p.part_o + at * D + d) = A;
-            if (d == 0) p.part_ml[at] = make_float2(M, L);
-        }
+        const size_t at = ((size_t)r * p.heads + h) * ns + slot;
+        *reinterpret_cast<float4*>(p.part_o + at * D + d) = A;
+        if (d == 0) p.part_ml[at] = make_float2(M, L);
     }
 }
 
-// One row's own positions: item i of [row][kv head][split].
-template <int D, typename T>
-__device__ __forceinline__ void private_item(const KvAttnParams& p, int i, int* lim, int* page_ids, float* cmul, int* found,
-                                             uint8_t* smem) {
-    const int tid = threadIdx.x, split = i % p.nsp;
-    i /= p.nsp;
+constexpr int kPrWarps = 4;
+constexpr int kPrStages = 2;      // 16 positions of K and V each, per warp (three: fewer CTAs per SM, 192 against 187 us)
+constexpr int kPrWhole = 1024;    // private ranges up to this stay whole (and no split is longer)
+__host__ __device__ constexpr size_t pr_smem(int D) { return (size_t)kPrWarps * kPrStages * 2 * 16 * D * 2; }
+
+// One row's own positions, every warp on its own ring of 16-position stages.
+// WHOLE: a CTA per [row][kv head], its warps take every fourth block of 16 positions; at the end they
+// and the row's shared items (the kernel before this one) are joined and the output written.
+// Else: a warp per item of [row][kv head][split], no barrier between the warps.
+// PK: FP32 rows of at most four columns, hi parts in columns 0-3, lo parts in 4-7 of the tile.
+template <int D, typename T, bool PK, bool WHOLE>
+__global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAttnParams p) {
+    constexpr bool HL = sizeof(T) == 4 && !PK;
+    constexpr int HN = HL ? 2 : 1, KS = D / 16, CPR = D / 8, NST = kPrStages;
+    constexpr uint32_t STAGE = 2 * 16 * D * 2;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int page_ids[kPrWarps][kPrWhole / 16 + 2];
+    __shared__ uint32_t qf[kPrWarps][KS][HN][32][2];
+    __shared__ float cmul[kPrWarps][8];
+    __shared__ int found[kPrWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int gq = lane >> 2, c = lane & 3;
+    pdl_launch_dependents();  // (the merge waits for this grid's end; nothing else follows)
+    int i = WHOLE ? blockIdx.x : blockIdx.x * kPrWarps + warp;
+    const bool in = WHOLE || i < p.private_items;
+    if (!in) i = 0;
+    const int split = WHOLE ? 0 : i % p.nsp;
+    if (!WHOLE) i /= p.nsp;
     const int kvh = i % p.kv_heads, r = i / p.kv_heads;
     const int len = p.len[r], sq = p.seq ? p.seq[r] : r;  // under way while the groups are searched
     int shared = 0;
     if (p.groups) {
-        if (tid == 0) *found = 0;
-        __syncthreads();
-        find_group(p, r, tid, kPaWarps * 32, found);
-        __syncthreads();
-        shared = *found;
+        if (lane == 0) found[warp] = 0;
+        __syncwarp();
+        find_group(p, r, lane, 32, &found[warp]);
+        __syncwarp();
+        shared = found[warp];
     }
     const RowView v = row_view(p, len, sq, shared);
-    if (v.n < 0) return;
-    if (v.n - v.shared > p.max_private && tid == 0) kv_flag(p.err, kKvBadPos);
-    const int t0 = v.shared + split * p.lp, t1 = min(min(v.n, v.shared + p.max_private), t0 + p.lp);
-    if (t0 >= t1) {
-        if (p.direct) {  // a row that sees nothing
-            T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)kvh * p.G * D;
-            for (int e = tid; e < p.G * D; e += kPaWarps * 32) dst[e] = kv_out<T>(0.f);
-        }
+    if (v.n - v.shared > p.max_private && lane == 0) kv_flag(p.err, kKvBadPos);
+    if (WHOLE && v.n < 0) {  // padding
+        if (blockIdx.x == 0) pdl_wait();
         return;
     }
-    if (tid < 8) lim[tid] = tid < p.G ? t1 : 0;
-    const int slot = p.nss + split;
-    if constexpr (sizeof(T) == 4) {
-        if (p.G <= 4) {
-            pa_item<D, 1, T, true>(p, r, 0, p.G, kvh, v.seq, t0, t1, slot, lim, t1, page_ids, cmul, smem);
-            return;
+    const int t0 = v.shared + split * p.lp, t1 = in ? min(min(v.n, v.shared + p.max_private), t0 + p.lp) : 0;
+    constexpr int STRIDE = WHOLE ? kPrWarps : 1;
+    const int a0 = t0 & ~15, first = WHOLE ? warp : 0;  // blocks first, first + STRIDE, ... of 16 positions from a0
+    const int nb = in && v.n >= 0 && t0 < t1 ? (((t1 - a0 + 15) >> 4) - first + STRIDE - 1) / STRIDE : 0;
+    float m_[2] = {-INFINITY, -INFINITY}, l_[2] = {0.f, 0.f}, o[KS][4];
+#pragma unroll
+    for (int mt = 0; mt < KS; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+    if (nb > 0) {
+        // ---- the range's page ids, each checked once; blocks of 16 positions lie in one page
+        const int first_page = a0 >> p.page_shift, npages = ((t1 - 1) >> p.page_shift) - first_page + 1;
+        for (int k = lane; k < npages; k += 32) {
+            int id = p.table[(size_t)v.seq * p.pages_per_seq + first_page + k];
+            if (id < 0 || id >= p.num_pages) {
+                kv_flag(p.err, kKvBadPage);
+                id = 0;
+            }
+            page_ids[warp][k] = id;
+        }
+        __syncwarp();
+        const uint32_t ring = smem_u32(smem) + (uint32_t)warp * (NST * STAGE);
+        constexpr int RPP = 32 / CPR;  // rows a pass of the warp covers
+        const int lrow = lane / CPR, lcc = lane % CPR;
+        const int page_mask = (1 << p.page_shift) - 1;
+        const size_t src0 = (size_t)lrow * D + lcc * 8;
+        auto load = [&](int b) {
+            if (b < nb) {
+                const int tb = a0 + (first + b * STRIDE) * 16;
+                const size_t at = ((((size_t)page_ids[warp][(tb >> p.page_shift) - first_page] * p.kv_heads + kvh) << p.page_shift) +
+                                   (tb & page_mask)) * D + src0;
+                const uint32_t kd = ring + (uint32_t)(b % NST) * STAGE;
+#pragma unroll
+                for (int q = 0; q < 16 / RPP; ++q) {
+                    const int rr = lrow + q * RPP;
+                    const bool ok = tb + rr < t1;  // rows past the end: zeros
+                    cp_async16_z(kd + 2 * attn_swz<D>(rr, lcc), p.kp + at + (size_t)q * RPP * D, ok);
+                    cp_async16_z(kd + 16 * D * 2 + 2 * attn_swz<D>(rr, lcc), p.vp + at + (size_t)q * RPP * D, ok);
+                }
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int b = 0; b < NST - 1; ++b) load(b);
+
+        // ---- query fragments, column by column
+        constexpr int PL = (D / 2 + 31) / 32;  // pairs per lane
+        float qa[8][PL][2];
+#pragma unroll
+        for (int col = 0; col < (PK ? 4 : 8); ++col)
+#pragma unroll
+            for (int k = 0; k < PL; ++k) {
+                const int pi = lane + 32 * k, hh = (kvh * p.G + col) * D;
+                const bool got = col < p.G && pi < D / 2;
+                qa[col][k][0] = got ? q_at<T>(p, r, hh, 2 * pi) : 0.f;
+                qa[col][k][1] = got ? q_at<T>(p, r, hh, 2 * pi + 1) : 0.f;
+            }
+#pragma unroll
+        for (int col = 0; col < (PK ? 4 : 8); ++col) {
+            float fac = 1.f, inv = 1.f;
+            if (HL || PK) {
+                float mx = 0.f;
+#pragma unroll
+                for (int k = 0; k < PL; ++k) mx = fmaxf(mx, fmaxf(fabsf(qa[col][k][0]), fabsf(qa[col][k][1])));
+                mx = warp_max(mx);
+                const int e = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
+                fac = __uint_as_float((uint32_t)(127 - e) << 23);
+                inv = __uint_as_float((uint32_t)(127 + e) << 23);
+            }
+            if (lane == 0) cmul[warp][col] = p.scale_log2 * inv;
+#pragma unroll
+            for (int k = 0; k < PL; ++k) {
+                const int pi = lane + 32 * k;
+                if (pi < D / 2) {
+                    const int ks = pi >> 3, j = (pi >> 2) & 1, cl = pi & 3;
+                    const float va = qa[col][k][0] * fac, vb = qa[col][k][1] * fac;
+                    const __half ha = __float2half_rn(va), hb = __float2half_rn(vb);
+                    qf[warp][ks][0][col * 4 + cl][j] = pack_h2(ha, hb);
+                    if (HL || PK) {
+                        const uint32_t lo = pack_h2(__float2half_rn(va - __half2float(ha)), __float2half_rn(vb - __half2float(hb)));
+                        if (HL) qf[warp][ks][HN - 1][col * 4 + cl][j] = lo;
+                        else qf[warp][ks][0][(col + 4) * 4 + cl][j] = lo;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        uint2 qr[KS][HN];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int hl = 0; hl < HN; ++hl) qr[ks][hl] = *reinterpret_cast<const uint2*>(qf[warp][ks][hl][lane]);
+        const float cm2[2] = {cmul[warp][PK ? (2 * c) & 3 : 2 * c], cmul[warp][PK ? (2 * c + 1) & 3 : 2 * c + 1]};
+
+        const int li = lane >> 3, lr = lane & 7;  // ldmatrix: this lane addresses row lr of matrix li
+        for (int b = 0; b < nb; ++b) {
+            cp_async_wait<NST - 2>();
+            __syncwarp();
+            const uint32_t ks_a = ring + (uint32_t)(b % NST) * STAGE, vs_a = ks_a + 16 * D * 2;
+            float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                uint32_t a[4];
+                ldsm_x4(ks_a + 2 * attn_swz<D>((li & 1) * 8 + lr, ks * 2 + (li >> 1)), a);
+                // (two accumulators: the second takes the lo parts, or every other step)
+                if (HL) {
+                    mma16816_acc(s, a[0], a[1], a[2], a[3], qr[ks][0].x, qr[ks][0].y);
+                    mma16816_acc(s2, a[0], a[1], a[2], a[3], qr[ks][HN - 1].x, qr[ks][HN - 1].y);
+                } else if (ks & 1) {
+                    mma16816_acc(s2, a[0], a[1], a[2], a[3], qr[ks][0].x, qr[ks][0].y);
+                } else {
+                    mma16816_acc(s, a[0], a[1], a[2], a[3], qr[ks][0].x, qr[ks][0].y);
+                }
+            }
+            const int c0 = a0 + (first + b * STRIDE) * 16, pos = c0 + gq;
+            const bool full = c0 >= t0 && c0 + 16 <= t1;
+            float mx[2] = {-INFINITY, -INFINITY}, corr[2], sum[2] = {0.f, 0.f}, pv[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[e] += s2[e];
+                if (PK) s[e] += __shfl_xor_sync(0xffffffffu, s[e], 2);
+                const int at = pos + (e >> 1) * 8;
+                if (full || (at >= t0 && at < t1)) mx[e & 1] = fmaxf(mx[e & 1], s[e] * cm2[e & 1]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16));
+                const float mnew = fmaxf(m_[h], mx[h]);
+                const float mu = mnew == -INFINITY ? 0.f : mnew;  // (every score -inf: every weight is 0)
+                corr[h] = ex2(m_[h] - mu);
+                m_[h] = mnew;
+                mx[h] = mu;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                pv[e] = ex2(fmaf(s[e], cm2[e & 1], -mx[e & 1]));
+                const int at = pos + (e >> 1) * 8;
+                if (!full && (at < t0 || at >= t1)) pv[e] = 0.f;
+                sum[e & 1] += pv[e];
+                pv[e] *= kPaGain;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) l_[h] = fmaf(l_[h], corr[h], sum[h]);  // this lane's positions
+            uint32_t ph[2], pl[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                __half h0 = __float2half_rn(pv[2 * j]), h1 = __float2half_rn(pv[2 * j + 1]);
+                if (HL || PK) {
+                    const __half l0 = __float2half_rn(pv[2 * j] - __half2float(h0)), l1 = __float2half_rn(pv[2 * j + 1] - __half2float(h1));
+                    if (HL) pl[j] = movm_t(pack_h2(l0, l1));
+                    if (PK && c >= 2) { h0 = l0; h1 = l1; }
+                }
+                ph[j] = movm_t(pack_h2(h0, h1));
+            }
+            if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt) {
+                    o[mt][0] *= corr[0]; o[mt][1] *= corr[1];
+                    o[mt][2] *= corr[0]; o[mt][3] *= corr[1];
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt) {
+                uint32_t a[4];
+                ldsm_x4_t(vs_a + 2 * attn_swz<D>((li >> 1) * 8 + lr, mt * 2 + (li & 1)), a);
+                mma16816_acc(o[mt], a[0], a[1], a[2], a[3], ph[0], ph[1]);
+                if (HL) mma16816_acc(o[mt], a[0], a[1], a[2], a[3], pl[0], pl[1]);
+            }
+            __syncwarp();  // the stage is free
+            load(b + NST - 1);
+        }
+        cp_async_wait<0>();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float x = l_[h];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            l_[h] = x * kPaGain;
         }
     }
-    pa_item<D, 1, T, false>(p, r, 0, p.G, kvh, v.seq, t0, t1, slot, lim, t1, page_ids, cmul, smem);
+    const int ns = p.nss + p.nsp;
+    if constexpr (!WHOLE) {
+        if (nb > 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int col = 2 * c + h;
+                const bool mine = col < p.G;  // (PK: the lo columns' outputs are added to the hi columns')
+                const size_t at = ((size_t)r * p.heads + kvh * p.G + min(col, p.G - 1)) * ns + p.nss + split;
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float x = o[mt][2 * k + h];
+                        if (PK) x += __shfl_xor_sync(0xffffffffu, x, 2);
+                        if (mine) p.part_o[at * D + mt * 16 + gq + 8 * k] = x;
+                    }
+                if (mine && gq == 0) p.part_ml[at] = make_float2(m_[h], l_[h]);
+            }
+        }
+        if (blockIdx.x == 0) pdl_wait();  // this kernel's end then stands for the shared items' too
+    } else {
+        __shared__ float2 wml[kPrWarps][8];
+        __syncthreads();  // every warp is done with its ring: it takes the warps' outputs
+        float* red = reinterpret_cast<float*>(smem);  // [warp][column][D + 4]
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int col = 2 * c + h;
+            const bool mine = col < p.G;
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float x = o[mt][2 * k + h];
+                    if (PK) x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    if (mine) red[((size_t)warp * 8 + col) * (D + 4) + mt * 16 + gq + 8 * k] = x;
+                }
+            if (mine && gq == 0) wml[warp][col] = make_float2(m_[h], l_[h]);
+        }
+        __syncthreads();
+        const int live_s = v.shared > 0 ? (v.shared + p.ls * p.lc - 1) / (p.ls * p.lc) : 0;
+        if (live_s || blockIdx.x == 0) pdl_wait();  // the shared items' results
+        for (int e = threadIdx.x; e < p.G * (D / 4); e += kPrWarps * 32) {
+            const int col = e / (D / 4), d = e % (D / 4) * 4, head = kvh * p.G + col;
+            const size_t at = ((size_t)r * p.heads + head) * ns;
+            float M = -INFINITY, L = 0.f;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto add = [&](float2 ml, const float4& x, float top) {
+                if (ml.x == -INFINITY) return;
+                const float w = ex2(ml.x - top);
+                L = fmaf(ml.y, w, L);
+                a.x = fmaf(x.x, w, a.x); a.y = fmaf(x.y, w, a.y);
+                a.z = fmaf(x.z, w, a.z); a.w = fmaf(x.w, w, a.w);
+            };
+#pragma unroll
+            for (int w = 0; w < kPrWarps; ++w) M = fmaxf(M, wml[w][col].x);
+            for (int q = 0; q < live_s; ++q) M = fmaxf(M, p.part_ml[at + q].x);
+#pragma unroll 4
+            for (int q = 0; q < live_s; ++q) add(p.part_ml[at + q], *reinterpret_cast<const float4*>(p.part_o + (at + q) * D + d), M);
+#pragma unroll
+            for (int w = 0; w < kPrWarps; ++w)
+                add(wml[w][col], *reinterpret_cast<const float4*>(red + ((size_t)w * 8 + col) * (D + 4) + d), M);
+            const float iv = M == -INFINITY ? 0.f : 1.f / L;
+            T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)head * D + d;
+            const float x[4] = {a.x * iv, a.y * iv, a.z * iv, a.w * iv};
+            if (p.out_vec) {
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+                } else {
+                    const __half2 y = __floats2half2_rn(x[0], x[1]), z = __floats2half2_rn(x[2], x[3]);
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&y), *reinterpret_cast<const uint32_t*>(&z));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) dst[k] = kv_out<T>(x[k]);
+            }
+        }
+    }
 }
 
 // One tile of a group's columns over a split of the shared positions:
@@ -549,21 +798,17 @@ __device__ __forceinline__ void shared_item(const KvAttnParams& p, int i, int* l
     const int t0 = split * p.ls, t1 = min(range[0], t0 + p.ls);
     if (t0 >= t1) return;  // no row of the tile sees this far
     const int seq = max(0, row_seq(p, r0));  // (a bad one is recorded, and reads some sequence's pages)
-    pa_item<D, NT, T, false>(p, r0, col0, ncol, kvh, seq, t0, t1, split, lim, range[1], page_ids, cmul, smem);
+    pa_item<D, NT, T>(p, r0, col0, ncol, kvh, seq, t0, t1, split, lim, range[1], page_ids, cmul, smem);
 }
 
-// Grid: the shared items, then the private ones.
+// Grid: the shared items.
 template <int D, int NT, typename T>
 __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const KvAttnParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int lim[NT * 8], page_ids[kPaMaxSplit / 16 + 2], range[2];
     __shared__ float cmul[NT * 8];
-    __shared__ int found;
-    const int i = blockIdx.x;
-    if (i < p.shared_items) shared_item<D, NT, T>(p, i, lim, page_ids, cmul, range, smem);
-    else private_item<D, T>(p, i - p.shared_items, lim, page_ids, cmul, &found, smem);
-    pdl_launch_dependents();
-    if (i == 0) pdl_wait();  // this kernel's end then stands for the bulk kernel's too
+    pdl_launch_dependents();  // the private items need nothing of this kernel
+    shared_item<D, NT, T>(p, blockIdx.x, lim, page_ids, cmul, range, smem);
 }
 
 constexpr int kPmWarps = 4;

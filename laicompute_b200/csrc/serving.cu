@@ -138,7 +138,8 @@ struct AttnPlan {
     int shared_items = 0, private_items = 0;
     bool bulk = false;     // the shared items run in paged_bulk.cuh,
     int cluster = 1;       // this many splits of a set of columns in a cluster (nss counts clusters)
-    bool direct = false;
+    bool whole = false;    // a CTA per row and kv head finishes the row
+    bool direct = false;   // the bulk kernel's clusters do
     size_t ml_off = 0, bytes = 0;
 };
 
@@ -166,19 +167,21 @@ int check_attention(const laic_kv_pages& g, const laic_kv_attention_args& a) {
 int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, AttnPlan& pl) {
     const int G = a.heads / g.kv_heads;
     const int max_private = a.max_private < 0 ? a.max_len : std::min(a.max_private, a.max_len);
-    // splits: about `want` items, each a whole number of chunks; not below 128 positions (a join costs
-    // more than another chunk) and a range of 256 stays whole; at most 512 (a partial costs 2 % of such
-    // an item's bytes, and ragged rows balance)
-    const long long want = 4LL * device_sms(g.device);
-    auto split = [&](long long pairs, int len) {
-        if (len <= 256) return round_up(std::max(len, 1), kPaChunk);
+    // splits of `len` positions over `pairs` items each: about `want` items; a range of up to `whole` stays in
+    // one piece and none is shorter than 128 (a join costs more than that many positions)
+    auto split = [&](long long pairs, int len, long long want, int unit, int whole, int most) {
+        if (len <= whole) return round_up(std::max(len, 1), unit);
         const long long l = ((long long)len * pairs + want - 1) / want;
-        return std::max(128, std::min(round_up(l, kPaChunk), 512));
+        return std::max(128, std::min(round_up(l, unit), most));
     };
-    pl.lp = split((long long)a.rows * g.kv_heads, max_private);
-    pl.nsp = std::max(1, (max_private + pl.lp - 1) / pl.lp);
+    const int sms = device_sms(g.device);
+    // private: ranges up to kPrWhole by one CTA, which writes the output; longer ones by a warp per split, 8 to 12
+    // on an SM (256 positions: a partial costs 2 % of their bytes, and ragged rows balance)
+    pl.whole = max_private <= kPrWhole;
+    pl.lp = pl.whole ? kPrWhole : split((long long)a.rows * g.kv_heads, max_private, 12LL * sms, 16, 128, 256);
+    pl.nsp = pl.whole ? 0 : (max_private + pl.lp - 1) / pl.lp;
     if (a.groups) {
-        if (max_private == 0) pl.nsp = 0;
+        if (max_private == 0) pl.whole = false;  // nothing private: shared items alone, joined by the merge
         const int cols = a.max_group_rows * G;
         const long long pool_rows = (long long)g.num_pages * g.kv_heads * g.page_size;
         pl.bulk = g.head_dim >= 64 && cols >= kBulkMinCols && a.max_shared >= kBulkMinShared && pool_rows <= INT_MAX;
@@ -202,17 +205,17 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
         } else {
             pl.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
             pl.ctiles = (cols + 8 * pl.nt - 1) / (8 * pl.nt);
-            pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared);
+            pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared, 4LL * sms, kPaChunk, 256, 512);
         }
         if (!pl.bulk) pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
     }
     const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss * pl.cluster;
-    const long long pi = (long long)a.rows * g.kv_heads * pl.nsp;
+    const long long pi = (long long)a.rows * g.kv_heads * (pl.whole ? 1 : pl.nsp);
     if (si + pi > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
     pl.shared_items = (int)si;
     pl.private_items = (int)pi;
-    pl.direct = a.groups == 0 ? pl.nsp == 1 : pl.bulk && pl.nss == 1 && pl.nsp == 0;
-    if (!pl.direct) {
+    pl.direct = pl.bulk && pl.nss == 1 && pi == 0;
+    if (!pl.direct && pl.nss + pl.nsp) {
         const size_t parts = (size_t)a.rows * a.heads * (pl.nss + pl.nsp);
         pl.ml_off = parts * g.head_dim * 4;
         pl.bytes = pl.ml_off + parts * 8;
@@ -230,6 +233,17 @@ PaFn pa_fn(int D, int nt) {
     return D == 32 ? pa_fn_nt<32, T>(nt) : D == 64 ? pa_fn_nt<64, T>(nt) : pa_fn_nt<128, T>(nt);
 }
 PaFn pa_pick(int D, int nt, int type) { return type == LAIC_GGML_F32 ? pa_fn<float>(D, nt) : pa_fn<__half>(D, nt); }
+template <typename T, bool PK, bool WHOLE>
+PaFn pr_fn(int D) {
+    return D == 32   ? paged_private_kernel<32, T, PK, WHOLE>
+           : D == 64 ? paged_private_kernel<64, T, PK, WHOLE>
+                     : paged_private_kernel<128, T, PK, WHOLE>;
+}
+template <bool WHOLE>
+PaFn pr_fn_type(int D, int type, int G) {
+    return type == LAIC_GGML_F16 ? pr_fn<__half, false, WHOLE>(D) : G <= 4 ? pr_fn<float, true, WHOLE>(D) : pr_fn<float, false, WHOLE>(D);
+}
+PaFn pr_pick(int D, int type, int G, bool whole) { return whole ? pr_fn_type<true>(D, type, G) : pr_fn_type<false>(D, type, G); }
 template <typename T>
 PaFn pm_fn(int D) {
     return D == 32 ? paged_merge_kernel<32, T> : D == 64 ? paged_merge_kernel<64, T> : paged_merge_kernel<128, T>;
@@ -273,6 +287,12 @@ cudaError_t serving_set_attributes() {
             for (int type : {LAIC_GGML_F32, LAIC_GGML_F16}) {
                 e = cudaFuncSetAttribute(pa_pick(D, nt, type), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)pa_smem(D, nt, type == LAIC_GGML_F32));
+                if (e != cudaSuccess) return e;
+            }
+    for (int D : {32, 64, 128})
+        for (bool whole : {false, true})
+            for (PaFn fn : {pr_pick(D, LAIC_GGML_F16, 1, whole), pr_pick(D, LAIC_GGML_F32, 4, whole), pr_pick(D, LAIC_GGML_F32, 8, whole)}) {
+                e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pr_smem(D));
                 if (e != cudaSuccess) return e;
             }
     for (int D : {64, 128})
@@ -387,11 +407,11 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     const float scale = a.scale != 0.f ? a.scale : 1.f / sqrtf((float)g.head_dim);
     p.scale_log2 = scale * 1.44269504f;
     p.lp = pl.lp; p.nsp = pl.nsp; p.ls = pl.ls; p.nss = pl.nss; p.ctiles = pl.ctiles; p.lc = pl.cluster;
-    p.shared_items = pl.bulk ? 0 : pl.shared_items;
+    p.private_items = pl.private_items;
     p.direct = pl.direct;
     p.out_vec = aligned16(a.out_dev) && (a.rows == 1 || a.ldo * type_size(a.type) % 16 == 0);
     p.q_vec = aligned16(a.q_dev) && (a.rows == 1 || a.ldq * type_size(a.type) % 16 == 0);
-    if (!pl.direct) {
+    if (pl.bytes) {
         p.part_o = static_cast<float*>(a.workspace_dev);
         p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(a.workspace_dev) + pl.ml_off);
     }
@@ -406,15 +426,18 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
             e = launch_cluster_k(bulk_pick(g.head_dim, f32), dim3(pl.shared_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32),
                                  st, false, pl.cluster, p, mk, mv);
         }
-        const int items = p.shared_items + pl.private_items;
-        const bool before = pl.bulk && pl.shared_items;  // (a kernel of this call, which nothing earlier runs beside)
-        if (e == cudaSuccess && items)
-            e = launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(items), dim3(kPaWarps * 32),
-                         pa_smem(g.head_dim, pl.nt, f32), st, before, p);
-        if (e == cudaSuccess && !pl.direct)
+        if (e == cudaSuccess && !pl.bulk && pl.shared_items)
+            e = launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(pl.shared_items), dim3(kPaWarps * 32),
+                         pa_smem(g.head_dim, pl.nt, f32), st, false, p);
+        // (launched early only behind kernels of this call, which nothing earlier runs beside)
+        if (e == cudaSuccess && pl.private_items)
+            e = launch_k(pr_pick(g.head_dim, a.type, p.G, pl.whole),
+                         dim3(pl.whole ? pl.private_items : (pl.private_items + kPrWarps - 1) / kPrWarps), dim3(kPrWarps * 32),
+                         pr_smem(g.head_dim), st, pl.shared_items > 0, p);
+        if (e == cudaSuccess && !pl.direct && !pl.whole)
             e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
                          dim3((unsigned)(((long long)a.rows * a.heads + kPmWarps - 1) / kPmWarps)), dim3(kPmWarps * 32), 0,
-                         st, before || items, p);
+                         st, pl.shared_items || pl.private_items, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "kv_attention");
     });
 }
