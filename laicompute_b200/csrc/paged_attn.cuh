@@ -812,60 +812,90 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const KvAttnP
 }
 
 constexpr int kPmWarps = 4;
-// Join the items of each (row, head): one warp per pair, grid ceil(rows * heads / kPmWarps).
+// Join the items of a (row, head) pair: a CTA per pair, its warps take every fourth item (one warp alone
+// walked a long row's 32 items in 21 us on 64 rows of 32 heads), their sums meet in shared memory.
 template <int D, typename T>
 __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttnParams p) {
-    constexpr int E = D / 32;
-    __shared__ int found[kPmWarps];
+    constexpr int E = D / 32, U = 8;  // U items' loads in flight
+    __shared__ int found;
+    __shared__ float acc_s[kPmWarps][D], l_s[kPmWarps], m_s[kPmWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int pair = blockIdx.x * kPmWarps + warp;
-    const bool in = pair < p.rows * p.heads;
-    const int r = in ? pair / p.heads : 0, h = in ? pair % p.heads : 0;
+    const int r = blockIdx.x / p.heads, h = blockIdx.x % p.heads;
     const int len = p.len[r], sq = p.seq ? p.seq[r] : r;
-    if (lane == 0) found[warp] = 0;
-    __syncwarp();
-    find_group(p, r, lane, 32, &found[warp]);
-    __syncwarp();
-    const RowView v = row_view(p, len, sq, found[warp]);
+    int shared = 0;
+    if (p.groups) {
+        if (threadIdx.x == 0) found = 0;
+        __syncthreads();
+        find_group(p, r, threadIdx.x, kPmWarps * 32, &found);
+        __syncthreads();
+        shared = found;
+    }
+    const RowView v = row_view(p, len, sq, shared);
     pdl_wait();
-    if (!in || v.n < 0) return;
+    if (v.n < 0) return;
     const int ns = p.nss + p.nsp;
     const int priv = min(v.n - v.shared, p.max_private);
-    if (v.n - v.shared > p.max_private && lane == 0) kv_flag(p.err, kKvBadPos);
+    if (v.n - v.shared > p.max_private && threadIdx.x == 0) kv_flag(p.err, kKvBadPos);
     const int live_s = v.shared > 0 ? (v.shared + p.ls * p.lc - 1) / (p.ls * p.lc) : 0;
     const int live = live_s + (priv > 0 ? (priv + p.lp - 1) / p.lp : 0);
-    const size_t base = (size_t)pair * ns;
+    const size_t base = (size_t)blockIdx.x * ns;
     auto slot = [&](int i) { return i < live_s ? i : p.nss + (i - live_s); };
-    float M = -INFINITY;
-    for (int i = lane; i < live; i += 32) M = fmaxf(M, p.part_ml[base + slot(i)].x);
-    M = warp_max(M);
-    float L = 0.f, acc[E] = {};
-    for (int i0 = 0; i0 < live; i0 += 32) {
-        float w = 0.f;
-        if (i0 + lane < live) {
-            const float2 ml = p.part_ml[base + slot(i0 + lane)];
-            w = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-            L = fmaf(ml.y, w, L);
-        }
-        const int n = min(32, live - i0);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            const float* src = p.part_o + (base + slot(i0 + i)) * D + lane * E;
-            float x[E];
-            if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
-            else if constexpr (E == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
-            else x[0] = *src;
+    // this warp's items i = warp, warp + 4, ...: U at a time against the running maximum
+    float M = -INFINITY, L = 0.f, acc[E] = {};
+    for (int i0 = warp; i0 < live; i0 += kPmWarps * U) {
+        float2 ml[U];
+        float x[U][E];
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (wi != 0.f) acc[e] = fmaf(x[e], wi, acc[e]);
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * kPmWarps;
+            ml[u] = make_float2(-INFINITY, 0.f);
+            if (i < live) {
+                ml[u] = p.part_ml[base + slot(i)];
+                const float* src = p.part_o + (base + slot(i)) * D + lane * E;
+                if constexpr (E == 4) *reinterpret_cast<float4*>(x[u]) = *reinterpret_cast<const float4*>(src);
+                else if constexpr (E == 2) *reinterpret_cast<float2*>(x[u]) = *reinterpret_cast<const float2*>(src);
+                else x[u][0] = *src;
+            }
         }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) top = fmaxf(top, ml[u].x);
+        if (top == -INFINITY) continue;
+        const float corr = ex2(M - top);
+        M = top;
+        L *= corr;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] *= corr;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (ml[u].x != -INFINITY) {
+                const float w = ex2(ml[u].x - M);
+                L = fmaf(ml[u].y, w, L);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = fmaf(x[u][e], w, acc[e]);
+            }
     }
-    L = warp_sum(L);
-    const float iv = M == -INFINITY ? 0.f : 1.f / L;
-    T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)h * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = kv_out<T>(acc[e] * iv);
+    for (int e = 0; e < E; ++e) acc_s[warp][lane * E + e] = acc[e];
+    if (lane == 0) { m_s[warp] = M; l_s[warp] = L; }
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f, w[kPmWarps];
+#pragma unroll
+    for (int k = 0; k < kPmWarps; ++k) top = fmaxf(top, m_s[k]);
+#pragma unroll
+    for (int k = 0; k < kPmWarps; ++k) {
+        w[k] = m_s[k] == -INFINITY ? 0.f : ex2(m_s[k] - top);
+        sum = fmaf(l_s[k], w[k], sum);
+    }
+    const float iv = top == -INFINITY ? 0.f : 1.f / sum;
+    T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)h * D;
+    for (int d = threadIdx.x; d < D; d += kPmWarps * 32) {
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < kPmWarps; ++k)
+            if (w[k] != 0.f) a = fmaf(acc_s[k][d], w[k], a);
+        dst[d] = kv_out<T>(a * iv);
+    }
 }
 
 }  // namespace laic

@@ -211,7 +211,7 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
     }
     const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss * pl.cluster;
     const long long pi = (long long)a.rows * g.kv_heads * (pl.whole ? 1 : pl.nsp);
-    if (si + pi > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
+    if (si + pi > INT_MAX || (long long)a.rows * a.heads > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
     pl.shared_items = (int)si;
     pl.private_items = (int)pi;
     pl.direct = pl.bulk && pl.nss == 1 && pi == 0;
@@ -436,7 +436,7 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
                          pr_smem(g.head_dim), st, pl.shared_items > 0, p);
         if (e == cudaSuccess && !pl.direct && !pl.whole)
             e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
-                         dim3((unsigned)(((long long)a.rows * a.heads + kPmWarps - 1) / kPmWarps)), dim3(kPmWarps * 32), 0,
+                         dim3((unsigned)(a.rows * a.heads)), dim3(kPmWarps * 32), 0,
                          st, pl.shared_items || pl.private_items, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "kv_attention");
     });

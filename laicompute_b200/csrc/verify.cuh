@@ -41,9 +41,9 @@ struct ProbsPart {
 };
 
 // A cluster per row, each CTA a slice held in shared memory (SM; vocab <= cluster * kProbsSlice), so
-// the row is read once: the slice's maximum and its sum of 2^((x - slice maximum) k) meet in one
-// exchange, then every element is formed against the row's maximum. Else (larger vocabularies) a
-// CTA per row reads it three times. VEC: 16-byte aligned rows.
+// the row is read once and every exponential formed once: the slice's weights against its own maximum
+// stay there, the maxima and sums meet in one exchange, and a product per element is left. Else
+// (larger vocabularies) a CTA per row reads it three times. VEC: 16-byte aligned rows.
 template <bool SM, bool VEC>
 __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsParams p) {
     namespace cg = cooperative_groups;
@@ -78,7 +78,6 @@ __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsPara
         if constexpr (VEC) cp_async_wait_all();
         __syncthreads();
     }
-    auto get = [&](float v) { return v == v ? v : -INFINITY; };  // a NaN cannot be chosen
     // f(element, its index) over this thread's elements, in ascending order
     auto each = [&](auto&& f) {
         if constexpr (SM) {
@@ -108,8 +107,24 @@ __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsPara
         __syncthreads();
         at = __reduce_min_sync(0xffffffffu, lane < NW ? redi[lane] : 0x7fffffff);
     } else if (m != -INFINITY) {
-        if (m == INFINITY) each([&](float v, int) { s += v == INFINITY ? 1.f : 0.f; });
-        else each([&](float v, int) { s += ex2(__fmul_rn(__fsub_rn(get(v), m), k)); });
+        if (m == INFINITY) {
+            each([&](float v, int) { s += v == INFINITY ? 1.f : 0.f; });
+        } else if constexpr (SM) {  // the weights against the slice's maximum take the logits' place
+            float s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+            for (int i = tid * 4; i < n; i += NT * 4) {
+                float4 w = *reinterpret_cast<const float4*>(slice + i);
+                w.x = prob_exp(w.x, m, k, kl);
+                w.y = i + 1 < n ? prob_exp(w.y, m, k, kl) : 0.f;
+                w.z = i + 2 < n ? prob_exp(w.z, m, k, kl) : 0.f;
+                w.w = i + 3 < n ? prob_exp(w.w, m, k, kl) : 0.f;
+                *reinterpret_cast<float4*>(slice + i) = w;
+                s4[0] += w.x; s4[1] += w.y; s4[2] += w.z; s4[3] += w.w;
+            }
+            s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        } else {
+            each([&](float v, int) { s += prob_exp(v, m, k, kl); });
+        }
         s = warp_sum(s);
         __syncthreads();
         if (lane == 0) red[warp] = s;
@@ -123,15 +138,18 @@ __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsPara
         ProbsPart o{-INFINITY, 0.f, 0x7fffffff};
         if (lane < C) o = *cluster.map_shared_rank(&part, lane);  // every warp for itself
         M = warp_max(o.m);
-        S = warp_sum(o.m == -INFINITY ? 0.f : o.m == M ? o.s : o.s * ex2(__fmul_rn(__fsub_rn(o.m, M), k)));
+        S = warp_sum(o.m == -INFINITY ? 0.f : o.m == M ? o.s : o.s * prob_exp(o.m, M, k, kl));
         at = __reduce_min_sync(0xffffffffu, o.m == M ? o.at : 0x7fffffff);
         cluster.sync();  // no CTA leaves while another may still read its part
     }
     const float iv = 1.f / S;
+    // (a slice of -inf kept its logits)
+    const float part_of = m == M ? iv : m == -INFINITY ? 0.f : prob_exp(m, M, k, kl) * iv;
     auto term = [&](float v, int i) {
         if (M == -INFINITY) return 0.f;  // nothing can be chosen
         if (greedy) return i + v0 == at ? 1.f : 0.f;
         if (M == INFINITY) return v == INFINITY ? iv : 0.f;
+        if (SM) return m == -INFINITY ? 0.f : v * part_of;
         return prob_exp(v, M, k, kl) * iv;  // (0 for a NaN: its exponent is not above any bound)
     };
     if constexpr (SM && VEC) {
@@ -225,12 +243,12 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     const int run_len = ((p.vocab + C * NW - 1) / (C * NW) + 3) & ~3;
     const long long first = (long long)(rank * NW + warp) * run_len;
     const int v0 = (int)min((long long)p.vocab, first), v1 = min(p.vocab, v0 + run_len);
-    auto four = [&](const float* src, int i, float (&x)[4]) {  // elements i.. of the run, zeros past its end
-        if (VEC && i + 3 < v1) {
+    auto four = [&](const float* src, int i, int end, float (&x)[4]) {  // elements i.., zeros from `end` on
+        if (VEC && i + 3 < end) {
             *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src + i);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = i + e < v1 ? src[i + e] : 0.f;
+            for (int e = 0; e < 4; ++e) x[e] = i + e < end ? src[i + e] : 0.f;
         }
     };
     double total = 0.0, before = 0.0;
@@ -267,8 +285,8 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         a -= a2;
         for (; i < v1; i += 128) {
             float x[4], q[4] = {};
-            four(P, i, x);
-            if (sub) four(Q, i, q);
+            four(P, i, v1, x);
+            if (sub) four(Q, i, v1, q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) a += value(x[e], q[e], i + e);
         }
@@ -333,19 +351,24 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
         if (tid == 0) out[acc] = 0;  // no positive probability anywhere
         return;
     }
-    if (warp != who) return;
+    // the CTA's warps take 128 elements each of that run, 2,048 at a time (one warp alone waited for every
+    // load in turn: 29 us on 64 sequences of the 8B vocabulary)
+    const long long first_of = (long long)(rank * NW + who) * run_len;
+    const int r0 = (int)min((long long)p.vocab, first_of), r1 = min(p.vocab, r0 + run_len);
+    __shared__ double s_blk[NW];
+    __shared__ int s_hit, s_last;
+    if (tid == 0) { s_hit = 0x7fffffff; s_last = r0; }
     double run = at_base;
-    int pick = v0;  // the last positive element so far
-    for (int i0 = v0; i0 < v1; i0 += 128) {
-        const int i = i0 + lane * 4;
+    for (int i0 = r0; i0 < r1; i0 += NW * 128) {
+        const int i = i0 + warp * 128 + lane * 4;
         float x[4] = {}, q[4] = {};
-        four(P, i, x);
-        if (mode && Q) four(Q, i, q);
+        four(P, i, r1, x);
+        if (mode && Q) four(Q, i, r1, q);
         double c[4], mine = 0.0;
         int lastpos = -1;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const double w = i + e < v1 ? value(x[e], q[e], i + e) : 0.0;
+            const double w = i + e < r1 ? value(x[e], q[e], i + e) : 0.0;
             if (w > 0.0) lastpos = i + e;
             mine += w;
             c[e] = mine;
@@ -356,20 +379,24 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
             const double u = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += u;
         }
-        const double start = run + (incl - mine);
+        __syncthreads();  // (the block before is read)
+        if (lane == 31) s_blk[warp] = incl;
+        __syncthreads();
+        double start = run + (incl - mine);
+        for (int w = 0; w < NW; ++w) {
+            if (w < warp) start += s_blk[w];
+            run += s_blk[w];
+        }
         int hit = 0x7fffffff;
 #pragma unroll
         for (int e = 3; e >= 0; --e)
-            if (i + e < v1 && start + c[e] > t && (e == 0 ? c[0] > 0.0 : c[e] > c[e - 1])) hit = i + e;
-        hit = __reduce_min_sync(0xffffffffu, hit);
-        if (hit != 0x7fffffff) {
-            if (lane == 0) out[acc] = (unsigned)hit;
-            return;
-        }
-        pick = max(pick, __reduce_max_sync(0xffffffffu, lastpos));
-        run += __shfl_sync(0xffffffffu, incl, 31);
+            if (i + e < r1 && start + c[e] > t && (e == 0 ? c[0] > 0.0 : c[e] > c[e - 1])) hit = i + e;
+        if (hit != 0x7fffffff) atomicMin(&s_hit, hit);
+        if (lastpos >= 0) atomicMax(&s_last, lastpos);
+        __syncthreads();
+        if (s_hit != 0x7fffffff) break;
     }
-    if (lane == 0) out[acc] = (unsigned)pick;
+    if (tid == 0) out[acc] = (unsigned)(s_hit != 0x7fffffff ? s_hit : s_last);
 }
 
 }  // namespace laic
