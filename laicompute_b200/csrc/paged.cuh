@@ -41,7 +41,7 @@ struct KvAppendParams {
     void* q_out;
     long long ldq, ldk, ldv, ldqo;
     __half *kp, *vp;
-    int heads, kv_heads, head_dim, page_shift, num_pages;
+    int rows, heads, kv_heads, head_dim, page_shift, num_pages;
     const int *pos, *seq, *table;
     int nseq, pages_per_seq;
     const float2* rope;
@@ -88,76 +88,91 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
     }
 }
 
-constexpr int kAppendUnits = 4;  // units per thread
+constexpr int kAppendUnits = 4;  // units per thread and row
 
-// Grid (rows, slices of a row). A thread owns whole rotation pairs, so q_out may be q itself; it
-// loads all its units before the chain position -> sequence -> page is resolved. The rotation is
-// the reference's unfused multiply and add (src/inference_v2.cpp:25) in FP32; k and v are rounded
-// to binary16 once, which is the cache's precision.
-template <typename TI, typename TQ, bool VEC>
+// Grid (rows / R, slices of a row). A thread owns whole rotation pairs, so q_out may be q itself; it
+// loads all its units of R rows before the chains position -> sequence -> page are resolved (two rows
+// at a time fill the waits of many rows: 35 us against 40 for 8,188 rows of the 8B shape). The
+// rotation is the reference's unfused multiply and add (src/inference_v2.cpp:25) in FP32; k and v are
+// rounded to binary16 once, which is the cache's precision.
+template <typename TI, typename TQ, bool VEC, int R>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p) {
-    const int t = blockIdx.x;
-    const int pos = p.pos[t];
-    const int seq = p.seq ? p.seq[t] : t;
-    if (pos < 0) return;
     const int sh = __ffs(p.head_dim) - 4;  // units per head: 2^sh
     const int u0 = blockIdx.y * blockDim.x * kAppendUnits + threadIdx.x;
-    Raw8<TI> raw[kAppendUnits];
+    int pos[R], seq[R];
 #pragma unroll
-    for (int j = 0; j < kAppendUnits; ++j) {
-        const int u = u0 + j * blockDim.x;
-        if (u < p.units) {
-            const int head = u >> sh, hk = head - p.heads, hv = hk - p.kv_heads;
-            const TI* src = hk < 0   ? static_cast<const TI*>(p.q) + (size_t)t * p.ldq + (size_t)u * 8
-                            : hv < 0 ? static_cast<const TI*>(p.k) + (size_t)t * p.ldk + (size_t)(u - (p.heads << sh)) * 8
-                                     : static_cast<const TI*>(p.v) + (size_t)t * p.ldv +
-                                           (size_t)(u - ((p.heads + p.kv_heads) << sh)) * 8;
-            load8<TI, VEC>(src, raw[j]);
+    for (int q = 0; q < R; ++q) {
+        const int t = blockIdx.x * R + q;
+        pos[q] = t < p.rows ? p.pos[t] : -1;
+        seq[q] = t < p.rows && p.seq ? p.seq[t] : t;
+    }
+    Raw8<TI> raw[R][kAppendUnits];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+        const int t = blockIdx.x * R + q;
+#pragma unroll
+        for (int j = 0; j < kAppendUnits; ++j) {
+            const int u = u0 + j * blockDim.x;
+            if (u < p.units && t < p.rows) {
+                const int head = u >> sh, hk = head - p.heads, hv = hk - p.kv_heads;
+                const TI* src = hk < 0   ? static_cast<const TI*>(p.q) + (size_t)t * p.ldq + (size_t)u * 8
+                                : hv < 0 ? static_cast<const TI*>(p.k) + (size_t)t * p.ldk + (size_t)(u - (p.heads << sh)) * 8
+                                         : static_cast<const TI*>(p.v) + (size_t)t * p.ldv +
+                                               (size_t)(u - ((p.heads + p.kv_heads) << sh)) * 8;
+                load8<TI, VEC>(src, raw[q][j]);
+            }
         }
     }
-    // the units of a thread lie blockDim.x apart, a whole number of heads: one set of angles
+    // the units of a thread lie blockDim.x apart, a whole number of heads: one set of angles per row
     const int d = (u0 & ((1 << sh) - 1)) * 8, pr = d >> 1;
-    const float2* cs = p.rope + (size_t)min(pos, p.rope_positions - 1) * p.rope_pairs;
-    float2 c[4];
-    if (p.vec_rope && pr + 4 <= p.rope_pairs) {
-        *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cs + pr));
-        *reinterpret_cast<float4*>(c + 2) = __ldg(reinterpret_cast<const float4*>(cs + pr + 2));
-    } else {
+    float2 c[R][4];
+    int page[R];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (pr + i < p.rope_pairs) c[i] = __ldg(cs + pr + i);
-    }
-    int bad;
-    const int page = kv_place(seq, pos, p.table, p.nseq, p.pages_per_seq, p.page_shift, p.num_pages, p.rope_positions, bad);
-    if (page < 0) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) kv_flag(p.err, bad);
-        return;
-    }
-    const int off = pos & ((1 << p.page_shift) - 1);
-#pragma unroll
-    for (int j = 0; j < kAppendUnits; ++j) {
-        const int u = u0 + j * blockDim.x;
-        if (u >= p.units) break;
-        const int head = u >> sh, hk = head - p.heads, hv = hk - p.kv_heads;
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = raw[j].at(i);
-        if (hv < 0) {
+    for (int q = 0; q < R; ++q) {
+        const float2* cs = p.rope + (size_t)min(max(pos[q], 0), p.rope_positions - 1) * p.rope_pairs;
+        if (p.vec_rope && pr + 4 <= p.rope_pairs) {
+            *reinterpret_cast<float4*>(c[q]) = __ldg(reinterpret_cast<const float4*>(cs + pr));
+            *reinterpret_cast<float4*>(c[q] + 2) = __ldg(reinterpret_cast<const float4*>(cs + pr + 2));
+        } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (pr + i < p.rope_pairs) {
-                    const float a = x[2 * i], b = x[2 * i + 1];
-                    x[2 * i] = __fsub_rn(__fmul_rn(a, c[i].x), __fmul_rn(b, c[i].y));
-                    x[2 * i + 1] = __fadd_rn(__fmul_rn(a, c[i].y), __fmul_rn(b, c[i].x));
-                }
+                if (pr + i < p.rope_pairs) c[q][i] = __ldg(cs + pr + i);
         }
-        if (hk < 0) {
-            store8<TQ, VEC>(static_cast<TQ*>(p.q_out) + (size_t)t * p.ldqo + (size_t)u * 8, x);
-        } else {
-            const int h = hv < 0 ? hk : hv;
-            __half* dst = (hv < 0 ? p.kp : p.vp) +
-                          (((((size_t)page * p.kv_heads + h) << p.page_shift) + off) * p.head_dim + d);
-            store8<__half, true>(dst, x);  // pages are 16-byte aligned and head_dim a multiple of 8
+        int bad = 0;
+        page[q] = pos[q] < 0 ? -1 : kv_place(seq[q], pos[q], p.table, p.nseq, p.pages_per_seq, p.page_shift, p.num_pages,
+                                             p.rope_positions, bad);
+        if (bad && threadIdx.x == 0 && blockIdx.y == 0) kv_flag(p.err, bad);
+    }
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+        if (page[q] < 0) continue;  // padding, or refused
+        const int t = blockIdx.x * R + q;
+        const int off = pos[q] & ((1 << p.page_shift) - 1);
+#pragma unroll
+        for (int j = 0; j < kAppendUnits; ++j) {
+            const int u = u0 + j * blockDim.x;
+            if (u >= p.units) break;
+            const int head = u >> sh, hk = head - p.heads, hv = hk - p.kv_heads;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = raw[q][j].at(i);
+            if (hv < 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (pr + i < p.rope_pairs) {
+                        const float a = x[2 * i], b = x[2 * i + 1];
+                        x[2 * i] = __fsub_rn(__fmul_rn(a, c[q][i].x), __fmul_rn(b, c[q][i].y));
+                        x[2 * i + 1] = __fadd_rn(__fmul_rn(a, c[q][i].y), __fmul_rn(b, c[q][i].x));
+                    }
+            }
+            if (hk < 0) {
+                store8<TQ, VEC>(static_cast<TQ*>(p.q_out) + (size_t)t * p.ldqo + (size_t)u * 8, x);
+            } else {
+                const int h = hv < 0 ? hk : hv;
+                __half* dst = (hv < 0 ? p.kp : p.vp) +
+                              (((((size_t)page[q] * p.kv_heads + h) << p.page_shift) + off) * p.head_dim + d);
+                store8<__half, true>(dst, x);  // pages are 16-byte aligned and head_dim a multiple of 8
+            }
         }
     }
 }

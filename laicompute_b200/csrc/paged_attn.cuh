@@ -7,8 +7,8 @@
 //   range is short (it then joins the shared items' results and writes the output), else a warp per split;
 //   shared item (a CTA): up to 8 NT columns of a group's rows over a split of [0, shared), so the keys
 //   and values of a shared position are read once for all of them (wide groups: paged_bulk.cuh).
-// An item keeps, per column, the running maximum m of the scores (log2 domain), l = sum 2^(s - m)
-// and the unnormalised output; where a row has several items the merge kernel joins them by
+// An item keeps, per column, a reference m (a maximum of the scores seen, log2 domain, renewed when
+// they outgrow it by 2^8), l = sum 2^(s - m) and the unnormalised output; where a row has several items the merge kernel joins them by
 // out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
 //
 // Products run transposed on mma.m16n8k16: S^T = K Q^T (16 positions x 8 columns) and
@@ -16,7 +16,7 @@
 // from accumulators to B fragments by movmatrix. FP32 queries and weights are split into binary16
 // hi + lo (two products, 22 bits); a query row is first scaled by a power of two to [1, 2), so no
 // magnitude leaves binary16's range, and the weights carry a factor 2^7 that keeps small ones
-// out of its subnormals (both sides of the final division have it). The hi and lo products have
+// out of its subnormals (both sides of the final division have it, and 2^8 2^7 stay below its largest). The hi and lo products have
 // accumulators of their own: the tensor cores truncate as they accumulate, and lo parts added to a
 // large sum would only lengthen that chain. A private item of at most four columns (a decode step of
 // the usual groups) has hi and lo side by side in one tile's eight columns (PK), so the split costs no
@@ -55,6 +55,7 @@ struct KvAttnParams {
 constexpr int kPaWarps = 4;
 constexpr int kPaChunk = 64;      // positions per ring stage: 16 per warp
 constexpr int kPaMaxSplit = 2048; // positions per item at most (its page ids are held in shared memory)
+constexpr float kPaSlack = 8.f;  // log2 of how far a maximum may outgrow its reference before sums are rescaled
 constexpr float kPaGain = 128.f;  // the factor the weights carry (bulk items too: a row's items are summed)
 
 __host__ __device__ constexpr int pa_stages(int D) { return D == 128 ? 3 : 4; }
@@ -301,45 +302,62 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             const int pos = c0 + wp + gq;
             const bool full = c0 + wp >= t0 && c0 + wp + 16 <= min(t1, minlim);  // every live column sees all 16 positions
             uint32_t ph[NT][2], pl[NT][2];
+            float cm2[NT][2], mx[NT][2];
+            int lm[NT][2];
+            bool grew = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float mx[2] = {-INFINITY, -INFINITY}, corr[2], sum[2] = {0.f, 0.f}, cm2[2];
-                int lm[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int col = nt * 8 + 2 * c + h;
-                    cm2[h] = cmul[col];
-                    lm[h] = min(t1, lim[col]);
+                    cm2[nt][h] = cmul[col];
+                    lm[nt][h] = min(t1, lim[col]);
+                    mx[nt][h] = -INFINITY;
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (HL) s[nt][e] += sl[nt][e];
-                    const float x = s[nt][e] * cm2[e & 1];
+                    const float x = s[nt][e] * cm2[nt][e & 1];
                     const int at = pos + (e >> 1) * 8;
-                    if (full || (at < lm[e & 1] && at >= t0)) mx[e & 1] = fmaxf(mx[e & 1], x);
+                    if (full || (at < lm[nt][e & 1] && at >= t0)) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], x);
                 }
+                grew |= mx[nt][0] > m_[nt][0] + kPaSlack || mx[nt][1] > m_[nt][1] + kPaSlack;
+            }
+            if (__any_sync(0xffffffffu, grew)) {  // new reference maxima
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
-                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16));
-                    const float mnew = fmaxf(m_[nt][h], mx[h]);
-                    const float mu = mnew == -INFINITY ? 0.f : mnew;  // nothing seen yet: every weight is 0
-                    corr[h] = ex2(m_[nt][h] - mu);
-                    m_[nt][h] = mnew;
-                    mx[h] = mu;
+                for (int nt = 0; nt < NT; ++nt) {
+                    float corr[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float x = mx[nt][h];
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        const float mnew = fmaxf(m_[nt][h], x);
+                        corr[h] = mnew == -INFINITY ? 1.f : ex2(m_[nt][h] - mnew);
+                        m_[nt][h] = mnew;
+                        l_[nt][h] *= corr[h];
+                    }
+#pragma unroll
+                    for (int mt = 0; mt < KS; ++mt) {
+                        o[mt][nt][0] *= corr[0]; o[mt][nt][1] *= corr[1];
+                        o[mt][nt][2] *= corr[0]; o[mt][nt][3] *= corr[1];
+                    }
                 }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) mx[nt][h] = m_[nt][h] == -INFINITY ? 0.f : m_[nt][h];  // (nothing seen yet)
                 float pv[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    pv[e] = ex2(fmaf(s[nt][e], cm2[e & 1], -mx[e & 1]));
+                    pv[e] = ex2(fmaf(s[nt][e], cm2[nt][e & 1], -mx[nt][e & 1]));
                     const int at = pos + (e >> 1) * 8;
-                    if (!full && (at >= lm[e & 1] || at < t0)) pv[e] = 0.f;
-                    sum[e & 1] += pv[e];
+                    if (!full && (at >= lm[nt][e & 1] || at < t0)) pv[e] = 0.f;
+                    l_[nt][e & 1] += pv[e];  // this lane's positions
                     pv[e] *= kPaGain;
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) l_[nt][h] = fmaf(l_[nt][h], corr[h], sum[h]);  // this lane's positions
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const __half h0 = __float2half_rn(pv[2 * j]), h1 = __float2half_rn(pv[2 * j + 1]);
@@ -347,13 +365,6 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
                         pl[nt][j] = movm_t(pack_h2(__float2half_rn(pv[2 * j] - __half2float(h0)),
                                                    __float2half_rn(pv[2 * j + 1] - __half2float(h1))));
                     ph[nt][j] = movm_t(pack_h2(h0, h1));
-                }
-                if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-#pragma unroll
-                    for (int mt = 0; mt < KS; ++mt) {
-                        o[mt][nt][0] *= corr[0]; o[mt][nt][1] *= corr[1];
-                        o[mt][nt][2] *= corr[0]; o[mt][nt][3] *= corr[1];
-                    }
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[nt][e] = pv[e];
@@ -622,7 +633,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
             }
             const int c0 = a0 + (first + b * STRIDE) * 16, pos = c0 + gq;
             const bool full = c0 >= t0 && c0 + 16 <= t1;
-            float mx[2] = {-INFINITY, -INFINITY}, corr[2], sum[2] = {0.f, 0.f}, pv[4];
+            float mx[2] = {-INFINITY, -INFINITY}, pv[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 s[e] += s2[e];
@@ -630,27 +641,34 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                 const int at = pos + (e >> 1) * 8;
                 if (full || (at >= t0 && at < t1)) mx[e & 1] = fmaxf(mx[e & 1], s[e] * cm2[e & 1]);
             }
+            if (__any_sync(0xffffffffu, mx[0] > m_[0] + kPaSlack || mx[1] > m_[1] + kPaSlack)) {  // new reference maxima
+                float corr[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16));
-                const float mnew = fmaxf(m_[h], mx[h]);
-                const float mu = mnew == -INFINITY ? 0.f : mnew;  // (every score -inf: every weight is 0)
-                corr[h] = ex2(m_[h] - mu);
-                m_[h] = mnew;
-                mx[h] = mu;
+                for (int h = 0; h < 2; ++h) {
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16));
+                    const float mnew = fmaxf(m_[h], mx[h]);
+                    corr[h] = mnew == -INFINITY ? 1.f : ex2(m_[h] - mnew);
+                    m_[h] = mnew;
+                    l_[h] *= corr[h];
+                }
+#pragma unroll
+                for (int mt = 0; mt < KS; ++mt) {
+                    o[mt][0] *= corr[0]; o[mt][1] *= corr[1];
+                    o[mt][2] *= corr[0]; o[mt][3] *= corr[1];
+                }
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) mx[h] = m_[h] == -INFINITY ? 0.f : m_[h];  // (nothing seen yet)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 pv[e] = ex2(fmaf(s[e], cm2[e & 1], -mx[e & 1]));
                 const int at = pos + (e >> 1) * 8;
                 if (!full && (at < t0 || at >= t1)) pv[e] = 0.f;
-                sum[e & 1] += pv[e];
+                l_[e & 1] += pv[e];  // this lane's positions
                 pv[e] *= kPaGain;
             }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) l_[h] = fmaf(l_[h], corr[h], sum[h]);  // this lane's positions
             uint32_t ph[2], pl[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -661,13 +679,6 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                     if (PK && c >= 2) { h0 = l0; h1 = l1; }
                 }
                 ph[j] = movm_t(pack_h2(h0, h1));
-            }
-            if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
-#pragma unroll
-                for (int mt = 0; mt < KS; ++mt) {
-                    o[mt][0] *= corr[0]; o[mt][1] *= corr[1];
-                    o[mt][2] *= corr[0]; o[mt][3] *= corr[1];
-                }
             }
 #pragma unroll
             for (int mt = 0; mt < KS; ++mt) {

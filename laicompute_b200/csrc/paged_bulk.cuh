@@ -40,7 +40,6 @@ constexpr int kBulkCols = 256;        // score columns of a CTA
 constexpr int kBulkThreads = 352;
 constexpr int kBulkMaxCluster = 8;   // clusters of 1, 2, 4 or 8
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
-constexpr float kBulkSlack = 8.f;     // log2 of how far a maximum may outgrow its reference
 
 constexpr int kBulkKeys = 128;        // positions per tile
 __host__ __device__ constexpr int bulk_slot_bytes(int D) { return kBulkKeys * D * 2; }  // a tile of K or of V
@@ -470,7 +469,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * cm;
             if (j == 0) {
                 mref = mx > -INFINITY ? mx : 0.f;
-            } else if (__any_sync(0xffffffffu, mx > mref + kBulkSlack)) {
+            } else if (__any_sync(0xffffffffu, mx > mref + kPaSlack)) {
                 const float next = fmaxf(mref, mx), corr = ex2(mref - next);
                 mref = next;
                 l *= corr;  // (PV(j - 1) is complete: QK(j), which S is of, was issued behind it)

@@ -76,8 +76,9 @@ int on_device(int device, F&& f) {
 
 template <typename TI, typename TQ>
 void append_launch(bool vec, dim3 grid, int block, cudaStream_t st, const KvAppendParams& p) {
-    if (vec) kv_append_kernel<TI, TQ, true><<<grid, block, 0, st>>>(p);
-    else kv_append_kernel<TI, TQ, false><<<grid, block, 0, st>>>(p);
+    if (!vec) kv_append_kernel<TI, TQ, false, 1><<<grid, block, 0, st>>>(p);
+    else if (grid.x < (unsigned)p.rows) kv_append_kernel<TI, TQ, true, 2><<<grid, block, 0, st>>>(p);
+    else kv_append_kernel<TI, TQ, true, 1><<<grid, block, 0, st>>>(p);
 }
 
 int device_sms(int dev) {
@@ -100,7 +101,25 @@ BulkFn bulk_pick(int D, bool f32) {
     return f32 ? paged_bulk_kernel<128, float> : paged_bulk_kernel<128, __half>;
 }
 
-// Clusters of c bulk CTAs that are resident at once on `device` (asked once; without a device, by the SM count).
+// Clusters of c CTAs of a kernel that are resident at once on the current device, 0 where that cannot be asked.
+template <typename K>
+int resident_clusters(K kernel, int threads, size_t smem, int c, int sms) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(c * sms);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)c;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0) return n;
+    cudaGetLastError();
+    return 0;
+}
+// Of c bulk CTAs (asked once per device; without one, by the SM count).
 int bulk_clusters(int device, int c) {
     static std::atomic<int> known[64][kBulkMaxCluster + 1];
     const int guess = device_sms(device) / c;
@@ -112,24 +131,11 @@ int bulk_clusters(int device, int c) {
         cudaGetLastError();
         return guess;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(c * device_sms(device));
-    cfg.blockDim = dim3(kBulkThreads);
-    cfg.dynamicSmemBytes = bulk_smem(128, true);  // the largest
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)c;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, bulk_pick(128, true), &cfg) != cudaSuccess || n < 1) {
-        cudaGetLastError();
-        return guess;
-    }
+    n = resident_clusters(bulk_pick(128, true), kBulkThreads, bulk_smem(128, true), c, device_sms(device));  // (the largest)
+    if (!n) return guess;
     known[device][c].store(n);
     return n;
 }
-
 // ---- attention: how a call is cut into items
 struct AttnPlan {
     int nt = 1;            // column tiles of 8 of a shared item
@@ -203,7 +209,7 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
             pl.ls = std::min(kBulkMaxSplit, std::max(2 * kBulkKeys, round_up((a.max_shared + best * count - 1) / (best * count), kBulkKeys)));
             pl.nss = (int)((a.max_shared + (long long)pl.ls * best - 1) / ((long long)pl.ls * best));
         } else {
-            pl.nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+            pl.nt = cols <= 24 ? (cols + 7) / 8 : 4;
             pl.ctiles = (cols + 8 * pl.nt - 1) / (8 * pl.nt);
             pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared, 4LL * sms, kPaChunk, 256, 512);
         }
@@ -226,7 +232,10 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
 using PaFn = void (*)(KvAttnParams);
 template <int D, typename T>
 PaFn pa_fn_nt(int nt) {
-    return nt == 1 ? paged_attn_kernel<D, 1, T> : nt == 2 ? paged_attn_kernel<D, 2, T> : paged_attn_kernel<D, 4, T>;
+    return nt == 1   ? paged_attn_kernel<D, 1, T>
+           : nt == 2 ? paged_attn_kernel<D, 2, T>
+           : nt == 3 ? paged_attn_kernel<D, 3, T>
+                     : paged_attn_kernel<D, 4, T>;
 }
 template <typename T>
 PaFn pa_fn(int D, int nt) {
@@ -283,7 +292,7 @@ cudaError_t serving_set_attributes() {
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64 && done[dev].load()) return cudaSuccess;
     for (int D : {32, 64, 128})
-        for (int nt : {1, 2, 4})
+        for (int nt : {1, 2, 3, 4})
             for (int type : {LAIC_GGML_F32, LAIC_GGML_F16}) {
                 e = cudaFuncSetAttribute(pa_pick(D, nt, type), cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)pa_smem(D, nt, type == LAIC_GGML_F32));
@@ -301,7 +310,7 @@ cudaError_t serving_set_attributes() {
             if (e != cudaSuccess) return e;
         }
     for (auto fn : {probs_kernel<true, true>, probs_kernel<true, false>}) {
-        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (kProbsSlice + 8) * 4);
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kProbsSlice * 4);
         if (e != cudaSuccess) return e;
     }
     if (dev >= 0 && dev < 64) done[dev].store(true);
@@ -341,7 +350,7 @@ int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t
     p.q = a.q_dev; p.k = a.k_dev; p.v = a.v_dev; p.q_out = a.q_out_dev;
     p.ldq = a.ldq; p.ldk = a.ldk; p.ldv = a.ldv; p.ldqo = a.ldqo;
     p.kp = static_cast<__half*>(g.k_dev); p.vp = static_cast<__half*>(g.v_dev);
-    p.heads = a.heads; p.kv_heads = g.kv_heads; p.head_dim = g.head_dim;
+    p.rows = a.rows; p.heads = a.heads; p.kv_heads = g.kv_heads; p.head_dim = g.head_dim;
     p.page_shift = log2i(g.page_size); p.num_pages = g.num_pages;
     p.pos = a.pos_dev; p.seq = a.seq_dev; p.table = a.page_table_dev;
     p.nseq = a.nseq; p.pages_per_seq = a.pages_per_seq;
@@ -355,7 +364,8 @@ int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t
     const int units = (a.heads + 2 * g.kv_heads) * (g.head_dim / 8);
     p.units = units;
     const int block = std::min(256, (units + 31) / 32 * 32), cta = block * kAppendUnits;
-    const dim3 grid(a.rows, (units + cta - 1) / cta);
+    // two rows per CTA where there are enough of them to fill the GPU several times over
+    const dim3 grid(vec && a.rows >= 16 * device_sms(g.device) ? (a.rows + 1) / 2 : a.rows, (units + cta - 1) / cta);
     if (grid.y > 65535) return api_fail(LAIC_E_UNSUPPORTED, "rows too wide");
     return on_device(g.device, [&]() -> int {
         if (a.in_type == LAIC_GGML_F32) {
@@ -459,11 +469,11 @@ int logits_probs(int device, int rows, int vocab, const float* x, long long ldx,
         if (vocab >= 8 * kProbsThreads && 8LL * rows <= device_sms(device)) c = 8;
         const bool sm = (long long)c * kProbsSlice >= vocab;
         if (!sm) c = 1;
-        const size_t smem = sm ? ((size_t)(vocab + c - 1) / c + 8) * 4 : 0;
+        const auto fn = sm ? (vec ? probs_kernel<true, true> : probs_kernel<true, false>) : probs_kernel<false, false>;
+        const size_t smem = sm ? ((((size_t)vocab + c - 1) / c + 3) & ~(size_t)3) * 4 : 0;
         cudaError_t e = serving_set_attributes();
         if (e == cudaSuccess)
-            e = launch_cluster_k(sm ? (vec ? probs_kernel<true, true> : probs_kernel<true, false>) : probs_kernel<false, false>,
-                                 dim3((unsigned)rows * c), dim3(kProbsThreads), smem, st, false, c, p);
+            e = launch_cluster_k(fn, dim3((unsigned)rows * c), dim3(kProbsThreads), smem, st, false, c, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "logits_probs");
     });
 }

@@ -18,20 +18,45 @@ struct ProbsParams {
     int vocab;
 };
 
-// 2^((x - m) log2(e) / T) with the product's rounding error carried along: the FP32 difference and
-// product alone would lose |exponent| * 2^-24 of the result. k + kl = log2(e) / T.
-__device__ __forceinline__ float prob_exp(float x, float m, float k, float kl) {
-    const float d = __fsub_rn(x, m);
-    const float bb = __fsub_rn(d, x);
-    const float e = __fsub_rn(__fsub_rn(x, __fsub_rn(d, bb)), __fadd_rn(m, bb));  // (x - m) - d, exactly
-    const float h = __fmul_rn(d, k);
-    if (!(h > -150.f)) return 0.f;  // below binary32 (a mask of the lowest value overflows d and h)
-    const float l = fmaf(d, kl, fmaf(e, k, fmaf(d, k, -h)));
-    const float p = ex2(h);
-    return fmaf(p, l * 0.69314718f, p);
+// log2(e) / T as hi + lo: the lo part matters, an error of the factor tilts the whole row.
+struct ProbFactor {
+    float k, kl;
+    __device__ __forceinline__ explicit ProbFactor(float t) {
+        k = 1.44269502f / t;  // log2(e) = 1.44269502162933 (binary32) + 1.9259630e-8
+        kl = (fmaf(-k, t, 1.44269502f) + 1.9259630e-8f) / t;
+    }
+};
+// The weight of logit x against the slice's maximum m, 2^(x k - c0): c0 is m k to a 1024th, so that c0 + n
+// is exact for the nearest integer n of the exponent and the fraction f = x k - (c0 + n) is rounded at
+// its own size (2^-26), not at the exponent's. `off` takes
+// 2^(m k - c0), the same for the whole slice, out again. A NaN counts as -inf. Maxima too large for
+// that take the difference first.
+struct ProbExp {
+    float k, kl, c0, m, off;
+    bool huge;
+    __device__ __forceinline__ ProbExp(float m_, ProbFactor f)
+        : k(f.k), kl(f.kl), c0(rintf(m_ * f.k * 1024.f) * 0x1p-10f), m(m_), off(1.f), huge(!(fabsf(m_ * f.k) < 4096.f)) {
+        if (!huge) off = exp2f(-fmaf(m, kl, fmaf(m, k, -c0)));
+    }
+    __device__ __forceinline__ float operator()(float x) const {
+        if (huge) return ex2(fmaxf((x - m) * k, -200.f));
+        const float t = fmaf(x, k, 12582912.f - c0);  // 1.5 2^23: the sum's last bits are n
+        const float c = (t - 12582912.f) + c0;
+        const float f = fmaf(x, kl, fmaf(x, k, -c));
+        const float p = ex2(f);
+        return t >= 12582912.f - 126.f ? p * __int_as_float((__float_as_int(t) << 23) + 0x3f800000) : 0.f;
+    }
+};
+// 2^((a - b) k) of two slices' maxima, a <= b, to binary32: an error here is a whole slice's.
+__device__ __forceinline__ float prob_scale(float a, float b, ProbFactor f) {
+    if (a == b) return 1.f;
+    const float d = a - b, bb = d - a, e = (a - (d - bb)) - (b + bb);  // (a - b) - d exactly
+    const float h = d * f.k, l = fmaf(d, f.kl, fmaf(e, f.k, fmaf(d, f.k, -h)));
+    const float p = exp2f(fmaxf(h, -200.f));
+    return fmaf(p, h > -200.f ? l * 0.69314718f : 0.f, p);
 }
 
-constexpr int kProbsThreads = 512;
+constexpr int kProbsThreads = 256;
 constexpr int kProbsSlice = 16384;  // elements of a row's slice in shared memory
 
 // The row's slices exchange through this (distributed shared memory).
@@ -40,26 +65,25 @@ struct ProbsPart {
     int at;
 };
 
-// A cluster per row, each CTA a slice held in shared memory (SM; vocab <= cluster * kProbsSlice), so
-// the row is read once and every exponential formed once: the slice's weights against its own maximum
-// stay there, the maxima and sums meet in one exchange, and a product per element is left. Else
-// (larger vocabularies) a CTA per row reads it three times. VEC: 16-byte aligned rows.
+// SM (vocab <= cluster * kProbsSlice): a cluster per row, each CTA a slice in shared memory. The row is
+// read once and every exponential formed once: the slice's weights against its own maximum take the
+// logits' place, the maxima and sums meet in one exchange, and a product per element is left.
+// Else (larger vocabularies) a CTA per row reads it three times. VEC: 16-byte aligned rows.
 template <bool SM, bool VEC>
-__global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsParams p) {
+__global__ void __launch_bounds__(kProbsThreads) probs_kernel(const ProbsParams p) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(16) float slice[];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = SM ? (int)cluster.num_blocks() : 1, rank = SM ? (int)cluster.block_rank() : 0;
     const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int NW = kProbsThreads / 32, NT = kProbsThreads;
-    __shared__ float red[NW];
+    __shared__ float red[2][NW];
     __shared__ int redi[NW];
     __shared__ ProbsPart part;
     const int per = SM ? ((p.vocab + C - 1) / C + 3) & ~3 : p.vocab;
     const int v0 = min(p.vocab, rank * per), n = min(p.vocab, v0 + per) - v0;
     const float* x = p.x + (size_t)row * p.ldx + v0;
     float* y = p.y + (size_t)row * p.ldy + v0;
-    const float* src = SM ? slice : x;
     if constexpr (SM) {
         if constexpr (VEC) {
             for (int i = tid * 4; i + 3 < n; i += NT * 4) cp_async16(slice + i, x + i);
@@ -69,11 +93,11 @@ __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsPara
 #pragma unroll 4
             for (int i = tid; i < n; i += NT) slice[i] = x[i];
         }
+        if ((n & 3) && tid < 4 - (n & 3)) slice[n + tid] = -INFINITY;  // whole groups of four
     }
     const float t = p.temp[row];
     const bool greedy = !(t > 0.f);
-    const double kd = 1.4426950408889634 / (double)(greedy ? 1.f : t);
-    const float k = (float)kd, kl = (float)(kd - (double)k);
+    const ProbFactor k(greedy ? 1.f : t);
     if constexpr (SM) {
         if constexpr (VEC) cp_async_wait_all();
         __syncthreads();
@@ -81,25 +105,26 @@ __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsPara
     // f(element, its index) over this thread's elements, in ascending order
     auto each = [&](auto&& f) {
         if constexpr (SM) {
-#pragma unroll 2
+#pragma unroll 4
             for (int i = tid * 4; i < n; i += NT * 4) {
-                const float4 w = *reinterpret_cast<const float4*>(slice + i);  // (the slice is padded to four)
+                const float4 w = *reinterpret_cast<const float4*>(slice + i);
                 f(w.x, i);
-                if (i + 1 < n) f(w.y, i + 1);
-                if (i + 2 < n) f(w.z, i + 2);
-                if (i + 3 < n) f(w.w, i + 3);
+                f(w.y, i + 1);
+                f(w.z, i + 2);
+                f(w.w, i + 3);
             }
         } else {
-            for (int i = tid; i < n; i += NT) f(src[i], i);
+            for (int i = tid; i < n; i += NT) f(x[i], i);
         }
     };
     float m = -INFINITY, s = 0.f;
     int at = 0x7fffffff;
     each([&](float v, int) { m = fmaxf(m, v); });  // (fmaxf passes a NaN over)
     m = warp_max(m);
-    if (lane == 0) red[warp] = m;
+    if (lane == 0) red[0][warp] = m;
     __syncthreads();
-    m = warp_max(lane < NW ? red[lane] : -INFINITY);
+    m = warp_max(lane < NW ? red[0][lane] : -INFINITY);
+    const ProbExp e(m, k);
     if (greedy) {  // the slice's first maximum
         each([&](float v, int i) { if (v == m) at = min(at, i + v0); });
         at = __reduce_min_sync(0xffffffffu, at);
@@ -109,27 +134,24 @@ __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsPara
     } else if (m != -INFINITY) {
         if (m == INFINITY) {
             each([&](float v, int) { s += v == INFINITY ? 1.f : 0.f; });
-        } else if constexpr (SM) {  // the weights against the slice's maximum take the logits' place
+        } else if constexpr (SM) {  // the weights take the logits' place
             float s4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
+#pragma unroll 4
             for (int i = tid * 4; i < n; i += NT * 4) {
                 float4 w = *reinterpret_cast<const float4*>(slice + i);
-                w.x = prob_exp(w.x, m, k, kl);
-                w.y = i + 1 < n ? prob_exp(w.y, m, k, kl) : 0.f;
-                w.z = i + 2 < n ? prob_exp(w.z, m, k, kl) : 0.f;
-                w.w = i + 3 < n ? prob_exp(w.w, m, k, kl) : 0.f;
+                w.x = e(w.x); w.y = e(w.y); w.z = e(w.z); w.w = e(w.w);
                 *reinterpret_cast<float4*>(slice + i) = w;
                 s4[0] += w.x; s4[1] += w.y; s4[2] += w.z; s4[3] += w.w;
             }
             s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         } else {
-            each([&](float v, int) { s += prob_exp(v, m, k, kl); });
+            each([&](float v, int) { s += e(v); });
         }
         s = warp_sum(s);
+        if (lane == 0) red[1][warp] = s;
         __syncthreads();
-        if (lane == 0) red[warp] = s;
-        __syncthreads();
-        s = warp_sum(lane < NW ? red[lane] : 0.f);
+        s = warp_sum(lane < NW ? red[1][lane] : 0.f);
+        if (m != INFINITY) s *= e.off;
     }
     float M = m, S = s;
     if (SM && C > 1) {
@@ -138,22 +160,33 @@ __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsPara
         ProbsPart o{-INFINITY, 0.f, 0x7fffffff};
         if (lane < C) o = *cluster.map_shared_rank(&part, lane);  // every warp for itself
         M = warp_max(o.m);
-        S = warp_sum(o.m == -INFINITY ? 0.f : o.m == M ? o.s : o.s * prob_exp(o.m, M, k, kl));
+        S = warp_sum(o.m == -INFINITY || greedy ? 0.f : o.s * prob_scale(o.m, M, k));
         at = __reduce_min_sync(0xffffffffu, o.m == M ? o.at : 0x7fffffff);
         cluster.sync();  // no CTA leaves while another may still read its part
     }
     const float iv = 1.f / S;
-    // (a slice of -inf kept its logits)
-    const float part_of = m == M ? iv : m == -INFINITY ? 0.f : prob_exp(m, M, k, kl) * iv;
+    const float part_of = greedy || m == -INFINITY || m == INFINITY ? 0.f : prob_scale(m, M, k) * iv * e.off;
     auto term = [&](float v, int i) {
         if (M == -INFINITY) return 0.f;  // nothing can be chosen
         if (greedy) return i + v0 == at ? 1.f : 0.f;
-        if (M == INFINITY) return v == INFINITY ? iv : 0.f;
-        if (SM) return m == -INFINITY ? 0.f : v * part_of;
-        return prob_exp(v, M, k, kl) * iv;  // (0 for a NaN: its exponent is not above any bound)
+        if (M == INFINITY) return m == INFINITY && v == INFINITY ? iv : 0.f;  // (a finite slice holds weights)
+        if (SM) return m == -INFINITY ? 0.f : v * part_of;  // (a slice of -inf kept its logits)
+        return e(v) * part_of;
     };
-    if constexpr (SM && VEC) {
-#pragma unroll 2
+    if (SM && VEC && !greedy && m != -INFINITY && M != INFINITY) {  // the usual row
+#pragma unroll 4
+        for (int i = tid * 4; i < n; i += NT * 4) {
+            float4 w = *reinterpret_cast<const float4*>(slice + i);
+            w.x *= part_of; w.y *= part_of; w.z *= part_of; w.w *= part_of;
+            if (i + 3 < n) {
+                *reinterpret_cast<float4*>(y + i) = w;
+            } else {
+                y[i] = w.x;
+                if (i + 1 < n) y[i + 1] = w.y;
+                if (i + 2 < n) y[i + 2] = w.z;
+            }
+        }
+    } else if constexpr (SM && VEC) {
         for (int i = tid * 4; i < n; i += NT * 4) {
             const float4 w = *reinterpret_cast<const float4*>(slice + i);
             const float4 o = make_float4(term(w.x, i), term(w.y, i + 1), term(w.z, i + 2), term(w.w, i + 3));
@@ -166,7 +199,7 @@ __global__ void __launch_bounds__(kProbsThreads, 3) probs_kernel(const ProbsPara
             }
         }
     } else {
-        for (int i = tid; i < n; i += NT) y[i] = term(src[i], i);
+        for (int i = tid; i < n; i += NT) y[i] = term(SM ? slice[i] : x[i], i);
     }
 }
 
