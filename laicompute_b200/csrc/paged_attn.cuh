@@ -147,9 +147,13 @@ __host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int sh
     return row_view(p, p.len[r], p.seq ? p.seq[r] : r, shared);
 }
 
+// Elements e and e + 1 (e even) of query row r.
 template <typename T>
-__device__ __forceinline__ float q_at(const KvAttnParams& p, int r, int h, int d) {
-    return kv_in<T>(static_cast<const T*>(p.q)[(size_t)r * p.ldq + d + (size_t)h]);
+__device__ __forceinline__ float2 q_pair(const KvAttnParams& p, int r, int e) {
+    const T* q = static_cast<const T*>(p.q) + (size_t)r * p.ldq + e;
+    if (!p.q_vec) return make_float2(kv_in<T>(q[0]), kv_in<T>(q[1]));
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float2*>(q);
+    else return __half22float2(*reinterpret_cast<const __half2*>(q));
 }
 
 // One item: columns [col0, col0 + 8 NT) of rows r0.. (column = row offset * G + head), positions
@@ -227,8 +231,9 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
         for (int i = 0; i < PL; ++i) {
             const int pi = lane + 32 * i;
             const bool in = live && pi < D / 2;
-            a[i] = in ? q_at<T>(p, rr, hh, 2 * pi) : 0.f;
-            b[i] = in ? q_at<T>(p, rr, hh, 2 * pi + 1) : 0.f;
+            const float2 x = in ? q_pair<T>(p, rr, hh + 2 * pi) : make_float2(0.f, 0.f);
+            a[i] = x.x;
+            b[i] = x.y;
             mx = fmaxf(mx, fmaxf(fabsf(a[i]), fabsf(b[i])));
         }
         float fac = 1.f, inv = 1.f;
@@ -478,27 +483,30 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
 constexpr int kPrWarps = 4;
 constexpr int kPrStages = 2;      // 16 positions of K and V each, per warp (three: fewer CTAs per SM, 192 against 187 us)
 constexpr int kPrWhole = 1024;    // private ranges up to this stay whole (and no split is longer)
-__host__ __device__ constexpr size_t pr_smem(int D) { return (size_t)kPrWarps * kPrStages * 2 * 16 * D * 2; }
+// Warps of a CTA: three where a CTA takes a whole row, so that four of head_dim 128 fit an SM.
+__host__ __device__ constexpr int pr_warps(bool whole) { return whole ? 3 : kPrWarps; }
+__host__ __device__ constexpr size_t pr_smem(int D, bool whole) { return (size_t)pr_warps(whole) * kPrStages * 2 * 16 * D * 2; }
 
 // One row's own positions, every warp on its own ring of 16-position stages.
-// WHOLE: a CTA per [row][kv head], its warps take every fourth block of 16 positions; at the end they
+// WHOLE: a CTA per [row][kv head], its warps take turns at the blocks of 16 positions; at the end they
 // and the row's shared items (the kernel before this one) are joined and the output written.
 // Else: a warp per item of [row][kv head][split], no barrier between the warps.
 // PK: FP32 rows of at most four columns, hi parts in columns 0-3, lo parts in 4-7 of the tile.
 template <int D, typename T, bool PK, bool WHOLE>
-__global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAttnParams p) {
+__global__ void __launch_bounds__(pr_warps(WHOLE) * 32) paged_private_kernel(const KvAttnParams p) {
+    constexpr int NW = pr_warps(WHOLE);
     constexpr bool HL = sizeof(T) == 4 && !PK;
     constexpr int HN = HL ? 2 : 1, KS = D / 16, CPR = D / 8, NST = kPrStages;
     constexpr uint32_t STAGE = 2 * 16 * D * 2;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int page_ids[kPrWarps][kPrWhole / 16 + 2];
-    __shared__ uint32_t qf[kPrWarps][KS][HN][32][2];
-    __shared__ float cmul[kPrWarps][8];
-    __shared__ int found[kPrWarps];
+    __shared__ int page_ids[NW][kPrWhole / 16 + 2];
+    __shared__ uint32_t qf[NW][KS][HN][32][2];
+    __shared__ float cmul[NW][8];
+    __shared__ int found[NW];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gq = lane >> 2, c = lane & 3;
     pdl_launch_dependents();  // (the merge waits for this grid's end; nothing else follows)
-    int i = WHOLE ? blockIdx.x : blockIdx.x * kPrWarps + warp;
+    int i = WHOLE ? blockIdx.x : blockIdx.x * NW + warp;
     const bool in = WHOLE || i < p.private_items;
     if (!in) i = 0;
     const int split = WHOLE ? 0 : i % p.nsp;
@@ -520,7 +528,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
         return;
     }
     const int t0 = v.shared + split * p.lp, t1 = in ? min(min(v.n, v.shared + p.max_private), t0 + p.lp) : 0;
-    constexpr int STRIDE = WHOLE ? kPrWarps : 1;
+    constexpr int STRIDE = WHOLE ? NW : 1;
     const int a0 = t0 & ~15, first = WHOLE ? warp : 0;  // blocks first, first + STRIDE, ... of 16 positions from a0
     const int nb = in && v.n >= 0 && t0 < t1 ? (((t1 - a0 + 15) >> 4) - first + STRIDE - 1) / STRIDE : 0;
     float m_[2] = {-INFINITY, -INFINITY}, l_[2] = {0.f, 0.f}, o[KS][4];
@@ -571,8 +579,9 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
             for (int k = 0; k < PL; ++k) {
                 const int pi = lane + 32 * k, hh = (kvh * p.G + col) * D;
                 const bool got = col < p.G && pi < D / 2;
-                qa[col][k][0] = got ? q_at<T>(p, r, hh, 2 * pi) : 0.f;
-                qa[col][k][1] = got ? q_at<T>(p, r, hh, 2 * pi + 1) : 0.f;
+                const float2 x = got ? q_pair<T>(p, r, hh + 2 * pi) : make_float2(0.f, 0.f);
+                qa[col][k][0] = x.x;
+                qa[col][k][1] = x.y;
             }
 #pragma unroll
         for (int col = 0; col < (PK ? 4 : 8); ++col) {
@@ -721,7 +730,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
         }
         if (blockIdx.x == 0) pdl_wait();  // this kernel's end then stands for the shared items' too
     } else {
-        __shared__ float2 wml[kPrWarps][8];
+        __shared__ float2 wml[NW][8];
         __syncthreads();  // every warp is done with its ring: it takes the warps' outputs
         float* red = reinterpret_cast<float*>(smem);  // [warp][column][D + 4]
 #pragma unroll
@@ -741,7 +750,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
         __syncthreads();
         const int live_s = v.shared > 0 ? (v.shared + p.ls * p.lc - 1) / (p.ls * p.lc) : 0;
         if (live_s || blockIdx.x == 0) pdl_wait();  // the shared items' results
-        for (int e = threadIdx.x; e < p.G * (D / 4); e += kPrWarps * 32) {
+        for (int e = threadIdx.x; e < p.G * (D / 4); e += NW * 32) {
             const int col = e / (D / 4), d = e % (D / 4) * 4, head = kvh * p.G + col;
             const size_t at = ((size_t)r * p.heads + head) * ns;
             float M = -INFINITY, L = 0.f;
@@ -754,13 +763,32 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                 a.z = fmaf(x.z, w, a.z); a.w = fmaf(x.w, w, a.w);
             };
 #pragma unroll
-            for (int w = 0; w < kPrWarps; ++w) M = fmaxf(M, wml[w][col].x);
-            for (int q = 0; q < live_s; ++q) M = fmaxf(M, p.part_ml[at + q].x);
-#pragma unroll 4
-            for (int q = 0; q < live_s; ++q) add(p.part_ml[at + q], *reinterpret_cast<const float4*>(p.part_o + (at + q) * D + d), M);
+            for (int w = 0; w < NW; ++w) M = fmaxf(M, wml[w][col].x);
+            // the shared items' results, up to four at a time against the maximum so far
 #pragma unroll
-            for (int w = 0; w < kPrWarps; ++w)
+            for (int w = 0; w < NW; ++w)
                 add(wml[w][col], *reinterpret_cast<const float4*>(red + ((size_t)w * 8 + col) * (D + 4) + d), M);
+            for (int q0 = 0; q0 < live_s; q0 += 4) {
+                float2 ml[4];
+                float4 x[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    ml[q] = make_float2(-INFINITY, 0.f);
+                    if (q0 + q < live_s) {
+                        ml[q] = p.part_ml[at + q0 + q];
+                        x[q] = *reinterpret_cast<const float4*>(p.part_o + (at + q0 + q) * D + d);
+                    }
+                }
+                const float top = fmaxf(fmaxf(M, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+                if (top > M) {
+                    const float corr = ex2(M - top);
+                    L *= corr;
+                    a.x *= corr; a.y *= corr; a.z *= corr; a.w *= corr;
+                    M = top;
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) add(ml[q], x[q], M);
+            }
             const float iv = M == -INFINITY ? 0.f : 1.f / L;
             T* dst = static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)head * D + d;
             const float x[4] = {a.x * iv, a.y * iv, a.z * iv, a.w * iv};

@@ -7,8 +7,7 @@
 // Roles: warp 8 loads (TMA boxes of up to a page, 128-byte swizzle, a lane per box: one lane alone
 // took 125 cycles a box, 4,000 for a tile of 16-position pages; a ring of K and V tiles); warps 9 and
 // 10 multiply, one lane for each tile of columns (tcgen05.mma, S and O in tensor memory, P read from tensor memory, where it
-// takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S (twice, 32
-// columns at a time: a column's 128 scores do not fit the registers beside the rest), keep the
+// takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S, keep the
 // running maximum and sum, and write P in two halves, so that PV starts on the first. One tile's products run under the other's exponentials. 128 positions
 // per tile: a product of N = 64 takes about as long as one of N = 128 (100 against 85 cycles
 // measured), and two score buffers of 64 ran slower than one of 128. O is rescaled only when a
@@ -38,6 +37,10 @@ namespace laic {
 
 constexpr int kBulkCols = 256;        // score columns of a CTA
 constexpr int kBulkThreads = 352;
+// Of 16 pairs of binary16 exponentials, this many go to the FMA pipe (f2_exp2): the special-function unit
+// alone (16 a clock) bounds a tile's softmax.
+constexpr int kBulkPoly = 6;
+constexpr float kExpC0 = 1.f, kExpC1 = 0.693121045f, kExpC2 = 0.24022349f, kExpC3 = 0.0559219758f, kExpC4 = 0.00966636852f;
 constexpr int kBulkMaxCluster = 8;   // clusters of 1, 2, 4 or 8
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
 
@@ -169,10 +172,31 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ uint64_t f2_sub(uint64_t a, uint64_t b) { return f2_fma(b, f2_pack(-1.f, -1.f), a); }
 __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+
+// 2^x of two numbers below 2^7 on the FMA pipe, for binary16 weights: n the nearest integer, f the rest,
+// 2^f by the polynomial of degree 4 that interpolates it at the Chebyshev points of [-1/2, 1/2] (relative
+// error 3.5e-6, below a hundredth of binary16's half step), times 2^n. From 2^-126 down: 2^-126.
+__device__ __forceinline__ uint64_t f2_exp2(uint64_t x) {
+    float a, b;
+    f2_unpack(x, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+    x = f2_pack(a, b);
+    const uint64_t magic = f2_pack(12582912.f, 12582912.f);  // 1.5 2^23: a sum's last bits are n
+    const uint64_t t = f2_add(x, magic), f = f2_sub(x, f2_sub(t, magic));
+    uint64_t y = f2_pack(kExpC4, kExpC4);
+    y = f2_fma(y, f, f2_pack(kExpC3, kExpC3));
+    y = f2_fma(y, f, f2_pack(kExpC2, kExpC2));
+    y = f2_fma(y, f, f2_pack(kExpC1, kExpC1));
+    y = f2_fma(y, f, f2_pack(kExpC0, kExpC0));
+    f2_unpack(t, a, b);
+    return f2_mul(y, f2_pack(__int_as_float((__float_as_int(a) << 23) + 0x3f800000), __int_as_float((__float_as_int(b) << 23) + 0x3f800000)));
 }
 
 // Grid [group][pair of column tiles][kv head][split], clusters of bulk_cluster consecutive splits.
@@ -187,7 +211,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
     uint8_t* ring = base + bulk_q_bytes(D, F32);
     __shared__ int page_ids[kBulkMaxSplit / 16 + 2];
-    __shared__ uint64_t kv_full[NS], kv_free[NS], s_full[2], p_ready[2][2], o_done;
+    __shared__ uint64_t kv_full[NS], kv_free[NS], s_full[2], p_ready[2][2], pv_half[2], o_done;
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;
     __shared__ int lim_max, lim_min;
@@ -314,6 +338,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], tiles); }
         for (int w = 0; w < 2; ++w) {
             mbar_init(&s_full[w], 1);
+            mbar_init(&pv_half[w], 1);
             for (int h = 0; h < 2; ++h) mbar_init(&p_ready[w][h], 128);
         }
         mbar_init(&o_done, tiles);
@@ -418,6 +443,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                     if (!(ok = bulk_wait(&p_ready[w][h], (uint32_t)j & 1, &dead, p.err))) break;
                     tc_fence_after();
                     pv(j, h);
+                    if (h == 0) tc_commit(&pv_half[w]);
                 }
                 if (!ok) break;
                 tc_commit(&kv_free[(2 * j + 1) % NS]);
@@ -442,50 +468,6 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             ok = __all_sync(0xffffffffu, bulk_wait(&s_full[wg], (uint32_t)j & 1, &dead, p.err));
             if (!ok) break;
             tc_fence_after();
-            // S in blocks of 32 columns, the next one on its way: f(block, its first column)
-            auto each_block = [&](auto&& f) {
-                uint32_t s[2][32];
-                tc_ld32(S, s[0]);
-#pragma unroll
-                for (int k = 0; k < NK; k += 32) {
-                    uint32_t* cur = s[k >> 5 & 1];
-                    tc_wait_ld();
-                    tc_loaded(cur);
-                    if (k + 32 < NK) tc_ld32(S + k + 32, s[(k >> 5 & 1) ^ 1]);
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (c0 + k + e >= lim) cur[e] = 0xff800000u;  // -inf
-                    }
-                    f(cur, k);
-                }
-            };
-            // ---- the maximum
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            each_block([&](const uint32_t* s, int) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
-            });
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * cm;
-            if (j == 0) {
-                mref = mx > -INFINITY ? mx : 0.f;
-            } else if (__any_sync(0xffffffffu, mx > mref + kPaSlack)) {
-                const float next = fmaxf(mref, mx), corr = ex2(mref - next);
-                mref = next;
-                l *= corr;  // (PV(j - 1) is complete: QK(j), which S is of, was issued behind it)
-#pragma unroll 1
-                for (int k = 0; k < D; k += 16) {
-                    uint32_t o[16];
-                    tc_ld16(O + k, o);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                    tc_st16(O + k, o);
-                }
-            }
-            // ---- the weights: binary16 rows carry the factor in the exponent (their rounding is 2^-11 anyway)
-            const float shift = F32 ? -mref : 7.f - mref;
-            const uint64_t cm2 = f2_pack(cm, cm), sh2 = f2_pack(shift, shift), gain2 = f2_pack(kPaGain, kPaGain);
-            uint64_t sum2[2] = {0, 0};
             if (masked) {  // V where not every column sees: nothing but finite values may meet a zero weight
                 full(2 * j + 1);
                 uint8_t* V = ring + (size_t)((2 * j + 1) % NS) * SLOT;
@@ -510,37 +492,88 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             }
-            uint32_t lo[F32 ? 32 : 1];  // of a half: stored once both its blocks of S are read
-            each_block([&](const uint32_t* s, int k) {
-                uint32_t hi[16];
+            uint64_t sum2[2] = {0, 0};
+            const uint64_t cm2 = f2_pack(cm, cm), gain2 = f2_pack(kPaGain, kPaGain);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float a, b;
-                    f2_unpack(f2_fma(f2_pack(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), cm2, sh2), a, b);
-                    a = ex2(a);
-                    b = ex2(b);
-                    uint64_t ab = f2_pack(a, b);
-                    sum2[e & 1] = f2_add(sum2[e & 1], ab);
-                    if constexpr (F32) {
-                        ab = f2_mul(ab, gain2);
-                        f2_unpack(ab, a, b);
+            for (int h = 0; h < 2; ++h) {  // halves of 64 positions, each with its own look at the maximum
+                uint32_t s[64];
+                tc_ld32(S + h * 64, s);
+                tc_ld32(S + h * 64 + 32, s + 32);
+                tc_wait_ld();
+                tc_loaded(s);
+                tc_loaded(s + 32);
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 64; ++e)
+                        if (c0 + h * 64 + e >= lim) s[e] = 0xff800000u;  // -inf
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 64; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * cm;
+                if (j == 0 && h == 0) {
+                    mref = mx > -INFINITY ? mx : 0.f;
+                } else if (__any_sync(0xffffffffu, mx > mref + kPaSlack)) {
+                    const float next = fmaxf(mref, mx), corr = ex2(mref - next);
+                    mref = next;
+                    l *= corr;
+                    sum2[0] = f2_mul(sum2[0], f2_pack(corr, corr));
+                    sum2[1] = f2_mul(sum2[1], f2_pack(corr, corr));
+                    // every product into O so far has to be complete: before S(j) the earlier tiles', before its
+                    // second half the first half's
+                    if (h == 1) {
+                        ok = __all_sync(0xffffffffu, bulk_wait(&pv_half[wg], (uint32_t)j & 1, &dead, p.err));
+                        tc_fence_after();
                     }
-                    const __half2 h = __floats2half2_rn(a, b);
-                    hi[e] = *reinterpret_cast<const uint32_t*>(&h);
-                    if constexpr (F32) {
-                        const float2 f = __half22float2(h);
-                        const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
-                        lo[(k >> 1 & 16) + e] = *reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll 1
+                    for (int k = 0; k < D; k += 16) {
+                        uint32_t o[16];
+                        tc_ld16(O + k, o);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                        tc_st16(O + k, o);
                     }
                 }
-                tc_st16(S + (k >> 6) * 64 + (k >> 1 & 16), hi);
-                if (k & 32) {  // a half is written
-                    if constexpr (F32) tc_st32(S + (k >> 6) * 64 + 32, lo);
-                    tc_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(&p_ready[wg][k >> 6]);
+                // ---- the weights: binary16 rows carry the factor in the exponent (their rounding is 2^-11 anyway)
+                const float shift = F32 ? -mref : 7.f - mref;
+                const uint64_t sh2 = f2_pack(shift, shift);
+#pragma unroll
+                for (int k = 0; k < 64; k += 32) {
+                    uint32_t hi[16], lo[F32 ? 16 : 1];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        uint64_t ab = f2_fma(f2_pack(__uint_as_float(s[k + 2 * e]), __uint_as_float(s[k + 2 * e + 1])), cm2, sh2);
+                        float a, b;
+                        if (!F32 && e % 16 < kBulkPoly) {
+                            ab = f2_exp2(ab);
+                            f2_unpack(ab, a, b);
+                        } else {
+                            f2_unpack(ab, a, b);
+                            a = ex2(a);
+                            b = ex2(b);
+                            ab = f2_pack(a, b);
+                        }
+                        sum2[e & 1] = f2_add(sum2[e & 1], ab);
+                        if constexpr (F32) {
+                            ab = f2_mul(ab, gain2);
+                            f2_unpack(ab, a, b);
+                        }
+                        const __half2 x = __floats2half2_rn(a, b);
+                        hi[e] = *reinterpret_cast<const uint32_t*>(&x);
+                        if constexpr (F32) {
+                            const float2 f = __half22float2(x);
+                            const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+                            lo[e] = *reinterpret_cast<const uint32_t*>(&r);
+                        }
+                    }
+                    tc_st16(S + h * 64 + k / 2, hi);
+                    if constexpr (F32) tc_st16(S + h * 64 + 32 + k / 2, lo);
                 }
-            });
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_ready[wg][h]);
+            }
+            if (!ok) break;
             float a, b;
             f2_unpack(f2_add(sum2[0], sum2[1]), a, b);
             l += a + b;
@@ -573,8 +606,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
-            // (l is zero only where the column saw nothing: its largest weight is at least 2^-8)
-            row_ml[tid] = make_float2(l == 0.f ? -INFINITY : mref, live && view.n < 0 ? -1.f : F32 ? l * kPaGain : l);
+            row_ml[tid] = make_float2(lim <= t0 ? -INFINITY : mref, live && view.n < 0 ? -1.f : F32 ? l * kPaGain : l);
         }
         tc_fence_before();
     }

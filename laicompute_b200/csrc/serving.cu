@@ -301,7 +301,7 @@ cudaError_t serving_set_attributes() {
     for (int D : {32, 64, 128})
         for (bool whole : {false, true})
             for (PaFn fn : {pr_pick(D, LAIC_GGML_F16, 1, whole), pr_pick(D, LAIC_GGML_F32, 4, whole), pr_pick(D, LAIC_GGML_F32, 8, whole)}) {
-                e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pr_smem(D));
+                e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pr_smem(D, whole));
                 if (e != cudaSuccess) return e;
             }
     for (int D : {64, 128})
@@ -442,8 +442,8 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
         // (launched early only behind kernels of this call, which nothing earlier runs beside)
         if (e == cudaSuccess && pl.private_items)
             e = launch_k(pr_pick(g.head_dim, a.type, p.G, pl.whole),
-                         dim3(pl.whole ? pl.private_items : (pl.private_items + kPrWarps - 1) / kPrWarps), dim3(kPrWarps * 32),
-                         pr_smem(g.head_dim), st, pl.shared_items > 0, p);
+                         dim3(pl.whole ? pl.private_items : (pl.private_items + kPrWarps - 1) / kPrWarps), dim3(pr_warps(pl.whole) * 32),
+                         pr_smem(g.head_dim, pl.whole), st, pl.shared_items > 0, p);
         if (e == cudaSuccess && !pl.direct && !pl.whole)
             e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
                          dim3((unsigned)(a.rows * a.heads)), dim3(kPmWarps * 32), 0,
