@@ -6,13 +6,19 @@
 //
 // Roles: warp 8 loads (TMA boxes of up to a page, 128-byte swizzle, a lane per box: one lane alone
 // took 125 cycles a box, 4,000 for a tile of 16-position pages; a ring of K and V tiles); warps 9 and
-// 10 multiply, one lane for each tile of columns (tcgen05.mma, S and O in tensor memory, P read from tensor memory, where it
-// takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S, keep the
-// running maximum and sum, and write P in two halves, so that PV starts on the first. One tile's products run under the other's exponentials. 128 positions
-// per tile: a product of N = 64 takes about as long as one of N = 128 (100 against 85 cycles
-// measured), and two score buffers of 64 ran slower than one of 128. O is rescaled only when a
-// maximum grew by more than 2^8 since the last time (weights stay below 2^15 in binary16 with the
-// factor 2^7 they carry). Both tiles' S and O fill the 512 columns of tensor memory.
+// 10 multiply (one lane each: tcgen05.mma, S and O in tensor memory, P read from tensor memory, where
+// it takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S, keep the
+// running maximum and sum, and write P in two halves, so that PV starts on the first.
+// Binary16 rows, where a tile's exponentials take longer than its products: one lane multiplies for
+// both tiles in turn, which keeps one tile's products under the other's exponentials (attn of 512
+// prompt rows behind 1,537: 39.0 us; a lane per tile let them fall into step, 41.0). FP32 rows, with
+// twice the products: a lane per tile (64 rows behind 4,101 shared positions: 44.0 us against 48.6).
+// 128 positions per tile: a product of N = 64 takes about as long as one of N = 128 (100 against 85
+// cycles), and two score buffers of 64 ran slower than one of 128. O is rescaled only when a maximum
+// grew by more than 2^8 since the last time (weights stay below 2^15 in binary16 with the factor 2^7
+// they carry). Both tiles' S and O fill the 512 columns of tensor memory. What bounds it: the chain
+// softmax -> PV -> QK of a tile (about 4,000 cycles a pair of 128-position tiles, 2,000 of them
+// exponentials at 16 a clock), and, for few tiles per CTA, set-up and the join.
 //
 // The splits of a set of columns form a thread-block cluster and join through distributed shared
 // memory: one partial per cluster goes to global memory, or the output itself where the cluster holds
@@ -37,10 +43,6 @@ namespace laic {
 
 constexpr int kBulkCols = 256;        // score columns of a CTA
 constexpr int kBulkThreads = 352;
-// Of 16 pairs of binary16 exponentials, this many go to the FMA pipe (f2_exp2): the special-function unit
-// alone (16 a clock) bounds a tile's softmax.
-constexpr int kBulkPoly = 6;
-constexpr float kExpC0 = 1.f, kExpC1 = 0.693121045f, kExpC2 = 0.24022349f, kExpC3 = 0.0559219758f, kExpC4 = 0.00966636852f;
 constexpr int kBulkMaxCluster = 8;   // clusters of 1, 2, 4 or 8
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
 
@@ -172,31 +174,10 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ uint64_t f2_sub(uint64_t a, uint64_t b) { return f2_fma(b, f2_pack(-1.f, -1.f), a); }
 __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
-}
-
-// 2^x of two numbers below 2^7 on the FMA pipe, for binary16 weights: n the nearest integer, f the rest,
-// 2^f by the polynomial of degree 4 that interpolates it at the Chebyshev points of [-1/2, 1/2] (relative
-// error 3.5e-6, below a hundredth of binary16's half step), times 2^n. From 2^-126 down: 2^-126.
-__device__ __forceinline__ uint64_t f2_exp2(uint64_t x) {
-    float a, b;
-    f2_unpack(x, a, b);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
-    x = f2_pack(a, b);
-    const uint64_t magic = f2_pack(12582912.f, 12582912.f);  // 1.5 2^23: a sum's last bits are n
-    const uint64_t t = f2_add(x, magic), f = f2_sub(x, f2_sub(t, magic));
-    uint64_t y = f2_pack(kExpC4, kExpC4);
-    y = f2_fma(y, f, f2_pack(kExpC3, kExpC3));
-    y = f2_fma(y, f, f2_pack(kExpC2, kExpC2));
-    y = f2_fma(y, f, f2_pack(kExpC1, kExpC1));
-    y = f2_fma(y, f, f2_pack(kExpC0, kExpC0));
-    f2_unpack(t, a, b);
-    return f2_mul(y, f2_pack(__int_as_float((__float_as_int(a) << 23) + 0x3f800000), __int_as_float((__float_as_int(b) << 23) + 0x3f800000)));
 }
 
 // Grid [group][pair of column tiles][kv head][split], clusters of bulk_cluster consecutive splits.
@@ -335,13 +316,13 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (tid == 0) {
-        for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], tiles); }
+        for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], F32 ? tiles : 1); }
         for (int w = 0; w < 2; ++w) {
             mbar_init(&s_full[w], 1);
             mbar_init(&pv_half[w], 1);
             for (int h = 0; h < 2; ++h) mbar_init(&p_ready[w][h], 128);
         }
-        mbar_init(&o_done, tiles);
+        mbar_init(&o_done, F32 ? tiles : 1);
         mbar_fence_init();
         dead = 0;
         any_odd = 0;
@@ -406,10 +387,11 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 while (!mbar_try_wait(&kv_full[q % NS], (uint32_t)(q / NS) & 1) && clock64() - since < 200000000LL) {}
             }
     } else if (warp >= 9) {
-        const int w = warp - 9;
-        if (lane == 0 && w < tiles) {
+        // the column tiles this warp multiplies for: FP32, one each for warps 9 and 10; binary16, warp 9 both in turn
+        const int w0 = F32 ? warp - 9 : 0, w1 = F32 ? min(w0 + 1, tiles) : warp == 9 ? tiles : 0;
+        if (lane == 0 && w0 < w1) {
             constexpr uint32_t iqk = umma_idesc(NK, false), ipv = umma_idesc(D, true);
-            auto qk = [&](int j) {
+            auto qk = [&](int w, int j) {
                 uint32_t ks = slot(2 * j), qa = smem_u32(base) + (uint32_t)(w * HN * QPART);
                 asm volatile("" : "+r"(ks), "+r"(qa));  // (descriptors are formed here, not kept over the loop)
 #pragma unroll
@@ -421,9 +403,9 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                                   umma_desc(ks + (k >> 2) * (NK * 128) + off, 16, 1024), iqk, part != HN - 1 || k > 0);
                     }
                 tc_commit(&s_full[w]);
-                tc_commit(&kv_free[2 * j % NS]);
+                if (w == w1 - 1) tc_commit(&kv_free[2 * j % NS]);
             };
-            auto pv = [&](int j, int h) {
+            auto pv = [&](int w, int j, int h) {
                 uint32_t vs = slot(2 * j + 1);
                 asm volatile("" : "+r"(vs));
 #pragma unroll
@@ -433,26 +415,27 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                         tc_mma_ts(o_at(w), s_at(w) + h * (NK / 2) + part * (NK / 4) + k * 8,
                                   umma_desc(vs + (h * (NK / 32) + k) * 2048, NK * 128, 1024), ipv,
                                   j > 0 || h > 0 || part != HN - 1 || k > 0);
+                if (h == 0) tc_commit(&pv_half[w]);
             };
             bool ok = full(0);
             tc_fence_after();
-            if (ok) qk(0);
-            for (int j = 0; j < nt && ok; ++j) {
-                ok = full(2 * j + 1);
-                for (int h = 0; h < 2 && ok; ++h) {
-                    if (!(ok = bulk_wait(&p_ready[w][h], (uint32_t)j & 1, &dead, p.err))) break;
-                    tc_fence_after();
-                    pv(j, h);
-                    if (h == 0) tc_commit(&pv_half[w]);
+            for (int w = w0; w < w1 && ok; ++w) qk(w, 0);
+            for (int j = 0; j < nt && ok; ++j)
+                for (int w = w0; w < w1 && ok; ++w) {
+                    if (w == w0 && !(ok = full(2 * j + 1))) break;
+                    for (int h = 0; h < 2 && ok; ++h) {
+                        if (!(ok = bulk_wait(&p_ready[w][h], (uint32_t)j & 1, &dead, p.err))) break;
+                        tc_fence_after();
+                        pv(w, j, h);
+                    }
+                    if (!ok) break;
+                    if (w == w1 - 1) tc_commit(&kv_free[(2 * j + 1) % NS]);
+                    if (j + 1 < nt) {
+                        if (w == w0 && !(ok = full(2 * j + 2))) break;
+                        tc_fence_after();
+                        qk(w, j + 1);
+                    }
                 }
-                if (!ok) break;
-                tc_commit(&kv_free[(2 * j + 1) % NS]);
-                if (j + 1 < nt) {
-                    if (!(ok = full(2 * j + 2))) break;
-                    tc_fence_after();
-                    qk(j + 1);
-                }
-            }
             tc_commit(&o_done);  // after a failed wait too: whatever was issued ends before tensor memory is freed
         }
     } else if (wg < tiles) {
@@ -542,17 +525,11 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                     uint32_t hi[16], lo[F32 ? 16 : 1];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        uint64_t ab = f2_fma(f2_pack(__uint_as_float(s[k + 2 * e]), __uint_as_float(s[k + 2 * e + 1])), cm2, sh2);
                         float a, b;
-                        if (!F32 && e % 16 < kBulkPoly) {
-                            ab = f2_exp2(ab);
-                            f2_unpack(ab, a, b);
-                        } else {
-                            f2_unpack(ab, a, b);
-                            a = ex2(a);
-                            b = ex2(b);
-                            ab = f2_pack(a, b);
-                        }
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[k + 2 * e]), __uint_as_float(s[k + 2 * e + 1])), cm2, sh2), a, b);
+                        a = ex2(a);
+                        b = ex2(b);
+                        uint64_t ab = f2_pack(a, b);
                         sum2[e & 1] = f2_add(sum2[e & 1], ab);
                         if constexpr (F32) {
                             ab = f2_mul(ab, gain2);
