@@ -99,6 +99,7 @@ template <typename TI, typename TQ, bool VEC, int R>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvAppendParams p) {
     const int sh = __ffs(p.head_dim) - 4;  // units per head: 2^sh
     const int u0 = blockIdx.y * blockDim.x * kAppendUnits + threadIdx.x;
+    pdl_wait();
     int pos[R], seq[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {

@@ -48,6 +48,7 @@ struct KvAttnParams {
     uint32_t g_inv;               // 2^16 / G rounded up
     float* part_o;                // [rows][heads][nss + nsp][head_dim]
     float2* part_ml;              // [rows][heads][nss + nsp] (m, l)
+    int first;                    // private items: no kernel of this call before them
     int direct;                   // the bulk kernel's clusters hold all that their rows see: they write the output
     int* err;
 };
@@ -58,7 +59,7 @@ constexpr int kPaMaxSplit = 2048; // positions per item at most (its page ids ar
 constexpr float kPaSlack = 8.f;  // log2 of how far a maximum may outgrow its reference before sums are rescaled
 constexpr float kPaGain = 128.f;  // the factor the weights carry (bulk items too: a row's items are summed)
 
-__host__ __device__ constexpr int pa_stages(int D) { return D == 128 ? 3 : 4; }
+__host__ __device__ constexpr int pa_stages(int D) { (void)D; return 3; }
 __host__ __device__ constexpr size_t pa_ring_bytes(int D) { return (size_t)pa_stages(D) * 2 * kPaChunk * D * 2; }
 __host__ __device__ constexpr size_t pa_smem(int D, int NT, bool hl) {
     const size_t ring = pa_ring_bytes(D), red = (size_t)kPaWarps * NT * 8 * (D + 4) * 4;
@@ -505,6 +506,7 @@ __global__ void __launch_bounds__(pr_warps(WHOLE) * 32) paged_private_kernel(con
     __shared__ int found[NW];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gq = lane >> 2, c = lane & 3;
+    if (p.first) pdl_wait();  // what the stream held before this call
     pdl_launch_dependents();  // (the merge waits for this grid's end; nothing else follows)
     int i = WHOLE ? blockIdx.x : blockIdx.x * NW + warp;
     const bool in = WHOLE || i < p.private_items;
@@ -842,10 +844,11 @@ __device__ __forceinline__ void shared_item(const KvAttnParams& p, int i, int* l
 
 // Grid: the shared items.
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const KvAttnParams p) {
+__global__ void __launch_bounds__(kPaWarps * 32, D == 128 ? 2 : 4) paged_attn_kernel(const KvAttnParams p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int lim[NT * 8], page_ids[kPaMaxSplit / 16 + 2], range[2];
     __shared__ float cmul[NT * 8];
+    pdl_wait();               // what the stream held before this call
     pdl_launch_dependents();  // the private items need nothing of this kernel
     shared_item<D, NT, T>(p, blockIdx.x, lim, page_ids, cmul, range, smem);
 }

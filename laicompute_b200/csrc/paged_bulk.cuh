@@ -205,6 +205,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     if (tid == 0) { tma_prefetch(&mk); tma_prefetch(&mv); }
+    pdl_wait();  // what the stream held before this call
     int i = blockIdx.x;
     const int nsplit = p.nss * C, split = i % nsplit;
     i /= nsplit;

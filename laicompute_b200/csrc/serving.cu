@@ -74,11 +74,14 @@ int on_device(int device, F&& f) {
     return f();
 }
 
+// Every first kernel of a call may start while its predecessor in the stream drains; it waits before it
+// reads or writes anything.
 template <typename TI, typename TQ>
-void append_launch(bool vec, dim3 grid, int block, cudaStream_t st, const KvAppendParams& p) {
-    if (!vec) kv_append_kernel<TI, TQ, false, 1><<<grid, block, 0, st>>>(p);
-    else if (grid.x < (unsigned)p.rows) kv_append_kernel<TI, TQ, true, 2><<<grid, block, 0, st>>>(p);
-    else kv_append_kernel<TI, TQ, true, 1><<<grid, block, 0, st>>>(p);
+cudaError_t append_launch(bool vec, dim3 grid, int block, cudaStream_t st, const KvAppendParams& p) {
+    return launch_k(!vec                         ? kv_append_kernel<TI, TQ, false, 1>
+                    : grid.x < (unsigned)p.rows ? kv_append_kernel<TI, TQ, true, 2>
+                                                 : kv_append_kernel<TI, TQ, true, 1>,
+                    grid, dim3(block), 0, st, true, p);
 }
 
 int device_sms(int dev) {
@@ -368,14 +371,9 @@ int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t
     const dim3 grid(vec && a.rows >= 16 * device_sms(g.device) ? (a.rows + 1) / 2 : a.rows, (units + cta - 1) / cta);
     if (grid.y > 65535) return api_fail(LAIC_E_UNSUPPORTED, "rows too wide");
     return on_device(g.device, [&]() -> int {
-        if (a.in_type == LAIC_GGML_F32) {
-            if (a.q_type == LAIC_GGML_F32) append_launch<float, float>(vec, grid, block, st, p);
-            else append_launch<float, __half>(vec, grid, block, st, p);
-        } else {
-            if (a.q_type == LAIC_GGML_F32) append_launch<__half, float>(vec, grid, block, st, p);
-            else append_launch<__half, __half>(vec, grid, block, st, p);
-        }
-        const cudaError_t e = cudaGetLastError();
+        const bool i32 = a.in_type == LAIC_GGML_F32, q32 = a.q_type == LAIC_GGML_F32;
+        const cudaError_t e = i32 ? (q32 ? append_launch<float, float>(vec, grid, block, st, p) : append_launch<float, __half>(vec, grid, block, st, p))
+                                  : (q32 ? append_launch<__half, float>(vec, grid, block, st, p) : append_launch<__half, __half>(vec, grid, block, st, p));
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "kv_append");
     });
 }
@@ -418,6 +416,7 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     p.scale_log2 = scale * 1.44269504f;
     p.lp = pl.lp; p.nsp = pl.nsp; p.ls = pl.ls; p.nss = pl.nss; p.ctiles = pl.ctiles; p.lc = pl.cluster;
     p.private_items = pl.private_items;
+    p.first = pl.shared_items == 0;
     p.direct = pl.direct;
     p.out_vec = aligned16(a.out_dev) && (a.rows == 1 || a.ldo * type_size(a.type) % 16 == 0);
     p.q_vec = aligned16(a.q_dev) && (a.rows == 1 || a.ldq * type_size(a.type) % 16 == 0);
@@ -434,16 +433,15 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
             if (!encode_pages(g, g.k_dev, &mk) || !encode_pages(g, g.v_dev, &mv))
                 return api_fail(LAIC_E_CUDA, "kv_attention: tensor map");
             e = launch_cluster_k(bulk_pick(g.head_dim, f32), dim3(pl.shared_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32),
-                                 st, false, pl.cluster, p, mk, mv);
+                                 st, true, pl.cluster, p, mk, mv);
         }
         if (e == cudaSuccess && !pl.bulk && pl.shared_items)
             e = launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(pl.shared_items), dim3(kPaWarps * 32),
-                         pa_smem(g.head_dim, pl.nt, f32), st, false, p);
-        // (launched early only behind kernels of this call, which nothing earlier runs beside)
+                         pa_smem(g.head_dim, pl.nt, f32), st, true, p);
         if (e == cudaSuccess && pl.private_items)
             e = launch_k(pr_pick(g.head_dim, a.type, p.G, pl.whole),
                          dim3(pl.whole ? pl.private_items : (pl.private_items + kPrWarps - 1) / kPrWarps), dim3(pr_warps(pl.whole) * 32),
-                         pr_smem(g.head_dim, pl.whole), st, pl.shared_items > 0, p);
+                         pr_smem(g.head_dim, pl.whole), st, true, p);
         if (e == cudaSuccess && !pl.direct && !pl.whole)
             e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
                          dim3((unsigned)(a.rows * a.heads)), dim3(kPmWarps * 32), 0,
@@ -473,7 +471,7 @@ int logits_probs(int device, int rows, int vocab, const float* x, long long ldx,
         const size_t smem = sm ? ((((size_t)vocab + c - 1) / c + 3) & ~(size_t)3) * 4 : 0;
         cudaError_t e = serving_set_attributes();
         if (e == cudaSuccess)
-            e = launch_cluster_k(fn, dim3((unsigned)rows * c), dim3(kProbsThreads), smem, st, false, c, p);
+            e = launch_cluster_k(fn, dim3((unsigned)rows * c), dim3(kProbsThreads), smem, st, true, c, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "logits_probs");
     });
 }
@@ -497,7 +495,7 @@ int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st) {
         // the largest cluster that still runs in one wave (two CTAs per SM)
         int c = kVerifyMaxCluster;
         while (c > 1 && (long long)a.nseq * c > 2LL * device_sms(device)) c /= 2;
-        const cudaError_t e = launch_cluster_k(vec ? verify_kernel<true> : verify_kernel<false>, dim3((unsigned)a.nseq * c), dim3(kVerifyThreads), 0, st, false, c, p);
+        const cudaError_t e = launch_cluster_k(vec ? verify_kernel<true> : verify_kernel<false>, dim3((unsigned)a.nseq * c), dim3(kVerifyThreads), 0, st, true, c, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "verify_drafts");
     });
 }

@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kProbsThreads) probs_kernel(const ProbsParams 
     const int v0 = min(p.vocab, rank * per), n = min(p.vocab, v0 + per) - v0;
     const float* x = p.x + (size_t)row * p.ldx + v0;
     float* y = p.y + (size_t)row * p.ldy + v0;
+    pdl_wait();
     if constexpr (SM) {
         if constexpr (VEC) {
             for (int i = tid * 4; i + 3 < n; i += NT * 4) cp_async16(slice + i, x + i);
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(const VerifyP
     constexpr int NW = kVerifyThreads / 32;
     __shared__ int s_acc;
     __shared__ double s_sum[2], s_run[NW];
+    pdl_wait();
     int n = p.n_draft[s];
     if (n < 0) return;  // the whole cluster alike
     n = min(n, p.max_draft);
