@@ -180,6 +180,21 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
     return r;
 }
 
+// Where the clusters write the output themselves, the first CTA leaves the zeros of the rows of no group.
+template <int D, typename T>
+__device__ __forceinline__ void groupless_rows(const KvAttnParams& p) {
+    if (!p.direct || blockIdx.x != 0) return;
+    const int lane = threadIdx.x & 31;
+    const int g0 = max(0, min(p.rows, p.group_rows[0])), g1 = max(g0, min(p.rows, p.group_rows[p.groups]));
+    for (int r = threadIdx.x >> 5; r < p.rows; r += kBulkThreads / 32) {
+        if (r >= g0 && r < g1) continue;
+        const RowView v = row_view(p, r, 0);
+        if (v.n < 0) continue;
+        if (v.n > 0 && lane == 0) kv_flag(p.err, kKvBadPos);
+        for (int e = lane; e < p.heads * D; e += 32) static_cast<T*>(p.out)[(size_t)r * p.ldo + e] = kv_out<T>(0.f);
+    }
+}
+
 // Grid [group][pair of column tiles][kv head][split], clusters of bulk_cluster consecutive splits.
 template <int D, typename T>
 __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAttnParams p, const __grid_constant__ CUtensorMap mk,
@@ -214,9 +229,12 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     const int pair = i % p.ctiles, g = i / p.ctiles;
     int r0, r1;
     const int glen = p.group_len[g];
-    if (!group_rows(p, g, r0, r1)) return;
+    if (!group_rows(p, g, r0, r1)) r1 = r0;
     const int ncol = (r1 - r0) * p.G, col0 = pair * kBulkCols;
-    if (col0 >= ncol) return;
+    if (col0 >= ncol) {  // (alike for all CTAs of a cluster)
+        groupless_rows<D, T>(p);
+        return;
+    }
     const int t0 = split * p.ls;
     const int shared = max(0, kv_clamp_len(p, glen, p.max_shared));
     const int tiles = ncol - col0 > 128 ? 2 : 1;  // M tiles with columns
@@ -677,16 +695,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     else if (C == 4) join(std::integral_constant<int, 4>{});
     else join(std::integral_constant<int, 8>{});
     if (C > 1) cluster.sync();  // no CTA leaves while another may still read its rows
-    if (p.direct && blockIdx.x == 0) {  // rows of no group see nothing here
-        const int g0 = max(0, min(p.rows, p.group_rows[0])), g1 = max(g0, min(p.rows, p.group_rows[p.groups]));
-        for (int r = warp; r < p.rows; r += kBulkThreads / 32) {
-            if (r >= g0 && r < g1) continue;
-            const RowView v = row_view(p, r, 0);
-            if (v.n < 0) continue;
-            if (v.n > 0 && lane == 0) kv_flag(p.err, kKvBadPos);
-            for (int e = lane; e < p.heads * D; e += 32) static_cast<T*>(p.out)[(size_t)r * p.ldo + e] = kv_out<T>(0.f);
-        }
-    }
+    groupless_rows<D, T>(p);
 }
 
 }  // namespace laic

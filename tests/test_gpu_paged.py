@@ -436,6 +436,41 @@ def test_attention_captured_and_on_two_streams():
         close(outs[i], ref, tol)
 
 
+@pytest.mark.parametrize("shared", [0, 600])
+def test_offsets_beyond_32_bits(shared):
+    """A pool of more than 2^31 elements per side: append and both attentions at its last pages."""
+    from laicompute_b200.serving import KvPages
+    hkv, d, page, heads, n = 8, 128, 64, 32, 12
+    num_pages = (1 << 31) // (hkv * page * d) + 40
+    small = Cache([640] * n, hkv, d, page, seed=3, shared=[(list(range(n)), shared)] if shared else None)
+    k = torch.empty(num_pages, hkv, page, d, dtype=torch.float16, device="cuda")
+    v = torch.empty_like(k)
+    base = num_pages - small.num_pages
+    k[base:], v[base:] = small.k, small.v
+    table = torch.where(small.table >= 0, small.table + base, small.table)
+    assert table.dtype == torch.int32
+    pages = KvPages(k.data_ptr(), v.data_ptr(), num_pages, hkv, page, d, err=small.err.data_ptr())
+    # the last position of every row is appended again, at a place past 2^31 elements
+    new = torch.randn(n, 2 * hkv * d).half()
+    ld = 2 * hkv * d
+    x, pos = new.cuda(), ints([639] * n)
+    plan = pages.append_plan(n, 0, n, table.shape[1], in_type=F16, q_type=F16, ldk=ld, ldv=ld)
+    plan(0, x.data_ptr(), x.data_ptr() + 2 * hkv * d, 0, pos.data_ptr(), table.data_ptr())
+    for i in range(n):
+        small.seq_k[i][639] = new[i, :hkv * d].view(hkv, d)
+        small.seq_v[i][639] = new[i, hkv * d:].view(hkv, d)
+    q = _q(n, heads, d, F32, seed=8)
+    big = Cache.__new__(Cache)
+    big.__dict__.update(small.__dict__)
+    big.k, big.v, big.table, big.num_pages = k, v, table, num_pages
+    lens = [640] * n
+    out = attend(big, q, lens, groups=([0, n], [shared]) if shared else None)
+    big.pages().check()
+    rows = [0, 5, n - 1]
+    ref, tol = reference(small, q[rows], [640] * 3, rows)
+    close(out[rows], ref, tol)
+
+
 def test_attention_is_repeatable():
     """The same call gives the same bits (no order of arrival enters a sum)."""
     cache = Cache([1200] * 6, 2, 128, 16, seed=1, shared=[(list(range(6)), 1000)])
@@ -443,6 +478,42 @@ def test_attention_is_repeatable():
     a = attend(cache, q, [1200] * 6, groups=([0, 6], [1000]))
     for _ in range(3):
         assert torch.equal(a, attend(cache, q, [1200] * 6, groups=([0, 6], [1000])))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_rows_of_no_group(dtype):
+    """Rows before, between and behind the groups, with and without positions of their own; groups without rows."""
+    cache = Cache([400] * 30, 1, 64, 32, seed=9, shared=[(list(range(2, 22)), 400)])
+    lens = [0, -1] + [400] * 20 + [0, -1] + [0] * 6
+    q = _q(30, 4, 64, dtype, seed=6)
+    out = attend(cache, q, lens, groups=([2, 2, 22, 22], [64, 400, 10]), bounds=dict(max_private=0))
+    cache.pages().check()
+    rows = [2, 11, 21]
+    ref, tol = reference(cache, q[rows], [400] * 3, rows)
+    close(out[rows], ref, tol)
+    assert not out[[0, 22, 24, 29]].any() and torch.all(out[[1, 23]] == 7.0)
+    lens = [37, 5] + [400] * 20 + [1, 0, 399] + [12] * 5
+    out = attend(cache, q, lens, groups=([2, 2, 22, 22], [64, 400, 10]))
+    cache.pages().check()
+    rows = list(range(0, 30, 3)) + [1, 22, 23, 24]
+    ref, tol = reference(cache, q[rows], [lens[r] for r in rows], rows)
+    close(out[rows], ref, tol)
+
+
+def test_long_bounds_and_many_groups():
+    """A bound far above the lengths (its splits are empty), and a group per pair of rows."""
+    n = 40
+    lens = [70 + 13 * i for i in range(n)]
+    cache = Cache(lens, 2, 64, 16, seed=2, shared=[([2 * i, 2 * i + 1], 64) for i in range(n // 2)], room=4000)
+    q = _q(n, 8, 64, F32, seed=4)
+    ref, tol = reference(cache, q, lens)
+    groups = (list(range(0, n + 1, 2)), [64] * (n // 2))
+    for kw in (dict(max_len=60000, max_private=60000, max_shared=60000), dict(max_len=60000, max_private=2000)):
+        out = attend(cache, q, lens, groups=groups, bounds=kw)
+        cache.pages().check()
+        close(out, ref, tol)
+    out = attend(cache, q, lens, bounds=dict(max_len=60000))
+    close(out, ref, tol)
 
 
 # ------------------------------------------------------------------------------------------------
