@@ -314,6 +314,7 @@ typedef struct laic_kv_pages {
 #define LAIC_KV_BAD_POS 2   /* a position or length beyond the page table, the rotation table or a given bound */
 #define LAIC_KV_BAD_PAGE 4  /* a page id outside [0, num_pages) */
 #define LAIC_KV_BAD_GROUP 8 /* group_rows_dev not ascending within the rows, or a group above max_group_rows */
+#define LAIC_KV_WAIT 16     /* a kernel's bounded wait ran out (the call's output is incomplete) */
 
 typedef struct laic_kv_append_args {
     int32_t rows;             /* tokens */
@@ -367,7 +368,8 @@ typedef struct laic_kv_attention_args {
  * once, through the page table row of the group's first row. Rows that share a
  * whole sequence with causal lengths (a prompt's tokens, drafted tokens) are a
  * group whose length is the longest. Masked positions never reach a row's output,
- * whatever they hold. */
+ * whatever they hold. out_dev must not overlap an input. Two calls with the same
+ * inputs give the same bits. */
 LAIC_API int laic_kv_attention(const laic_kv_pages* pages, const laic_kv_attention_args* args, void* stream);
 /* Bytes of workspace the call needs (0 possible); reads no pointer of `args`. */
 LAIC_API int laic_kv_attention_workspace(const laic_kv_pages* pages, const laic_kv_attention_args* args,

@@ -1962,7 +1962,9 @@ int laic_dev_reset_slot(laic_dev* d, int32_t slot) {
     return LAIC_OK;
 }
 
-int laic_dev_fork_slot(laic_dev* d, int32_t src, int32_t dst) {
+}  // extern "C"
+
+static int fork_slot(laic_dev* d, int32_t src, int32_t dst) {
     if (!d || src < 0 || src >= d->S || dst < 0 || dst >= d->S) return fail(LAIC_E_INVALID, "slot out of range");
     if (!d->paged) return fail(LAIC_E_UNSUPPORTED, "forking a slot needs a paged cache (LAIC_FLAG_PAGED_KV)");
     if (src == dst) return LAIC_OK;
@@ -1994,9 +1996,9 @@ int laic_dev_fork_slot(laic_dev* d, int32_t src, int32_t dst) {
     return LAIC_OK;
 }
 
-int laic_dev_verify(laic_dev* d, int32_t nseq, const int32_t* slots, int32_t max_draft, const uint32_t* tokens,
-                    const int32_t* n_draft, const float* draft_probs_dev, const laic_sample_params* params, int32_t nparams,
-                    uint32_t* out_ids, int32_t* out_n) {
+static int verify_step(laic_dev* d, int32_t nseq, const int32_t* slots, int32_t max_draft, const uint32_t* tokens,
+                       const int32_t* n_draft, const float* draft_probs_dev, const laic_sample_params* params,
+                       int32_t nparams, uint32_t* out_ids, int32_t* out_n) {
     if (!d) return fail(LAIC_E_INVALID, "null device");
     if (!d->paged) return fail(LAIC_E_UNSUPPORTED, "verifying drafted tokens needs a paged cache (LAIC_FLAG_PAGED_KV)");
     if (!slots || !tokens || !n_draft || !out_ids || !out_n) return fail(LAIC_E_INVALID, "null argument");
@@ -2103,6 +2105,30 @@ int laic_dev_verify(laic_dev* d, int32_t nseq, const int32_t* slots, int32_t max
     std::copy(got.begin(), got.end(), out_ids);
     std::copy(cnt.begin(), cnt.end(), out_n);
     return check_sampler_err(d);
+}
+
+// No exception crosses the C boundary (these calls allocate on the host).
+template <typename F>
+static int no_throw(F&& f) {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        return fail(LAIC_E_INVALID, e.what());
+    }
+}
+
+extern "C" {
+
+int laic_dev_fork_slot(laic_dev* d, int32_t src, int32_t dst) {
+    return no_throw([&] { return fork_slot(d, src, dst); });
+}
+
+int laic_dev_verify(laic_dev* d, int32_t nseq, const int32_t* slots, int32_t max_draft, const uint32_t* tokens,
+                    const int32_t* n_draft, const float* draft_probs_dev, const laic_sample_params* params, int32_t nparams,
+                    uint32_t* out_ids, int32_t* out_n) {
+    return no_throw([&] {
+        return verify_step(d, nseq, slots, max_draft, tokens, n_draft, draft_probs_dev, params, nparams, out_ids, out_n);
+    });
 }
 
 int laic_dev_slot_pos(laic_dev* d, int32_t slot, int64_t* pos) {

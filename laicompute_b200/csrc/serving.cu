@@ -185,9 +185,11 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
     };
     const int sms = device_sms(g.device);
     // private: ranges up to kPrWhole by one CTA, which writes the output; longer ones by a warp per split, 8 to 12
-    // on an SM (256 positions: a partial costs 2 % of their bytes, and ragged rows balance)
+    // on an SM (256 positions: a partial costs 2 % of their bytes, and ragged rows balance; more where the
+    // bound is far, which would ask for thousands of partials per row)
     pl.whole = max_private <= kPrWhole;
-    pl.lp = pl.whole ? kPrWhole : split((long long)a.rows * g.kv_heads, max_private, 12LL * sms, 16, 128, 256);
+    const int most = std::max(256, std::min(kPrWhole, max_private / 64 / 16 * 16));
+    pl.lp = pl.whole ? kPrWhole : split((long long)a.rows * g.kv_heads, max_private, 12LL * sms, 16, 128, most);
     pl.nsp = pl.whole ? 0 : (max_private + pl.lp - 1) / pl.lp;
     if (a.groups) {
         if (max_private == 0) pl.whole = false;  // nothing private: shared items alone, joined by the merge
