@@ -18,10 +18,13 @@ struct ProbsParams {
     int vocab;
 };
 
-// log2(e) / T as hi + lo: the lo part matters, an error of the factor tilts the whole row.
+// log2(e) / T as hi + lo: the lo part matters, an error of the factor tilts the whole row. An infinite T
+// makes all finite logits alike; one below the smallest normal number counts as that.
 struct ProbFactor {
-    float k, kl;
+    float k = 0.f, kl = 0.f;
     __device__ __forceinline__ explicit ProbFactor(float t) {
+        if (t == INFINITY) return;
+        t = fmaxf(t, 0x1p-126f);
         k = 1.44269502f / t;  // log2(e) = 1.44269502162933 (binary32) + 1.9259630e-8
         kl = (fmaf(-k, t, 1.44269502f) + 1.9259630e-8f) / t;
     }

@@ -516,6 +516,110 @@ def test_long_bounds_and_many_groups():
     close(out, ref, tol)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_wide_group_captured_on_two_streams(dtype):
+    """Wide groups and private positions: a captured call replays over other lengths, groups and queries, with
+    padding rows and one sequence named by several rows; then calls at once, each with its own workspace."""
+    n, heads, hkv, d = 36, 8, 2, 64
+    cache = Cache([900 + 3 * i for i in range(n)], hkv, d, 32, seed=4, shared=[(list(range(n)), 850)])
+    pages = cache.pages()
+    kw = dict(type=dtype, groups=2, max_group_rows=32, max_shared=850, max_private=400)
+    plan = pages.attention_plan(n, heads, n, cache.per_seq, 1024, **kw)
+    ws = [torch.full((plan.workspace_bytes,), 255, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    q, out = _q(n, heads, d, dtype, 1), torch.full((n, heads * d), 7.0, dtype=TORCH[dtype], device="cuda")
+    lens, seq = ints([0] * n), ints([0] * n)
+    starts, shared = ints([0, 0, 0]), ints([0, 0])
+
+    def call(k, stream, qk, ok):
+        plan(qk.data_ptr(), ok.data_ptr(), lens.data_ptr(), cache.table.data_ptr(), workspace=ws[k].data_ptr(),
+             seq=seq.data_ptr(), group_rows=starts.data_ptr(), group_len=shared.data_ptr(), stream=stream)
+    call(0, 0, q, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(0, torch.cuda.current_stream().cuda_stream, q, out)
+    cases = [([0, 20, 36], [850, 700], [900 + 3 * i for i in range(n)], list(range(n))),
+             ([4, 4, 34], [850, 850], [30, -1, 0, 250] + [860] * 30 + [399, 1], [5] * n),
+             ([0, 32, 36], [64, 850], [450] * 31 + [-1] + [851, 850, 849, 0], [0, 0, 1, 2] * 9)]
+    for seed, (gr, gl, ln, sq) in enumerate(cases):
+        q.copy_(_q(n, heads, d, dtype, seed + 2))
+        for t, x in ((lens, ln), (seq, sq), (starts, gr), (shared, gl)):
+            t.copy_(ints(x))
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        pages.check()
+        rows = [r for r in range(0, n, 3) if ln[r] >= 0] + [35]
+        ref, tol = reference(cache, q[rows], [ln[r] for r in rows], [sq[r] for r in rows])
+        close(out[rows], ref, tol)
+        assert all(torch.all(out[r] == 7.0) for r in range(n) if ln[r] < 0)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    qs = [_q(n, heads, d, dtype, 30 + i) for i in range(2)]
+    outs = [torch.zeros_like(out) for _ in range(2)]
+    alone = []
+    for i in range(2):
+        call(i, 0, qs[i], outs[i])
+        torch.cuda.synchronize()
+        alone.append(outs[i].clone())
+        outs[i].zero_()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i in range(2):
+            call(i, streams[i].cuda_stream, qs[i], outs[i])
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], alone[0]) and torch.equal(outs[1], alone[1])
+
+
+FIRST_CALL = """
+import torch
+from laicompute_b200.serving import KvPages, logits_probs, verify_drafts
+d, page, n = 64, 32, 64
+k, v = (torch.randn(40, 1, page, d, device="cuda").half() for _ in range(2))
+err, table = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.arange(40, dtype=torch.int32, device="cuda")[None].contiguous()
+pages = KvPages(k.data_ptr(), v.data_ptr(), 40, 1, page, d, err=err.data_ptr())
+q, out = torch.randn(n, d, device="cuda"), torch.zeros(n, d, device="cuda")
+ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+lens, seq, gr, gl, one = ints([1280] * n), ints([0] * n), ints([0, n]), ints([1280]), ints([1])
+x, t, pr = torch.randn(3, 20000, device="cuda"), torch.ones(3, device="cuda"), torch.zeros(3, 20000, device="cuda")
+u, ids, cnt = torch.full((2,), 0.5, device="cuda"), ints([5, 6]), ints([0])
+oid = ints([0, 0, 0])
+new = torch.randn(1, d, device="cuda")
+app = pages.append_plan(1, 0, 1, 40)
+plan = pages.attention_plan(n, 1, 1, 40, 1280, groups=1, max_group_rows=n, max_shared=1280, max_private=0)
+ws = torch.zeros(max(16, plan.workspace_bytes), dtype=torch.uint8, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    st = torch.cuda.current_stream().cuda_stream
+    app(0, new.data_ptr(), new.data_ptr(), 0, one.data_ptr(), table.data_ptr(), stream=st)
+    plan(q.data_ptr(), out.data_ptr(), lens.data_ptr(), table.data_ptr(), workspace=ws.data_ptr(), seq=seq.data_ptr(),
+         group_rows=gr.data_ptr(), group_len=gl.data_ptr(), stream=st)
+    logits_probs(3, 20000, x.data_ptr(), t.data_ptr(), pr.data_ptr(), stream=st)
+    verify_drafts(1, 2, 20000, pr.data_ptr(), 0, ids.data_ptr(), gr.data_ptr(), u.data_ptr(), u.data_ptr(),
+                  oid.data_ptr(), cnt.data_ptr(), stream=st)
+graph.replay()
+torch.cuda.synchronize()
+pages.check()
+ref = torch.nn.functional.scaled_dot_product_attention(q[None, None].double(), k.view(1, 1, 1280, d).double(), v.view(1, 1, 1280, d).double())
+# as in reference(): scores to 35 * 1.2e-6 + 2e-6, weights to twice that and 2e-5, values to 0.8 on average
+assert float((out - ref[0, 0]).abs().max()) < 1e-4
+assert float((pr.double() - torch.softmax(x.double(), 1)).abs().max()) < 1e-6
+assert int(cnt[0]) == 1
+print("captured")
+"""
+
+
+def test_first_call_is_captured():
+    """A process whose first call of each operator is made under stream capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 # ------------------------------------------------------------------------------------------------
 # append and attention together, as a decode loop uses them
 # ------------------------------------------------------------------------------------------------

@@ -66,6 +66,31 @@ def test_probs_strides_and_in_place(ld, ldp, in_place):
     _check_probs(_probs(x, temp, ld=ld, ldp=ldp, in_place=in_place), x, temp)
 
 
+@pytest.mark.parametrize("v", [40, 1000, 40000, 140000])
+def test_probs_extreme_temperatures(v):
+    """From the smallest binary32 numbers to the largest and infinity, ordinary logits and huge ones."""
+    inf = float("inf")
+    x = torch.randn(8, v, generator=torch.Generator().manual_seed(v)) * 3
+    x[:, 7] = 20.0                                    # one clear first
+    x[1] = 0.0                                        # a constant row
+    x[5] *= 1e37
+    temp = [1e-45, 1e-45, 1e-30, inf, 3e38, 3e38, 1e-39, inf]
+    x[7, 3] = -inf
+    p = _probs(x, temp)
+    uniform = torch.full((v,), 1 / v, dtype=torch.float64)
+    _check_probs(p[2:3], x[2:3], [1e-30])
+    _check_probs(p[5:6], x[5:6], [3e38])
+    rel = 2.0 ** -20 + (v / 256 + 40) * 2.0 ** -24    # of the sum and the products, as in _check_probs
+    one = torch.zeros(v, dtype=torch.float64)
+    one[7] = 1.0
+    assert torch.equal(p[0].double(), one) and torch.equal(p[6].double(), one)
+    for r in (1, 3, 4):                               # (row 4: exponents below 1e-36)
+        assert float((p[r].double() / uniform - 1).abs().max()) <= rel
+    assert p[7, 3] == 0
+    rest = torch.cat([p[7, :3], p[7, 4:]]).double() * (v - 1)
+    assert float((rest - 1).abs().max()) <= rel
+
+
 def test_probs_ties_masks_and_infinities():
     inf, nan = float("inf"), float("nan")
     lowest = torch.finfo(torch.float32).min
