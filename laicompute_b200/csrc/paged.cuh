@@ -91,8 +91,9 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 constexpr int kAppendUnits = 4;  // units per thread and row
 
 // Grid (rows / R, slices of a row). A thread owns whole rotation pairs, so q_out may be q itself; it
-// loads all its units of R rows before the chains position -> sequence -> page are resolved (two rows
-// at a time fill the waits of many rows: 38 us against 40 for 8,188 rows of the 8B shape, 5.3 TB/s). The
+// loads all its units of R rows before the chains position -> sequence -> page are resolved, and the
+// grid covers many rows per SM: memory bounds long appends (8,188 rows of 32 + 16 heads of 128 in
+// binary16: 38 us, 5.3 TB/s, 81 % of a copy's rate), the chain of three loads short ones. The
 // rotation is the reference's unfused multiply and add (src/inference_v2.cpp:25) in FP32; k and v are
 // rounded to binary16 once, which is the cache's precision.
 template <typename TI, typename TQ, bool VEC, int R>

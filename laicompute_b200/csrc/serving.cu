@@ -78,10 +78,10 @@ int on_device(int device, F&& f) {
 // reads or writes anything.
 template <typename TI, typename TQ>
 cudaError_t append_launch(bool vec, dim3 grid, int block, cudaStream_t st, const KvAppendParams& p) {
-    return launch_k(!vec                         ? kv_append_kernel<TI, TQ, false, 1>
-                    : grid.x < (unsigned)p.rows ? kv_append_kernel<TI, TQ, true, 2>
-                                                 : kv_append_kernel<TI, TQ, true, 1>,
-                    grid, dim3(block), 0, st, true, p);
+    void (*fn)(KvAppendParams) = vec ? kv_append_kernel<TI, TQ, true, 1> : kv_append_kernel<TI, TQ, false, 1>;
+    if constexpr (sizeof(TI) == 2 && sizeof(TQ) == 2)
+        if (grid.x < (unsigned)p.rows) fn = kv_append_kernel<TI, TQ, true, 2>;
+    return launch_k(fn, grid, dim3(block), 0, st, true, p);
 }
 
 int device_sms(int dev) {
@@ -122,10 +122,10 @@ int resident_clusters(K kernel, int threads, size_t smem, int c, int sms) {
     cudaGetLastError();
     return 0;
 }
-// Of c bulk CTAs (asked once per device; without one, by the SM count).
-int bulk_clusters(int device, int c) {
-    static std::atomic<int> known[64][kBulkMaxCluster + 1];
-    const int guess = device_sms(device) / c;
+// The same, asked once per device and size (`known` of the kernel); where it cannot be, per_sm CTAs on each SM.
+template <typename K>
+int known_clusters(std::atomic<int> (&known)[64][9], K kernel, int threads, size_t smem, int device, int c, int per_sm) {
+    const int guess = per_sm * device_sms(device) / c;
     if (device < 0 || device >= 64) return guess;
     int n = known[device][c].load();
     if (n) return n;
@@ -134,11 +134,20 @@ int bulk_clusters(int device, int c) {
         cudaGetLastError();
         return guess;
     }
-    n = resident_clusters(bulk_pick(128, true), kBulkThreads, bulk_smem(128, true), c, device_sms(device));  // (the largest)
+    n = resident_clusters(kernel, threads, smem, c, device_sms(device));
     if (!n) return guess;
     known[device][c].store(n);
     return n;
 }
+int bulk_clusters(int device, int c) {
+    static std::atomic<int> known[64][9];
+    return known_clusters(known, bulk_pick(128, true), kBulkThreads, bulk_smem(128, true), device, c, 1);  // (the largest)
+}
+int verify_clusters(int device, int c) {
+    static std::atomic<int> known[64][9];
+    return known_clusters(known, verify_kernel<true>, kVerifyThreads, 0, device, c, 2);
+}
+static_assert(kBulkMaxCluster <= 8 && kVerifyMaxCluster <= 8, "known_clusters' tables");
 // ---- attention: how a call is cut into items
 struct AttnPlan {
     int nt = 1;            // column tiles of 8 of a shared item
@@ -153,7 +162,13 @@ struct AttnPlan {
 };
 
 // A group goes to the bulk kernel from this many columns (query rows x heads per kv head) and shared positions on.
-constexpr int kBulkMinCols = 48, kBulkMinShared = 256;
+// Measured on 8 kv heads, 1 to 8 groups, 128 to 8,192 positions, us of the items / of the bulk kernel:
+//   head_dim 64: 24 columns 34 / 42, 28: 54 / 42; with private positions, whose CTAs run beside items but not beside
+//   bulk CTAs (which fill their SM), 32: 58 / 69, 64: 110 / 71;
+//   head_dim 128: 16 columns 47 / 50 (FP32), 20: 60 / 50 and 52 / 37 (binary16);
+//   128 positions: 32 columns 13 / 10 and 14 / 12; 64 positions at head_dim 128: 12 / 14.
+int bulk_min_cols(int head_dim, bool has_private) { return head_dim == 128 ? 20 : has_private ? 40 : 28; }
+constexpr int kBulkMinShared = 128;
 
 int round_up(long long v, int m) { return (int)((v + m - 1) / m * m); }
 
@@ -184,10 +199,12 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
         return std::max(128, std::min(round_up(l, unit), most));
     };
     const int sms = device_sms(g.device);
-    // private: ranges up to kPrWhole by one CTA, which writes the output; longer ones by a warp per split, 8 to 12
-    // on an SM (256 positions: a partial costs 2 % of their bytes, and ragged rows balance; more where the
+    // private: short ranges by one CTA, which writes the output; longer ones by a warp per split, 8 to 12 on an SM (256 positions: a partial costs 2 % of their bytes, and ragged rows balance; more where the
     // bound is far, which would ask for thousands of partials per row)
-    pl.whole = max_private <= kPrWhole;
+    // (a CTA's warps walk a range of 1,024 in 16 to 25 us whatever the rows, splits and their merge take 9 to 14 for
+    // 64 (row, kv head) pairs, but 62 against 45 for 512; they meet near 448 positions, or 370 pairs)
+    const bool many = 2LL * a.rows * g.kv_heads >= 5LL * sms;
+    pl.whole = max_private <= (many ? kPrWhole : 448);
     const int most = std::max(256, std::min(kPrWhole, max_private / 64 / 16 * 16));
     pl.lp = pl.whole ? kPrWhole : split((long long)a.rows * g.kv_heads, max_private, 12LL * sms, 16, 128, most);
     pl.nsp = pl.whole ? 0 : (max_private + pl.lp - 1) / pl.lp;
@@ -195,7 +212,7 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
         if (max_private == 0) pl.whole = false;  // nothing private: shared items alone, joined by the merge
         const int cols = a.max_group_rows * G;
         const long long pool_rows = (long long)g.num_pages * g.kv_heads * g.page_size;
-        pl.bulk = g.head_dim >= 64 && cols >= kBulkMinCols && a.max_shared >= kBulkMinShared && pool_rows <= INT_MAX;
+        pl.bulk = g.head_dim >= 64 && cols >= bulk_min_cols(g.head_dim, max_private > 0) && a.max_shared >= kBulkMinShared && pool_rows <= INT_MAX;
         if (pl.bulk) {
             // about one CTA per SM (a bulk CTA fills one), in whole tiles, as few clusters per set of columns
             // as that allows
@@ -369,8 +386,10 @@ int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t
     const int units = (a.heads + 2 * g.kv_heads) * (g.head_dim / 8);
     p.units = units;
     const int block = std::min(256, (units + 31) / 32 * 32), cta = block * kAppendUnits;
-    // two rows per CTA where there are enough of them to fill the GPU several times over
-    const dim3 grid(vec && a.rows >= 16 * device_sms(g.device) ? (a.rows + 1) / 2 : a.rows, (units + cta - 1) / cta);
+    // two rows per CTA of binary16 in and out from 40 rows per SM on (8,192 rows of 32 + 16 heads of 128: 37.5 us
+    // against 38.5; 4,096: 19.0 against 18.7; FP32 on either side has the bytes in flight with one: 59 against 69)
+    const bool two = vec && bi == 2 && bq == 2 && a.rows >= 40 * device_sms(g.device);
+    const dim3 grid(two ? (a.rows + 1) / 2 : a.rows, (units + cta - 1) / cta);
     if (grid.y > 65535) return api_fail(LAIC_E_UNSUPPORTED, "rows too wide");
     return on_device(g.device, [&]() -> int {
         const bool i32 = a.in_type == LAIC_GGML_F32, q32 = a.q_type == LAIC_GGML_F32;
@@ -463,10 +482,11 @@ int logits_probs(int device, int rows, int vocab, const float* x, long long ldx,
     ProbsParams p{x, y, temp, ldx, ldy, vocab};
     return on_device(device, [&]() -> int {
         const bool vec = aligned16(x) && aligned16(y) && (rows == 1 || (ldx % 4 == 0 && ldy % 4 == 0));
-        // the smallest cluster whose shared memory holds the row; for few rows the largest, to spread them over the SMs
+        // the smallest cluster whose shared memory holds the row; for few rows of some length the largest, to spread
+        // them over the SMs (8 rows of 16,384: 4.4 us against 5.6; of 10,000: 4.3 against 4.5; of 8,192: 4.1 against 3.8)
         int c = 1;
         while (c < 8 && c * kProbsSlice < vocab) c *= 2;
-        if (vocab >= 8 * kProbsThreads && 8LL * rows <= device_sms(device)) c = 8;
+        if (vocab >= 10000 && 8LL * rows <= device_sms(device)) c = 8;
         const bool sm = (long long)c * kProbsSlice >= vocab;
         if (!sm) c = 1;
         const auto fn = sm ? (vec ? probs_kernel<true, true> : probs_kernel<true, false>) : probs_kernel<false, false>;
@@ -494,9 +514,10 @@ int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st) {
     return on_device(device, [&]() -> int {
         const bool vec = aligned16(a.target_dev) && a.ld_target % 4 == 0 &&
                          (!a.draft_dev || (aligned16(a.draft_dev) && a.ld_draft % 4 == 0));
-        // the largest cluster that still runs in one wave (two CTAs per SM)
+        // the largest cluster of which all fit at once (vocabulary 128,256: 32 sequences in clusters of 8, 4, 2 take
+        // 11.6, 13.0, 19.8 us, 36 take 17.9, 14.2, 19.5, 72 take 28, 25, 21)
         int c = kVerifyMaxCluster;
-        while (c > 1 && (long long)a.nseq * c > 2LL * device_sms(device)) c /= 2;
+        while (c > 1 && a.nseq > verify_clusters(device, c)) c /= 2;
         const cudaError_t e = launch_cluster_k(vec ? verify_kernel<true> : verify_kernel<false>, dim3((unsigned)a.nseq * c), dim3(kVerifyThreads), 0, st, true, c, p);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "verify_drafts");
     });
