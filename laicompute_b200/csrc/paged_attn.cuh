@@ -482,11 +482,11 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
 }
 
 constexpr int kPrWarps = 4;
-constexpr int kPrStages = 2;      // 16 positions of K and V each, per warp (three: fewer CTAs per SM, 192 against 187 us)
-constexpr int kPrWhole = 1024;    // private ranges up to this stay whole (and no split is longer)
-// Warps of a CTA: three where a CTA takes a whole row, so that four of head_dim 128 fit an SM.
-__host__ __device__ constexpr int pr_warps(bool whole) { return whole ? 3 : kPrWarps; }
-__host__ __device__ constexpr size_t pr_smem(int D, bool whole) { return (size_t)pr_warps(whole) * kPrStages * 2 * 16 * D * 2; }
+// 16 positions of K and V each, per warp (three: fewer CTAs per SM, 192 us against 187 for 64 rows of 1 to 8,000
+// positions, 8 kv heads of 128)
+constexpr int kPrStages = 2;
+constexpr int kPrWhole = 1024;    // no split is longer, and no range that stays whole
+__host__ __device__ constexpr size_t pr_smem(int D) { return (size_t)kPrWarps * kPrStages * 2 * 16 * D * 2; }
 
 // One row's own positions, every warp on its own ring of 16-position stages.
 // WHOLE: a CTA per [row][kv head], its warps take turns at the blocks of 16 positions; at the end they
@@ -494,8 +494,8 @@ __host__ __device__ constexpr size_t pr_smem(int D, bool whole) { return (size_t
 // Else: a warp per item of [row][kv head][split], no barrier between the warps.
 // PK: FP32 rows of at most four columns, hi parts in columns 0-3, lo parts in 4-7 of the tile.
 template <int D, typename T, bool PK, bool WHOLE>
-__global__ void __launch_bounds__(pr_warps(WHOLE) * 32) paged_private_kernel(const KvAttnParams p) {
-    constexpr int NW = pr_warps(WHOLE);
+__global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAttnParams p) {
+    constexpr int NW = kPrWarps;
     constexpr bool HL = sizeof(T) == 4 && !PK;
     constexpr int HN = HL ? 2 : 1, KS = D / 16, CPR = D / 8, NST = kPrStages;
     constexpr uint32_t STAGE = 2 * 16 * D * 2;

@@ -41,22 +41,29 @@
 
 namespace laic {
 
-constexpr int kBulkCols = 256;        // score columns of a CTA
-constexpr int kBulkThreads = 352;
+// TILES (1 or 2): M tiles of a CTA
+constexpr int kBulkTiles = 2;
+constexpr int kBulkThreads = 352;     // with two; a warpgroup per tile, then loads, then two that multiply
+__host__ __device__ constexpr int bulk_cols(int tiles) { return 128 * tiles; }  // score columns of a CTA
+__host__ __device__ constexpr int bulk_threads(int tiles) { return 128 * tiles + 96; }
 constexpr int kBulkMaxCluster = 8;   // clusters of 1, 2, 4 or 8
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
 
 constexpr int kBulkKeys = 128;        // positions per tile
+constexpr int kBulkEarly = 2;         // ring items loaded before the CTA meets (a box takes 70 to 150 cycles to issue)
 __host__ __device__ constexpr int bulk_slot_bytes(int D) { return kBulkKeys * D * 2; }  // a tile of K or of V
-__host__ __device__ constexpr int bulk_q_bytes(int D, bool f32) { return kBulkCols * D * 2 * (f32 ? 2 : 1); }
-__host__ __device__ constexpr int bulk_slots(int D, bool f32) { return D == 64 ? 6 : f32 ? 3 : 5; }
-__host__ __device__ constexpr int bulk_smem(int D, bool f32) {
-    return bulk_q_bytes(D, f32) + bulk_slots(D, f32) * bulk_slot_bytes(D) + 1024;  // (aligned to 1024)
+__host__ __device__ constexpr int bulk_q_bytes(int D, bool f32, int tiles) { return bulk_cols(tiles) * D * 2 * (f32 ? 2 : 1); }
+// (one tile: room for private items' CTAs on the SM)
+__host__ __device__ constexpr int bulk_slots(int D, bool f32, int tiles) { return D == 64 ? 6 : f32 ? 3 : tiles == 2 ? 5 : 4; }
+__host__ __device__ constexpr int bulk_smem(int D, bool f32, int tiles) {
+    return bulk_q_bytes(D, f32, tiles) + bulk_slots(D, f32, tiles) * bulk_slot_bytes(D) + 1024;  // (aligned to 1024)
 }
 // (at the end the ring and Q hold O's rows and their maxima and sums)
-__host__ __device__ constexpr int bulk_rows_bytes(int D) { return kBulkCols * (D + 4) * 4; }
-static_assert(bulk_smem(64, false) - 1024 >= bulk_rows_bytes(64) + kBulkCols * 8 &&
-              bulk_smem(128, false) - 1024 >= bulk_rows_bytes(128) + kBulkCols * 8, "O's rows fit");
+__host__ __device__ constexpr int bulk_rows_bytes(int D, int tiles) { return bulk_cols(tiles) * (D + 4) * 4; }
+__host__ __device__ constexpr bool bulk_rows_fit(int D, int tiles) {
+    return bulk_smem(D, false, tiles) - 1024 >= bulk_rows_bytes(D, tiles) + bulk_cols(tiles) * 8;
+}
+static_assert(bulk_rows_fit(64, 1) && bulk_rows_fit(64, 2) && bulk_rows_fit(128, 1) && bulk_rows_fit(128, 2), "O's rows fit");
 
 // ---- PTX
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
@@ -129,6 +136,11 @@ __device__ __forceinline__ void tc_loaded(uint32_t* r) {
                        "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
                        "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Shared-memory operand descriptor, 128-byte swizzle: start, strides between core groups (bytes).
@@ -186,7 +198,7 @@ __device__ __forceinline__ void groupless_rows(const KvAttnParams& p) {
     if (!p.direct || blockIdx.x != 0) return;
     const int lane = threadIdx.x & 31;
     const int g0 = max(0, min(p.rows, p.group_rows[0])), g1 = max(g0, min(p.rows, p.group_rows[p.groups]));
-    for (int r = threadIdx.x >> 5; r < p.rows; r += kBulkThreads / 32) {
+    for (int r = threadIdx.x >> 5; r < p.rows; r += blockDim.x / 32) {
         if (r >= g0 && r < g1) continue;
         const RowView v = row_view(p, r, 0);
         if (v.n < 0) continue;
@@ -196,22 +208,22 @@ __device__ __forceinline__ void groupless_rows(const KvAttnParams& p) {
 }
 
 // Grid [group][pair of column tiles][kv head][split], clusters of bulk_cluster consecutive splits.
-template <int D, typename T>
+template <int D, typename T, int TILES>
 __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAttnParams p, const __grid_constant__ CUtensorMap mk,
                                                                      const __grid_constant__ CUtensorMap mv) {
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int HN = F32 ? 2 : 1, NK = kBulkKeys, NS = bulk_slots(D, F32), HALVES = D / 64;
-    constexpr int SLOT = bulk_slot_bytes(D);
+    constexpr int HN = F32 ? 2 : 1, NK = kBulkKeys, NS = bulk_slots(D, F32, TILES), HALVES = D / 64;
+    constexpr int SLOT = bulk_slot_bytes(D), COLS = bulk_cols(TILES), LOADER = 4 * TILES, MMA = LOADER + 1;  // (warps)
     constexpr int QPART = 128 * D * 2;  // one tile's hi or lo part
     extern __shared__ uint8_t dyn[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~(uintptr_t)1023);
-    uint8_t* ring = base + bulk_q_bytes(D, F32);
+    uint8_t* ring = base + bulk_q_bytes(D, F32, TILES);
     __shared__ int page_ids[kBulkMaxSplit / 16 + 2];
     __shared__ uint64_t kv_full[NS], kv_free[NS], s_full[2], p_ready[2][2], pv_half[2], o_done;
     __shared__ uint32_t tmem_at;
     __shared__ volatile int dead;
     __shared__ int lim_max, lim_min;
-    __shared__ float cmul[kBulkCols];
+    __shared__ float cmul[COLS];
     __shared__ uint32_t odd[kBulkMaxSplit / 32];  // positions of the split whose V was not finite in a masked tile
     __shared__ int any_odd;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -230,31 +242,76 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     int r0, r1;
     const int glen = p.group_len[g];
     if (!group_rows(p, g, r0, r1)) r1 = r0;
-    const int ncol = (r1 - r0) * p.G, col0 = pair * kBulkCols;
+    const int ncol = (r1 - r0) * p.G, col0 = pair * COLS;
     if (col0 >= ncol) {  // (alike for all CTAs of a cluster)
         groupless_rows<D, T>(p);
         return;
     }
     const int t0 = split * p.ls;
     const int shared = max(0, kv_clamp_len(p, glen, p.max_shared));
-    const int tiles = ncol - col0 > 128 ? 2 : 1;  // M tiles with columns
+    const int tiles = TILES == 2 && ncol - col0 > 128 ? 2 : 1;  // M tiles with columns
 
     // ---- a softmax thread's column and how far it sees
     const int wg = warp >> 2, col = col0 + tid;
-    const bool live = tid < kBulkCols && col < ncol;
+    const bool live = tid < COLS && col < ncol;
     const int base_row = col0 / p.G, base_head = col0 - base_row * p.G;  // of the pair's first column
     // column cw of the pair: its row and query head (cw + base_head < 2^9: the product by 2^16 / G rounds right)
     auto row_of = [&](int cw) { return (int)((uint32_t)(cw + base_head) * p.g_inv >> 16); };
     const int my_row = row_of(live ? tid : 0);
-    const int rr = r0 + base_row + my_row, hh = kvh * p.G + (live ? tid : 0) + base_head - my_row * p.G;
-    const RowView view = row_view(p, rr, shared);
-    if (live && split == 0 && view.n - view.shared > p.max_private) kv_flag(p.err, kKvBadPos);
-    const int lim = live ? max(0, view.shared) : 0;
-    int seq = row_seq(p, r0);
-    if (seq < 0) seq = 0;  // (recorded) reads some sequence's pages
+    const int rr = r0 + base_row + my_row;
+    const int my_len = p.len[rr], my_seq = p.seq ? p.seq[rr] : rr;  // under way while Q is loaded
     const int first_page = t0 >> p.page_shift;
-    const int npages = min(((t0 + p.ls - 1) >> p.page_shift) + 1, p.pages_per_seq) - first_page;
-    for (int k = tid; k < npages; k += kBulkThreads) page_ids[k] = p.table[(size_t)seq * p.pages_per_seq + first_page + k];
+
+    // ring item m: K of tile m / 2, then its V; a lane per box: (piece of the tile, half of the row)
+    auto slot = [&](int m) { return smem_u32(ring) + (uint32_t)(m % NS * SLOT); };
+    auto load = [&](int m, int t1) {
+        const int box = min(1 << p.page_shift, NK), half = lane % HALVES, k = lane / HALVES * box, s = m % NS;
+        if (lane == 0) mbar_expect_tx(&kv_full[s], SLOT);
+        __syncwarp();
+        if (lane < NK / box * HALVES) {
+            const int t = t0 + (m >> 1) * NK + k;
+            int id = 0;  // past the last position seen: any page (masked, and cleared in V)
+            if (t < t1) {
+                id = page_ids[(t >> p.page_shift) - first_page];
+                if (id < 0 || id >= p.num_pages) {
+                    kv_flag(p.err, kKvBadPage);
+                    id = 0;
+                }
+            }
+            const int y = ((id * p.kv_heads + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
+            tma_2d(slot(m) + half * (NK * 128) + k * 128, m & 1 ? &mv : &mk, half * 64, y, &kv_full[s]);
+        }
+    };
+    if (warp == LOADER) {  // the first loads, while the others bring Q: the chain lengths -> sequence -> pages is its own
+        if (lane == 0) {
+            for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], F32 ? tiles : 1); }
+            for (int w = 0; w < 2; ++w) {
+                mbar_init(&s_full[w], 1);
+                mbar_init(&pv_half[w], 1);
+                for (int h = 0; h < 2; ++h) mbar_init(&p_ready[w][h], 128);
+            }
+            mbar_init(&o_done, F32 ? tiles : 1);
+            mbar_fence_init();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        const int first_seq = row_seq(p, r0);
+        // (rows that see nothing do not keep the others' tiles from being whole)
+        int hi = 0, lo = 0x7fffffff;
+        for (int k = lane; k <= row_of(min(COLS, ncol - col0) - 1); k += 32) {
+            const int n = row_view(p, r0 + base_row + k, shared).shared;
+            if (n > 0) { hi = max(hi, n); lo = min(lo, n); }
+        }
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        const int seq = max(0, first_seq);  // (a bad one is recorded, and reads some sequence's pages)
+        const int npages = min(((t0 + p.ls - 1) >> p.page_shift) + 1, p.pages_per_seq) - first_page;
+        for (int k = lane; k < npages; k += 32) page_ids[k] = p.table[(size_t)seq * p.pages_per_seq + first_page + k];
+        if (lane == 0) { lim_max = hi; lim_min = lo; }
+        __syncwarp();
+        const int t1 = min(hi, t0 + p.ls), items = t0 < t1 ? 2 * ((t1 - t0 + NK - 1) / NK) : 0;
+        for (int m = 0; m < min(kBulkEarly, items); ++m) load(m, t1);
+    }
+    if (warp == MMA) tc_alloc(smem_u32(&tmem_at), 256 * TILES);
 
     // ---- Q in 128-byte swizzled rows
     auto q_at = [&](int cw) {  // row of q of the pair's column cw
@@ -266,8 +323,9 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         return base + (size_t)(cw >> 7) * HN * QPART + (ch >> 3) * (128 * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
     };
     constexpr int CH = D / 8;  // chunks per row
-    if constexpr (!F32) {
-        for (int k = tid; k < tiles * 128 * CH; k += kBulkThreads) {
+    if (warp >= LOADER) {
+    } else if constexpr (!F32) {
+        for (int k = tid; k < tiles * 128 * CH; k += COLS) {
             const int cw = k / CH, ch = k % CH;
             const bool in = col0 + cw < ncol;
             if (p.q_vec) {
@@ -279,12 +337,12 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 *reinterpret_cast<uint4*>(q_dst(cw, ch)) = *reinterpret_cast<const uint4*>(x);
             }
         }
-        if (tid < kBulkCols) cmul[tid] = p.scale_log2;
+        cmul[tid] = p.scale_log2;
         cp_async_commit();
         cp_async_wait_all();
     } else if (warp < 4 * tiles) {
-        // a warp takes 32 columns, CH lanes a row; four steps' loads in flight
-        constexpr int RPI = 32 / CH, STEPS = 32 / RPI, B = 4;
+        // a warp takes 32 columns, CH lanes a row; eight steps' loads in flight
+        constexpr int RPI = 32 / CH, STEPS = 32 / RPI, B = 8;
         const int sub = lane / CH, ch = lane % CH;
 #pragma unroll 1
         for (int it0 = 0; it0 < STEPS; it0 += B) {
@@ -335,79 +393,44 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     if (tid == 0) {
-        for (int s = 0; s < NS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_free[s], F32 ? tiles : 1); }
-        for (int w = 0; w < 2; ++w) {
-            mbar_init(&s_full[w], 1);
-            mbar_init(&pv_half[w], 1);
-            for (int h = 0; h < 2; ++h) mbar_init(&p_ready[w][h], 128);
-        }
-        mbar_init(&o_done, F32 ? tiles : 1);
-        mbar_fence_init();
         dead = 0;
         any_odd = 0;
-        lim_max = 0;
-        lim_min = 0x7fffffff;
     }
     if (tid < kBulkMaxSplit / 32) odd[tid] = 0;
-    __syncthreads();
-    if (warp < 8) {  // (rows that see nothing do not keep the others' tiles from being whole)
-        const int hi = __reduce_max_sync(0xffffffffu, lim);
-        const int lo = __reduce_min_sync(0xffffffffu, lim > 0 ? lim : 0x7fffffff);
-        if (lane == 0) { atomicMax(&lim_max, hi); atomicMin(&lim_min, lo); }
-    }
-    __syncthreads();
-    const int t1 = min(lim_max, t0 + p.ls), seen_by_all = lim_min;
-    const int nt = t0 < t1 ? (t1 - t0 + NK - 1) / NK : 0;  // 0: no column sees this far
-    float* rows = reinterpret_cast<float*>(base);           // at the end: O's rows, [column][D + 4]
-    float2* row_ml = reinterpret_cast<float2*>(base + bulk_rows_bytes(D));  // (m, l); l -1: padding
-    if (nt > 0) {
-    if (warp == 9) tc_alloc(smem_u32(&tmem_at), 512);
+    const RowView view = row_view(p, my_len, my_seq, shared);
+    if (live && split == 0 && view.n - view.shared > p.max_private) kv_flag(p.err, kKvBadPos);
+    const int lim = live ? max(0, view.shared) : 0;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     pdl_launch_dependents();  // the private items need nothing of this kernel
     const uint32_t tmem = tmem_at;
+    const int t1 = min(lim_max, t0 + p.ls), seen_by_all = lim_min;
+    const int nt = t0 < t1 ? (t1 - t0 + NK - 1) / NK : 0;  // 0: no column sees this far
+    float* rows = reinterpret_cast<float*>(base);           // at the end: O's rows, [column][D + 4]
+    float2* row_ml = reinterpret_cast<float2*>(base + bulk_rows_bytes(D, TILES));  // (m, l); l -1: padding
+    if (nt > 0) {
     // S; then, in the place of each half of its positions, P hi (32 columns) and P lo (32)
     auto s_at = [&](int w) { return tmem + (uint32_t)(w * NK); };
-    auto o_at = [&](int w) { return tmem + 256u + (uint32_t)(w * D); };
+    auto o_at = [&](int w) { return tmem + (uint32_t)(TILES * NK + w * D); };
 
-    // ring item m: K of tile m / 2, then its V
-    auto slot = [&](int m) { return smem_u32(ring) + (uint32_t)(m % NS * SLOT); };
     auto full = [&](int m) { return bulk_wait(&kv_full[m % NS], (uint32_t)(m / NS) & 1, &dead, p.err); };
 
-    if (warp == 8) {
-        // a lane per box: (piece of the tile, half of the row)
-        const int box = min(1 << p.page_shift, NK), boxes = NK / box * HALVES;
-        const int half = lane % HALVES, k = lane / HALVES * box;
-        int m = 0;
+    if (warp == LOADER) {
+        int m = min(kBulkEarly, 2 * nt);  // (these are under way)
         for (; m < 2 * nt; ++m) {
-            const int s = m % NS;
-            const bool ok = m < NS || bulk_wait(&kv_free[s], (uint32_t)(m / NS - 1) & 1, &dead, p.err);
+            const bool ok = m < NS || bulk_wait(&kv_free[m % NS], (uint32_t)(m / NS - 1) & 1, &dead, p.err);
             if (!__all_sync(0xffffffffu, ok)) break;
-            if (lane == 0) mbar_expect_tx(&kv_full[s], SLOT);
-            __syncwarp();
-            if (lane < boxes) {
-                const int t = t0 + (m >> 1) * NK + k;
-                int id = 0;  // past the last position seen: any page (masked, and cleared in V)
-                if (t < t1) {
-                    id = page_ids[(t >> p.page_shift) - first_page];
-                    if (id < 0 || id >= p.num_pages) {
-                        kv_flag(p.err, kKvBadPage);
-                        id = 0;
-                    }
-                }
-                const int y = ((id * p.kv_heads + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1));
-                tma_2d(slot(m) + half * (NK * 128) + k * 128, m & 1 ? &mv : &mk, half * 64, y, &kv_full[s]);
-            }
+            load(m, t1);
         }
         if (lane == 0 && dead)  // copies still in flight land before the CTA's memory is given up
             for (int q = max(0, m - NS); q < m; ++q) {
                 const long long since = clock64();
                 while (!mbar_try_wait(&kv_full[q % NS], (uint32_t)(q / NS) & 1) && clock64() - since < 200000000LL) {}
             }
-    } else if (warp >= 9) {
-        // the column tiles this warp multiplies for: FP32, one each for warps 9 and 10; binary16, warp 9 both in turn
-        const int w0 = F32 ? warp - 9 : 0, w1 = F32 ? min(w0 + 1, tiles) : warp == 9 ? tiles : 0;
+    } else if (warp >= MMA) {
+        // the column tiles this warp multiplies for: FP32, one each; binary16, the first warp both in turn
+        const int w0 = F32 ? warp - MMA : 0, w1 = F32 ? min(w0 + 1, tiles) : warp == MMA ? tiles : 0;
         if (lane == 0 && w0 < w1) {
             constexpr uint32_t iqk = umma_idesc(NK, false), ipv = umma_idesc(D, true);
             auto qk = [&](int w, int j) {
@@ -496,11 +519,11 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             }
             uint64_t sum2[2] = {0, 0};
             const uint64_t cm2 = f2_pack(cm, cm), gain2 = f2_pack(kPaGain, kPaGain);
+            uint32_t s[64];
+            tc_ld32(S, s);
+            tc_ld32(S + 32, s + 32);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {  // halves of 64 positions, each with its own look at the maximum
-                uint32_t s[64];
-                tc_ld32(S + h * 64, s);
-                tc_ld32(S + h * 64 + 32, s + 32);
                 tc_wait_ld();
                 tc_loaded(s);
                 tc_loaded(s + 32);
@@ -511,8 +534,8 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 }
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < 64; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * cm;
+                for (int e = 0; e < 64; e += 2) mx4[(e >> 1) & 3] = max3(mx4[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+                const float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * cm;
                 if (j == 0 && h == 0) {
                     mref = mx > -INFINITY ? mx : 0.f;
                 } else if (__any_sync(0xffffffffu, mx > mref + kPaSlack)) {
@@ -564,6 +587,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                     }
                     tc_st16(S + h * 64 + k / 2, hi);
                     if constexpr (F32) tc_st16(S + h * 64 + 32 + k / 2, lo);
+                    if (h == 0) tc_ld32(S + 64 + k, s + k);  // the second half's scores take the used ones' registers
                 }
                 tc_wait_st();
                 tc_fence_before();
@@ -608,14 +632,14 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     }
     __syncwarp();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == MMA) {
         if (lane == 0) bulk_wait(&o_done, 0, &dead, p.err);
         __syncwarp();
         tc_fence_after();
-        tc_dealloc(tmem, 512);
+        tc_dealloc(tmem, 256 * TILES);
     }
     } else {
-        pdl_launch_dependents();
+        if (warp == MMA) tc_dealloc(tmem, 256 * TILES);
         if (tid < 128 * tiles) row_ml[tid] = make_float2(-INFINITY, live && view.n < 0 ? -1.f : 0.f);
     }
     // ---- join the cluster's splits: CTA `rank` takes every C-th block of rows, a warp a row at a time
@@ -623,7 +647,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     if (C > 1) cluster.sync();
     else __syncthreads();
     constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp and step
-    const int ns = p.nss + p.nsp, slot_at = split / C, cols = min(kBulkCols, ncol - col0);
+    const int ns = p.nss + p.nsp, slot_at = split / C, cols = min(COLS, ncol - col0);
     auto join = [&](auto cc) {
         constexpr int CC = decltype(cc)::value, U = 8 / CC;  // U rows at a time: eight loads in flight
         const float* far_rows[CC];
@@ -635,7 +659,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         }
         constexpr int STEP = RPW * CC;
         const int e0 = lane % LPR * 4;
-        for (int r = (warp * U * CC + rank) * RPW; r < cols; r += (kBulkThreads / 32) * U * STEP) {
+        for (int r = (warp * U * CC + rank) * RPW; r < cols; r += (bulk_threads(TILES) / 32) * U * STEP) {
             float2 ml[U][CC];
             float4 v[U][CC];
 #pragma unroll

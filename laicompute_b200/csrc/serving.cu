@@ -99,10 +99,12 @@ int device_sms(int dev) {
 }
 
 using BulkFn = void (*)(KvAttnParams, CUtensorMap, CUtensorMap);
-BulkFn bulk_pick(int D, bool f32) {
-    if (D == 64) return f32 ? paged_bulk_kernel<64, float> : paged_bulk_kernel<64, __half>;
-    return f32 ? paged_bulk_kernel<128, float> : paged_bulk_kernel<128, __half>;
+template <int TILES>
+BulkFn bulk_fn(int D, bool f32) {
+    if (D == 64) return f32 ? paged_bulk_kernel<64, float, TILES> : paged_bulk_kernel<64, __half, TILES>;
+    return f32 ? paged_bulk_kernel<128, float, TILES> : paged_bulk_kernel<128, __half, TILES>;
 }
+BulkFn bulk_pick(int D, bool f32, int tiles) { return tiles == 1 ? bulk_fn<1>(D, f32) : bulk_fn<2>(D, f32); }
 
 // Clusters of c CTAs of a kernel that are resident at once on the current device, 0 where that cannot be asked.
 template <typename K>
@@ -139,9 +141,9 @@ int known_clusters(std::atomic<int> (&known)[64][9], K kernel, int threads, size
     known[device][c].store(n);
     return n;
 }
-int bulk_clusters(int device, int c) {
+int bulk_clusters(int device, int c) {  // (the largest's: a CTA takes an SM's tensor memory or shared memory)
     static std::atomic<int> known[64][9];
-    return known_clusters(known, bulk_pick(128, true), kBulkThreads, bulk_smem(128, true), device, c, 1);  // (the largest)
+    return known_clusters(known, bulk_pick(128, true, 2), bulk_threads(2), bulk_smem(128, true, 2), device, c, 1);
 }
 int verify_clusters(int device, int c) {
     static std::atomic<int> known[64][9];
@@ -155,6 +157,7 @@ struct AttnPlan {
     int ls = 64, nss = 0, ctiles = 0;
     int shared_items = 0, private_items = 0;
     bool bulk = false;     // the shared items run in paged_bulk.cuh,
+    int mt = 1;            // M tiles per CTA there
     int cluster = 1;       // this many splits of a set of columns in a cluster (nss counts clusters)
     bool whole = false;    // a CTA per row and kv head finishes the row
     bool direct = false;   // the bulk kernel's clusters do
@@ -199,30 +202,32 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
         return std::max(128, std::min(round_up(l, unit), most));
     };
     const int sms = device_sms(g.device);
-    // private: short ranges by one CTA, which writes the output; longer ones by a warp per split, 8 to 12 on an SM (256 positions: a partial costs 2 % of their bytes, and ragged rows balance; more where the
-    // bound is far, which would ask for thousands of partials per row)
-    // (a CTA's warps walk a range of 1,024 in 16 to 25 us whatever the rows, splits and their merge take 9 to 14 for
-    // 64 (row, kv head) pairs, but 62 against 45 for 512; they meet near 448 positions, or 370 pairs)
+    // private: short ranges by one CTA, which writes the output; longer ones by a warp per split, 8 to 12 on an SM
+    // (256 positions: a partial costs 2 % of their bytes, and ragged rows balance; more where the bound is far,
+    // which would ask for thousands of partials per row).
+    // A CTA's warps walk a range of 1,024 in 16 to 25 us whatever the rows; splits and their merge take 9 to 14 for
+    // 64 (row, kv head) pairs, but 62 against 45 for 512: they meet near 448 positions, or 370 pairs.
     const bool many = 2LL * a.rows * g.kv_heads >= 5LL * sms;
+    const int cols = a.max_group_rows * G;
+    pl.bulk = a.groups && g.head_dim >= 64 && cols >= bulk_min_cols(g.head_dim, max_private > 0) &&
+              a.max_shared >= kBulkMinShared && (long long)g.num_pages * g.kv_heads * g.page_size <= INT_MAX;
     pl.whole = max_private <= (many ? kPrWhole : 448);
     const int most = std::max(256, std::min(kPrWhole, max_private / 64 / 16 * 16));
     pl.lp = pl.whole ? kPrWhole : split((long long)a.rows * g.kv_heads, max_private, 12LL * sms, 16, 128, most);
     pl.nsp = pl.whole ? 0 : (max_private + pl.lp - 1) / pl.lp;
     if (a.groups) {
         if (max_private == 0) pl.whole = false;  // nothing private: shared items alone, joined by the merge
-        const int cols = a.max_group_rows * G;
-        const long long pool_rows = (long long)g.num_pages * g.kv_heads * g.page_size;
-        pl.bulk = g.head_dim >= 64 && cols >= bulk_min_cols(g.head_dim, max_private > 0) && a.max_shared >= kBulkMinShared && pool_rows <= INT_MAX;
         if (pl.bulk) {
             // about one CTA per SM (a bulk CTA fills one), in whole tiles, as few clusters per set of columns
             // as that allows
-            pl.ctiles = (cols + kBulkCols - 1) / kBulkCols;
+            pl.mt = cols <= 128 ? 1 : kBulkTiles;
+            pl.ctiles = (cols + bulk_cols(pl.mt) - 1) / bulk_cols(pl.mt);
             const long long sets = (long long)a.groups * pl.ctiles * g.kv_heads;
-            const long long most = std::max(1LL, (a.max_shared + 2LL * kBulkKeys - 1) / (2 * kBulkKeys));  // two tiles each
+            const long long splits = std::max(1LL, (a.max_shared + 2LL * kBulkKeys - 1) / (2 * kBulkKeys));  // two tiles each
             int best = 1, count = 1;
             for (int c = kBulkMaxCluster; c >= 1; c /= 2) {
-                const long long fit = std::min(bulk_clusters(g.device, c) / sets, (most + c - 1) / c);
-                if (c <= 2 * most && fit * c > (long long)best * count) {
+                const long long fit = std::min(bulk_clusters(g.device, c) / sets, (splits + c - 1) / c);
+                if (c <= 2 * splits && fit * c > (long long)best * count) {
                     best = c;
                     count = (int)fit;
                 }
@@ -234,8 +239,8 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
             pl.nt = cols <= 24 ? (cols + 7) / 8 : 4;
             pl.ctiles = (cols + 8 * pl.nt - 1) / (8 * pl.nt);
             pl.ls = split((long long)a.groups * pl.ctiles * g.kv_heads, a.max_shared, 4LL * sms, kPaChunk, 256, 512);
+            pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
         }
-        if (!pl.bulk) pl.nss = (a.max_shared + pl.ls - 1) / pl.ls;
     }
     const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss * pl.cluster;
     const long long pi = (long long)a.rows * g.kv_heads * (pl.whole ? 1 : pl.nsp);
@@ -323,13 +328,15 @@ cudaError_t serving_set_attributes() {
     for (int D : {32, 64, 128})
         for (bool whole : {false, true})
             for (PaFn fn : {pr_pick(D, LAIC_GGML_F16, 1, whole), pr_pick(D, LAIC_GGML_F32, 4, whole), pr_pick(D, LAIC_GGML_F32, 8, whole)}) {
-                e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pr_smem(D, whole));
+                e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pr_smem(D));
                 if (e != cudaSuccess) return e;
             }
     for (int D : {64, 128})
         for (bool f32 : {false, true}) {
-            e = cudaFuncSetAttribute(bulk_pick(D, f32), cudaFuncAttributeMaxDynamicSharedMemorySize, bulk_smem(D, f32));
-            if (e != cudaSuccess) return e;
+            for (int mt = 1; mt <= kBulkTiles; ++mt) {
+                e = cudaFuncSetAttribute(bulk_pick(D, f32, mt), cudaFuncAttributeMaxDynamicSharedMemorySize, bulk_smem(D, f32, mt));
+                if (e != cudaSuccess) return e;
+            }
         }
     for (auto fn : {probs_kernel<true, true>, probs_kernel<true, false>}) {
         e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kProbsSlice * 4);
@@ -453,7 +460,7 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
             CUtensorMap mk, mv;
             if (!encode_pages(g, g.k_dev, &mk) || !encode_pages(g, g.v_dev, &mv))
                 return api_fail(LAIC_E_CUDA, "kv_attention: tensor map");
-            e = launch_cluster_k(bulk_pick(g.head_dim, f32), dim3(pl.shared_items), dim3(kBulkThreads), bulk_smem(g.head_dim, f32),
+            e = launch_cluster_k(bulk_pick(g.head_dim, f32, pl.mt), dim3(pl.shared_items), dim3(bulk_threads(pl.mt)), bulk_smem(g.head_dim, f32, pl.mt),
                                  st, true, pl.cluster, p, mk, mv);
         }
         if (e == cudaSuccess && !pl.bulk && pl.shared_items)
@@ -461,8 +468,8 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
                          pa_smem(g.head_dim, pl.nt, f32), st, true, p);
         if (e == cudaSuccess && pl.private_items)
             e = launch_k(pr_pick(g.head_dim, a.type, p.G, pl.whole),
-                         dim3(pl.whole ? pl.private_items : (pl.private_items + kPrWarps - 1) / kPrWarps), dim3(pr_warps(pl.whole) * 32),
-                         pr_smem(g.head_dim, pl.whole), st, true, p);
+                         dim3(pl.whole ? pl.private_items : (pl.private_items + kPrWarps - 1) / kPrWarps), dim3(kPrWarps * 32),
+                         pr_smem(g.head_dim), st, true, p);
         if (e == cudaSuccess && !pl.direct && !pl.whole)
             e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
                          dim3((unsigned)(a.rows * a.heads)), dim3(kPmWarps * 32), 0,
