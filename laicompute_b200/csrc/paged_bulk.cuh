@@ -1,24 +1,30 @@
 // Shared positions of wide groups on the 5th-generation tensor cores.
 //
 // A group with many columns (rows x query heads of one KV head) makes its attention a pair of dense
-// products: S = Q K^T and O += P V over 256 columns per CTA, two tiles of M = 128, and a split of the
-// group's positions in tiles of bulk_keys.
+// products: S = Q K^T and O += P V over one or two tiles of M = 128 columns per CTA (two from 129 columns
+// on: one tile's softmax then runs under the other's products) and a split of the group's positions, 128
+// at a time.
 //
-// Roles: warp 8 loads (TMA boxes of up to a page, 128-byte swizzle, a lane per box: one lane alone
-// took 125 cycles a box, 4,000 for a tile of 16-position pages; a ring of K and V tiles); warps 9 and
-// 10 multiply (one lane each: tcgen05.mma, S and O in tensor memory, P read from tensor memory, where
-// it takes S's place); warps 0-3 and 4-7 each own a tile, a thread a column: they read S, keep the
-// running maximum and sum, and write P in two halves, so that PV starts on the first.
+// Roles: a warpgroup per tile, a thread a column: it reads S, keeps the running maximum and sum, and
+// writes P in two halves, so that PV starts on the first; a warp that loads (TMA boxes of up to a page,
+// 128-byte swizzle, a lane per box: one lane alone took 125 cycles a box, 4,000 for a tile of 16-position
+// pages; a ring of K and V tiles; its first loads start while the others bring Q); two warps that
+// multiply (one lane each: tcgen05.mma, S and O in tensor memory, P read from tensor memory, where
+// it takes S's place).
 // Binary16 rows, where a tile's exponentials take longer than its products: one lane multiplies for
-// both tiles in turn, which keeps one tile's products under the other's exponentials (attn of 512
-// prompt rows behind 1,537: 39.0 us; a lane per tile let them fall into step, 41.0). FP32 rows, with
-// twice the products: a lane per tile (64 rows behind 4,101 shared positions: 44.0 us against 48.6).
+// both tiles in turn, which keeps one tile's products under the other's exponentials (512 prompt rows
+// behind 1,537 positions, 32 heads over 8 of 128: 39.0 us; a lane per tile let them fall into step, 41.0).
+// FP32 rows, with twice the products: a lane per tile (64 rows behind 4,101 shared positions: 44.0 us
+// against 48.6).
 // 128 positions per tile: a product of N = 64 takes about as long as one of N = 128 (100 against 85
 // cycles), and two score buffers of 64 ran slower than one of 128. O is rescaled only when a maximum
 // grew by more than 2^8 since the last time (weights stay below 2^15 in binary16 with the factor 2^7
 // they carry). Both tiles' S and O fill the 512 columns of tensor memory. What bounds it: the chain
-// softmax -> PV -> QK of a tile (about 4,000 cycles a pair of 128-position tiles, 2,000 of them
-// exponentials at 16 a clock), and, for few tiles per CTA, set-up and the join.
+// softmax -> PV -> QK of a tile (4,200 cycles a pair of 128-position tiles in binary16, of which
+// the exponentials fill 2,048 at 16 a clock and the 32 products 2,700; 3,200 for one tile alone), and, for few tiles per CTA,
+// the way to the first scores (7,000 to 11,000 cycles: Q for every CTA out of L2) and the join (8,000
+// over a cluster's shared memory at about 14 bytes a clock). 512 prompt rows behind 1,537 positions:
+// 37 us, 404 TFLOP/s; 64 FP32 rows over 4,101 shared positions: 16 to 22 us of the call's 41.
 //
 // The splits of a set of columns form a thread-block cluster and join through distributed shared
 // memory: one partial per cluster goes to global memory, or the output itself where the cluster holds
