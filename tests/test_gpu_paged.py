@@ -500,6 +500,35 @@ def test_rows_of_no_group(dtype):
     close(out[rows], ref, tol)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("heads,hkv,d", [(8, 2, 64), (8, 2, 128), (7, 1, 128), (10, 2, 64)])
+@pytest.mark.parametrize("cols", [20, 28, 40, 124, 128, 132, 256, 260])
+def test_widths_around_the_tiles(cols, heads, hkv, d, dtype):
+    """Widths at the kernels' thresholds and tiles' ends, causal (no private positions) and with private ones."""
+    n = max(1, cols // (heads // hkv))
+    cache = Cache([330] * n, hkv, d, 32, seed=cols, shared=[(list(range(n)), 300)])
+    q = _q(n, heads, d, dtype, seed=cols)
+    rows = sorted({0, n // 3, n // 2, n - 1})
+    for lens in ([300 - (n - 1 - r) for r in range(n)], [301 + (r * 7) % 29 for r in range(n)]):
+        out = attend(cache, q, lens, groups=([0, n], [300]))
+        cache.pages().check()
+        ref, tol = reference(cache, q[rows], [lens[r] for r in rows], rows)
+        close(out[rows], ref, tol)
+
+
+@pytest.mark.parametrize("n,length", [(3, 448), (3, 449), (3, 1024), (60, 448), (60, 1024), (60, 1025)])
+def test_private_ranges_around_the_split(n, length):
+    """Few and many rows whose ranges end at and behind what one CTA takes, ragged."""
+    lens = [max(1, length - (37 * r) % length) for r in range(n)]
+    cache = Cache(lens, 8, 64, 64, seed=n)
+    q = _q(n, 16, 64, F32, seed=length)
+    out = attend(cache, q, lens)
+    cache.pages().check()
+    rows = sorted({0, 1, n // 2, n - 1})
+    ref, tol = reference(cache, q[rows], [lens[r] for r in rows], rows)
+    close(out[rows], ref, tol)
+
+
 def test_long_bounds_and_many_groups():
     """A bound far above the lengths (its splits are empty), and a group per pair of rows."""
     n = 40
