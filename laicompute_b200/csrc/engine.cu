@@ -72,6 +72,19 @@ int laic::api_fail(int code, const std::string& msg) { return fail(code, msg); }
 
 namespace {
 
+// Device memory set before work on a non-blocking stream uses it: cudaMemset, and a cudaMemcpy from pageable
+// memory, may return with the transfer still queued on the legacy stream, for which such a stream does not wait.
+int zero_now(void* p, size_t bytes) {
+    CK(cudaMemset(p, 0, bytes));
+    CK(cudaStreamSynchronize(cudaStreamLegacy));
+    return LAIC_OK;
+}
+int copy_now(void* dst, const void* src, size_t bytes) {
+    CK(cudaMemcpy(dst, src, bytes, cudaMemcpyHostToDevice));
+    CK(cudaStreamSynchronize(cudaStreamLegacy));
+    return LAIC_OK;
+}
+
 using laic::T_F16;
 using laic::T_F32;
 using laic::T_Q4_0;
@@ -153,11 +166,11 @@ int mat_alloc(Mat& m, int type, int rows, int in) {
     m.type = type; m.rows = rows; m.in = in; m.nb = in / 32; m.ntiles = (rows + 15) / 16;
     const size_t qbytes = (size_t)m.ntiles * m.nb * laic::tile_qbytes(type);
     CK(cudaMalloc(&m.q, qbytes));
-    CK(cudaMemset(m.q, 0, qbytes));
+    if (int rc = zero_now(m.q, qbytes)) return rc;
     if (type != T_F16) {
         const size_t sbytes = (size_t)m.ntiles * m.nb * laic::kTileSBytes;
         CK(cudaMalloc(&m.s, sbytes));
-        CK(cudaMemset(m.s, 0, sbytes));
+        if (int rc = zero_now(m.s, sbytes)) return rc;
     }
     return LAIC_OK;
 }
@@ -371,7 +384,7 @@ int mv_scratch_reserve(MvScratch& sc, const MvNeed& need, bool* moved = nullptr)
     bool mv = false;
     if (!sc.err) {
         CK(cudaMalloc(&sc.err, 4));
-        CK(cudaMemset(sc.err, 0, 4));
+        if (int rc = zero_now(sc.err, 4)) return rc;
     }
     if (need.part_floats > sc.part_cap) {
         if (sc.part) cudaFree(sc.part);
@@ -384,7 +397,7 @@ int mv_scratch_reserve(MvScratch& sc, const MvNeed& need, bool* moved = nullptr)
         if (sc.tile_cnt) cudaFree(sc.tile_cnt);
         sc.tile_cnt = nullptr;
         CK(cudaMalloc(&sc.tile_cnt, need.ntiles * 4));
-        CK(cudaMemset(sc.tile_cnt, 0, need.ntiles * 4));
+        if (int rc = zero_now(sc.tile_cnt, need.ntiles * 4)) return rc;
         sc.cnt_cap = need.ntiles;
         mv = true;
     }
@@ -853,16 +866,16 @@ struct laic_dev {
         const int nmax = S * h;
         CK(cudaMalloc(&ar_box, (size_t)2 * tp * nmax * 4));
         CK(cudaMalloc(&ar_flags, (size_t)2 * tp * laic::kArCtas * 4));
-        CK(cudaMemset(ar_flags, 0, (size_t)2 * tp * laic::kArCtas * 4));
+        if (int rc = zero_now(ar_flags, (size_t)2 * tp * laic::kArCtas * 4)) return rc;
         CK(cudaMalloc(&ar_ctr, 8));
-        CK(cudaMemset(ar_ctr, 0, 8));
+        if (int rc = zero_now(ar_ctr, 8)) return rc;
         cudaIpcMemHandle_t hd[2];
         CK(cudaIpcGetMemHandle(&hd[0], ar_box));
         CK(cudaIpcGetMemHandle(&hd[1], ar_flags));
         const size_t hb = sizeof hd;
         void* dev = nullptr;
         CK(cudaMalloc(&dev, hb * (tp + 1)));
-        CK(cudaMemcpy((char*)dev + hb * tp, hd, hb, cudaMemcpyHostToDevice));
+        if (int rc = copy_now((char*)dev + hb * tp, hd, hb)) return rc;
         const laic::ncclResult_t r = nccl->AllGather((char*)dev + hb * tp, dev, hb / 4, laic::ncclFloat32, comm, st);
         if (r != laic::ncclSuccess) { cudaFree(dev); return fail(LAIC_E_NCCL, std::string("ncclAllGather: ") + nccl->GetErrorString(r)); }
         std::vector<cudaIpcMemHandle_t> all(2 * tp);
@@ -1172,7 +1185,7 @@ struct laic_dev {
         }
         ls_free();
         CK(cudaMalloc(&ls_layers, sizeof(laic::LsLayer) * L));
-        CK(cudaMemcpy(ls_layers, tab.data(), sizeof(laic::LsLayer) * L, cudaMemcpyHostToDevice));
+        if (int rc = copy_now(ls_layers, tab.data(), sizeof(laic::LsLayer) * L)) return rc;
         const int Gc = num_sms();
         const int cp = laic::ls_positions_per_chunk(D);
         const int gm = G <= 1 ? 1 : G <= 2 ? 2 : G <= 4 ? 4 : 8;
@@ -1190,7 +1203,7 @@ struct laic_dev {
             const size_t tb = ((size_t)Gc * laic::ls_phases(L) * laic::ls_trace_stamps() +
                                (size_t)Gc * laic::ls_trace_warp_words()) * 8;
             CK(cudaMalloc(&ls_trace, tb));
-            CK(cudaMemset(ls_trace, 0, tb));
+            CK(cudaMemsetAsync(ls_trace, 0, tb, st));
         }
         if (int rc = ls_reset()) return rc;
         ls_type = type;
@@ -1206,9 +1219,9 @@ struct laic_dev {
     // step whose bounded waits ran out and may have left them part-way).
     int ls_reset() {
         if (!ls_done) return LAIC_OK;
-        CK(cudaMemset(ls_head_tick, 0, (size_t)Hkv * 4));
-        CK(cudaMemset(ls_done, 0, ls_done_bytes));
-        CK(cudaMemset(ls_epoch, 0, 8));
+        CK(cudaMemsetAsync(ls_head_tick, 0, (size_t)Hkv * 4, st));
+        CK(cudaMemsetAsync(ls_done, 0, ls_done_bytes, st));
+        CK(cudaMemsetAsync(ls_epoch, 0, 8, st));
         return LAIC_OK;
     }
 
@@ -1447,7 +1460,7 @@ int upload_norm(float** dst, int type, const void* data, size_t n, size_t nbytes
         }
     }
     if (!*dst) CK(cudaMalloc(dst, n * 4));
-    CK(cudaMemcpy(*dst, v.data(), n * 4, cudaMemcpyHostToDevice));
+    if (int rc = copy_now(*dst, v.data(), n * 4)) return rc;
     return LAIC_OK;
 }
 
@@ -1543,8 +1556,8 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     if (!d->paged) {
         CK(cudaMalloc(&d->kc, kv_bytes));
         CK(cudaMalloc(&d->vc, kv_bytes));
-        CK(cudaMemset(d->kc, 0, kv_bytes));
-        CK(cudaMemset(d->vc, 0, kv_bytes));
+        if (int rc = zero_now(d->kc, kv_bytes)) return rc;
+        if (int rc = zero_now(d->vc, kv_bytes)) return rc;
     } else {
         CK(laic::serving_set_attributes());
         if (int rc = mv_scratch_reserve(d->mvs, MvNeed{})) return rc;  // the error word, which the pages' kernels share
@@ -1565,7 +1578,7 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
         CK(cudaMalloc(&d->qkv, RB * (d->hq + 2 * d->kv) * 4));
     }
     CK(cudaMalloc(&d->pos, S * 4));
-    CK(cudaMemset(d->pos, 0, S * 4));
+    if (int rc = zero_now(d->pos, S * 4)) return rc;
     if (d->tile_step(S) || d->tp == 1) {  // activation records between the projections
         CK(cudaMalloc(&d->rec_x, RB * d->h * 4));
         CK(cudaMalloc(&d->rec_act, RB * d->F * 4));
@@ -1573,7 +1586,7 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
         CK(cudaMalloc(&d->rec_ss, RB * ((d->h + 15) / 16) * 4));
     }
     CK(cudaMalloc(&d->counts, S * d->V * 4));
-    CK(cudaMemset(d->counts, 0, S * d->V * 4));
+    if (int rc = zero_now(d->counts, S * d->V * 4)) return rc;
 
     // RoPE table with the reference's float arithmetic (src/inference_v2.cpp:25):
     // a = float(pos) * pow(theta, -float(i)/float(head_dim)), (cos a, sin a)
@@ -1586,22 +1599,23 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
             cs[(size_t)p * d->rope_pairs + j] = make_float2(std::cos(ang), std::sin(ang));
         }
     CK(cudaMalloc(&d->rope_cs, std::max<size_t>(1, cs.size()) * sizeof(float2)));
-    if (!cs.empty()) CK(cudaMemcpy(d->rope_cs, cs.data(), cs.size() * sizeof(float2), cudaMemcpyHostToDevice));
+    if (!cs.empty())
+        if (int rc = copy_now(d->rope_cs, cs.data(), cs.size() * sizeof(float2))) return rc;
 
     d->max_split = std::max(1, std::min(64, (cap + 31) / 32));
     CK(cudaMalloc(&d->attn_part, S * d->Hkv * d->max_split * d->G * (D + 2) * 4));
     CK(cudaMalloc(&d->attn_cnt, S * d->Hkv * 4));
-    CK(cudaMemset(d->attn_cnt, 0, S * d->Hkv * 4));
+    if (int rc = zero_now(d->attn_cnt, S * d->Hkv * 4)) return rc;
 
     CK(cudaMalloc(&d->d_tokens, RB * 4));
     CK(cudaMalloc(&d->d_out_ids, S * 4));
     CK(cudaMalloc(&d->d_slots, RB * 4));
     CK(cudaMalloc(&d->d_err, 4));
-    CK(cudaMemset(d->d_err, 0, 4));
+    if (int rc = zero_now(d->d_err, 4)) return rc;
     CK(cudaMalloc(&d->samp_v, S * laic::kSampleSlices * 4));
     CK(cudaMalloc(&d->samp_i, S * laic::kSampleSlices * 4));
     CK(cudaMalloc(&d->samp_cnt, S * 4));
-    CK(cudaMemset(d->samp_cnt, 0, S * 4));
+    if (int rc = zero_now(d->samp_cnt, S * 4)) return rc;
     CK(cudaMalloc(&d->d_hist_count, 4));
     CK(cudaMalloc(&d->d_params, S * sizeof(laic::SampleDev)));
     CK(cudaMallocHost(&d->h_tokens, RB * 4));
@@ -1853,13 +1867,13 @@ static std::string wait_error_text(int code) {
 static int check_step_err(laic_dev* d, int buf = 0) {
     const int mv_err = d->h_err[2 * buf], sample_err = d->h_err[2 * buf + 1];
     if (mv_err) {
-        CK(cudaMemset(d->mvs.err, 0, 4));
+        CK(cudaMemsetAsync(d->mvs.err, 0, 4, d->st));
         d->h_err[2 * buf] = 0;
         if (int rc = d->ls_reset()) return rc;
         return fail(LAIC_E_CUDA, wait_error_text(mv_err));
     }
     if (sample_err) {
-        CK(cudaMemset(d->d_err, 0, 4));
+        CK(cudaMemsetAsync(d->d_err, 0, 4, d->st));
         d->h_err[2 * buf + 1] = 0;
         return fail(LAIC_E_UNSUPPORTED, "sampling request needs more than 1024 candidates (top_k or top_p mass)");
     }
@@ -1871,14 +1885,14 @@ static int check_sampler_err(laic_dev* d) {
     if (d->mvs.err) {
         CK(cudaMemcpy(&err, d->mvs.err, 4, cudaMemcpyDeviceToHost));
         if (err) {
-            CK(cudaMemset(d->mvs.err, 0, 4));
+            CK(cudaMemsetAsync(d->mvs.err, 0, 4, d->st));
             if (int rc = d->ls_reset()) return rc;
             return fail(LAIC_E_CUDA, wait_error_text(err));
         }
     }
     CK(cudaMemcpy(&err, d->d_err, 4, cudaMemcpyDeviceToHost));
     if (err) {
-        CK(cudaMemset(d->d_err, 0, 4));
+        CK(cudaMemsetAsync(d->d_err, 0, 4, d->st));
         return fail(LAIC_E_UNSUPPORTED, "sampling request needs more than 1024 candidates (top_k or top_p mass)");
     }
     return LAIC_OK;
@@ -1956,8 +1970,8 @@ int laic_dev_reset_slot(laic_dev* d, int32_t slot) {
     if (int rc_ = d->spec_cancel()) return rc_;  // (a pending speculative step assumed the old state)
     CK(cudaStreamSynchronize(d->st));
     if (d->paged) d->drop_slot(slot);
-    CK(cudaMemset(d->pos + slot, 0, 4));
-    CK(cudaMemset(d->counts + (size_t)slot * d->V, 0, (size_t)d->V * 4));
+    CK(cudaMemsetAsync(d->pos + slot, 0, 4, d->st));
+    CK(cudaMemsetAsync(d->counts + (size_t)slot * d->V, 0, (size_t)d->V * 4, d->st));
     d->h_pos[slot] = 0;
     return LAIC_OK;
 }
@@ -2486,8 +2500,10 @@ int laic_tensor_check(laic_tensor* t, void* stream) {
     unsigned char* base = nullptr;
     if (int rc = fixed_scratch_base(t->device, &base)) return rc;
     CK(cudaMemcpy(&fixed, base, 4, cudaMemcpyDeviceToHost));
-    if (own) CK(cudaMemset(t->sc.err, 0, 4));
-    if (fixed) CK(cudaMemset(base, 0, 4));
+    if (own)
+        if (int rc = zero_now(t->sc.err, 4)) return rc;
+    if (fixed)
+        if (int rc = zero_now(base, 4)) return rc;
     if (own || fixed) return fail(LAIC_E_CUDA, wait_error_text(own ? own : fixed));
     return LAIC_OK;
 }
