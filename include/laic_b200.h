@@ -162,9 +162,10 @@ LAIC_API int laic_dev_fork_slot(laic_dev* dev, int32_t src, int32_t dst);
  * (nseq * (max_draft + 1) <= 64), and laic_verify_drafts decides on the drafted ones with the target's
  * probabilities softmax(logits / temperature) (temperature <= 0: the first maximum) and numbers from
  * mt19937_64(seed). draft_probs_dev: device memory [nseq][max_draft][vocab] the drafts were drawn from, or NULL
- * (drafted with certainty). out_ids [nseq][max_draft + 1] receives the tokens that follow, out_n how many; the
- * last one is not in the cache yet. Positions advance by out_n. top_k, top_p and repeat_penalty must be off. No
- * counterpart in the reference. */
+ * (drafted with certainty); they are read behind what the legacy default stream holds at the call, and behind a
+ * stream given to laic_dev_wait_stream before. out_ids [nseq][max_draft + 1] receives the tokens that follow, out_n
+ * how many; the last one is not in the cache yet. Positions advance by out_n. top_k, top_p and repeat_penalty must
+ * be off. No counterpart in the reference. */
 LAIC_API int laic_dev_verify(laic_dev* dev, int32_t nseq, const int32_t* slots, int32_t max_draft, const uint32_t* tokens,
                              const int32_t* n_draft, const float* draft_probs_dev, const laic_sample_params* params,
                              int32_t nparams, uint32_t* out_ids, int32_t* out_n);
@@ -288,6 +289,12 @@ LAIC_API int laic_selftest_peer_timeout(int32_t device, int64_t spin_cycles, int
  * host. */
 LAIC_API int laic_tensor_matvec_noalloc(laic_tensor* t, const float* x_dev, float* y_dev, int32_t batch,
                                         void* stream);
+
+/* What the engine does from now on runs behind the work that `stream` (cudaStream_t of the engine's device, not
+ * under capture; NULL: the legacy default stream) holds at this call, on the device: the engine's own stream waits
+ * for no other by itself. For device memory that another stream writes, as laic_dev_verify's draft_probs_dev. No
+ * counterpart in the reference. */
+LAIC_API int laic_dev_wait_stream(laic_dev* dev, void* stream);
 
 /* ---- serving: a KV cache in pages, attention over it, drafted tokens -------
  * No counterpart in the reference, which holds one sequence's cache in host

@@ -26,7 +26,7 @@ EXPORTS = (
     "laic_dev_prefill_batch", "laic_tensor_check", "laic_selftest_peer_timeout",
     "laic_dev_step_trace", "laic_blocks_convert",
     "laic_kv_append", "laic_kv_attention", "laic_kv_attention_workspace", "laic_kv_check", "laic_logits_probs",
-    "laic_verify_drafts", "laic_dev_fork_slot", "laic_dev_verify",
+    "laic_verify_drafts", "laic_dev_fork_slot", "laic_dev_verify", "laic_dev_wait_stream",
 )
 
 
@@ -141,6 +141,7 @@ def lib() -> ctypes.CDLL:
     L.laic_selftest_peer_timeout.argtypes = [I32, ctypes.c_int64, ctypes.POINTER(I32)]
     L.laic_blocks_convert.argtypes = [I32, P, U64, ctypes.c_uint32, ctypes.POINTER(I32), P, U64, ctypes.POINTER(U64)]
     L.laic_dev_fork_slot.argtypes = [P, I32, I32]
+    L.laic_dev_wait_stream.argtypes = [P, P]
     L.laic_dev_verify.argtypes = [P, I32, P, I32, P, P, P, ctypes.POINTER(SampleParams), I32, P, P]
     KP = ctypes.POINTER(KvPagesDesc)
     I64 = ctypes.c_int64
@@ -151,7 +152,8 @@ def lib() -> ctypes.CDLL:
     L.laic_logits_probs.argtypes = [I32, I32, I32, P, I64, P, P, I64, P]
     L.laic_verify_drafts.argtypes = [I32, ctypes.POINTER(VerifyArgs), P]
     for name in ("laic_kv_append", "laic_kv_attention", "laic_kv_attention_workspace", "laic_kv_check",
-                 "laic_logits_probs", "laic_verify_drafts", "laic_dev_fork_slot", "laic_dev_verify", "laic_dev_create", "laic_dev_upload", "laic_dev_prefill", "laic_dev_step", "laic_dev_reset_slot",
+                 "laic_logits_probs", "laic_verify_drafts", "laic_dev_fork_slot", "laic_dev_verify", "laic_dev_wait_stream",
+                 "laic_dev_create", "laic_dev_upload", "laic_dev_prefill", "laic_dev_step", "laic_dev_reset_slot",
                  "laic_dev_slot_pos", "laic_dev_fill_kv", "laic_dev_sync", "laic_dev_stats_get",
                  "laic_dev_decode", "laic_dev_profile", "laic_nccl_unique_id", "laic_tensor_create", "laic_tensor_matvec",
                  "laic_tensor_dequant", "laic_tensor_matvec_noalloc", "laic_dev_prefill_batch", "laic_tensor_check",

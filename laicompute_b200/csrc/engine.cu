@@ -661,8 +661,19 @@ struct laic_dev {
     unsigned* vf_ids = nullptr;  // drafted ids [nseq][max_draft], then out ids [nseq][max_draft + 1]
     int* vf_n = nullptr;         // drafted counts, then out counts
     const float* vf_draft = nullptr;
+    cudaEvent_t other_ev = nullptr;  // laic_dev_wait_stream
     int vf_nseq = 0, vf_max = 0;
 
+    // `st` goes on behind what `other` holds now.
+    int wait_stream(cudaStream_t other) {
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        CK(cudaStreamIsCapturing(other, &cap));
+        if (cap != cudaStreamCaptureStatusNone) return fail(LAIC_E_INVALID, "the stream is being captured");
+        if (!other_ev) CK(cudaEventCreateWithFlags(&other_ev, cudaEventDisableTiming));
+        CK(cudaEventRecord(other_ev, other));
+        CK(cudaStreamWaitEvent(st, other_ev, 0));
+        return LAIC_OK;
+    }
     // The whole-page prefix that two slots' page tables share, in pages.
     int common_pages(int a, int b) const {
         int n = 0;
@@ -1647,6 +1658,7 @@ void laic_dev_destroy(laic_dev* d) {
     cudaSetDevice(d->device);
     cudaStreamSynchronize(d->st);
     for (cudaEvent_t ev : d->spec_ev) if (ev) cudaEventDestroy(ev);
+    if (d->other_ev) cudaEventDestroy(d->other_ev);
     d->drop_graphs();  // graphs holding NCCL calls go first
     for (int q = 0; q < d->tp && d->ar_p2p; ++q) {
         if (q == d->tr) continue;
@@ -2094,7 +2106,8 @@ static int verify_step(laic_dev* d, int32_t nseq, const int32_t* slots, int32_t 
     CK(cudaMemcpyAsync(d->vf_n, nd.data(), nseq * 4, cudaMemcpyHostToDevice, st));
     d->kb = b;
     d->vf_nseq = nseq; d->vf_max = max_draft; d->vf_draft = draft_probs_dev;
-    int rc = d->reserve_attn_ws(rows, b);
+    int rc = draft_probs_dev ? d->wait_stream(nullptr) : LAIC_OK;
+    if (!rc) rc = d->reserve_attn_ws(rows, b);
     if (!rc) rc = d->run(rows, MODE_VERIFY);
     if (rc) { cudaStreamSynchronize(st); return rc; }
     std::vector<uint32_t> got(rows);
@@ -2135,6 +2148,14 @@ extern "C" {
 
 int laic_dev_fork_slot(laic_dev* d, int32_t src, int32_t dst) {
     return no_throw([&] { return fork_slot(d, src, dst); });
+}
+
+int laic_dev_wait_stream(laic_dev* d, void* stream) {
+    return no_throw([&]() -> int {
+        if (!d) return fail(LAIC_E_INVALID, "null device");
+        CK(cudaSetDevice(d->device));
+        return d->wait_stream((cudaStream_t)stream);
+    });
 }
 
 int laic_dev_verify(laic_dev* d, int32_t nseq, const int32_t* slots, int32_t max_draft, const uint32_t* tokens,

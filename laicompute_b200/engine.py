@@ -113,9 +113,14 @@ class Engine:
         """Slot dst becomes a copy of slot src, sharing its whole pages (engines with paged=True)."""
         check(lib().laic_dev_fork_slot(self.h, src, dst))
 
-    def verify(self, tokens, n_draft, slots=None, params=None, draft_probs: int = 0):
+    def wait_stream(self, stream: int) -> None:
+        """What the engine does from now on runs behind what `stream` (cudaStream_t) holds now."""
+        check(lib().laic_dev_wait_stream(self.h, stream))
+
+    def verify(self, tokens, n_draft, slots=None, params=None, draft_probs: int = 0, stream: int = 0):
         """One speculative step (engines with paged=True): tokens [nseq][1 + max_draft], each row the next token
-        and then n_draft[i] drafted ones; draft_probs: device pointer [nseq][max_draft][vocab] or 0. Returns
+        and then n_draft[i] drafted ones; draft_probs: device pointer [nseq][max_draft][vocab] or 0, read behind
+        what `stream` (where they are written; 0: the legacy default stream) holds at the call. Returns
         (ids [nseq][1 + max_draft], counts): the tokens that follow, counts[i] of them valid."""
         t = np.ascontiguousarray(np.atleast_2d(tokens), dtype=np.uint32)
         n = np.ascontiguousarray(np.atleast_1d(n_draft), dtype=np.int32)
@@ -123,6 +128,8 @@ class Engine:
         s = np.arange(nseq, dtype=np.int32) if slots is None else np.ascontiguousarray(np.atleast_1d(slots), np.int32)
         if len(n) != nseq or len(s) != nseq:
             raise ValueError("one n_draft and slot per row of tokens")
+        if draft_probs and stream:
+            self.wait_stream(stream)
         arr = self._params(params, nseq)
         ids, cnt = np.zeros((nseq, m1), dtype=np.uint32), np.zeros(nseq, dtype=np.int32)
         check(lib().laic_dev_verify(self.h, nseq, s.ctypes.data, m1 - 1, t.ctypes.data, n.ctypes.data, draft_probs, arr,
