@@ -4,7 +4,7 @@ drafted tokens (``laic_kv_*``, ``laic_logits_probs``, ``laic_verify_drafts`` of 
 
 As in ``engine.Matrix``, pointers are plain integers (``tensor.data_ptr()``) and ``stream`` a
 ``cudaStream_t``; calls return when their kernels are queued. A plan holds a call's shape, so that a
-loop passes only its pointers.
+loop passes only its pointers; threads may call one plan at once, each with outputs and a workspace of its own.
 """
 from __future__ import annotations
 
@@ -50,14 +50,14 @@ class AppendPlan:
                                  ldq=ldq or heads * d.head_dim, ldk=ldk or kvw, ldv=ldv or kvw,
                                  ldqo=ldqo or heads * d.head_dim)
         self._call = lib().laic_kv_append
-        self._refs = ctypes.byref(d), ctypes.byref(self.args)
+        self._desc = ctypes.byref(d)
 
     def __call__(self, q: int, k: int, v: int, q_out: int, pos: int, table: int, rope: int = 0, seq: int = 0,
                  stream: int = 0) -> None:
-        a = self.args
+        a = KvAppendArgs.from_buffer_copy(self.args)  # this call's own: another thread may be in one of its own
         a.q_dev, a.k_dev, a.v_dev, a.q_out_dev = q, k, v, q_out
         a.pos_dev, a.page_table_dev, a.rope_dev, a.seq_dev = pos, table, rope, seq
-        rc = self._call(*self._refs, stream)
+        rc = self._call(self._desc, ctypes.byref(a), stream)
         if rc:
             check(rc)
 
@@ -77,17 +77,17 @@ class AttentionPlan:
                                     max_len=max_len, groups=groups, max_group_rows=max_group_rows, max_shared=max_shared,
                                     max_private=max_private, scale=scale, ldq=ldq or w, ldo=ldo or w)
         self._call = lib().laic_kv_attention
-        self._refs = ctypes.byref(pages.desc), ctypes.byref(self.args)
+        self._desc = ctypes.byref(pages.desc)
         n = ctypes.c_uint64()
-        check(lib().laic_kv_attention_workspace(*self._refs, ctypes.byref(n)))
+        check(lib().laic_kv_attention_workspace(self._desc, ctypes.byref(self.args), ctypes.byref(n)))
         self.workspace_bytes = self.args.workspace_bytes = int(n.value)
 
     def __call__(self, q: int, out: int, lens: int, table: int, workspace: int = 0, seq: int = 0, group_rows: int = 0,
                  group_len: int = 0, stream: int = 0) -> None:
-        a = self.args
+        a = KvAttentionArgs.from_buffer_copy(self.args)  # this call's own: another thread may be in one of its own
         a.q_dev, a.out_dev, a.len_dev, a.page_table_dev, a.workspace_dev = q, out, lens, table, workspace
         a.seq_dev, a.group_rows_dev, a.group_len_dev = seq, group_rows, group_len
-        rc = self._call(*self._refs, stream)
+        rc = self._call(self._desc, ctypes.byref(a), stream)
         if rc:
             check(rc)
 
