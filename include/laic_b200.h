@@ -351,7 +351,7 @@ typedef struct laic_kv_attention_args {
     int32_t type;             /* of q and out: LAIC_GGML_F32 (products to 22 bits of q and of the weights) or
                                  LAIC_GGML_F16 (weights rounded to binary16) */
     int32_t nseq, pages_per_seq;
-    int32_t max_len;          /* bound on len_dev */
+    int32_t max_len;          /* bound on len_dev (as max_shared, at most 1,073,000,000) */
     int32_t groups;           /* groups of rows that share their first positions (0: none) */
     int32_t max_group_rows, max_shared; /* bounds on the groups' rows and shared lengths */
     int32_t max_private;      /* bound on a row's positions beyond its group's shared ones (-1: max_len) */

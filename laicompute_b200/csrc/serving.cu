@@ -175,6 +175,9 @@ constexpr int kBulkMinShared = 128;
 
 int round_up(long long v, int m) { return (int)((v + m - 1) / m * m); }
 
+constexpr int kMaxPositions = 1073000000;
+static_assert(2LL * kMaxPositions + 16 * kBulkMaxCluster * kBulkMaxSplit <= INT_MAX, "positions past a row's end stay within an int");
+
 int check_attention(const laic_kv_pages& g, const laic_kv_attention_args& a) {
     if (int rc = check_pages(g)) return rc;
     if (a.rows < 0) return api_fail(LAIC_E_INVALID, "rows must be >= 0");
@@ -185,6 +188,9 @@ int check_attention(const laic_kv_pages& g, const laic_kv_attention_args& a) {
     if (a.max_len < 0 || a.groups < 0 || a.max_private < -1) return api_fail(LAIC_E_INVALID, "negative bound");
     if (a.groups && (a.max_group_rows < 1 || a.max_shared < 0 || a.max_group_rows > a.rows))
         return api_fail(LAIC_E_INVALID, "groups need max_group_rows in [1, rows] and max_shared >= 0");
+    // (a shared length, a private one and a split added up stay within 32 bits)
+    if (a.max_len > kMaxPositions || (a.groups && a.max_shared > kMaxPositions))
+        return api_fail(LAIC_E_UNSUPPORTED, "max_len and max_shared must not exceed 1,073,000,000 positions");
     const long long cap = (long long)a.pages_per_seq * g.page_size;
     if (a.max_len > cap || (a.groups && a.max_shared > cap))
         return api_fail(LAIC_E_INVALID, "max_len and max_shared must not exceed pages_per_seq * page_size");

@@ -1,0 +1,32 @@
+"""Far bounds of an attention call (no GPU): what would leave the kernels' 32-bit positions is refused."""
+import pytest
+
+from test_serving_refusals import UNSUPPORTED, _pages, _refused
+
+MOST = 1073000000
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_far_bounds_are_refused_or_planned(page):
+    per_seq = (2 ** 31 - 1) // page
+    far = per_seq * page
+    pages = _pages(page_size=page, kv_heads=1)
+    grouped = dict(groups=1, max_group_rows=1)
+    for kw in (dict(max_len=far), dict(max_len=MOST + 1), dict(max_len=100, max_shared=far, **grouped),
+               dict(max_len=far, max_shared=64, max_private=10, **grouped)):
+        _refused(UNSUPPORTED, "1,073,000,000", lambda: pages.attention_plan(1, 1, 1, per_seq, **kw))
+    for kw in (dict(max_len=MOST), dict(max_len=MOST, max_shared=MOST, **grouped), dict(max_len=MOST, max_shared=64, **grouped)):
+        plan = pages.attention_plan(1, 1, 1, per_seq, **kw)
+        # a partial of 64 + 2 floats for every split of each bound: neither negative nor wrapped
+        most = 2 * (MOST // 128 + 1) * 66 * 4
+        assert 0 < plan.workspace_bytes <= most
+
+
+def test_positions_of_far_bounds_stay_within_an_int():
+    """The largest start of a private split, as the kernel adds it up, and its end."""
+    i32 = lambda x: (x + 2 ** 31) % 2 ** 32 - 2 ** 31  # noqa: E731
+    for split in (128, 1024, 2048 * 8):
+        last = (MOST + split - 1) // split - 1
+        for shared in (0, 1, MOST):
+            assert i32(shared + last * split) >= 0 and i32(shared + MOST) >= 0
+        assert i32(MOST + split) >= 0 and i32(MOST + split - 1) >= 0
