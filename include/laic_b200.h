@@ -372,9 +372,9 @@ typedef struct laic_kv_attention_args {
 /* out[r] = softmax(scale * q[r] . K) V over the row's first len_dev[r] positions,
  * query head h with kv head h / (heads / kv_heads). The rows of group g hold the
  * same keys and values in positions [0, group_len_dev[g]): the kernels read them
- * once, through the page table row of the group's first row. Rows that share a
- * whole sequence with causal lengths (a prompt's tokens, drafted tokens) are a
- * group whose length is the longest. Masked positions never reach a row's output,
+ * once, through the page table row of the group's first row that sees any. Rows that
+ * share a whole sequence with causal lengths (a prompt's tokens, drafted tokens) are
+ * a group whose length is the longest. Masked positions never reach a row's output,
  * whatever they hold. out_dev must not overlap an input. Two calls with the same
  * inputs give the same bits. */
 LAIC_API int laic_kv_attention(const laic_kv_pages* pages, const laic_kv_attention_args* args, void* stream);

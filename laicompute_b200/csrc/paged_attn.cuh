@@ -103,12 +103,6 @@ __host__ __device__ inline int kv_clamp_len(const KvAttnParams& p, int n, int bo
     }
     return n;
 }
-__host__ __device__ inline int row_seq(const KvAttnParams& p, int r) {
-    const int s = p.seq ? p.seq[r] : r;
-    if (s >= 0 && s < p.nseq) return s;
-    kv_flag(p.err, kKvBadSeq);
-    return -1;
-}
 // Rows [r0, r1) of group g, false (and recorded) where they are not within the call's rows and bounds.
 __host__ __device__ inline bool group_rows(const KvAttnParams& p, int g, int& r0, int& r1) {
     r0 = p.group_rows[g];
@@ -118,6 +112,20 @@ __host__ __device__ inline bool group_rows(const KvAttnParams& p, int g, int& r0
         return false;
     }
     return true;
+}
+// The page table row through which the group of rows [r0, r1) is read: that of its first row that sees any
+// position (padding may name any sequence, and one that sees nothing need hold nothing). A bad one is recorded, and
+// reads some sequence's pages.
+__host__ __device__ inline int group_seq(const KvAttnParams& p, int r0, int r1) {
+    int n = p.len[r0], s = p.seq ? p.seq[r0] : r0;  // (under way together: the first row mostly sees something)
+    for (int r = r0 + 1; n <= 0 && r < r1; ++r) {
+        n = p.len[r];
+        s = p.seq ? p.seq[r] : r;
+    }
+    if (n <= 0) return 0;  // nothing is read
+    if (s >= 0 && s < p.nseq) return s;
+    kv_flag(p.err, kKvBadSeq);
+    return 0;
 }
 // Shared positions of group g.
 __host__ __device__ inline int group_shared(const KvAttnParams& p, int g) {
@@ -842,8 +850,7 @@ __device__ __forceinline__ void shared_item(const KvAttnParams& p, int i, int* l
     __syncthreads();
     const int t0 = split * p.ls, t1 = min(range[0], t0 + p.ls);
     if (t0 >= t1) return;  // no row of the tile sees this far
-    const int seq = max(0, row_seq(p, r0));  // (a bad one is recorded, and reads some sequence's pages)
-    pa_item<D, NT, T>(p, r0, col0, ncol, kvh, seq, t0, t1, split, lim, range[1], page_ids, cmul, smem);
+    pa_item<D, NT, T>(p, r0, col0, ncol, kvh, group_seq(p, r0, r1), t0, t1, split, lim, range[1], page_ids, cmul, smem);
 }
 
 // Grid: the shared items.

@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             mbar_fence_init();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        const int first_seq = row_seq(p, r0);
+        const int seq = group_seq(p, r0, r1);
         // (rows that see nothing do not keep the others' tiles from being whole)
         int hi = 0, lo = 0x7fffffff;
         for (int k = lane; k <= row_of(min(COLS, ncol - col0) - 1); k += 32) {
@@ -309,7 +309,6 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         }
         hi = __reduce_max_sync(0xffffffffu, hi);
         lo = __reduce_min_sync(0xffffffffu, lo);
-        const int seq = max(0, first_seq);  // (a bad one is recorded, and reads some sequence's pages)
         const int npages = min(((t0 + p.ls - 1) >> p.page_shift) + 1, p.pages_per_seq) - first_page;
         for (int k = lane; k < npages; k += 32) page_ids[k] = p.table[(size_t)seq * p.pages_per_seq + first_page + k];
         if (lane == 0) { lim_max = hi; lim_min = lo; }
