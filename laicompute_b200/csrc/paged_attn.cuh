@@ -160,6 +160,10 @@ __host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int sh
     return row_view(p, p.len[r], p.seq ? p.seq[r] : r, shared);
 }
 
+// The maximum that an item reports beside its sum: a column all of whose scores are NaN has none, but its sum (NaN)
+// has to reach the row.
+__device__ __forceinline__ float seen_max(float m, float sum) { return m == -INFINITY && sum != sum ? 0.f : m; }
+
 // Elements e and e + 1 (e even) of query row r.
 template <typename T>
 __device__ __forceinline__ float2 q_pair(const KvAttnParams& p, int r, int e) {
@@ -449,6 +453,7 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             v += __shfl_xor_sync(0xffffffffu, v, 8);
             v += __shfl_xor_sync(0xffffffffu, v, 16);
             l_[nt][h] = v * kPaGain;
+            m_[nt][h] = seen_max(m_[nt][h], v);
         }
 
     // ---- join the warps (the ring holds their outputs now)
@@ -721,6 +726,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
             x += __shfl_xor_sync(0xffffffffu, x, 8);
             x += __shfl_xor_sync(0xffffffffu, x, 16);
             l_[h] = x * kPaGain;
+            m_[h] = seen_max(m_[h], x);
         }
     }
     const int ns = p.nss + p.nsp;
