@@ -164,6 +164,28 @@ __host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int sh
 // has to reach the row.
 __device__ __forceinline__ float seen_max(float m, float sum) { return m == -INFINITY && sum != sum ? 0.f : m; }
 
+// A value that is not finite reaches the rows that see it whatever its weight. The products may make NaN of an
+// infinite one (a weight rounded to zero, or its lo part's zero or sign), so where an output is NaN and its weights'
+// sum is not, it is the sum of the values of dimension d that are not finite, at the positions [t0, t1) whose block
+// of 16 is the `first` of every `stride`; x where there is none. (Out of line: the usual call never comes here.)
+__device__ __noinline__ float odd_values(const __half* vp, const int* page_ids, int page_shift, int kv_heads, int kvh, int D,
+                                         int d, int t0, int t1, int first, int stride, float x) {
+    const int a0 = t0 & ~15, first_page = t0 >> page_shift;
+    float sum = 0.f;
+    bool any = false;
+    for (int t = t0; t < t1; ++t) {
+        if (((t - a0) >> 4) % stride != first) continue;
+        const int page = page_ids[(t >> page_shift) - first_page];
+        const float v = __half2float(vp[((((size_t)page * kv_heads + kvh) << page_shift) + (t & ((1 << page_shift) - 1))) * D + d]);
+        if (fabsf(v) <= 65504.f) continue;
+        sum += v;
+        any = true;
+    }
+    return any ? sum : x;
+}
+// The weight of an item against the largest maximum of its row, kept above zero: an infinite output stays one.
+__device__ __forceinline__ float item_weight(float m, float top) { return fmaxf(ex2(m - top), 0x1p-126f); }
+
 // Elements e and e + 1 (e even) of query row r.
 template <typename T>
 __device__ __forceinline__ float2 q_pair(const KvAttnParams& p, int r, int e) {
@@ -419,6 +441,13 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
             } else {
                 const __half* V = reinterpret_cast<const __half*>(smem + (size_t)(ch % NST) * (2 * kPaChunk * D * 2) +
                                                                   kPaChunk * D * 2);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {  // (a weight that is seen is not zero)
+                        const int at = pos + (e >> 1) * 8;
+                        if (at < lm[nt][e & 1] && at >= t0) s[nt][e] = fmaxf(s[nt][e], 0x1p-126f);
+                    }
 #pragma unroll 1
                 for (int i = 0; i < 16; ++i) {
 #pragma unroll
@@ -483,13 +512,19 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
         float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
-            w[k] = cm[k][col] == -INFINITY ? 0.f : ex2(cm[k][col] - M);
+            w[k] = cm[k][col] == -INFINITY ? 0.f : item_weight(cm[k][col], M);
             L = fmaf(cl[k][col], w[k], L);
             if (w[k] != 0.f) {
                 const float4 v = *reinterpret_cast<const float4*>(red + ((size_t)k * NC + col) * (D + 4) + d);
                 A.x = fmaf(v.x, w[k], A.x); A.y = fmaf(v.y, w[k], A.y);
                 A.z = fmaf(v.z, w[k], A.z); A.w = fmaf(v.w, w[k], A.w);
             }
+        }
+        if (A.x + A.y + A.z + A.w != A.x + A.y + A.z + A.w && L == L) {
+            auto seen = [&](float x, int k) {
+                return x == x ? x : odd_values(p.vp, page_ids, p.page_shift, p.kv_heads, kvh, D, d + k, t0, min(t1, lim[col]), 0, 1, x);
+            };
+            A = make_float4(seen(A.x, 0), seen(A.y, 1), seen(A.z, 2), seen(A.w, 3));
         }
         const int r = r0 + cc / p.G, h = kvh * p.G + cc % p.G;
         const size_t at = ((size_t)r * p.heads + h) * ns + slot;
@@ -729,6 +764,10 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
             m_[h] = seen_max(m_[h], x);
         }
     }
+    auto seen = [&](float x, int h, int d) {  // column h's output, where a product made NaN of it
+        return x == x || l_[h] != l_[h] ? x
+                                        : odd_values(p.vp, page_ids[warp], p.page_shift, p.kv_heads, kvh, D, d, t0, t1, first, STRIDE, x);
+    };
     const int ns = p.nss + p.nsp;
     if constexpr (!WHOLE) {
         if (nb > 0) {
@@ -743,7 +782,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                     for (int k = 0; k < 2; ++k) {
                         float x = o[mt][2 * k + h];
                         if (PK) x += __shfl_xor_sync(0xffffffffu, x, 2);
-                        if (mine) p.part_o[at * D + mt * 16 + gq + 8 * k] = x;
+                        if (mine) p.part_o[at * D + mt * 16 + gq + 8 * k] = seen(x, h, mt * 16 + gq + 8 * k);
                     }
                 if (mine && gq == 0) p.part_ml[at] = make_float2(m_[h], l_[h]);
             }
@@ -763,7 +802,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                 for (int k = 0; k < 2; ++k) {
                     float x = o[mt][2 * k + h];
                     if (PK) x += __shfl_xor_sync(0xffffffffu, x, 2);
-                    if (mine) red[((size_t)warp * 8 + col) * (D + 4) + mt * 16 + gq + 8 * k] = x;
+                    if (mine) red[((size_t)warp * 8 + col) * (D + 4) + mt * 16 + gq + 8 * k] = seen(x, h, mt * 16 + gq + 8 * k);
                 }
             if (mine && gq == 0) wml[warp][col] = make_float2(m_[h], l_[h]);
         }
@@ -777,7 +816,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
             auto add = [&](float2 ml, const float4& x, float top) {
                 if (ml.x == -INFINITY) return;
-                const float w = ex2(ml.x - top);
+                const float w = item_weight(ml.x, top);
                 L = fmaf(ml.y, w, L);
                 a.x = fmaf(x.x, w, a.x); a.y = fmaf(x.y, w, a.y);
                 a.z = fmaf(x.z, w, a.z); a.w = fmaf(x.w, w, a.w);
@@ -801,7 +840,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                 }
                 const float top = fmaxf(fmaxf(M, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
                 if (top > M) {
-                    const float corr = ex2(M - top);
+                    const float corr = item_weight(M, top);
                     L *= corr;
                     a.x *= corr; a.y *= corr; a.z *= corr; a.w *= corr;
                     M = top;
@@ -921,7 +960,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
 #pragma unroll
         for (int u = 0; u < U; ++u) top = fmaxf(top, ml[u].x);
         if (top == -INFINITY) continue;
-        const float corr = ex2(M - top);
+        const float corr = item_weight(M, top);
         M = top;
         L *= corr;
 #pragma unroll
@@ -929,7 +968,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (ml[u].x != -INFINITY) {
-                const float w = ex2(ml[u].x - M);
+                const float w = item_weight(ml[u].x, M);
                 L = fmaf(ml[u].y, w, L);
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] = fmaf(x[u][e], w, acc[e]);
@@ -944,7 +983,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
     for (int k = 0; k < kPmWarps; ++k) top = fmaxf(top, m_s[k]);
 #pragma unroll
     for (int k = 0; k < kPmWarps; ++k) {
-        w[k] = m_s[k] == -INFINITY ? 0.f : ex2(m_s[k] - top);
+        w[k] = m_s[k] == -INFINITY ? 0.f : item_weight(m_s[k], top);
         sum = fmaf(l_s[k], w[k], sum);
     }
     const float iv = top == -INFINITY ? 0.f : 1.f / sum;

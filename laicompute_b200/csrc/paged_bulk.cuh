@@ -33,7 +33,7 @@
 // Tiles that some column does not see to their end are masked. There 0 * V must not be 0 * inf: the
 // softmax threads clear what is not finite in V before the product (all of it past the positions any
 // column sees), note the positions, and the columns that do see one take its infinities and NaN at
-// the end.
+// the end, as do columns whose output a product with one made NaN.
 //
 // FP32 rows: Q as binary16 hi + lo after a scaling by a power of two, P likewise, the lo products
 // first (the accumulators then start from small terms); binary16 rows: one product each, P rounded to
@@ -614,9 +614,18 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 tc_ld32(O + k, o);
                 tc_wait_ld();
                 tc_loaded(o);
-                if (any_odd)
+                bool nan = false;  // (an infinite value that every column sees, or scores that are NaN)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) nan |= __uint_as_float(o[e]) != __uint_as_float(o[e]);
+                nan &= l == l;
+                if (nan) {  // as odd_values
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (__uint_as_float(o[e]) != __uint_as_float(o[e])) o[e] = 0;
+                }
+                if (nan || any_odd)
                     for (int t = t0; t < min(t1, lim); ++t)
-                        if (odd[(t - t0) >> 5] >> ((t - t0) & 31) & 1) {
+                        if (nan || (odd[(t - t0) >> 5] >> ((t - t0) & 31) & 1)) {
                             int id = page_ids[(t >> p.page_shift) - first_page];
                             if (id < 0 || id >= p.num_pages) id = 0;
                             const __half* v = p.vp + (((((size_t)id * p.kv_heads + kvh) << p.page_shift) +
@@ -687,7 +696,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
 #pragma unroll
                 for (int c = 0; c < CC; ++c)
                     if (ml[u][c].x != -INFINITY) {
-                        const float w = ex2(ml[u][c].x - M);
+                        const float w = item_weight(ml[u][c].x, M);
                         L = fmaf(ml[u][c].y, w, L);
                         a.x = fmaf(v[u][c].x, w, a.x); a.y = fmaf(v[u][c].y, w, a.y);
                         a.z = fmaf(v[u][c].z, w, a.z); a.w = fmaf(v[u][c].w, w, a.w);

@@ -63,3 +63,53 @@ def test_a_row_that_sees_only_nan_keys(n, dtype):
     out = attend(cache, q, [n, 40])
     assert torch.isnan(out[0]).all()
     close(out[1:], ref[1:], tol[1:])
+
+
+def _close_nonfinite(out, ref, tol):
+    """Finite elements within their bound; the others are the definition's infinities and NaN."""
+    out = out.double().cpu()
+    odd = ~torch.isfinite(ref)
+    assert odd.any()
+    same = (out[odd] == ref[odd]) | (torch.isnan(out[odd]) & torch.isnan(ref[odd]))
+    assert same.all(), (out[odd][~same][:8], ref[odd][~same][:8])
+    close(out[~odd], ref[~odd], tol[~odd])
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("heads,hkv,d", [(8, 2, 64), (4, 2, 32), (8, 1, 128), (6, 1, 64)])
+@pytest.mark.parametrize("kind", ["whole", "split", "narrow", "wide"])
+def test_seen_values_that_are_not_finite(kind, heads, hkv, d, dtype, scale):
+    """Infinities and NaN in values that every row sees, in the first and last tiles and in the row's own positions,
+    of each sign and both, at weights down to e^-200 of the sum (beyond binary32 and binary16)."""
+    cache, lens, seqs, groups = _shape(kind, heads, hkv, d, seed=4)
+    n, all_ = lens[0], range(len(lens))
+    for pos, dim, value in ((3, 1, INF), (n - 40, 2, -INF), (50, 3, INF), (60, 3, -INF), (70, 4, NAN), (n - 30, 5, INF),
+                            (n - 29, 5, INF), (0, 6, -INF)):
+        _put(cache, "v", all_, pos, value, dim)
+    _put(cache, "v", [1], n - 1, INF, 7)   # (one row alone)
+    q = _q(len(lens), heads, d, dtype, seed=6)
+    out = attend(cache, q, lens, groups=groups, scale=scale)
+    cache.pages().check()
+    ref, tol = reference(cache, q[:3], lens[:3], scale=scale)
+    _close_nonfinite(out[:3], ref, tol)
+
+
+@pytest.mark.parametrize("scale", [0.0, 2.0])
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("heads,hkv,d,rows,start", [(4, 2, 64, 30, 150), (32, 8, 128, 12, 150), (2, 2, 32, 9, 150),
+                                                    (8, 1, 128, 40, 300), (4, 1, 64, 80, 490)])
+def test_values_that_some_rows_see(heads, hkv, d, rows, start, dtype, scale):
+    """Causal rows: infinite values seen by all, by the last rows only, and by none but the last."""
+    total = start + rows
+    cache = Cache([total], hkv, d, 16, seed=2)
+    lens = [start + j + 1 for j in range(rows)]
+    for pos, dim, value in ((5, 0, INF), (start - 1, 1, -INF), (total - 4, 2, INF), (total - 3, 2, -INF), (total - 5, 3, NAN),
+                            (total - 1, 4, INF), (start + 1, 5, -INF)):
+        _put(cache, "v", [0], pos, value, dim)
+    q = _q(rows, heads, d, dtype, seed=4)
+    out = attend(cache, q, lens, seqs=[0] * rows, groups=([0, rows], [total]), scale=scale)
+    cache.pages().check()
+    at = sorted({0, 1, 2, rows // 2, rows - 6, rows - 5, rows - 4, rows - 3, rows - 2, rows - 1})
+    ref, tol = reference(cache, q[at], [lens[r] for r in at], [0] * len(at), scale=scale)
+    _close_nonfinite(out[at], ref, tol)
