@@ -375,9 +375,10 @@ typedef struct laic_kv_attention_args {
  * once, through the page table row of the group's first row that sees any. Rows that
  * share a whole sequence with causal lengths (a prompt's tokens, drafted tokens) are
  * a group whose length is the longest. Masked positions never reach a row's output,
- * whatever they hold; a NaN score that a row sees makes its head's output NaN, and a value
- * that is not finite reaches the outputs of all rows that see it, whatever its weight. out_dev
- * must not overlap an input. Two calls with the same inputs give the same bits. */
+ * whatever they hold; a NaN score that a row sees makes its head's output NaN, scores
+ * that are all -inf give zeros (FP32 rows: an infinite key's score may be NaN), and otherwise a
+ * value that is not finite reaches the outputs of all rows that see it, whatever its weight. out_dev must not overlap an input. Two calls
+ * with the same inputs give the same bits. */
 LAIC_API int laic_kv_attention(const laic_kv_pages* pages, const laic_kv_attention_args* args, void* stream);
 /* Bytes of workspace the call needs (0 possible); reads no pointer of `args`. */
 LAIC_API int laic_kv_attention_workspace(const laic_kv_pages* pages, const laic_kv_attention_args* args,

@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         const uint32_t S = s_at(wg) + lane_at, O = o_at(wg) + lane_at;
         const float cm = fmaxf(cmul[tid], 1e-36f);  // (-inf * 0 would be NaN; below this every score is 0)
         const int wtid = tid & 127;
-        float mref = 0.f, l = 0.f;
+        float mref = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < nt; ++j) {
             const int c0 = t0 + j * NK;
@@ -542,9 +542,10 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 for (int e = 0; e < 64; e += 2) mx4[(e >> 1) & 3] = max3(mx4[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                 const float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * cm;
                 if (j == 0 && h == 0) {
-                    mref = mx > -INFINITY ? mx : 0.f;
+                    mref = mx != mx ? 0.f : mx;  // (scores that are NaN alone: their sum says so)
                 } else if (__any_sync(0xffffffffu, mx > mref + kPaSlack)) {
-                    const float next = fmaxf(mref, mx), corr = ex2(mref - next);
+                    // (no finite score so far: nothing to rescale)
+                    const float next = fmaxf(mref, mx), corr = mref == -INFINITY ? 1.f : ex2(mref - next);
                     mref = next;
                     l *= corr;
                     sum2[0] = f2_mul(sum2[0], f2_pack(corr, corr));
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                     }
                 }
                 // ---- the weights: binary16 rows carry the factor in the exponent (their rounding is 2^-11 anyway)
-                const float shift = F32 ? -mref : 7.f - mref;
+                const float shift = (F32 ? 0.f : 7.f) - (mref == -INFINITY ? 0.f : mref);
                 const uint64_t sh2 = f2_pack(shift, shift);
 #pragma unroll
                 for (int k = 0; k < 64; k += 32) {

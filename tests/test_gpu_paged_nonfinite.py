@@ -113,3 +113,39 @@ def test_values_that_some_rows_see(heads, hkv, d, rows, start, dtype, scale):
     at = sorted({0, 1, 2, rows // 2, rows - 6, rows - 5, rows - 4, rows - 3, rows - 2, rows - 1})
     ref, tol = reference(cache, q[at], [lens[r] for r in at], [0] * len(at), scale=scale)
     _close_nonfinite(out[at], ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("heads,hkv,d", [(8, 2, 64), (4, 2, 32), (8, 1, 128)])
+@pytest.mark.parametrize("kind", ["whole", "split", "narrow", "wide"])
+def test_scores_of_minus_infinity(kind, heads, hkv, d, dtype):
+    """Infinite keys whose scores are -inf at the head of the positions, with all other scores far below zero: they
+    weigh nothing. Where every score is -inf, zeros."""
+    cache, lens, seqs, groups = _shape(kind, heads, hkv, d, seed=7)
+    n = lens[0]
+    q = _q(len(lens), heads, d, dtype, seed=8).view(len(lens), heads, d)
+    # q[0] k[0] = -inf with both parts of the split q of one sign, q[1] k[1] = -500 / scale
+    q[:, :, 0], q[:, :, 1] = (1.0 + 2.0 ** -13 if dtype == F32 else 1.0), 1.0
+    q = q.flatten(1).contiguous()
+
+    class Rest:  # the positions behind the infinite keys
+        head_dim, kv_heads = d, hkv
+    for s in range(len(lens)):
+        for t in range(n):
+            _put(cache, "k", [s], t, -1000.0, 1)
+    for first in (64, 70, 200 if n > 200 else 80):
+        for t in range(first):
+            _put(cache, "k", range(len(lens)), t, -INF, 0)
+        Rest.seq_k = [k[first:] for k in cache.seq_k]
+        Rest.seq_v = [v[first:] for v in cache.seq_v]
+        out = attend(cache, q, lens, groups=groups, scale=0.5)
+        cache.pages().check()
+        ref, tol = reference(Rest, q[:3], [m - first for m in lens[:3]], scale=0.5)
+        close(out[:3], ref, tol)
+    for t in range(n):
+        _put(cache, "k", range(len(lens)), t, -INF, 0)
+    out = attend(cache, q, lens, groups=groups, scale=0.5)
+    assert not out.any()
+    if groups:  # and where a group's rows see the shared positions alone
+        out = attend(cache, q, [groups[1][0]] * len(lens), groups=groups, scale=0.5)
+        assert not out.any()
