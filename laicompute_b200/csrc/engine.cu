@@ -591,8 +591,8 @@ struct laic_dev {
         CK(cudaMemsetAsync(mvs.err, 0, 4, st));  // the discarded step's wait or sampler errors are not the caller's
         CK(cudaMemsetAsync(d_err, 0, 4, st));
         CK(cudaStreamSynchronize(st));
-        const bool waits_failed = h_err[2 * spec_buf] != 0;
-        h_err[0] = h_err[1] = h_err[2] = h_err[3] = 0;
+        const bool waits_failed = h_err[3 * spec_buf] != 0;
+        std::fill(h_err, h_err + 6, 0);
         if (waits_failed)
             if (int rc = ls_reset()) return rc;  // a failed wait may have left the step kernel's counters part-way
         return LAIC_OK;
@@ -629,11 +629,11 @@ struct laic_dev {
     int max_split = 1;
 
     unsigned *d_tokens = nullptr, *d_out_ids = nullptr, *d_hist = nullptr;
-    int *d_slots = nullptr, *d_err = nullptr, *d_hist_count = nullptr;
+    int *d_slots = nullptr, *d_err = nullptr /* [2]: sampler, pages */, *d_hist_count = nullptr;
     size_t hist_cap = 0;  // entries of d_hist
     laic::SampleDev* d_params = nullptr;
     unsigned *h_tokens = nullptr, *h_out_ids = nullptr;
-    int* h_err = nullptr;  // pinned [2][2]: a step's copies of the two device error flags (matvec waits, sampler)
+    int* h_err = nullptr;  // pinned [2][3]: a step's copies of the device error words (matvec waits, sampler, pages)
     float* samp_v = nullptr;  // sampler slices: [S][kSampleSlices] maxima, ids and per-sequence tickets
     int* samp_i = nullptr;
     unsigned* samp_cnt = nullptr;
@@ -699,7 +699,7 @@ struct laic_dev {
     }
     laic_kv_pages layer_pages(int l) const {
         const size_t off = (size_t)l * npages * Hkv * kKvPage * D;
-        return laic_kv_pages{device, Hkv, D, kKvPage, npages, pk + off, pv + off, mvs.err};
+        return laic_kv_pages{device, Hkv, D, kKvPage, npages, pk + off, pv + off, d_err + 1};
     }
     laic_kv_append_args append_args(int rows, const float* c, float* qout) const {
         laic_kv_append_args a{};
@@ -1138,11 +1138,11 @@ struct laic_dev {
                             d_hist_count, nseq));
                 ++nl;
             } else {
-                // the sampled ids and both error flags come back with the step (no extra round trip)
+                // the sampled ids and the error words come back with the step (no extra round trip)
                 const int ob = mode == MODE_SPEC1 ? 1 : 0;  // host output buffer
                 CK(cudaMemcpyAsync(h_out_ids + (size_t)ob * S, d_out_ids, nseq * sizeof(unsigned), cudaMemcpyDeviceToHost, s));
-                CK(cudaMemcpyAsync(h_err + 2 * ob, mvs.err, 4, cudaMemcpyDeviceToHost, s));
-                CK(cudaMemcpyAsync(h_err + 2 * ob + 1, d_err, 4, cudaMemcpyDeviceToHost, s));
+                CK(cudaMemcpyAsync(h_err + 3 * ob, mvs.err, 4, cudaMemcpyDeviceToHost, s));
+                CK(cudaMemcpyAsync(h_err + 3 * ob + 1, d_err, 8, cudaMemcpyDeviceToHost, s));
             }
         } else {
             t_begin("advance", 0);
@@ -1571,7 +1571,6 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
         if (int rc = zero_now(d->vc, kv_bytes)) return rc;
     } else {
         CK(laic::serving_set_attributes());
-        if (int rc = mv_scratch_reserve(d->mvs, MvNeed{})) return rc;  // the error word, which the pages' kernels share
         d->pps = (cap + kKvPage - 1) / kKvPage;
         d->npages = d->pps * (int)S;
         const size_t pool = (size_t)d->L * d->npages * d->Hkv * kKvPage * D * 2;
@@ -1621,8 +1620,8 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     CK(cudaMalloc(&d->d_tokens, RB * 4));
     CK(cudaMalloc(&d->d_out_ids, S * 4));
     CK(cudaMalloc(&d->d_slots, RB * 4));
-    CK(cudaMalloc(&d->d_err, 4));
-    if (int rc = zero_now(d->d_err, 4)) return rc;
+    CK(cudaMalloc(&d->d_err, 8));
+    if (int rc = zero_now(d->d_err, 8)) return rc;
     CK(cudaMalloc(&d->samp_v, S * laic::kSampleSlices * 4));
     CK(cudaMalloc(&d->samp_i, S * laic::kSampleSlices * 4));
     CK(cudaMalloc(&d->samp_cnt, S * 4));
@@ -1631,12 +1630,12 @@ int laic_dev_create(const laic_dev_desc* desc, const laic_dev_opts* opts, laic_d
     CK(cudaMalloc(&d->d_params, S * sizeof(laic::SampleDev)));
     CK(cudaMallocHost(&d->h_tokens, RB * 4));
     CK(cudaMallocHost(&d->h_out_ids, 2 * S * 4));
-    CK(cudaMallocHost(&d->h_err, 4 * sizeof(int)));
+    CK(cudaMallocHost(&d->h_err, 6 * sizeof(int)));
     CK(cudaEventCreateWithFlags(&d->spec_ev[0], cudaEventDisableTiming));
     CK(cudaEventCreateWithFlags(&d->spec_ev[1], cudaEventDisableTiming));
     CK(cudaMallocHost(&d->h_spec, 2 * (size_t)o.max_seqs * sizeof(int)));
     CK(cudaMalloc(&d->d_spec, 2 * (size_t)o.max_seqs * sizeof(int)));
-    d->h_err[0] = d->h_err[1] = d->h_err[2] = d->h_err[3] = 0;
+    std::fill(d->h_err, d->h_err + 6, 0);
     CK(cudaMallocHost(&d->h_slots, RB * 4));
     CK(cudaMallocHost(&d->h_params, S * sizeof(laic::SampleDev)));
     if (tp > 1) {
@@ -1863,51 +1862,36 @@ static int fill_params(laic_dev* d, int32_t nseq, const laic_sample_params* para
 }
 
 // The message of a bounded device wait that ran out (the codes of common.cuh).
-static std::string wait_error_text(int code) {
-    switch (code) {
-    case laic::kErrMbarrier: return "device wait timed out: a bulk copy into shared memory never completed";
-    case laic::kErrTeamMerge: return "device wait timed out: a matvec warp team's partial-sum slot was never released";
-    case laic::kErrGridBarrier: return "device wait timed out: a decode-step grid barrier was not reached by every CTA";
-    case laic::kErrPeerFlag: return "device wait timed out: a tensor-parallel peer never published its allreduce slice";
-    case laic::kKvWait: return "device wait timed out: a tile of the paged attention was never loaded or multiplied";
-    case laic::kErrDepCounter: return "device wait timed out: a decode-step dependency counter never reached its target";
-    }
-    return "device wait timed out (code " + std::to_string(code) + ")";
-}
-
-// After a synchronised MODE_STEP run: the error flags its graph copied to pinned memory.
-static int check_step_err(laic_dev* d, int buf = 0) {
-    const int mv_err = d->h_err[2 * buf], sample_err = d->h_err[2 * buf + 1];
-    if (mv_err) {
-        CK(cudaMemsetAsync(d->mvs.err, 0, 4, d->st));
-        d->h_err[2 * buf] = 0;
-        if (int rc = d->ls_reset()) return rc;
-        return fail(LAIC_E_CUDA, wait_error_text(mv_err));
+// The words a step left (zero: nothing): clear those that hold something and report them.
+static int report_step_err(laic_dev* d, int wait_code, int sample_err, int kv_bits) {
+    if (wait_code || kv_bits) {
+        if (wait_code) {
+            CK(cudaMemsetAsync(d->mvs.err, 0, 4, d->st));
+            if (int rc = d->ls_reset()) return rc;
+        }
+        if (kv_bits) CK(cudaMemsetAsync(d->d_err + 1, 0, 4, d->st));
+        return fail(LAIC_E_CUDA, laic::step_error_text(wait_code, kv_bits));
     }
     if (sample_err) {
         CK(cudaMemsetAsync(d->d_err, 0, 4, d->st));
-        d->h_err[2 * buf + 1] = 0;
         return fail(LAIC_E_UNSUPPORTED, "sampling request needs more than 1024 candidates (top_k or top_p mass)");
     }
     return LAIC_OK;
 }
 
+// After a synchronised MODE_STEP run: the error words its graph copied to pinned memory.
+static int check_step_err(laic_dev* d, int buf = 0) {
+    int* e = d->h_err + 3 * buf;
+    const int wait_code = e[0], sample_err = e[1], kv_bits = e[2];
+    std::fill(e, e + 3, 0);
+    return report_step_err(d, wait_code, sample_err, kv_bits);
+}
+
 static int check_sampler_err(laic_dev* d) {
-    int err = 0;
-    if (d->mvs.err) {
-        CK(cudaMemcpy(&err, d->mvs.err, 4, cudaMemcpyDeviceToHost));
-        if (err) {
-            CK(cudaMemsetAsync(d->mvs.err, 0, 4, d->st));
-            if (int rc = d->ls_reset()) return rc;
-            return fail(LAIC_E_CUDA, wait_error_text(err));
-        }
-    }
-    CK(cudaMemcpy(&err, d->d_err, 4, cudaMemcpyDeviceToHost));
-    if (err) {
-        CK(cudaMemsetAsync(d->d_err, 0, 4, d->st));
-        return fail(LAIC_E_UNSUPPORTED, "sampling request needs more than 1024 candidates (top_k or top_p mass)");
-    }
-    return LAIC_OK;
+    int wait_code = 0, e[2] = {0, 0};
+    if (d->mvs.err) CK(cudaMemcpy(&wait_code, d->mvs.err, 4, cudaMemcpyDeviceToHost));
+    CK(cudaMemcpy(e, d->d_err, 8, cudaMemcpyDeviceToHost));
+    return report_step_err(d, wait_code, e[0], e[1]);
 }
 
 int laic_dev_step(laic_dev* d, int32_t nseq, const uint32_t* tokens, const int32_t* slots,
@@ -2525,7 +2509,7 @@ int laic_tensor_check(laic_tensor* t, void* stream) {
         if (int rc = zero_now(t->sc.err, 4)) return rc;
     if (fixed)
         if (int rc = zero_now(base, 4)) return rc;
-    if (own || fixed) return fail(LAIC_E_CUDA, wait_error_text(own ? own : fixed));
+    if (own || fixed) return fail(LAIC_E_CUDA, laic::wait_error_text(own ? own : fixed));
     return LAIC_OK;
 }
 
@@ -2562,7 +2546,7 @@ int laic_selftest_peer_timeout(int32_t device, int64_t spin_cycles, int32_t* cod
     }
     release();
     if (e != cudaSuccess) return fail(LAIC_E_CUDA, std::string("self-test: ") + cudaGetErrorString(e));
-    if (*code) return fail(LAIC_E_CUDA, wait_error_text(*code));
+    if (*code) return fail(LAIC_E_CUDA, laic::wait_error_text(*code));
     return LAIC_OK;
 }
 

@@ -11,8 +11,6 @@
 
 namespace laic {
 
-enum : int { kKvBadSeq = 1, kKvBadPos = 2, kKvBadPage = 4, kKvBadGroup = 8, kKvWait = 16 };
-
 __host__ __device__ inline void kv_flag(int* err, int bits) {
 #ifdef __CUDA_ARCH__
     atomicOr(err, bits);

@@ -352,16 +352,8 @@ cudaError_t serving_set_attributes() {
     return cudaSuccess;
 }
 
-std::string kv_error_text(int bits) {
-    std::string s = "paged KV cache:";
-    if (bits & LAIC_KV_BAD_SEQ) s += " sequence index outside the page table;";
-    if (bits & LAIC_KV_BAD_POS) s += " position or length beyond its bound;";
-    if (bits & LAIC_KV_BAD_PAGE) s += " page id out of range;";
-    if (bits & LAIC_KV_BAD_GROUP) s += " group rows out of order or above their bound;";
-    if (bits & kKvWait) s += " a device wait timed out;";
-    s.pop_back();
-    return s;
-}
+static_assert(kKvBadSeq == LAIC_KV_BAD_SEQ && kKvBadPos == LAIC_KV_BAD_POS && kKvBadPage == LAIC_KV_BAD_PAGE &&
+              kKvBadGroup == LAIC_KV_BAD_GROUP && kKvWait == LAIC_KV_WAIT, "the public bits");
 
 int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t st) {
     if (int rc = check_pages(g)) return rc;

@@ -6,7 +6,7 @@
 
 #include "../../include/laic_b200.h"
 
-#include "paged.cuh"  // the error bits
+#include "errors.h"
 
 namespace laic {
 
@@ -20,7 +20,6 @@ int kv_attention(const laic_kv_pages& pages, const laic_kv_attention_args& a, cu
 int logits_probs(int device, int rows, int vocab, const float* x, long long ldx, const float* temp, float* y, long long ldy,
                  cudaStream_t st);
 int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st);
-std::string kv_error_text(int bits);
 // Kernel attributes (call before any graph capture; the entry points call it themselves).
 cudaError_t serving_set_attributes();
 
