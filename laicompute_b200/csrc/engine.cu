@@ -1013,12 +1013,12 @@ struct laic_dev {
                 laic_kv_append_args aa = append_args(nseq, qkv, q);
                 aa.pos_dev = d_rpos; aa.seq_dev = d_slots;
                 t_begin("kv_append", 4.0 * nseq * (2 * hq + 2 * kv) + 4.0 * nseq * kv);
-                if (int rc = laic::kv_append(pg, aa, s)) return rc;
+                if (int rc = laic::kv_append(pg, aa, s, {pdl})) return rc;
                 t_end();
                 laic_kv_attention_args at = attention_args(nseq, kb);
                 at.q_dev = q; at.out_dev = attn; at.len_dev = d_rlen; at.seq_dev = d_slots;
                 t_begin("attention", attn_bytes);
-                if (int rc = laic::kv_attention(pg, at, s)) return rc;
+                if (int rc = laic::kv_attention(pg, at, s, {pdl})) return rc;
                 t_end();
                 nl += 2;
             }
@@ -1111,14 +1111,14 @@ struct laic_dev {
             }
             if (mode == MODE_VERIFY) {
                 t_begin("verify", 0);
-                if (int rc = laic::logits_probs(device, nseq, V, logits, V, vf_temp, vf_probs, V, s)) return rc;
+                if (int rc = laic::logits_probs(device, nseq, V, logits, V, vf_temp, vf_probs, V, s, {pdl})) return rc;
                 laic_verify_args va{};
                 va.nseq = vf_nseq; va.max_draft = vf_max; va.vocab = V; va.ld_target = va.ld_draft = V;
                 va.target_dev = vf_probs; va.draft_dev = vf_draft;
                 va.draft_ids_dev = vf_ids; va.n_draft_dev = vf_n;
                 va.accept_u_dev = vf_u; va.sample_u_dev = vf_u + RB;
                 va.out_ids_dev = vf_ids + RB; va.out_n_dev = vf_n + RB;
-                if (int rc = laic::verify_drafts(device, va, s)) return rc;
+                if (int rc = laic::verify_drafts(device, va, s, {pdl})) return rc;
                 nl += 2;
                 t_end();
                 launches_step = nl;
@@ -1336,12 +1336,12 @@ struct laic_dev {
                     const laic_kv_pages pg = layer_pages(l);
                     laic_kv_append_args aa = append_args(T, pf_c, pf_q);
                     aa.pos_dev = pf_npos; aa.seq_dev = pf_slots;
-                    if (int rc = laic::kv_append(pg, aa, s)) return rc;
+                    if (int rc = laic::kv_append(pg, aa, s, {use_pdl})) return rc;
                     // the rows of the pass are one group: causal lengths over the sequence's positions
                     laic_kv_attention_args at = attention_args(T, fb);
                     at.q_dev = pf_q; at.out_dev = pf_attn; at.len_dev = pf_len; at.seq_dev = pf_slots;
                     at.group_rows_dev = pf_group; at.group_len_dev = pf_group + 2;
-                    if (int rc = laic::kv_attention(pg, at, s)) return rc;
+                    if (int rc = laic::kv_attention(pg, at, s, {use_pdl})) return rc;
                 } else {
                 laic::QkvPostParams qp{pf_c, T, hq, kv, D, rope_pairs, p0, rope_cs, pf_q, kcl, vcl, cap};
                 laic::qkv_post_kernel<<<grid, 256, 0, s>>>(qp);

@@ -74,14 +74,18 @@ int on_device(int device, F&& f) {
     return f();
 }
 
-// Every first kernel of a call may start while its predecessor in the stream drains; it waits before it
-// reads or writes anything.
+// The result of a launch, counted where it was made. (With LaunchOpts::pdl every first kernel of a call may start
+// while its predecessor in the stream drains; it waits before it reads or writes anything.)
+cudaError_t counted(cudaError_t e, const LaunchOpts& o) {
+    if (e == cudaSuccess && o.launches) ++*o.launches;
+    return e;
+}
 template <typename TI, typename TQ>
-cudaError_t append_launch(bool vec, dim3 grid, int block, cudaStream_t st, const KvAppendParams& p) {
+cudaError_t append_launch(bool vec, dim3 grid, int block, cudaStream_t st, const LaunchOpts& o, const KvAppendParams& p) {
     void (*fn)(KvAppendParams) = vec ? kv_append_kernel<TI, TQ, true, 1> : kv_append_kernel<TI, TQ, false, 1>;
     if constexpr (sizeof(TI) == 2 && sizeof(TQ) == 2)
         if (grid.x < (unsigned)p.rows) fn = kv_append_kernel<TI, TQ, true, 2>;
-    return launch_k(fn, grid, dim3(block), 0, st, true, p);
+    return counted(launch_k(fn, grid, dim3(block), 0, st, o.pdl, p), o);
 }
 
 int device_sms(int dev) {
@@ -355,7 +359,7 @@ cudaError_t serving_set_attributes() {
 static_assert(kKvBadSeq == LAIC_KV_BAD_SEQ && kKvBadPos == LAIC_KV_BAD_POS && kKvBadPage == LAIC_KV_BAD_PAGE &&
               kKvBadGroup == LAIC_KV_BAD_GROUP && kKvWait == LAIC_KV_WAIT, "the public bits");
 
-int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t st) {
+int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t st, LaunchOpts o) {
     if (int rc = check_pages(g)) return rc;
     if (a.rows < 0 || a.heads < 0) return api_fail(LAIC_E_INVALID, "rows and heads must be >= 0");
     if (!type_ok(a.in_type) || !type_ok(a.q_type)) return api_fail(LAIC_E_UNSUPPORTED, "q, k and v must be F32 or F16");
@@ -398,8 +402,8 @@ int kv_append(const laic_kv_pages& g, const laic_kv_append_args& a, cudaStream_t
     if (grid.y > 65535) return api_fail(LAIC_E_UNSUPPORTED, "rows too wide");
     return on_device(g.device, [&]() -> int {
         const bool i32 = a.in_type == LAIC_GGML_F32, q32 = a.q_type == LAIC_GGML_F32;
-        const cudaError_t e = i32 ? (q32 ? append_launch<float, float>(vec, grid, block, st, p) : append_launch<float, __half>(vec, grid, block, st, p))
-                                  : (q32 ? append_launch<__half, float>(vec, grid, block, st, p) : append_launch<__half, __half>(vec, grid, block, st, p));
+        const cudaError_t e = i32 ? (q32 ? append_launch<float, float>(vec, grid, block, st, o, p) : append_launch<float, __half>(vec, grid, block, st, o, p))
+                                  : (q32 ? append_launch<__half, float>(vec, grid, block, st, o, p) : append_launch<__half, __half>(vec, grid, block, st, o, p));
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "kv_append");
     });
 }
@@ -413,7 +417,7 @@ int kv_attention_bytes(const laic_kv_pages& g, const laic_kv_attention_args& a, 
     return LAIC_OK;
 }
 
-int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaStream_t st) {
+int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaStream_t st, LaunchOpts o) {
     if (int rc = check_attention(g, a)) return rc;
     if (int rc = check_table(a.rows, a.nseq, a.pages_per_seq, g.page_size, a.seq_dev)) return rc;
     if (a.rows == 0) return LAIC_OK;
@@ -458,26 +462,26 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
             CUtensorMap mk, mv;
             if (!encode_pages(g, g.k_dev, &mk) || !encode_pages(g, g.v_dev, &mv))
                 return api_fail(LAIC_E_CUDA, "kv_attention: tensor map");
-            e = launch_cluster_k(bulk_pick(g.head_dim, f32, pl.mt), dim3(pl.shared_items), dim3(bulk_threads(pl.mt)), bulk_smem(g.head_dim, f32, pl.mt),
-                                 st, true, pl.cluster, p, mk, mv);
+            e = counted(launch_cluster_k(bulk_pick(g.head_dim, f32, pl.mt), dim3(pl.shared_items), dim3(bulk_threads(pl.mt)),
+                                         bulk_smem(g.head_dim, f32, pl.mt), st, o.pdl, pl.cluster, p, mk, mv), o);
         }
         if (e == cudaSuccess && !pl.bulk && pl.shared_items)
-            e = launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(pl.shared_items), dim3(kPaWarps * 32),
-                         pa_smem(g.head_dim, pl.nt, f32), st, true, p);
+            e = counted(launch_k(pa_pick(g.head_dim, pl.nt, a.type), dim3(pl.shared_items), dim3(kPaWarps * 32),
+                                 pa_smem(g.head_dim, pl.nt, f32), st, o.pdl, p), o);
         if (e == cudaSuccess && pl.private_items)
-            e = launch_k(pr_pick(g.head_dim, a.type, p.G, pl.whole),
-                         dim3(pl.whole ? pl.private_items : (pl.private_items + kPrWarps - 1) / kPrWarps), dim3(kPrWarps * 32),
-                         pr_smem(g.head_dim), st, true, p);
+            e = counted(launch_k(pr_pick(g.head_dim, a.type, p.G, pl.whole),
+                                 dim3(pl.whole ? pl.private_items : (pl.private_items + kPrWarps - 1) / kPrWarps),
+                                 dim3(kPrWarps * 32), pr_smem(g.head_dim), st, o.pdl, p), o);
         if (e == cudaSuccess && !pl.direct && !pl.whole)
-            e = launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
-                         dim3((unsigned)(a.rows * a.heads)), dim3(kPmWarps * 32), 0,
-                         st, pl.shared_items || pl.private_items, p);
+            e = counted(launch_k(f32 ? pm_fn<float>(g.head_dim) : pm_fn<__half>(g.head_dim),
+                                 dim3((unsigned)(a.rows * a.heads)), dim3(kPmWarps * 32), 0,
+                                 st, o.pdl && (pl.shared_items || pl.private_items), p), o);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "kv_attention");
     });
 }
 
 int logits_probs(int device, int rows, int vocab, const float* x, long long ldx, const float* temp, float* y, long long ldy,
-                 cudaStream_t st) {
+                 cudaStream_t st, LaunchOpts o) {
     if (rows < 0 || vocab < 1) return api_fail(LAIC_E_INVALID, "rows must be >= 0 and vocab >= 1");
     if (rows > INT_MAX / 8) return api_fail(LAIC_E_UNSUPPORTED, "too many rows");
     if (rows == 0) return LAIC_OK;
@@ -498,12 +502,12 @@ int logits_probs(int device, int rows, int vocab, const float* x, long long ldx,
         const size_t smem = sm ? ((((size_t)vocab + c - 1) / c + 3) & ~(size_t)3) * 4 : 0;
         cudaError_t e = serving_set_attributes();
         if (e == cudaSuccess)
-            e = launch_cluster_k(fn, dim3((unsigned)rows * c), dim3(kProbsThreads), smem, st, true, c, p);
+            e = counted(launch_cluster_k(fn, dim3((unsigned)rows * c), dim3(kProbsThreads), smem, st, o.pdl, c, p), o);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "logits_probs");
     });
 }
 
-int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st) {
+int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st, LaunchOpts o) {
     if (a.nseq < 0 || a.vocab < 1) return api_fail(LAIC_E_INVALID, "nseq must be >= 0 and vocab >= 1");
     if (a.max_draft < 0) return api_fail(LAIC_E_INVALID, "max_draft must be >= 0");
     if (a.max_draft > LAIC_MAX_DRAFT) return api_fail(LAIC_E_UNSUPPORTED, "at most 64 drafted tokens per sequence");
@@ -523,7 +527,8 @@ int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st) {
         // 11.6, 13.0, 19.8 us, 36 take 17.9, 14.2, 19.5, 72 take 28, 25, 21)
         int c = kVerifyMaxCluster;
         while (c > 1 && a.nseq > verify_clusters(device, c)) c /= 2;
-        const cudaError_t e = launch_cluster_k(vec ? verify_kernel<true> : verify_kernel<false>, dim3((unsigned)a.nseq * c), dim3(kVerifyThreads), 0, st, true, c, p);
+        const cudaError_t e = counted(launch_cluster_k(vec ? verify_kernel<true> : verify_kernel<false>, dim3((unsigned)a.nseq * c),
+                                                       dim3(kVerifyThreads), 0, st, o.pdl, c, p), o);
         return e == cudaSuccess ? LAIC_OK : cuda_fail(e, "verify_drafts");
     });
 }
