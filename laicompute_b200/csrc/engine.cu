@@ -1013,14 +1013,13 @@ struct laic_dev {
                 laic_kv_append_args aa = append_args(nseq, qkv, q);
                 aa.pos_dev = d_rpos; aa.seq_dev = d_slots;
                 t_begin("kv_append", 4.0 * nseq * (2 * hq + 2 * kv) + 4.0 * nseq * kv);
-                if (int rc = laic::kv_append(pg, aa, s, {pdl})) return rc;
+                if (int rc = laic::kv_append(pg, aa, s, {pdl, &nl})) return rc;
                 t_end();
                 laic_kv_attention_args at = attention_args(nseq, kb);
                 at.q_dev = q; at.out_dev = attn; at.len_dev = d_rlen; at.seq_dev = d_slots;
                 t_begin("attention", attn_bytes);
-                if (int rc = laic::kv_attention(pg, at, s, {pdl})) return rc;
+                if (int rc = laic::kv_attention(pg, at, s, {pdl, &nl})) return rc;
                 t_end();
-                nl += 2;
             }
             // attention
             laic::AttnParams ap{};
@@ -1111,15 +1110,14 @@ struct laic_dev {
             }
             if (mode == MODE_VERIFY) {
                 t_begin("verify", 0);
-                if (int rc = laic::logits_probs(device, nseq, V, logits, V, vf_temp, vf_probs, V, s, {pdl})) return rc;
+                if (int rc = laic::logits_probs(device, nseq, V, logits, V, vf_temp, vf_probs, V, s, {pdl, &nl})) return rc;
                 laic_verify_args va{};
                 va.nseq = vf_nseq; va.max_draft = vf_max; va.vocab = V; va.ld_target = va.ld_draft = V;
                 va.target_dev = vf_probs; va.draft_dev = vf_draft;
                 va.draft_ids_dev = vf_ids; va.n_draft_dev = vf_n;
                 va.accept_u_dev = vf_u; va.sample_u_dev = vf_u + RB;
                 va.out_ids_dev = vf_ids + RB; va.out_n_dev = vf_n + RB;
-                if (int rc = laic::verify_drafts(device, va, s, {pdl})) return rc;
-                nl += 2;
+                if (int rc = laic::verify_drafts(device, va, s, {pdl, &nl})) return rc;
                 t_end();
                 launches_step = nl;
                 return LAIC_OK;

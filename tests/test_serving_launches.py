@@ -1,5 +1,5 @@
 """How the serving operators launch: early behind their predecessor or not, as asked, and counted (recorded by
-stand-ins for the runtime, no GPU); and the paged engine, which passes its flag on."""
+stand-ins for the runtime, no GPU); and the paged engine, which passes its flag on and reports the count."""
 import os
 import re
 import subprocess
@@ -37,7 +37,7 @@ def test_launches_follow_the_flag_and_are_counted(launches):
 def test_the_engine_passes_its_flag_to_every_operator():
     src = open(os.path.join(ROOT, "laicompute_b200", "csrc", "engine.cu")).read()
     calls = re.findall(r"laic::(?:kv_append|kv_attention|logits_probs|verify_drafts)\((.*)\)\) return rc;", src)
-    assert len(calls) == 6 and all(re.search(r"\{(?:use_)?pdl(?:, &nl)?\}$", c) for c in calls), calls
+    assert len(calls) == 6 and all(re.search(r"\{(?:pdl, &nl|use_pdl)\}$", c) for c in calls), calls
 
 
 @pytest.mark.gpu
@@ -63,3 +63,30 @@ def test_paged_engine_without_early_launches(graphs):
     (la, ia, ca), (lb, ib, cb) = got
     assert (np.abs(la - lb).max(axis=-1) / np.abs(lb).max(axis=-1)).max() <= 1e-4
     assert np.array_equal(ia, ib) and np.array_equal(ca, cb)
+
+
+@pytest.mark.gpu
+def test_paged_engine_counts_its_launches(tmp_path):
+    """launches_per_step: the contiguous engine's, the rows' kernel, and per layer an append, the preparation of the
+    o-projection's activations (the contiguous attention of this small model writes them itself) and as many attention
+    kernels as the lengths take, in the place of the contiguous engine's one."""
+    from laicompute_b200 import gguf, synth
+    from laicompute_b200.engine import Engine
+    a = synth.tiny_arch(gguf.Q8_0, gguf.F16, name="count", hidden=256, layers=2, heads=4, kv_heads=2, ffn=256, vocab=512,
+                        ctx=2048)
+    path = synth.write_model(os.path.join(str(tmp_path), "count.gguf"), a, seed=5)
+    rng = np.random.default_rng(0)
+    for n, forked, kernels in ((20, False, 1), (1200, False, 2), (100, True, 2), (20, True, 1)):
+        counts = []
+        for paged in (False, True):
+            e = Engine(path, max_seqs=2, paged=paged, speculate=False)
+            prompts = rng.integers(0, 512, size=(2, n)).astype(np.uint32)
+            e.prefill_batch(prompts[0], 0)
+            if paged and forked:
+                e.fork(0, 1)
+            else:
+                e.prefill_batch(prompts[1], 1)
+            e.step([1, 2])
+            counts.append(e.stats().launches_per_step)
+            e.close()
+        assert counts[1] - counts[0] == 1 + 2 * (1 + 1 + kernels - 1), (n, forked, counts)
