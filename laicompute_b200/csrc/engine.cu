@@ -41,6 +41,7 @@
 #include "../../include/laic_b200.h"
 #include "allreduce.cuh"
 #include "attention.cuh"
+#include "buffers.h"
 #include "launch.cuh"
 #include "misc.cuh"
 #include "mma_matvec.cuh"
@@ -611,6 +612,7 @@ struct laic_dev {
     unsigned* pf_tokens = nullptr;
     void* pf_ws = nullptr;
     size_t pf_ws_bytes = 0;
+    bool pf_ready = false;
     float* rec_ss = nullptr;  // [h / 16 row tiles][max_seqs] sums of squares of the residual
 
     Mat embd, lm;
@@ -664,6 +666,10 @@ struct laic_dev {
     cudaEvent_t other_ev = nullptr;  // laic_dev_wait_stream
     int vf_nseq = 0, vf_max = 0;
 
+    // The missing buffers of a set that a later call needs.
+    static cudaError_t make(std::initializer_list<laic::Want> set) {
+        return laic::alloc_missing(set, [](void** p, size_t bytes) { return cudaMalloc(p, bytes); });
+    }
     // `st` goes on behind what `other` holds now.
     int wait_stream(cudaStream_t other) {
         cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
@@ -1262,7 +1268,7 @@ struct laic_dev {
     }
 
     int prefill_alloc() {
-        if (pf_x) return LAIC_OK;
+        if (pf_ready) return LAIC_OK;
         const size_t T = kPfRows;
         size_t wmax = 0, cmax = 0;
         for (auto& l : layers)
@@ -1271,21 +1277,14 @@ struct laic_dev {
                 cmax = std::max(cmax, (size_t)m->rows);
             }
         const size_t amax = std::max((size_t)std::max(h, hq), (size_t)F);
-        CK(cudaMalloc(&pf_x, T * h * 4));
-        CK(cudaMalloc(&pf_c, T * cmax * 4));
-        CK(cudaMalloc(&pf_q, T * hq * 4));
-        CK(cudaMalloc(&pf_attn, T * hq * 4));
-        CK(cudaMalloc(&pf_a, T * amax * 2));
-        CK(cudaMalloc(&pf_w, wmax * 2));
-        CK(cudaMalloc(&pf_slots, T * 4));
-        CK(cudaMalloc(&pf_npos, T * 4));
-        CK(cudaMalloc(&pf_tokens, T * 4));
-        CK(cudaMalloc(&pf_len, T * 4));
-        CK(cudaMalloc(&pf_group, 3 * 4));
         for (auto& l : layers)
             for (const Mat* m : {&l.qkv, &l.o, &l.gu, &l.down})
                 pf_ws_bytes = std::max(pf_ws_bytes, laic::gemm_f16_workspace((int)T, m->rows, m->in));
-        if (pf_ws_bytes) CK(cudaMalloc(&pf_ws, pf_ws_bytes));
+        CK(make({{(void**)&pf_x, T * h * 4}, {(void**)&pf_c, T * cmax * 4}, {(void**)&pf_q, T * hq * 4},
+                 {(void**)&pf_attn, T * hq * 4}, {(void**)&pf_a, T * amax * 2}, {(void**)&pf_w, wmax * 2},
+                 {(void**)&pf_slots, T * 4}, {(void**)&pf_npos, T * 4}, {(void**)&pf_tokens, T * 4},
+                 {(void**)&pf_len, T * 4}, {(void**)&pf_group, 3 * 4}, {&pf_ws, pf_ws_bytes}}));
+        pf_ready = true;
         return LAIC_OK;
     }
 
@@ -2037,13 +2036,8 @@ static int verify_step(laic_dev* d, int32_t nseq, const int32_t* slots, int32_t 
     }
     CK(cudaSetDevice(d->device));
     const size_t RB = d->RB;
-    if (!d->vf_probs) {
-        CK(cudaMalloc(&d->vf_temp, RB * 4));
-        CK(cudaMalloc(&d->vf_u, 2 * RB * 4));
-        CK(cudaMalloc(&d->vf_ids, 2 * RB * 4));
-        CK(cudaMalloc(&d->vf_n, 2 * RB * 4));
-        CK(cudaMalloc(&d->vf_probs, RB * d->V * 4));
-    }
+    CK(laic_dev::make({{(void**)&d->vf_temp, RB * 4}, {(void**)&d->vf_u, 2 * RB * 4}, {(void**)&d->vf_ids, 2 * RB * 4},
+                       {(void**)&d->vf_n, 2 * RB * 4}, {(void**)&d->vf_probs, RB * d->V * 4}}));
     // rows: per sequence its token and the drafted ones, then padding (in no page, seen by nothing)
     std::vector<float> temp(rows, 0.f), u(2 * RB, 0.f);
     std::vector<uint32_t> ids(RB, 0);
