@@ -22,4 +22,22 @@ auto alloc_missing(std::initializer_list<Want> set, Alloc&& alloc) -> decltype(a
     return {};
 }
 
+// Replaces *p, which holds `cap` elements of `size` bytes, where `need` is above that. `moved` is set as soon as the old
+// buffer is gone; where the new one fails there is none, and `cap` is zero.
+template <typename Alloc, typename Free>
+auto regrow(void** p, size_t& cap, size_t need, size_t size, bool& moved, Alloc&& alloc, Free&& release)
+    -> decltype(alloc((void**)nullptr, (size_t)0)) {
+    if (need <= cap) return {};
+    if (*p) release(*p);
+    *p = nullptr;
+    cap = 0;
+    moved = true;
+    if (auto e = alloc(p, need * size)) {
+        *p = nullptr;
+        return e;
+    }
+    cap = need;
+    return {};
+}
+
 }  // namespace laic

@@ -380,43 +380,28 @@ MvNeed mv_need(const Mat& m, int B) {
     return n;
 }
 
-// Grow the scratch to `need`; returns whether any buffer moved (captured graphs are stale then).
+// Grow the scratch to `need`; `moved`: a buffer was replaced or lost, also where the call fails (captured graphs are
+// stale then).
 int mv_scratch_reserve(MvScratch& sc, const MvNeed& need, bool* moved = nullptr) {
-    bool mv = false;
+    bool mv = false, tickets = false;
+    bool& any = moved ? *moved : mv;
+    any = false;
     if (!sc.err) {
         CK(cudaMalloc(&sc.err, 4));
         if (int rc = zero_now(sc.err, 4)) return rc;
     }
-    if (need.part_floats > sc.part_cap) {
-        if (sc.part) cudaFree(sc.part);
-        sc.part = nullptr;
-        CK(cudaMalloc(&sc.part, need.part_floats * 4));
-        sc.part_cap = need.part_floats;
-        mv = true;
-    }
-    if (need.ntiles > sc.cnt_cap) {
-        if (sc.tile_cnt) cudaFree(sc.tile_cnt);
-        sc.tile_cnt = nullptr;
-        CK(cudaMalloc(&sc.tile_cnt, need.ntiles * 4));
+    auto grow = [&](void** p, size_t& cap, size_t n, size_t size, bool& m) {
+        return laic::regrow(p, cap, n, size, m, [](void** q, size_t bytes) { return cudaMalloc(q, bytes); },
+                            [](void* q) { cudaFree(q); });
+    };
+    CK(grow((void**)&sc.part, sc.part_cap, need.part_floats, 4, any));
+    const cudaError_t e = grow((void**)&sc.tile_cnt, sc.cnt_cap, need.ntiles, 4, tickets);
+    any |= tickets;
+    CK(e);
+    if (tickets)
         if (int rc = zero_now(sc.tile_cnt, need.ntiles * 4)) return rc;
-        sc.cnt_cap = need.ntiles;
-        mv = true;
-    }
-    if (need.xg_bytes > sc.xg_cap) {
-        if (sc.xg) cudaFree(sc.xg);
-        sc.xg = nullptr;
-        CK(cudaMalloc(&sc.xg, need.xg_bytes));
-        sc.xg_cap = need.xg_bytes;
-        mv = true;
-    }
-    if (need.xinv_floats > sc.xinv_cap) {
-        if (sc.xinv) cudaFree(sc.xinv);
-        sc.xinv = nullptr;
-        CK(cudaMalloc(&sc.xinv, need.xinv_floats * 4));
-        sc.xinv_cap = need.xinv_floats;
-        mv = true;
-    }
-    if (moved) *moved = mv;
+    CK(grow((void**)&sc.xg, sc.xg_cap, need.xg_bytes, 1, any));
+    CK(grow((void**)&sc.xinv, sc.xinv_cap, need.xinv_floats, 4, any));
     return LAIC_OK;
 }
 
@@ -736,13 +721,11 @@ struct laic_dev {
     int reserve_attn_ws(int rows, const KvBounds& b) {
         uint64_t need = 0;
         if (int rc = laic::kv_attention_bytes(layer_pages(0), attention_args(rows, b), &need)) return rc;
-        if (need <= attn_ws_cap) return LAIC_OK;
-        if (attn_ws) cudaFree(attn_ws);
-        attn_ws = nullptr;
-        attn_ws_cap = 0;
-        CK(cudaMalloc(&attn_ws, need));
-        attn_ws_cap = need;
-        drop_graphs();
+        bool moved = false;
+        const cudaError_t e = laic::regrow(&attn_ws, attn_ws_cap, need, 1, moved,
+                                           [](void** p, size_t bytes) { return cudaMalloc(p, bytes); }, [](void* p) { cudaFree(p); });
+        if (moved) drop_graphs();
+        CK(e);
         return LAIC_OK;
     }
     void drop_graphs() {
@@ -1383,7 +1366,7 @@ struct laic_dev {
         see(lm_head());
         bool moved = false;
         int rc = mv_scratch_reserve(mvs, need, &moved);
-        if (!rc && moved) drop_graphs();  // graphs captured the old buffers
+        if (moved) drop_graphs();  // graphs captured the old buffers
         return rc;
     }
 

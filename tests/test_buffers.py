@@ -33,3 +33,23 @@ def test_the_engine_makes_its_late_buffers_as_sets():
     src = open(os.path.join(ROOT, "laicompute_b200", "csrc", "engine.cu")).read()
     assert not re.search(r"cudaMalloc\(&(?:d->)?(?:vf_|pf_)", src)
     assert not re.search(r"if \(!?(?:d->)?(?:vf|pf)_(?!ready)\w+\) (?:return LAIC_OK|\{)", src)
+
+
+def test_a_growing_buffer_that_fails_is_known_to_be_gone(tmp_path):
+    """(error, moved, present, capacity) of each request: after a failure the smaller request allocates again."""
+    exe = str(tmp_path / "regrow_check")
+    subprocess.run(["g++", "-std=c++17", f"-I{ROOT}/laicompute_b200/csrc",
+                    os.path.join(ROOT, "tests", "host", "regrow_check.cpp"), "-o", exe], check=True)
+
+    def ask(fail_at, *needs):
+        out = subprocess.run([exe], input=" ".join(map(str, (fail_at, *needs))) + "\n", text=True, capture_output=True,
+                             check=True).stdout
+        return [tuple(map(int, x.split(":"))) for x in out.split()]
+    assert ask(9, 10, 5, 10, 20) == [(0, 1, 1, 10), (0, 0, 1, 10), (0, 0, 1, 10), (0, 1, 1, 20)]
+    assert ask(1, 10, 20, 5, 5) == [(0, 1, 1, 10), (2, 1, 0, 0), (0, 1, 1, 5), (0, 0, 1, 5)]
+    assert ask(0, 10, 0, 10) == [(2, 1, 0, 0), (0, 0, 0, 0), (0, 1, 1, 10)]
+
+
+def test_the_engine_grows_its_scratch_that_way():
+    src = open(os.path.join(ROOT, "laicompute_b200", "csrc", "engine.cu")).read()
+    assert not re.search(r"cudaMalloc\(&(?:sc\.(?!err)|attn_ws)", src) and src.count("laic::regrow(") == 2
