@@ -187,6 +187,7 @@ int check_attention(const laic_kv_pages& g, const laic_kv_attention_args& a) {
     if (a.rows < 0) return api_fail(LAIC_E_INVALID, "rows must be >= 0");
     if (a.heads < 1 || a.heads % g.kv_heads) return api_fail(LAIC_E_INVALID, "heads must be a multiple of kv_heads");
     if (a.heads / g.kv_heads > 8) return api_fail(LAIC_E_UNSUPPORTED, "at most 8 query heads per kv head");
+    if ((long long)a.rows * a.heads > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many rows of heads");
     if (!type_ok(a.type)) return api_fail(LAIC_E_UNSUPPORTED, "query and output type must be F32 or F16");
     if (!(a.scale >= 0.f)) return api_fail(LAIC_E_INVALID, "scale must not be negative");
     if (a.max_len < 0 || a.groups < 0 || a.max_private < -1) return api_fail(LAIC_E_INVALID, "negative bound");
@@ -208,7 +209,7 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
     // one piece and none is shorter than 128 (a join costs more than that many positions)
     auto split = [&](long long pairs, int len, long long want, int unit, int whole, int most) {
         if (len <= whole) return round_up(std::max(len, 1), unit);
-        const long long l = ((long long)len * pairs + want - 1) / want;
+        const long long l = std::min<long long>(((long long)len * pairs + want - 1) / want, kMaxPositions);
         return std::max(128, std::min(round_up(l, unit), most));
     };
     const int sms = device_sms(g.device);
@@ -254,7 +255,7 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
     }
     const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss * pl.cluster;
     const long long pi = (long long)a.rows * g.kv_heads * (pl.whole ? 1 : pl.nsp);
-    if (si + pi > INT_MAX || (long long)a.rows * a.heads > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
+    if (si + pi > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
     pl.shared_items = (int)si;
     pl.private_items = (int)pi;
     pl.direct = pl.bulk && pl.nss == 1 && pi == 0;

@@ -30,3 +30,17 @@ def test_positions_of_far_bounds_stay_within_an_int():
         for shared in (0, 1, MOST):
             assert i32(shared + last * split) >= 0 and i32(shared + MOST) >= 0
         assert i32(MOST + split) >= 0 and i32(MOST + split - 1) >= 0
+
+
+@pytest.mark.parametrize("rows,heads", [(1 << 29, 8), (1 << 28, 8), ((1 << 28) + 1, 8), ((1 << 31) - 1, 2)])
+def test_too_many_rows_are_refused(rows, heads):
+    """More (row, head) pairs than an int holds, with a group of them all (whose columns wrapped to zero)."""
+    for kw in (dict(groups=1, max_group_rows=rows, max_shared=16), dict(groups=1, max_group_rows=rows, max_shared=16, max_private=0),
+               {}):
+        _refused(UNSUPPORTED, "too many", lambda: _pages(kv_heads=1).attention_plan(rows, heads, rows, 2, 32, **kw))
+
+
+def test_the_most_rows_that_are_planned():
+    rows = ((1 << 31) - 1) // 8
+    plan = _pages(kv_heads=1).attention_plan(rows, 8, rows, 2, 32, groups=1, max_group_rows=rows, max_shared=16, max_private=0)
+    assert plan.workspace_bytes == rows * 8 * (64 * 4 + 8)  # one shared item per row and head
