@@ -113,17 +113,18 @@ __host__ __device__ inline bool group_rows(const KvAttnParams& p, int g, int& r0
     }
     return true;
 }
+// Length and sequence of row r.
+struct RowAt {
+    int n, seq;
+};
+__host__ __device__ inline RowAt row_at(const KvAttnParams& p, int r) { return RowAt{p.len[r], p.seq ? p.seq[r] : r}; }
 // The page table row through which the group of rows [r0, r1) is read: that of its first row that sees any
 // position (padding may name any sequence, and one that sees nothing need hold nothing). A bad one is recorded, and
-// reads some sequence's pages.
-__host__ __device__ inline int group_seq(const KvAttnParams& p, int r0, int r1) {
-    int n = p.len[r0], s = p.seq ? p.seq[r0] : r0;  // (under way together: the first row mostly sees something)
-    for (int r = r0 + 1; n <= 0 && r < r1; ++r) {
-        n = p.len[r];
-        s = p.seq ? p.seq[r] : r;
-    }
-    if (n <= 0) return 0;  // nothing is read
-    if (s >= 0 && s < p.nseq) return s;
+// reads some sequence's pages. `lead`: row r0, which the caller loads while other loads are under way.
+__host__ __device__ inline int group_seq(const KvAttnParams& p, int r0, int r1, RowAt lead) {
+    for (int r = r0 + 1; lead.n <= 0 && r < r1; ++r) lead = row_at(p, r);
+    if (lead.n <= 0) return 0;  // nothing is read
+    if (lead.seq >= 0 && lead.seq < p.nseq) return lead.seq;
     kv_flag(p.err, kKvBadSeq);
     return 0;
 }
@@ -165,26 +166,53 @@ __host__ __device__ inline RowView row_view(const KvAttnParams& p, int r, int sh
 __device__ __forceinline__ float seen_max(float m, float sum) { return m == -INFINITY && sum != sum ? 0.f : m; }
 
 // A value that is not finite reaches the rows that see it whatever its weight. The products may make NaN of an
-// infinite one (a weight rounded to zero, or its lo part's zero or sign), so where an output is NaN and its weights'
-// sum is not, it is the sum of the values of dimension d that are not finite, at the positions [t0, t1) whose block
-// of 16 is the `first` of every `stride`; x where there is none. (Out of line: the usual call never comes here.)
-__device__ __noinline__ float odd_values(const __half* vp, const int* page_ids, int page_shift, int kv_heads, int kvh, int D,
-                                         int d, int t0, int t1, int first, int stride, float x) {
-    const int a0 = t0 & ~15, first_page = t0 >> page_shift;
+// infinite one (a weight rounded to zero, its lo part's zero or sign, an item's weight in a join), so where an output
+// is NaN and the sum of its weights is not, it is the sum of the values of its dimension d that are not finite, over
+// the positions that row r sees; x where there is none. Outputs are looked up once they are stored: the usual call
+// pays for one test per output.
+__device__ __forceinline__ float odd_output(const KvAttnParams& p, int r, int kvh, int D, int d, float x) {
+    int shared = 0, lead = 0;
+    for (int g = 0; g < p.groups; ++g) {
+        int r0, r1;
+        if (!group_rows(p, g, r0, r1) || r < r0 || r >= r1) continue;
+        shared = group_shared(p, g);
+        lead = group_seq(p, r0, r1, row_at(p, r0));
+    }
+    const RowView v = row_view(p, r, shared);
+    const int end = min(v.n, v.shared + p.max_private);
     float sum = 0.f;
     bool any = false;
-    for (int t = t0; t < t1; ++t) {
-        if (((t - a0) >> 4) % stride != first) continue;
-        const int page = page_ids[(t >> page_shift) - first_page];
-        const float v = __half2float(vp[((((size_t)page * kv_heads + kvh) << page_shift) + (t & ((1 << page_shift) - 1))) * D + d]);
-        if (fabsf(v) <= 65504.f) continue;
-        sum += v;
-        any = true;
+#pragma unroll 1
+    for (int t0 = 0; t0 < end; t0 += 8) {  // (8 positions lie in one page)
+        auto page_of = [&](int seq) {
+            const int id = p.table[(size_t)max(0, seq) * p.pages_per_seq + (t0 >> p.page_shift)];
+            return id >= 0 && id < p.num_pages ? id : 0;
+        };
+        const int common = page_of(lead), own = page_of(v.seq);
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = t0 + i, page = t < v.shared ? common : own;
+            y[i] = t < end ? __half2float(p.vp[((((size_t)page * p.kv_heads + kvh) << p.page_shift) + (t & ((1 << p.page_shift) - 1))) * D + d])
+                           : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!(fabsf(y[i]) <= 65504.f)) {
+                sum += y[i];
+                any = true;
+            }
     }
     return any ? sum : x;
 }
-// The weight of an item against the largest maximum of its row, kept above zero: an infinite output stays one.
-__device__ __forceinline__ float item_weight(float m, float top) { return fmaxf(ex2(m - top), 0x1p-126f); }
+template <typename T>
+__device__ __forceinline__ void odd_outputs(const KvAttnParams& p, int r, int kvh, int D, int d, T* stored, int n) {
+#pragma unroll 1
+    for (int k = 0; k < n; ++k) {
+        const float x = kv_in<T>(stored[k]);
+        if (x != x) stored[k] = kv_out<T>(odd_output(p, r, kvh, D, d + k, x));
+    }
+}
 
 // Elements e and e + 1 (e even) of query row r.
 template <typename T>
@@ -512,19 +540,13 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
         float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < NW; ++k) {
-            w[k] = cm[k][col] == -INFINITY ? 0.f : item_weight(cm[k][col], M);
+            w[k] = cm[k][col] == -INFINITY ? 0.f : ex2(cm[k][col] - M);
             L = fmaf(cl[k][col], w[k], L);
-            if (w[k] != 0.f) {
+            if (cm[k][col] != -INFINITY) {
                 const float4 v = *reinterpret_cast<const float4*>(red + ((size_t)k * NC + col) * (D + 4) + d);
                 A.x = fmaf(v.x, w[k], A.x); A.y = fmaf(v.y, w[k], A.y);
                 A.z = fmaf(v.z, w[k], A.z); A.w = fmaf(v.w, w[k], A.w);
             }
-        }
-        if (A.x + A.y + A.z + A.w != A.x + A.y + A.z + A.w && L == L) {
-            auto seen = [&](float x, int k) {
-                return x == x ? x : odd_values(p.vp, page_ids, p.page_shift, p.kv_heads, kvh, D, d + k, t0, min(t1, lim[col]), 0, 1, x);
-            };
-            A = make_float4(seen(A.x, 0), seen(A.y, 1), seen(A.z, 2), seen(A.w, 3));
         }
         const int r = r0 + cc / p.G, h = kvh * p.G + cc % p.G;
         const size_t at = ((size_t)r * p.heads + h) * ns + slot;
@@ -764,10 +786,6 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
             m_[h] = seen_max(m_[h], x);
         }
     }
-    auto seen = [&](float x, int h, int d) {  // column h's output, where a product made NaN of it
-        return x == x || l_[h] != l_[h] ? x
-                                        : odd_values(p.vp, page_ids[warp], p.page_shift, p.kv_heads, kvh, D, d, t0, t1, first, STRIDE, x);
-    };
     const int ns = p.nss + p.nsp;
     if constexpr (!WHOLE) {
         if (nb > 0) {
@@ -782,7 +800,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                     for (int k = 0; k < 2; ++k) {
                         float x = o[mt][2 * k + h];
                         if (PK) x += __shfl_xor_sync(0xffffffffu, x, 2);
-                        if (mine) p.part_o[at * D + mt * 16 + gq + 8 * k] = seen(x, h, mt * 16 + gq + 8 * k);
+                        if (mine) p.part_o[at * D + mt * 16 + gq + 8 * k] = x;
                     }
                 if (mine && gq == 0) p.part_ml[at] = make_float2(m_[h], l_[h]);
             }
@@ -802,13 +820,14 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                 for (int k = 0; k < 2; ++k) {
                     float x = o[mt][2 * k + h];
                     if (PK) x += __shfl_xor_sync(0xffffffffu, x, 2);
-                    if (mine) red[((size_t)warp * 8 + col) * (D + 4) + mt * 16 + gq + 8 * k] = seen(x, h, mt * 16 + gq + 8 * k);
+                    if (mine) red[((size_t)warp * 8 + col) * (D + 4) + mt * 16 + gq + 8 * k] = x;
                 }
             if (mine && gq == 0) wml[warp][col] = make_float2(m_[h], l_[h]);
         }
         __syncthreads();
         const int live_s = v.shared > 0 ? (v.shared + p.ls * p.lc - 1) / (p.ls * p.lc) : 0;
         if (live_s || blockIdx.x == 0) pdl_wait();  // the shared items' results
+        bool odd = false;
         for (int e = threadIdx.x; e < p.G * (D / 4); e += NW * 32) {
             const int col = e / (D / 4), d = e % (D / 4) * 4, head = kvh * p.G + col;
             const size_t at = ((size_t)r * p.heads + head) * ns;
@@ -816,7 +835,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
             auto add = [&](float2 ml, const float4& x, float top) {
                 if (ml.x == -INFINITY) return;
-                const float w = item_weight(ml.x, top);
+                const float w = ex2(ml.x - top);
                 L = fmaf(ml.y, w, L);
                 a.x = fmaf(x.x, w, a.x); a.y = fmaf(x.y, w, a.y);
                 a.z = fmaf(x.z, w, a.z); a.w = fmaf(x.w, w, a.w);
@@ -840,7 +859,7 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
                 }
                 const float top = fmaxf(fmaxf(M, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
                 if (top > M) {
-                    const float corr = item_weight(M, top);
+                    const float corr = ex2(M - top);
                     L *= corr;
                     a.x *= corr; a.y *= corr; a.z *= corr; a.w *= corr;
                     M = top;
@@ -862,6 +881,15 @@ __global__ void __launch_bounds__(kPrWarps * 32) paged_private_kernel(const KvAt
 #pragma unroll
                 for (int k = 0; k < 4; ++k) dst[k] = kv_out<T>(x[k]);
             }
+            const float z = (a.x + a.y) + (a.z + a.w);
+            odd |= z - z != 0.f && L == L;
+        }
+        if (odd) {
+#pragma unroll 1
+            for (int e = threadIdx.x; e < p.G * (D / 4); e += NW * 32) {
+                const int d = e % (D / 4) * 4;
+                odd_outputs(p, r, kvh, D, d, static_cast<T*>(p.out) + (size_t)r * p.ldo + (size_t)(kvh * p.G + e / (D / 4)) * D + d, 4);
+            }
         }
     }
 }
@@ -880,6 +908,7 @@ __device__ __forceinline__ void shared_item(const KvAttnParams& p, int i, int* l
     if (!group_rows(p, g, r0, r1)) return;
     const int col0 = ct * NT * 8, ncol = (r1 - r0) * p.G;
     if (col0 >= ncol) return;
+    const RowAt lead = row_at(p, r0);
     const int shared = group_shared(p, g);
     if (tid < 32) {
         int n = 0;
@@ -895,7 +924,7 @@ __device__ __forceinline__ void shared_item(const KvAttnParams& p, int i, int* l
     __syncthreads();
     const int t0 = split * p.ls, t1 = min(range[0], t0 + p.ls);
     if (t0 >= t1) return;  // no row of the tile sees this far
-    pa_item<D, NT, T>(p, r0, col0, ncol, kvh, group_seq(p, r0, r1), t0, t1, split, lim, range[1], page_ids, cmul, smem);
+    pa_item<D, NT, T>(p, r0, col0, ncol, kvh, group_seq(p, r0, r1, lead), t0, t1, split, lim, range[1], page_ids, cmul, smem);
 }
 
 // Grid: the shared items.
@@ -960,7 +989,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
 #pragma unroll
         for (int u = 0; u < U; ++u) top = fmaxf(top, ml[u].x);
         if (top == -INFINITY) continue;
-        const float corr = item_weight(M, top);
+        const float corr = ex2(M - top);
         M = top;
         L *= corr;
 #pragma unroll
@@ -968,7 +997,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (ml[u].x != -INFINITY) {
-                const float w = item_weight(ml[u].x, M);
+                const float w = ex2(ml[u].x - M);
                 L = fmaf(ml[u].y, w, L);
 #pragma unroll
                 for (int e = 0; e < E; ++e) acc[e] = fmaf(x[u][e], w, acc[e]);
@@ -983,7 +1012,7 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
     for (int k = 0; k < kPmWarps; ++k) top = fmaxf(top, m_s[k]);
 #pragma unroll
     for (int k = 0; k < kPmWarps; ++k) {
-        w[k] = m_s[k] == -INFINITY ? 0.f : item_weight(m_s[k], top);
+        w[k] = m_s[k] == -INFINITY ? 0.f : ex2(m_s[k] - top);
         sum = fmaf(l_s[k], w[k], sum);
     }
     const float iv = top == -INFINITY ? 0.f : 1.f / sum;
@@ -992,8 +1021,9 @@ __global__ void __launch_bounds__(kPmWarps * 32) paged_merge_kernel(const KvAttn
         float a = 0.f;
 #pragma unroll
         for (int k = 0; k < kPmWarps; ++k)
-            if (w[k] != 0.f) a = fmaf(acc_s[k][d], w[k], a);
+            if (m_s[k] != -INFINITY) a = fmaf(acc_s[k][d], w[k], a);
         dst[d] = kv_out<T>(a * iv);
+        if (a - a != 0.f && sum == sum) odd_outputs(p, r, h / p.G, D, d, dst + d, 1);
     }
 }
 

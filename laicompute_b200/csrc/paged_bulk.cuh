@@ -33,7 +33,7 @@
 // Tiles that some column does not see to their end are masked. There 0 * V must not be 0 * inf: the
 // softmax threads clear what is not finite in V before the product (all of it past the positions any
 // column sees), note the positions, and the columns that do see one take its infinities and NaN at
-// the end, as do columns whose output a product with one made NaN.
+// the end. An output that is NaN all the same is looked up (odd_output).
 //
 // FP32 rows: Q as binary16 hi + lo after a scaling by a power of two, P likewise, the lo products
 // first (the accumulators then start from small terms); binary16 rows: one product each, P rounded to
@@ -56,6 +56,7 @@ constexpr int kBulkMaxCluster = 8;   // clusters of 1, 2, 4 or 8
 constexpr int kBulkMaxSplit = 2048;   // positions per item at most (its page ids are in shared memory)
 
 constexpr int kBulkKeys = 128;        // positions per tile
+constexpr float kBulkLowest = -3e38f; // the reference of a column that has seen no finite score
 constexpr int kBulkEarly = 2;         // ring items loaded before the CTA meets (a box takes 70 to 150 cycles to issue)
 __host__ __device__ constexpr int bulk_slot_bytes(int D) { return kBulkKeys * D * 2; }  // a tile of K or of V
 __host__ __device__ constexpr int bulk_q_bytes(int D, bool f32, int tiles) { return bulk_cols(tiles) * D * 2 * (f32 ? 2 : 1); }
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
             mbar_fence_init();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
-        const int seq = group_seq(p, r0, r1);
+        const RowAt lead = row_at(p, r0);
         // (rows that see nothing do not keep the others' tiles from being whole)
         int hi = 0, lo = 0x7fffffff;
         for (int k = lane; k <= row_of(min(COLS, ncol - col0) - 1); k += 32) {
@@ -309,6 +310,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         }
         hi = __reduce_max_sync(0xffffffffu, hi);
         lo = __reduce_min_sync(0xffffffffu, lo);
+        const int seq = group_seq(p, r0, r1, lead);
         const int npages = min(((t0 + p.ls - 1) >> p.page_shift) + 1, p.pages_per_seq) - first_page;
         for (int k = lane; k < npages; k += 32) page_ids[k] = p.table[(size_t)seq * p.pages_per_seq + first_page + k];
         if (lane == 0) { lim_max = hi; lim_min = lo; }
@@ -490,7 +492,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
         const uint32_t S = s_at(wg) + lane_at, O = o_at(wg) + lane_at;
         const float cm = fmaxf(cmul[tid], 1e-36f);  // (-inf * 0 would be NaN; below this every score is 0)
         const int wtid = tid & 127;
-        float mref = -INFINITY, l = 0.f;
+        float mref = 0.f, l = 0.f;
         bool ok = true;
         for (int j = 0; j < nt; ++j) {
             const int c0 = t0 + j * NK;
@@ -542,10 +544,9 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 for (int e = 0; e < 64; e += 2) mx4[(e >> 1) & 3] = max3(mx4[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                 const float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * cm;
                 if (j == 0 && h == 0) {
-                    mref = mx != mx ? 0.f : mx;  // (scores that are NaN alone: their sum says so)
+                    mref = fmaxf(mx, kBulkLowest);  // (below any finite score, where none has been seen)
                 } else if (__any_sync(0xffffffffu, mx > mref + kPaSlack)) {
-                    // (no finite score so far: nothing to rescale)
-                    const float next = fmaxf(mref, mx), corr = mref == -INFINITY ? 1.f : ex2(mref - next);
+                    const float next = fmaxf(mref, mx), corr = ex2(mref - next);
                     mref = next;
                     l *= corr;
                     sum2[0] = f2_mul(sum2[0], f2_pack(corr, corr));
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                     }
                 }
                 // ---- the weights: binary16 rows carry the factor in the exponent (their rounding is 2^-11 anyway)
-                const float shift = (F32 ? 0.f : 7.f) - (mref == -INFINITY ? 0.f : mref);
+                const float shift = F32 ? -mref : 7.f - mref;
                 const uint64_t sh2 = f2_pack(shift, shift);
 #pragma unroll
                 for (int k = 0; k < 64; k += 32) {
@@ -615,18 +616,9 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
                 tc_ld32(O + k, o);
                 tc_wait_ld();
                 tc_loaded(o);
-                bool nan = false;  // (an infinite value that every column sees, or scores that are NaN)
-#pragma unroll
-                for (int e = 0; e < 32; ++e) nan |= __uint_as_float(o[e]) != __uint_as_float(o[e]);
-                nan &= l == l;
-                if (nan) {  // as odd_values
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (__uint_as_float(o[e]) != __uint_as_float(o[e])) o[e] = 0;
-                }
-                if (nan || any_odd)
+                if (any_odd)
                     for (int t = t0; t < min(t1, lim); ++t)
-                        if (nan || (odd[(t - t0) >> 5] >> ((t - t0) & 31) & 1)) {
+                        if (odd[(t - t0) >> 5] >> ((t - t0) & 31) & 1) {
                             int id = page_ids[(t >> p.page_shift) - first_page];
                             if (id < 0 || id >= p.num_pages) id = 0;
                             const __half* v = p.vp + (((((size_t)id * p.kv_heads + kvh) << p.page_shift) +
@@ -641,7 +633,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
 #pragma unroll
                 for (int e = 0; e < 8; ++e) dst[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
             }
-            row_ml[tid] = make_float2(lim <= t0 ? -INFINITY : mref, live && view.n < 0 ? -1.f : F32 ? l * kPaGain : l);
+            row_ml[tid] = make_float2(lim <= t0 || l == 0.f ? -INFINITY : mref, live && view.n < 0 ? -1.f : F32 ? l * kPaGain : l);
         }
         tc_fence_before();
     }
@@ -663,6 +655,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     else __syncthreads();
     constexpr int LPR = D / 4, RPW = 32 / LPR;  // lanes per row, rows per warp and step
     const int ns = p.nss + p.nsp, slot_at = split / C, cols = min(COLS, ncol - col0);
+    bool odd_out = false;  // this thread has stored an output that is not finite
     auto join = [&](auto cc) {
         constexpr int CC = decltype(cc)::value, U = 8 / CC;  // U rows at a time: eight loads in flight
         const float* far_rows[CC];
@@ -697,7 +690,7 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
 #pragma unroll
                 for (int c = 0; c < CC; ++c)
                     if (ml[u][c].x != -INFINITY) {
-                        const float w = item_weight(ml[u][c].x, M);
+                        const float w = ex2(ml[u][c].x - M);
                         L = fmaf(ml[u][c].y, w, L);
                         a.x = fmaf(v[u][c].x, w, a.x); a.y = fmaf(v[u][c].y, w, a.y);
                         a.z = fmaf(v[u][c].z, w, a.z); a.w = fmaf(v[u][c].w, w, a.w);
@@ -721,6 +714,8 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
 #pragma unroll
                         for (int e = 0; e < 4; ++e) dst[e] = kv_out<T>(o[e]);
                     }
+                    const float z = (a.x + a.y) + (a.z + a.w);
+                    odd_out |= z - z != 0.f && L == L;
                 } else {
                     const size_t at = (row * p.heads + head) * ns + slot_at;
                     *reinterpret_cast<float4*>(p.part_o + at * D + e0) = a;
@@ -733,6 +728,18 @@ __global__ void __launch_bounds__(kBulkThreads, 1) paged_bulk_kernel(const KvAtt
     else if (C == 2) join(std::integral_constant<int, 2>{});
     else if (C == 4) join(std::integral_constant<int, 4>{});
     else join(std::integral_constant<int, 8>{});
+    if (odd_out) {  // (NaN: looked up, row by row as the join took them)
+        const int take = 8 / C;
+#pragma unroll 1
+        for (int k = 0;; ++k) {
+            const int cw = ((k / take * (bulk_threads(TILES) / 32) + warp) * take * C + rank + k % take * C) * RPW + lane / LPR;
+            if (cw >= COLS) break;
+            if (cw >= cols || row_ml[cw].y < 0.f) continue;
+            const int qr = row_of(cw), row = r0 + base_row + qr;
+            odd_outputs(p, row, kvh, D, lane % LPR * 4,
+                        static_cast<T*>(p.out) + (size_t)row * p.ldo + (size_t)(kvh * p.G + cw + base_head - qr * p.G) * D + lane % LPR * 4, 4);
+        }
+    }
     if (C > 1) cluster.sync();  // no CTA leaves while another may still read its rows
     groupless_rows<D, T>(p);
 }

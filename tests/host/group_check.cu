@@ -24,7 +24,7 @@ int main() {
         laic::KvAttnParams p{};
         p.err = &err;
         p.rows = a[2]; p.nseq = a[3]; p.len = len.data(); p.seq = a[4] ? seq.data() : nullptr;
-        const int s = laic::group_seq(p, a[0], a[1]);
+        const int s = laic::group_seq(p, a[0], a[1], laic::row_at(p, a[0]));
         std::printf("%d %d\n", s, err);
     }
     return 0;
