@@ -154,7 +154,8 @@ LAIC_API int laic_dev_step(laic_dev* dev, int32_t nseq, const uint32_t* tokens, 
 
 /* Engines with LAIC_FLAG_PAGED_KV: slot dst becomes a copy of slot src (cache, position, history). Whole pages
  * are shared, the partly filled one is copied. Slots that share pages and stand next to each other in a step's
- * list have their shared positions read once for all. No counterpart in the reference. */
+ * list have their shared positions read for all of them together (laic_kv_attention's groups). No counterpart in
+ * the reference. */
 LAIC_API int laic_dev_fork_slot(laic_dev* dev, int32_t src, int32_t dst);
 
 /* Engines with LAIC_FLAG_PAGED_KV: speculative decoding's step. tokens [nseq][max_draft + 1] holds for each
@@ -371,8 +372,9 @@ typedef struct laic_kv_attention_args {
 
 /* out[r] = softmax(scale * q[r] . K) V over the row's first len_dev[r] positions,
  * query head h with kv head h / (heads / kv_heads). The rows of group g hold the
- * same keys and values in positions [0, group_len_dev[g]): the kernels read them
- * once, through the page table row of the group's first row that sees any. Rows that
+ * same keys and values in positions [0, group_len_dev[g]): the kernels read them once
+ * for up to 256 columns (rows x heads / kv_heads; 32 in narrow groups and at head_dim
+ * 32), through the page table row of the group's first row that sees any. Rows that
  * share a whole sequence with causal lengths (a prompt's tokens, drafted tokens) are
  * a group whose length is the longest. Masked positions never reach a row's output,
  * whatever they hold; a NaN score that a row sees makes its head's output NaN, scores
@@ -416,7 +418,8 @@ typedef struct laic_verify_args {
  * everywhere), after n accepted tokens from p_n: the lowest v whose running sum
  * exceeds sample_u * total, in 64 bits. The tokens follow the target's
  * distribution. An id outside the vocabulary is refused; negative and NaN
- * probabilities count as zero. Padding sequences' outputs are left as they are. */
+ * probabilities count as zero. Padding sequences' outputs are left as they are. The
+ * outputs must not overlap an input. */
 LAIC_API int laic_verify_drafts(int32_t device, const laic_verify_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -1,4 +1,4 @@
-// Attention over a KV cache in pages, with shared prefixes read once.
+// Attention over a KV cache in pages, with shared prefixes read for all their rows together.
 //
 // out[r] = sum_t p_t v_t, p = softmax_t(scale q[r] . k_t) over the positions t < n_r of row r's
 // sequence. The work is cut into items, each a set of score columns (query row, query head of one
@@ -6,9 +6,11 @@
 //   private item: one row's G = heads / kv_heads columns over [shared, n_r): a CTA's four warps where the
 //   range is short (it then joins the shared items' results and writes the output), else a warp per split
 //   (memory bounds these: 64 rows of up to 8,000 positions, 8 kv heads of 128, 170 us, 6.0 TB/s, 92 % of a
-//   copy's rate; a warp's own ring needs no barrier, and eight to twelve warps an SM hide the loads);
-//   shared item (a CTA): up to 8 NT columns of a group's rows over a split of [0, shared), so the keys
-//   and values of a shared position are read once for all of them (wide groups: paged_bulk.cuh). What bounds
+//   copy's rate; a warp's own ring needs no barrier. Its next stage is loaded once the one before it is consumed, so
+//   a warp's loads do not run under its own products: the other eight to twelve warps of the SM hide them);
+//   shared item (a CTA): up to 8 NT columns (32 at most) of a group's rows over a split of [0, shared), so the keys
+//   and values of a shared position are read once for all of them (wide groups: paged_bulk.cuh, up to 256 columns at
+//   once; more columns, and at head_dim 32 more than 32, read them again, mostly out of L2). What bounds
 //   them is each warp's chain load -> QK -> softmax -> PV, so CTAs per SM count: eight groups of five rows,
 //   20 columns of head_dim 64, 500 to 8,000 positions take 33 us with four CTAs an SM, 45 with three.
 // An item keeps, per column, a reference m (a maximum of the scores seen, log2 domain, renewed when
@@ -556,8 +558,8 @@ __device__ __forceinline__ void pa_item(const KvAttnParams& p, int r0, int col0,
 }
 
 constexpr int kPrWarps = 4;
-// 16 positions of K and V each, per warp (three: fewer CTAs per SM, 192 us against 187 for 64 rows of 1 to 8,000
-// positions, 8 kv heads of 128)
+// 16 positions of K and V each, per warp (three: fewer CTAs per SM, 173.8 us against 172.4 for 64 rows of 1,024 to
+// 8,192 positions, 8 kv heads of 128, though 39.7 against 41.0 for 64 rows of up to 512 behind a shared prefix)
 constexpr int kPrStages = 2;
 constexpr int kPrWhole = 1024;    // no split is longer, and no range that stays whole
 __host__ __device__ constexpr size_t pr_smem(int D) { return (size_t)kPrWarps * kPrStages * 2 * 16 * D * 2; }

@@ -13,9 +13,9 @@
 // it takes S's place).
 // Binary16 rows, where a tile's exponentials take longer than its products: one lane multiplies for
 // both tiles in turn, which keeps one tile's products under the other's exponentials (512 prompt rows
-// behind 1,537 positions, 32 heads over 8 of 128: 39.0 us; a lane per tile let them fall into step, 41.0).
-// FP32 rows, with twice the products: a lane per tile (64 rows behind 4,101 shared positions: 44.0 us
-// against 48.6).
+// behind 1,537 positions, 32 heads over 8 of 128: 37.3 us; a lane per tile lets them fall into step, 39.3).
+// FP32 rows, with twice the products: a lane per tile, which won while a tile's way was longer; now the two are
+// alike (64 rows behind 4,101 shared positions: 41.0 us against 41.1; the prompt rows above: 52.1 against 50.1).
 // 128 positions per tile: a product of N = 64 takes about as long as one of N = 128 (100 against 85
 // cycles), and two score buffers of 64 ran slower than one of 128. O is rescaled only when a maximum
 // grew by more than 2^8 since the last time (weights stay below 2^15 in binary16 with the factor 2^7
@@ -23,8 +23,8 @@
 // softmax -> PV -> QK of a tile (4,200 cycles a pair of 128-position tiles in binary16, of which
 // the exponentials fill 2,048 at 16 a clock and the 32 products 2,700; 3,200 for one tile alone), and, for few tiles per CTA,
 // the way to the first scores (7,000 to 11,000 cycles: Q for every CTA out of L2) and the join (8,000
-// over a cluster's shared memory at about 14 bytes a clock). 512 prompt rows behind 1,537 positions:
-// 37 us, 404 TFLOP/s; 64 FP32 rows over 4,101 shared positions: 16 to 22 us of the call's 41.
+// over a cluster's shared memory at about 14 bytes a clock). The prompt rows above run at 404 TFLOP/s; the 64 FP32
+// rows over 4,101 shared positions take 16 to 22 us here, of the call's 41.
 //
 // The splits of a set of columns form a thread-block cluster and join through distributed shared
 // memory: one partial per cluster goes to global memory, or the output itself where the cluster holds

@@ -1,6 +1,7 @@
 """Serving operators on device pointers: a KV cache in pages (append with the position rotation,
-attention that reads shared prefixes once), probabilities of logits rows and the verification of
-drafted tokens (``laic_kv_*``, ``laic_logits_probs``, ``laic_verify_drafts`` of include/laic_b200.h).
+attention that reads shared prefixes for all their rows together), probabilities of logits rows and
+the verification of drafted tokens (``laic_kv_*``, ``laic_logits_probs``, ``laic_verify_drafts`` of
+include/laic_b200.h).
 
 As in ``engine.Matrix``, pointers are plain integers (``tensor.data_ptr()``) and ``stream`` a
 ``cudaStream_t``; calls return when their kernels are queued. A plan holds a call's shape, so that a
