@@ -477,7 +477,7 @@ def main() -> None:
             "rank_ms_per_step": [round(v / args.steps, 5) for v in r["rank_ms"]],
             "rank_spread": round(spread, 4),
             "e2e": {"value": round(r["e2e_value"], 2), "unit": "tokens/s", "h2d_bytes_per_step": batch * (4 + 4 + 24),
-                    "d2h_bytes_per_step": batch * 4 + 8},
+                    "d2h_bytes_per_step": batch * 4 + 12},
             "gpu_launches": int(args.steps * r["launches"]),
             "prefill": {"tokens_per_s": round(batch * (plen - 1) / r["prefill_s"], 1), "prompt_tokens": plen - 1,
                         "sequences": batch, "batched": r["tp"] == 1,

@@ -385,7 +385,7 @@ LAIC_API int laic_kv_attention(const laic_kv_pages* pages, const laic_kv_attenti
 /* Bytes of workspace the call needs (0 possible); reads no pointer of `args`. */
 LAIC_API int laic_kv_attention_workspace(const laic_kv_pages* pages, const laic_kv_attention_args* args,
                                          uint64_t* bytes);
-/* Synchronise `stream`, read and clear err_dev: LAIC_E_INVALID with the indices' description if any was refused. */
+/* Synchronise `stream`, read and clear err_dev: LAIC_E_INVALID with a description if an index was refused or a wait ran out. */
 LAIC_API int laic_kv_check(const laic_kv_pages* pages, void* stream);
 
 /* probs[r] = softmax(logits[r] / temperature[r]); temperature <= 0: one for the
