@@ -391,7 +391,7 @@ LAIC_API int laic_kv_check(const laic_kv_pages* pages, void* stream);
 /* probs[r] = softmax(logits[r] / temperature[r]); temperature <= 0: one for the
  * first maximum (sample()'s greedy choice, reference src/inference_v2.cpp:32), zeros elsewhere. A NaN
  * logit counts as -inf; equal +inf logits share the row; a row of -inf gives zeros. probs_dev
- * may be logits_dev with the same ld. */
+ * may be logits_dev with the same ld. vocab is at most 2^30 (here and below). */
 LAIC_API int laic_logits_probs(int32_t device, int32_t rows, int32_t vocab, const float* logits_dev, int64_t ld_logits,
                                const float* temperature_dev, float* probs_dev, int64_t ld_probs, void* stream);
 

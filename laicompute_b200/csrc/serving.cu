@@ -255,7 +255,7 @@ int plan_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, Attn
     }
     const long long si = (long long)a.groups * pl.ctiles * g.kv_heads * pl.nss * pl.cluster;
     const long long pi = (long long)a.rows * g.kv_heads * (pl.whole ? 1 : pl.nsp);
-    if (si + pi > INT_MAX) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
+    if (si + pi > INT_MAX - kPrWarps) return api_fail(LAIC_E_UNSUPPORTED, "too many attention items");
     pl.shared_items = (int)si;
     pl.private_items = (int)pi;
     pl.direct = pl.bulk && pl.nss == 1 && pi == 0;
@@ -481,10 +481,13 @@ int kv_attention(const laic_kv_pages& g, const laic_kv_attention_args& a, cudaSt
     });
 }
 
+constexpr int kMaxVocab = 1 << 30;  // (the kernels step past a row's end by less than that, in an int)
+
 int logits_probs(int device, int rows, int vocab, const float* x, long long ldx, const float* temp, float* y, long long ldy,
                  cudaStream_t st, LaunchOpts o) {
     if (rows < 0 || vocab < 1) return api_fail(LAIC_E_INVALID, "rows must be >= 0 and vocab >= 1");
     if (rows > INT_MAX / 8) return api_fail(LAIC_E_UNSUPPORTED, "too many rows");
+    if (vocab > kMaxVocab) return api_fail(LAIC_E_UNSUPPORTED, "a vocabulary of at most 2^30");
     if (rows == 0) return LAIC_OK;
     if (!x || !temp || !y) return api_fail(LAIC_E_INVALID, "null pointer");
     if (rows > 1 && (ldx < vocab || ldy < vocab)) return api_fail(LAIC_E_INVALID, "row strides must not be below the vocabulary");
@@ -512,6 +515,7 @@ int verify_drafts(int device, const laic_verify_args& a, cudaStream_t st, Launch
     if (a.nseq < 0 || a.vocab < 1) return api_fail(LAIC_E_INVALID, "nseq must be >= 0 and vocab >= 1");
     if (a.max_draft < 0) return api_fail(LAIC_E_INVALID, "max_draft must be >= 0");
     if (a.max_draft > LAIC_MAX_DRAFT) return api_fail(LAIC_E_UNSUPPORTED, "at most 64 drafted tokens per sequence");
+    if (a.vocab > kMaxVocab) return api_fail(LAIC_E_UNSUPPORTED, "a vocabulary of at most 2^30");
     if (a.nseq > INT_MAX / kVerifyMaxCluster) return api_fail(LAIC_E_UNSUPPORTED, "too many sequences");
     if (a.nseq == 0) return LAIC_OK;
     if (!a.target_dev || !a.n_draft_dev || !a.sample_u_dev || !a.out_ids_dev || !a.out_n_dev ||

@@ -44,3 +44,13 @@ def test_the_most_rows_that_are_planned():
     rows = ((1 << 31) - 1) // 8
     plan = _pages(kv_heads=1).attention_plan(rows, 8, rows, 2, 32, groups=1, max_group_rows=rows, max_shared=16, max_private=0)
     assert plan.workspace_bytes == rows * 8 * (64 * 4 + 8)  # one shared item per row and head
+
+
+@pytest.mark.parametrize("vocab", [(1 << 30) + 1, (1 << 31) - 1])
+def test_vocabularies_that_leave_an_int_are_refused(vocab):
+    """A row's loops step past its end: near 2^31 they would have wrapped to addresses before it."""
+    from laicompute_b200.serving import logits_probs, verify_drafts
+    _refused(UNSUPPORTED, "2^30", lambda: logits_probs(1, vocab, 4096, 4096, 4096))
+    _refused(UNSUPPORTED, "2^30", lambda: verify_drafts(1, 2, vocab, *[4096] * 8))
+    logits_probs(0, 1 << 30, 0, 0, 0)
+    verify_drafts(0, 2, 1 << 30, *[0] * 8)
